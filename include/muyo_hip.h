@@ -517,6 +517,141 @@ int muyo_sample_f32(float* logits, uint32_t vocab, const int32_t* history, uint3
                     const MuyoSamplerParams* params, void* state, void* workspace, int32_t* token, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Serving many requests: a cache in pages, shared by any number of sequences. The reference serves
+ * one chat from one contiguous cache (src/FullModel.cpp:622-625, src/KvCache.cpp:181-226), as the
+ * decoder above does; these launchers are for programs that batch sequences of many lengths.
+ *
+ * Layout: kcache and vcache are [pages][kv_heads][page_size][head_dim] fp16; slot s is row
+ * s % page_size of page s / page_size; row b of tables [sequences][table_pages] (int32) names the
+ * pages of sequence b in order. page_size is a power of two in 16..1024, pages * page_size < 2^31.
+ * Page ids, slots, positions and sequence numbers are device data: those outside their range are
+ * left out (as stated with each call), never read or written through.
+ *
+ * A step of a server:
+ *   muyo_paged_plan                   once: pages and slots for the step's new tokens
+ *   muyo_paged_rope_append_f16kv      per layer (a cache each, the same plan)
+ *   muyo_paged_attention_decode_f16kv per layer
+ *   muyo_token_logprobs_f32           on the step's logits
+ * None of them allocates or synchronises, so each may be captured into a graph.
+ * ------------------------------------------------------------------------------------------- */
+
+/* The plan of a step. lengths[b] keys of sequence b are in the cache and targets[b] are wanted: more
+ * for new tokens (a prompt starts at length 0), fewer to give pages back, 0 to end the sequence.
+ * free_pages [pages] is a ring of free page ids: pool[0] is the place of its first, pool[1] their
+ * number. Sequences are served in order, and one gets what it asks for when
+ *   - its length and target are in 0..table_pages * page_size,
+ *   - its new tokens fit in `tokens` behind those asked for by the sequences before it, and
+ *   - it needs no new page, or its pages are there behind those needed by the sequences before it;
+ * otherwise it stays as it is, with granted[b] = lengths[b] and no tokens. On return
+ *   granted[b]              the lengths after the step
+ *   pool_out                the ring's first place and number of free pages after the step
+ *   tables                  new pages entered from column ceil(length / page_size) on; the rest as it was
+ *   free_pages              pages given back entered behind the last free one (to be taken from the
+ *                           next call on); the rest as it was
+ *   starts [sequences + 1]  first entry of each sequence's new tokens in the three lists, then their number
+ *   token_sequence, positions, slots [tokens]   of each new token; -1 behind the last (a slot is -1 too
+ *                           where the page's id is outside the cache)
+ * granted may be lengths and pool_out may be pool; no other buffers may overlap. A page belongs to one
+ * sequence. A pool outside 0 <= pool[0] < pages, 0 <= pool[1] <= pages gives and takes no page. At most
+ * 4096 sequences, 2^24 tokens, table_pages * sequences and table_pages * page_size < 2^31. */
+int muyo_paged_plan(const int32_t* lengths, const int32_t* targets, uint32_t sequences, int32_t* tables,
+                    uint32_t table_pages, int32_t* free_pages, const int32_t* pool, uint32_t pages,
+                    uint32_t page_size, uint32_t tokens, int32_t* granted, int32_t* pool_out, int32_t* starts,
+                    int32_t* token_sequence, int32_t* positions, int32_t* slots, void* stream);
+
+/* Which values of a head form a rotated pair: (j, j + rotary_dim / 2), as rope_neox, or (2j, 2j + 1). */
+enum
+{
+    MUYO_ROPE_HALF = 0,
+    MUYO_ROPE_INTERLEAVED = 1
+};
+
+/* How positions past the trained context are taken into it. */
+enum
+{
+    MUYO_ROPE_SCALING_NONE = 0,
+    MUYO_ROPE_SCALING_LINEAR = 1, /* every pair turns 1 / factor as fast */
+    MUYO_ROPE_SCALING_BASE = 2,   /* the base times factor^(d / (d - 2)): the slowest pair turns 1 / factor as fast */
+    MUYO_ROPE_SCALING_YARN = 3,   /* pairs that turn over `high` times in trainedContext keep their speed, under `low`
+                                     times turn 1 / factor as fast, a ramp over the pairs between; the rotated
+                                     values times attnFactor * (1 + ln(factor) / 10). The ramp of
+                                     muyo_rope_neox_f32 with extFactor 1 (rope_funcs.glsl:17-35) */
+    MUYO_ROPE_SCALING_WAVELENGTH = 4 /* the same ends, a ramp over the turns between */
+};
+
+typedef struct MuyoRopeScaling
+{
+    uint32_t kind; /* MUYO_ROPE_SCALING_* */
+    float factor;
+    float low;  /* turns in the trained context (usually 1) */
+    float high; /* (usually 32 for YaRN, 4 by wavelength) */
+    float attnFactor; /* YaRN only (usually 1) */
+    uint32_t trainedContext;
+} MuyoRopeScaling;
+
+/* Host arithmetic, no device: turns[j] (j < rotary_dim / 2), the turns of pair j per position,
+ * base^(-2j / rotary_dim) / (2 pi) [/ pair_divisors[j]], scaled, in 64 bits; and the factor on rotated
+ * values. scaling and pair_divisors (the rope contract's frequency factors) may be NULL. */
+int muyo_rope_frequencies(double base, uint32_t rotary_dim, const MuyoRopeScaling* scaling,
+                          const float* pair_divisors, double* turns, float* magnitude);
+
+/* Rope and append of `tokens` new tokens: token t has position positions[t] and slot slots[t]. The
+ * first rotary_dim values of each head of q and k are rotated in pairs,
+ *   (x0, x1) -> magnitude * (x0 cos a - x1 sin a, x0 sin a + x1 cos a),  a = 2 pi positions[t] turns[j],
+ * the rest of a head stays. q goes to q_out [tokens][heads * head_dim] (f32), k and v as fp16 into their
+ * slots. q, k and v are f32 [tokens][heads * head_dim] with token strides of their own (in values,
+ * multiples of 4), so that they may be parts of stacked projection rows; q_out may be q where its
+ * stride is heads * head_dim. turns is device memory as muyo_rope_frequencies fills it.
+ * head_dim % 8 == 0 up to 1024, rotary_dim even. A token with a position below 0 is padding: its row
+ * of q_out and the caches stay as they were. One with a slot outside the cache is not appended. The
+ * slots of one call are distinct (as the plan makes them); the rows of a slot given twice are
+ * undefined. */
+int muyo_paged_rope_append_f16kv(const float* q, const float* k, const float* v, uint64_t q_stride,
+                                 uint64_t k_stride, uint64_t v_stride, float* q_out, void* kcache, void* vcache,
+                                 const int32_t* positions, const int32_t* slots, uint32_t tokens, uint32_t heads,
+                                 uint32_t kv_heads, uint32_t head_dim, uint32_t pages, uint32_t page_size,
+                                 uint32_t rope_layout, uint32_t rotary_dim, const double* turns, float magnitude,
+                                 void* stream);
+
+/* Attention of `queries` single tokens, each over the pages of its sequence: query i, at positions[i] of
+ * the sequence in row query_sequence[i] of tables, sees keys j <= positions[i], the last `window` of them
+ * where window > 0. For every head h (kv head h / (heads / kv_heads)):
+ *   out[i][h] = sum_j softmax_j(scale * q[i][h].k[j]) * v[j]
+ * q and out are f32 [queries][heads * head_dim]. A query without keys (a position below 0) gives 0. A
+ * query whose sequence is outside 0..sequences - 1 is padding: its row of out stays as it was. Keys past
+ * table_pages * page_size, or in pages with an id outside the cache, are left out. Queries may share a
+ * sequence (several new tokens of one). Which keys a workgroup takes depends on the whole batch, so a
+ * query's last bits may too; the same call gives the same bits.
+ * head_dim 64 or 128, at most 16 heads per kv head, 1024 heads, 65535 queries.
+ * `workspace` is caller-owned device memory (16-byte aligned) of at least
+ * muyo_paged_attention_decode_f16kv_workspace_bytes(...) bytes; it needs no clearing. Calls that
+ * overlap in time need their own. */
+size_t muyo_paged_attention_decode_f16kv_workspace_bytes(uint32_t queries, uint32_t heads, uint32_t kv_heads,
+                                                         uint32_t head_dim); /* 0: unsupported shape */
+int muyo_paged_attention_decode_f16kv(const float* q, const void* kcache, const void* vcache, float* out,
+                                      const int32_t* tables, uint32_t sequences, uint32_t table_pages,
+                                      const int32_t* query_sequence, const int32_t* positions, uint32_t queries,
+                                      uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t pages,
+                                      uint32_t page_size, uint32_t window, float scale, void* workspace,
+                                      uint64_t workspace_bytes, void* stream);
+
+/* Of each row of logits [rows][vocab] (f32, `row_stride` values apart), with p = softmax(row):
+ *   logprobs[r]     ln p of tokens[r]
+ *   ranks[r]        tokens before tokens[r] in the order of falling logits, equal ones by rising index
+ *   entropy[r]      -sum p ln p, in nats
+ *   top_ids[r][k], top_logprobs[r][k]   the first `top` tokens of that order, and their ln p
+ * logprobs, ranks and entropy may each be NULL (tokens too, without the first two), top 0..64 and at
+ * most vocab. A token outside the vocabulary has logprob -inf and rank -1. Logits of -inf have
+ * probability 0; a row of nothing else has logprobs -inf and entropy 0. A NaN or +inf among a row's
+ * logits makes its logprobs and entropy NaN; in the order NaN is last. `workspace` as above, of at least
+ * muyo_token_logprobs_workspace_bytes(...) bytes. */
+size_t muyo_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top); /* 0: unsupported */
+int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
+                            const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropy, uint32_t top,
+                            int32_t* top_ids, float* top_logprobs, void* workspace, uint64_t workspace_bytes,
+                            void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Synthetic-input helpers (portable seeded generator; bit-identical on host and device).
  *   word(seed, i)   = mix64(mix64(seed) + i)            mix64 = SplitMix64's finaliser
  *   uniform(i)      = (word >> 40) * 2^-23 - 1          in [-1, 1), exact in f32

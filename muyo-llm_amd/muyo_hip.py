@@ -110,6 +110,16 @@ class MuyoSamplerParams(ctypes.Structure):
     ]
 
 
+class MuyoRopeScaling(ctypes.Structure):
+    """How rope positions past the trained context are scaled; see muyo_rope_frequencies."""
+    _fields_ = [("kind", u32), ("factor", f32), ("low", f32), ("high", f32), ("attnFactor", f32),
+                ("trainedContext", u32)]
+
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALING = dict(NONE=0, LINEAR=1, BASE=2, YARN=3, WAVELENGTH=4)
+
+
 def sampler_params(temperature=0.0, top_k=40, top_p=0.95, repeat_penalty=1.0, repeat_last_n=64, seed=0):
     """The reference's defaults (src/Sampler.h:18-23)."""
     return MuyoSamplerParams(temperature, top_k, top_p, repeat_penalty, repeat_last_n, 0, seed)
@@ -214,6 +224,15 @@ _SIGNATURES = {
     "muyo_tokenizer_decode": (ctypes.c_int, [vp, vp, ctypes.c_uint64, vp, ctypes.c_uint64,
                                              ctypes.POINTER(ctypes.c_uint64)]),
     "muyo_tokenizer_token_bytes": (ctypes.c_int, [vp, i32, vp, ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint64)]),
+    "muyo_paged_plan": (ctypes.c_int, [vp, vp, u32, vp, u32, vp, vp, u32, u32, u32, vp, vp, vp, vp, vp, vp, vp]),
+    "muyo_rope_frequencies": (ctypes.c_int, [ctypes.c_double, u32, vp, vp, vp, ctypes.POINTER(f32)]),
+    "muyo_paged_rope_append_f16kv": (ctypes.c_int, [vp, vp, vp, u64, u64, u64, vp, vp, vp, vp, vp, u32, u32, u32, u32,
+                                                    u32, u32, u32, u32, vp, f32, vp]),
+    "muyo_paged_attention_decode_f16kv_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32, u32]),
+    "muyo_paged_attention_decode_f16kv": (ctypes.c_int, [vp, vp, vp, vp, vp, u32, u32, vp, vp, u32, u32, u32, u32, u32,
+                                                         u32, u32, f32, vp, u64, vp]),
+    "muyo_token_logprobs_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32]),
+    "muyo_token_logprobs_f32": (ctypes.c_int, [vp, u64, u32, u32, vp, vp, vp, vp, u32, vp, vp, vp, u64, vp]),
     "muyo_fill_normal_f16": (ctypes.c_int, [vp, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_double, ctypes.c_double, vp]),
     "muyo_fill_normal_f32": (ctypes.c_int, [vp, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_double, ctypes.c_double, vp]),
     "muyo_fill_uniform_f32": (ctypes.c_int, [vp, ctypes.c_uint64, ctypes.c_uint64, vp]),
@@ -685,6 +704,23 @@ class Decoder:
         check(self.lib.muyo_decoder_enqueue_kernel(self.handle, KERNEL[kernel], layer, stream))
 
 
+def rope_frequencies(base: float, rotary_dim: int, scaling: str = "NONE", factor: float = 1.0, low: float = 1.0,
+                     high: float = 32.0, attn_factor: float = 1.0, trained_context: int = 0, pair_divisors=None):
+    """muyo_rope_frequencies: (turns per position of each pair, a float64 array; the magnitude)."""
+    import numpy as np
+
+    s = MuyoRopeScaling(ROPE_SCALING[scaling], factor, low, high, attn_factor, trained_context)
+    turns, magnitude = np.empty(max(rotary_dim // 2, 1), np.float64), f32()
+    if pair_divisors is not None:
+        pair_divisors = np.ascontiguousarray(pair_divisors, dtype=np.float32)
+        if pair_divisors.size != rotary_dim // 2:
+            raise ValueError(f"pair_divisors has {pair_divisors.size} values for {rotary_dim // 2} pairs")
+    check(load().muyo_rope_frequencies(base, rotary_dim, ref(s),
+                                       None if pair_divisors is None else pair_divisors.ctypes.data,
+                                       turns.ctypes.data, ctypes.byref(magnitude)))
+    return turns, magnitude.value
+
+
 def tensor_seed(seed: int, kind: str, layer: int) -> int:
     return int(load().muyo_tensor_seed(seed, TENSOR[kind], layer))
 
@@ -693,6 +729,7 @@ def _self_check_sizes() -> None:
     for cls, words in CONTRACT_WORDS.items():
         assert ctypes.sizeof(cls) == 4 * words, cls.__name__
     assert ctypes.sizeof(MuyoSamplerParams) == 32
+    assert ctypes.sizeof(MuyoRopeScaling) == 24
 
 
 _self_check_sizes()
