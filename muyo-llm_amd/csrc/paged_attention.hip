@@ -16,13 +16,26 @@ constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / kWave;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kTile = 32;            // keys of a tile: what a wave takes at a time
+constexpr int kHalves = kTile / 16;       // matrix operands of 16 keys
 constexpr uint32_t kMaxGroup = 16;        // query heads per kv head: the columns of a matrix operation
 constexpr uint32_t kScanQueries = 1024;   // batches up to this many queries: each workgroup makes the sums itself
-constexpr uint32_t kWholeTiles = 32;      // caches of at most this many tiles are not split
-constexpr uint32_t kMinTiles = 16;        // a workgroup's share of the tiles is at least this long
+constexpr uint32_t kWholeKeys = 1024;     // caches of at most this many keys are not split
+constexpr uint32_t kMinTiles = kWaves;    // a workgroup's share of the tiles: at least one a wave
+constexpr uint32_t kSplitBlocks = 512;    // workgroups of a split launch: two on each of 256 CUs
 
-/// Workgroups of a split launch: as many as run at once on 256 CUs.
-constexpr uint32_t SplitBlocks(uint32_t headDim) { return headDim == 64 ? 1024 : 512; }
+/// *p for a p that is the same in the whole wave, of memory that nothing writes while the kernel runs: a
+/// scalar load. (Through a vector register the wait for it would also be one for every load before it:
+/// that took a third longer.)
+__device__ __forceinline__ int32_t ScalarLoad(const int32_t* p)
+{
+    return *(const __attribute__((address_space(4))) int32_t*)reinterpret_cast<uintptr_t>(p);
+}
+
+template <bool kOnce>
+__device__ __forceinline__ half8 LoadRow(const uint16_t* p)
+{
+    return kOnce ? __builtin_nontemporal_load(reinterpret_cast<const half8*>(p)) : *reinterpret_cast<const half8*>(p);
+}
 
 struct PagedAttentionArgs
 {
@@ -39,8 +52,10 @@ struct PagedAttentionArgs
     uint32_t pages, pageShift;
     uint32_t window;
     float scale;
-    uint64_t* tileSums;  // [queries + 1]: tiles of one kv head of the queries before
-    float* partials;     // [2 * blocks][group][2 + headDim]: max (log2 units), sum, weighted values
+    uint32_t* tileSums;  // [queries + 1]: tiles of one kv head of the queries before
+    uint4* cuts;         // what to join: query, kv head, first share, pieces (0: nothing)
+    uint32_t cutsByUnit; // cuts has an entry per (query, kv head); else one per share
+    float* partials;     // [2 * shares][group][4 + headDim]: max (log2 units), sum, -, -, weighted values
 };
 
 /// The keys begin..end - 1 that a query sees, and the tiles they lie in. A query without any has one
@@ -48,6 +63,7 @@ struct PagedAttentionArgs
 struct KeyRange
 {
     uint32_t begin, end, firstTile, tiles;
+    uint32_t row;  // of the tables
 };
 
 __device__ __forceinline__ KeyRange RangeOf(const PagedAttentionArgs& a, uint32_t query)
@@ -65,23 +81,20 @@ __device__ __forceinline__ KeyRange RangeOf(const PagedAttentionArgs& a, uint32_
         r.end = 0;
     }
     r.firstTile = r.begin / kTile;
-    r.tiles = max((r.end + kTile - 1) / kTile - r.firstTile, 1u);
-    if (row < 0 || static_cast<uint32_t>(row) >= a.sequences)
-    {
-        r.tiles = 0;
-    }
+    r.row = static_cast<uint32_t>(row);
+    r.tiles = r.row < a.sequences ? max((r.end + kTile - 1) / kTile - r.firstTile, 1u) : 0;
     return r;
 }
 
 /// Inclusive sum over the workgroup's threads, in thread order; `total` is the last one's.
 template <int kThreads>
-__device__ __forceinline__ uint64_t BlockSums(uint64_t v, uint64_t* waveSum, uint64_t& total)
+__device__ __forceinline__ uint32_t BlockSums(uint32_t v, uint32_t* waveSum, uint32_t& total)
 {
     const uint32_t lane = threadIdx.x & (kWave - 1);
 #pragma unroll
     for (uint32_t step = 1; step < kWave; step *= 2)
     {
-        const uint64_t other = __shfl_up(static_cast<unsigned long long>(v), step);
+        const uint32_t other = __shfl_up(v, step);
         v += lane >= step ? other : 0;
     }
     __syncthreads();
@@ -91,7 +104,7 @@ __device__ __forceinline__ uint64_t BlockSums(uint64_t v, uint64_t* waveSum, uin
     }
     __syncthreads();
     total = 0;
-    uint64_t before = 0;
+    uint32_t before = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kThreads / kWave; ++w)
     {
@@ -102,7 +115,7 @@ __device__ __forceinline__ uint64_t BlockSums(uint64_t v, uint64_t* waveSum, uin
 }
 
 /// The i with sums[i] <= at < sums[i + 1] (sums[0] = 0, at < sums[n]).
-__device__ __forceinline__ uint32_t OwnerOf(const uint64_t* sums, uint32_t n, uint64_t at)
+__device__ __forceinline__ uint32_t OwnerOf(const uint32_t* sums, uint32_t n, uint32_t at)
 {
     uint32_t low = 0;
     uint32_t high = n;
@@ -121,23 +134,17 @@ __device__ __forceinline__ uint32_t OwnerOf(const uint64_t* sums, uint32_t n, ui
     return low;
 }
 
-/// A workgroup's share of `total` tiles: the same for all but the last.
-__device__ __forceinline__ uint64_t ShareOf(uint64_t total, uint32_t blocks)
-{
-    return max((total + blocks - 1) / blocks, static_cast<uint64_t>(kMinTiles));
-}
-
 /// The sums of batches of more than kScanQueries queries, by one workgroup before the others start.
 __global__ __launch_bounds__(1024) void PagedTileSumsKernel(PagedAttentionArgs a)
 {
-    __shared__ uint64_t waveSum[1024 / kWave];
-    uint64_t before = 0;
+    __shared__ uint32_t waveSum[1024 / kWave];
+    uint32_t before = 0;
     for (uint32_t first = 0; first < a.queries; first += 1024)
     {
         const uint32_t i = first + threadIdx.x;
         const uint32_t tiles = i < a.queries ? RangeOf(a, i).tiles : 0;
-        uint64_t total;
-        const uint64_t sum = BlockSums<1024>(tiles, waveSum, total);
+        uint32_t total;
+        const uint32_t sum = BlockSums<1024>(tiles, waveSum, total);
         if (i < a.queries)
         {
             a.tileSums[i] = before + sum - tiles;
@@ -161,15 +168,15 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 
 /// The cache is read once: all the query heads of a kv head are columns of the same matrix operations
 /// (v_mfma_f32_16x16x32_f16: D = A.B with lane l supplying A[l % 16][8 (l / 16) .. +8] and
-/// B[8 (l / 16) .. +8][l % 16], receiving D[4 (l / 16) + r][l % 16]). Per tile of 32 keys a wave
-///   - takes K rows straight from memory as A operands (two of 16 keys) and forms S^T (keys x heads) =
+/// B[8 (l / 16) .. +8][l % 16], receiving D[4 (l / 16) + r][l % 16]). Per tile a wave
+///   - takes K rows straight from memory as A operands (of 16 keys each) and forms S^T (keys x heads) =
 ///     K . q^T, q in registers as two planes of f16 (hi + lo: 22 bits, of q over its largest value's
 ///     power of two);
 ///   - passes the V rows through its own part of LDS, to read them back transposed
 ///     (ds_read_b64_tr_b16: 16 lanes give 4 rows of 16 channels, each gets a channel of 4 rows);
 ///   - requests the next tile's K and V into the registers that are now free;
 ///   - makes the softmax weights of the running maximum and from them, in two planes again, the B operand:
-///     lane l's weights are keys 4 (l / 16) + r and 16 more, and the products sum over keys in any order,
+///     lane l's weights are keys 4 (l / 16) + r of each 16, and the products sum over keys in any order,
 ///     so the V^T operand just takes its rows in the same order: O^T (channels x heads) += V^T . P^T.
 /// f16 products are exact in f32 and the sums are f32 throughout; the planes keep what one f16 operand
 /// would lose (1e-4 of the result).
@@ -181,10 +188,17 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// kSplit: the tiles of all queries and kv heads in a row are dealt out in equal shares, whatever the
 /// sequences' lengths. A share may begin and end inside a (query, kv head); those pieces go to
 /// `partials` (a share has at most one that does not begin its (query, kv head) and one that does) for
-/// PagedAttentionMergeKernel. Otherwise a workgroup has one (query, kv head). Either way the
-/// workgroup's four waves take every fourth tile and join in LDS.
+/// PagedAttentionMergeKernel, which finds in `cuts` what to join. Otherwise a workgroup has one (query,
+/// kv head). Either way the workgroup's four waves take every fourth tile and join in LDS.
+///
+/// What bounds it: the cache's arrival. 64 sequences of 1 to 16384 keys (28 / 4 heads of 128, pages of 16,
+/// 1.07 GB of K and V): 169 us, 6.3 TB/s, where the best streaming read here has 6.9; 14 / 2 heads of 64,
+/// 0.27 GB: 47 us, 5.7 TB/s. Past the caches' size, loads without the non-temporal hint took 190 us; a
+/// split launch is for long caches, and loads K and V with it. Short ones are a chain of round trips
+/// (position, page, rows), 5 us: 8 or 16 waves a workgroup, tiles of 64 keys, and two or three tiles in
+/// flight at head_dim 64 all measured no better or worse.
 template <int kHd, bool kSplit>
-__global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKernel(PagedAttentionArgs a)
+__global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void PagedAttentionKernel(PagedAttentionArgs a)
 {
     constexpr int kSteps = kHd / 32;               // matrix operations over a head's channels
     constexpr int kChannels = kHd / 16;            // 16-channel blocks of the output
@@ -192,11 +206,13 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKerne
     constexpr uint32_t kRows = kWave / kChunks;    // V rows of one load of the wave
     constexpr int kHalfLoads = 16 / kRows;         // V loads of 16 keys
     constexpr uint32_t kWaveBytes = kTile * 2 * kHd;  // V of a tile; later O^T of 16 heads in f32
+    static_assert(kWaveBytes >= kMaxGroup * kHd * 4, "O^T fits where V was");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaves * kWaveBytes];
     __shared__ float waveMax[kWaves][kMaxGroup];
     __shared__ float waveTotal[kWaves][kMaxGroup];
-    __shared__ uint64_t tileSums[kSplit ? kScanQueries + 1 : 1];
-    __shared__ uint64_t waveSum[kWaves];
+    __shared__ uint32_t waveSum[kWaves];
+    __shared__ KeyRange firstRange;
+    __shared__ uint32_t firstAt[2];  // the share's first query, and the tiles before it
 
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -205,116 +221,209 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKerne
     const uint32_t pageSize = 1u << a.pageShift;
 
     uint32_t query, g;
-    uint64_t at = 0;   // this share's tiles, in the row of all
-    uint64_t stop = 0;
-    const uint64_t* sums = tileSums;
+    KeyRange range;
+    uint32_t at = 0;        // this share's next tile, in the row of all (the host keeps that below 2^32)
+    uint32_t stop = 0;
+    uint32_t share = 0;
+    uint32_t queryAt = 0;   // the first tile of the query
+    uint4 cut = make_uint4(0, 0, 0, 0);
     if constexpr (kSplit)
     {
+        uint32_t total;
         if (a.queries <= kScanQueries)
         {
+            // Every workgroup makes the sums; the thread that has the share's first query says so.
             constexpr uint32_t kPer = kScanQueries / kBlock;
-            uint32_t tiles[kPer];
-            uint64_t mine = 0;
+            KeyRange ranges[kPer];
+            uint32_t sum = 0;
 #pragma unroll
             for (uint32_t e = 0; e < kPer; ++e)
             {
                 const uint32_t i = threadIdx.x * kPer + e;
-                tiles[e] = i < a.queries ? RangeOf(a, i).tiles : 0;
-                mine += tiles[e];
+                ranges[e] = i < a.queries ? RangeOf(a, i) : KeyRange{};
+                sum += ranges[e].tiles;
             }
-            uint64_t total;
-            uint64_t sum = BlockSums<kBlock>(mine, waveSum, total) - mine;
+            const uint32_t all = sum;
+            sum = BlockSums<kBlock>(sum, waveSum, total) - all;
+            share = max((total * a.kvHeads + gridDim.x - 1) / gridDim.x, kMinTiles);
+            at = blockIdx.x * share;
 #pragma unroll
             for (uint32_t e = 0; e < kPer; ++e)
             {
-                const uint32_t i = threadIdx.x * kPer + e;
-                tileSums[i] = sum;
-                if (blockIdx.x == 0 && i < a.queries)
+                if (sum * a.kvHeads <= at && at < (sum + ranges[e].tiles) * a.kvHeads)
                 {
-                    a.tileSums[i] = sum;  // for the merge
+                    firstRange = ranges[e];
+                    firstAt[0] = threadIdx.x * kPer + e;
+                    firstAt[1] = sum;
                 }
-                sum += tiles[e];
-            }
-            if (threadIdx.x == 0)
-            {
-                tileSums[kScanQueries] = total;
-                if (blockIdx.x == 0)
-                {
-                    a.tileSums[a.queries] = total;
-                }
+                sum += ranges[e].tiles;
             }
             __syncthreads();
+            query = firstAt[0];
+            queryAt = firstAt[1] * a.kvHeads;
+            range = firstRange;
         }
         else
         {
-            sums = a.tileSums;
+            total = a.tileSums[a.queries];
+            share = max((total * a.kvHeads + gridDim.x - 1) / gridDim.x, kMinTiles);
+            at = blockIdx.x * share;
+            query = OwnerOf(a.tileSums, a.queries, min(at / a.kvHeads, total - 1));
+            queryAt = a.tileSums[query] * a.kvHeads;
+            range = RangeOf(a, query);
         }
-        const uint64_t total = sums[a.queries] * a.kvHeads;
-        const uint64_t share = ShareOf(total, gridDim.x);
-        at = blockIdx.x * share;
+        total *= a.kvHeads;
         stop = min(at + share, total);
-        if (at >= stop)
+        if (at >= total)
         {
+            if (a.cutsByUnit == 0 && threadIdx.x == 0)
+            {
+                a.cuts[blockIdx.x] = cut;
+            }
             return;
         }
-        query = OwnerOf(sums, a.queries, at / a.kvHeads);
         g = 0;
     }
     else
     {
         query = blockIdx.x / a.kvHeads;
         g = blockIdx.x % a.kvHeads;
+        range = RangeOf(a, query);
     }
 
     uint8_t* const mine = lds + wave * kWaveBytes;
     const uint32_t readAt = ValueAt<kHd>(4 * quad + column / 4, column % 4 / 2) + column % 2 * 8;
     do
     {
-        query = __builtin_amdgcn_readfirstlane(query);
-        const KeyRange range = RangeOf(a, query);
-        if (range.tiles == 0)
+        if constexpr (kSplit)
         {
-            if constexpr (kSplit)
-            {
-                ++query;  // padding has no tiles
-                continue;
-            }
-            else
-            {
-                return;
-            }
+            // The same for the whole workgroup, but read from LDS or counted up: scalars again.
+            query = __builtin_amdgcn_readfirstlane(query);
+            range.begin = __builtin_amdgcn_readfirstlane(range.begin);
+            range.end = __builtin_amdgcn_readfirstlane(range.end);
+            range.firstTile = __builtin_amdgcn_readfirstlane(range.firstTile);
+            range.tiles = __builtin_amdgcn_readfirstlane(range.tiles);
+            range.row = __builtin_amdgcn_readfirstlane(range.row);
         }
         uint32_t tile0 = 0;
         uint32_t tile1 = range.tiles;
         if constexpr (kSplit)
         {
-            const uint64_t inQuery = at - sums[query] * a.kvHeads;
-            g = static_cast<uint32_t>(inQuery / range.tiles);
-            tile0 = static_cast<uint32_t>(inQuery - static_cast<uint64_t>(g) * range.tiles);
-            tile1 = static_cast<uint32_t>(min(static_cast<uint64_t>(range.tiles), tile0 + (stop - at)));
+            if (range.tiles == 0)  // padding
+            {
+                ++query;
+                range = RangeOf(a, query);
+                continue;
+            }
+            g = __builtin_amdgcn_readfirstlane((at - queryAt) / range.tiles);
+            tile0 = __builtin_amdgcn_readfirstlane(at - queryAt - g * range.tiles);
+            tile1 = __builtin_amdgcn_readfirstlane(min(range.tiles, tile0 + (stop - at)));
+        }
+        else if (range.tiles == 0)
+        {
+            return;
         }
         const bool whole = tile0 == 0 && tile1 == range.tiles;
-        const int32_t* table = a.tables + static_cast<uint64_t>(a.querySequence[query]) * a.tablePages;
+        const int32_t* table = a.tables + static_cast<uint64_t>(range.row) * a.tablePages;
 
-        // The group's heads as columns; columns past it are 0. Planes of q / 2^e with 2^e above the head's
-        // largest value: f16 then holds any q.
-        half8 qhi[kSteps], qlo[kSteps];
-        float scaleLog2;
+        // q is requested before the first tile and made into operands while that arrives.
+        float4v qv[kSteps][2];
         {
-            float v[kSteps][8];
-            float largest = 0.0f;
             const float* from =
                 a.q + ((static_cast<uint64_t>(query) * a.kvHeads + g) * a.group + min(column, a.group - 1)) * kHd +
                 8 * quad;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
             {
-                *reinterpret_cast<float4*>(v[s]) = *reinterpret_cast<const float4*>(from + 32 * s);
-                *reinterpret_cast<float4*>(v[s] + 4) = *reinterpret_cast<const float4*>(from + 32 * s + 4);
+                qv[s][0] = *reinterpret_cast<const float4v*>(from + 32 * s);
+                qv[s][1] = *reinterpret_cast<const float4v*>(from + 32 * s + 4);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+
+        struct Pages
+        {
+            uint32_t of[kHalves];
+        };
+        // The part of a tile behind the table's end, if any, has the last page's id: its keys are past the
+        // range, and so masked.
+        auto pagesOf = [&](uint32_t tile) {
+            Pages ids;
+#pragma unroll
+            for (uint32_t half = 0; half < kHalves; ++half)
+            {
+                const uint32_t entry = ((range.firstTile + tile) * kTile + 16 * half) >> a.pageShift;
+                ids.of[half] = static_cast<uint32_t>(ScalarLoad(table + min(entry, a.tablePages - 1)));
+            }
+            return ids;
+        };
+        struct Tile
+        {
+            Pages pages;
+            half8 k[kHalves][kSteps];
+            half8 v[kHalves][kHalfLoads];
+        };
+        Tile now;
+        // A tile's K, then its V: loads complete in order, and the scores wait only for K. Pages outside the
+        // cache are read as page 0, whose rows are then masked.
+        auto request = [&](uint32_t tile, const Pages& pages) {
+            now.pages = pages;
+            uint64_t base[kHalves];
+#pragma unroll
+            for (uint32_t half = 0; half < kHalves; ++half)
+            {
+                const uint32_t page = pages.of[half] < a.pages ? pages.of[half] : 0;
+                const uint32_t row = ((range.firstTile + tile) * kTile + 16 * half) & (pageSize - 1);
+                base[half] = (((static_cast<uint64_t>(page) * a.kvHeads + g) << a.pageShift) + row) * kHd;
+            }
+#pragma unroll
+            for (uint32_t half = 0; half < kHalves; ++half)
+            {
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+                {
+                    now.k[half][s] = LoadRow<kSplit>(a.kcache + base[half] + (column * kHd + 8 * quad) + 32 * s);
+                }
+            }
+#pragma unroll
+            for (uint32_t half = 0; half < kHalves; ++half)
+            {
+#pragma unroll
+                for (int j = 0; j < kHalfLoads; ++j)
+                {
+                    now.v[half][j] = LoadRow<kSplit>(a.vcache + base[half] + lane * 8 + j * kRows * kHd);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+
+        float4v o[kChannels];
+#pragma unroll
+        for (int c = 0; c < kChannels; ++c)
+        {
+            o[c] = float4v{};
+        }
+        float runMax = -INFINITY;  // of the raw scores
+        float shift = 0.0f;        // in log2 units
+        float runSum = 0.0f;       // of this lane's keys
+        // A wave without a tile requests the last one and leaves it: a request under a condition would make
+        // the wait for q one for everything.
+        request(min(tile0 + wave, tile1 - 1), pagesOf(min(tile0 + wave, tile1 - 1)));
+        Pages next = pagesOf(min(tile0 + wave + kWaves, tile1 - 1));  // of the next tile to request
+
+        // The group's heads as columns; columns past it are 0. Planes of q / 2^e with 2^e above the head's
+        // largest value: f16 then holds any q.
+        half8 qhi[kSteps], qlo[kSteps];
+        float scaleLog2;
+        {
+            float largest = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+            {
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                 {
-                    largest = fmaxf(largest, fabsf(v[s][c]));
+                    largest = fmaxf(largest, fabsf(qv[s][c / 4][c % 4]));
                 }
             }
             largest = fmaxf(largest, PartnerLane<16>(largest));
@@ -333,7 +442,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKerne
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                 {
-                    const float x = column >= a.group ? 0.0f : ldexpf(v[s][c], -e) * sign;
+                    const float x = column >= a.group ? 0.0f : ldexpf(qv[s][c / 4][c % 4], -e) * sign;
                     const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);  // 11 bits: exact in f16
                     qhi[s][c] = static_cast<_Float16>(hi);
                     qlo[s][c] = static_cast<_Float16>(x - hi);
@@ -341,86 +450,53 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKerne
             }
         }
 
-        auto pageOf = [&](uint32_t tile, uint32_t half) {
-            const uint32_t column = ((range.firstTile + tile) * kTile + 16 * half) >> a.pageShift;
-            return column < a.tablePages ? static_cast<uint32_t>(table[column]) : 0xFFFFFFFFu;
-        };
-        half8 k[2][kSteps], v[2][kHalfLoads];
-        // A tile's K and V. Pages outside the cache are read as page 0, whose rows are then masked.
-        auto request = [&](uint32_t tile, uint32_t page0, uint32_t page1) {
-#pragma unroll
-            for (uint32_t half = 0; half < 2; ++half)
-            {
-                const uint32_t page = half == 0 ? page0 : page1;
-                const uint32_t row = ((range.firstTile + tile) * kTile + 16 * half) & (pageSize - 1);
-                const uint64_t base =
-                    (((static_cast<uint64_t>(page < a.pages ? page : 0) * a.kvHeads + g) << a.pageShift) + row) * kHd;
-                const uint16_t* kFrom = a.kcache + base + (column * kHd + 8 * quad);
-                const uint16_t* vFrom = a.vcache + base + lane * 8;
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s)
-                {
-                    k[half][s] = *reinterpret_cast<const half8*>(kFrom + 32 * s);
-                }
-#pragma unroll
-                for (int j = 0; j < kHalfLoads; ++j)
-                {
-                    v[half][j] = *reinterpret_cast<const half8*>(vFrom + j * kRows * kHd);
-                }
-            }
-        };
-
-        float4v o[kChannels];
-#pragma unroll
-        for (int c = 0; c < kChannels; ++c)
-        {
-            o[c] = float4v{};
-        }
-        float runMax = -INFINITY;  // of the raw scores
-        float shift = 0.0f;        // in log2 units
-        float runSum = 0.0f;       // of this lane's keys
-        uint32_t page0 = 0, page1 = 0;  // of the tile in registers
-        uint32_t next0 = 0, next1 = 0;  // of the one to request
-        if (tile0 + wave < tile1)
-        {
-            page0 = pageOf(tile0 + wave, 0);
-            page1 = pageOf(tile0 + wave, 1);
-            request(tile0 + wave, page0, page1);
-            const uint32_t later = min(tile0 + wave + kWaves, tile1 - 1);
-            next0 = pageOf(later, 0);
-            next1 = pageOf(later, 1);
-        }
         for (uint32_t tile = tile0 + wave; tile < tile1; tile += kWaves)
         {
-            float4v score[2] = {float4v{}, float4v{}};
+            const Pages afterNext = pagesOf(min(tile + 2 * kWaves, tile1 - 1));
+            float4v score[kHalves];
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
+            for (int half = 0; half < kHalves; ++half)
             {
-                score[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][s], qlo[s], score[0], 0, 0, 0);
-                score[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][s], qlo[s], score[1], 0, 0, 0);
+                score[half] = float4v{};
             }
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
             {
-                score[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[0][s], qhi[s], score[0], 0, 0, 0);
-                score[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[1][s], qhi[s], score[1], 0, 0, 0);
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half)
+                {
+                    score[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.k[half][s], qlo[s], score[half], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+            {
+#pragma unroll
+                for (int half = 0; half < kHalves; ++half)
+                {
+                    score[half] = __builtin_amdgcn_mfma_f32_16x16x32_f16(now.k[half][s], qhi[s], score[half], 0, 0, 0);
+                }
             }
             const uint32_t key0 = (range.firstTile + tile) * kTile;
-            const bool inside =
-                key0 >= range.begin && key0 + kTile <= range.end && page0 < a.pages && page1 < a.pages;
+            bool inside = key0 >= range.begin && key0 + kTile <= range.end;
+#pragma unroll
+            for (uint32_t half = 0; half < kHalves; ++half)
+            {
+                inside = inside && now.pages.of[half] < a.pages;
+            }
             if (!inside)
             {
 #pragma unroll
-                for (uint32_t half = 0; half < 2; ++half)
+                for (uint32_t half = 0; half < kHalves; ++half)
                 {
-                    const bool there = (half == 0 ? page0 : page1) < a.pages;
+                    const bool there = now.pages.of[half] < a.pages;
 #pragma unroll
                     for (int j = 0; j < kHalfLoads; ++j)
                     {
                         const uint32_t key = key0 + 16 * half + j * kRows + lane / kChunks;
                         if (!there || key < range.begin || key >= range.end)
                         {
-                            v[half][j] = half8{};
+                            now.v[half][j] = half8{};
                         }
                     }
 #pragma unroll
@@ -435,13 +511,13 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKerne
                 }
             }
 #pragma unroll
-            for (uint32_t half = 0; half < 2; ++half)
+            for (uint32_t half = 0; half < kHalves; ++half)
             {
 #pragma unroll
                 for (int j = 0; j < kHalfLoads; ++j)
                 {
                     const uint32_t row = 16 * half + j * kRows + lane / kChunks;
-                    *reinterpret_cast<half8*>(mine + ValueAt<kHd>(row, lane % kChunks)) = v[half][j];
+                    *reinterpret_cast<half8*>(mine + ValueAt<kHd>(row, lane % kChunks)) = now.v[half][j];
                 }
             }
             // The wave's LDS operations complete in order; this keeps the compiler's order too.
@@ -449,19 +525,16 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKerne
             __builtin_amdgcn_wave_barrier();
             if (tile + kWaves < tile1)
             {
-                page0 = next0;
-                page1 = next1;
-                request(tile + kWaves, page0, page1);
-                const uint32_t later = min(tile + 2 * kWaves, tile1 - 1);
-                next0 = pageOf(later, 0);
-                next1 = pageOf(later, 1);
+                request(tile + kWaves, next);
+                next = afterNext;
             }
 
             float tileMax = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int half = 0; half < kHalves; ++half)
             {
-                tileMax = fmaxf(tileMax, fmaxf(score[0][r], score[1][r]));
+                tileMax = fmaxf(tileMax, fmaxf(fmaxf(score[half][0], score[half][1]),
+                                               fmaxf(score[half][2], score[half][3])));
             }
             tileMax = fmaxf(tileMax, PartnerLane<16>(tileMax));
             tileMax = fmaxf(tileMax, PartnerLane<32>(tileMax));
@@ -481,34 +554,40 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKerne
                     o[c] *= factor;
                 }
             }
-            half8 phi, plo;
-            float sum[2] = {0.0f, 0.0f};
+            half8 phi[kHalves / 2], plo[kHalves / 2];
+            float sum = 0.0f;
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < kHalves; ++half)
             {
+                float4v p;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                 {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(score[half][r], scaleLog2, -shift));
-                    sum[half] += p;
-                    const _Float16 hi = static_cast<_Float16>(p);
-                    phi[4 * half + r] = hi;
-                    plo[4 * half + r] = static_cast<_Float16>(p - static_cast<float>(hi));
+                    p[r] = __builtin_amdgcn_exp2f(fmaf(score[half][r], scaleLog2, -shift));
+                    const _Float16 hi = static_cast<_Float16>(p[r]);
+                    phi[half / 2][4 * (half % 2) + r] = hi;
+                    plo[half / 2][4 * (half % 2) + r] = static_cast<_Float16>(p[r] - static_cast<float>(hi));
                 }
+                sum += (p[0] + p[1]) + (p[2] + p[3]);
             }
-            runSum += sum[0] + sum[1];
+            runSum += sum;
 #pragma unroll
             for (int c = 0; c < kChannels; ++c)
             {
-                uint8_t* from = mine + (readAt ^ (32u * c));
-                const half4 first = __builtin_bit_cast(
-                    half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)from));
-                const half4 second = __builtin_bit_cast(
-                    half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                               (__attribute__((address_space(3))) short4v*)(from + 16 * 2 * kHd)));
-                const half8 vt = __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7);
-                o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, plo, o[c], 0, 0, 0);
-                o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, phi, o[c], 0, 0, 0);
+#pragma unroll
+                for (int pair = 0; pair < kHalves / 2; ++pair)
+                {
+                    uint8_t* from = mine + ((readAt ^ (32u * c)) + pair * 32 * 2 * kHd);
+                    const half4 first = __builtin_bit_cast(
+                        half4,
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)from));
+                    const half4 second = __builtin_bit_cast(
+                        half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                   (__attribute__((address_space(3))) short4v*)(from + 16 * 2 * kHd)));
+                    const half8 vt = __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, plo[pair], o[c], 0, 0, 0);
+                    o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, phi[pair], o[c], 0, 0, 0);
+                }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -585,77 +664,130 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 4 : 2) void PagedAttentionKerne
         if constexpr (kSplit)
         {
             __syncthreads();  // the next piece overwrites the results
-            at += tile1 - tile0;
-            if (tile1 == range.tiles && g + 1 == a.kvHeads)
+            if (tile0 == 0)
             {
+                const uint32_t pieces = whole ? 0 : (at + range.tiles - 1) / share - blockIdx.x + 1;
+                const uint4 join = make_uint4(query, g, blockIdx.x, pieces);
+                if (a.cutsByUnit == 0)
+                {
+                    cut = join;  // only the last piece is not whole
+                }
+                else if (threadIdx.x == 0)
+                {
+                    a.cuts[query * a.kvHeads + g] = join;
+                }
+            }
+            at += tile1 - tile0;
+            if (at < stop && tile1 == range.tiles && g + 1 == a.kvHeads)
+            {
+                queryAt = at;
                 ++query;
+                range = RangeOf(a, query);
             }
         }
     } while (kSplit && at < stop);
+    if constexpr (kSplit)
+    {
+        if (a.cutsByUnit == 0 && threadIdx.x == 0)
+        {
+            a.cuts[blockIdx.x] = cut;
+        }
+    }
 }
 
-/// Joins the pieces of the (query, kv head) that the end of share blockIdx.x cuts, if no earlier share's
-/// end does: a workgroup per head, threads side by side over the channels and over every
-/// (256 / kHd)th piece. The pieces are added in their order.
-template <int kHd>
-__global__ __launch_bounds__(kBlock) void PagedAttentionMergeKernel(PagedAttentionArgs a, uint32_t blocks)
+/// Joins the pieces of a (query, kv head) that shares cut: blockIdx.x goes over those, or over the shares,
+/// whichever are fewer (a share's end cuts at most one that begins in it). A workgroup per head,
+/// kHd / 4 lanes over the channels of a piece, and kThreads / (kHd / 4) pieces side by side in slices,
+/// kDeep of each in flight. A slice's sums are relative to its own running maximum, so that nothing waits for
+/// a first pass over the maxima. The order is fixed.
+///
+/// 256 threads have 32 pieces of 128 channels in flight, 512 have 128: one sequence of 32749 keys (28 / 4
+/// heads, 28 workgroups of 128 pieces) takes 4.9 us with 512 threads and 7.6 with 256; 64 sequences (1792
+/// workgroups, most with three pieces) take 8.4 us with 512, whose waves start no faster, and 4.7 with 256.
+template <int kHd, int kThreads>
+__global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAttentionArgs a)
 {
-    constexpr uint32_t kSlices = kBlock / kHd;
-    __shared__ float sliceNum[kSlices][kHd];
+    constexpr uint32_t kLanes = kHd / 4;
+    constexpr uint32_t kSlices = kThreads / kLanes;
+    constexpr uint32_t kDeep = kThreads / 64;
+    __shared__ float4v sliceNum[kSlices][kLanes];
+    __shared__ float sliceMax[kSlices];
     __shared__ float sliceDen[kSlices];
-    const uint64_t total = a.tileSums[a.queries] * a.kvHeads;
-    const uint64_t share = ShareOf(total, blocks);
-    const uint64_t cut = (blockIdx.x + 1) * share;  // the end of share blockIdx.x
-    if (cut >= total)
+    const uint4 cut = a.cuts[blockIdx.x];
+    const uint32_t pieces = cut.w;
+    // By unit, padding has no entry.
+    if ((a.cutsByUnit != 0 && RangeOf(a, blockIdx.x / a.kvHeads).tiles == 0) || pieces == 0)
     {
         return;
     }
-    const uint32_t query = OwnerOf(a.tileSums, a.queries, cut / a.kvHeads);
-    const uint64_t tiles = a.tileSums[query + 1] - a.tileSums[query];
-    const uint64_t g = (cut - a.tileSums[query] * a.kvHeads) / tiles;
-    const uint64_t first = a.tileSums[query] * a.kvHeads + g * tiles;
-    if (cut == first || blockIdx.x * share > first)
-    {
-        return;
-    }
-    const uint32_t pieces = static_cast<uint32_t>((first + tiles - 1) / share) - blockIdx.x + 1;
     const uint32_t h = blockIdx.y;
-    // Piece 0 begins the (query, kv head), the others are their shares' first.
-    auto piece = [&](uint32_t p) {
-        return a.partials + (static_cast<uint64_t>(2 * (blockIdx.x + p) + (p == 0 ? 1 : 0)) * a.group + h) * (kHd + 4);
-    };
-    const uint32_t channel = threadIdx.x % kHd;
-    const uint32_t slice = threadIdx.x / kHd;
+    const uint32_t lane = threadIdx.x % kLanes;
+    const uint32_t slice = threadIdx.x / kLanes;
     float top = -INFINITY;
-    for (uint32_t p = 0; p < pieces; ++p)
-    {
-        top = fmaxf(top, piece(p)[0]);
-    }
-    float num = 0.0f;
     float den = 0.0f;
-    for (uint32_t p = slice; p < pieces; p += kSlices)
+    float4v num = float4v{};
+    for (uint32_t p0 = slice; p0 < pieces; p0 += kDeep * kSlices)
     {
-        const float* from = piece(p);
-        const float w = from[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(from[0] - top);
-        num = fmaf(w, from[4 + channel], num);
-        den = fmaf(w, from[1], den);
+        float4v head[kDeep], x[kDeep];
+        float best = top;
+#pragma unroll
+        for (uint32_t i = 0; i < kDeep; ++i)
+        {
+            // Piece 0 begins the (query, kv head), the others are their shares' first.
+            const uint32_t p = min(p0 + i * kSlices, pieces - 1);
+            const float* from = a.partials + (static_cast<uint64_t>(2 * (cut.z + p) + (p == 0 ? 1 : 0)) * a.group +
+                                              h) * (kHd + 4);
+            head[i] = *reinterpret_cast<const float4v*>(from);
+            x[i] = *reinterpret_cast<const float4v*>(from + 4 + 4 * lane);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kDeep; ++i)
+        {
+            best = p0 + i * kSlices < pieces ? fmaxf(best, head[i][0]) : best;
+        }
+        const float factor = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - best);
+        top = best;
+        den *= factor;
+        num *= factor;
+#pragma unroll
+        for (uint32_t i = 0; i < kDeep; ++i)
+        {
+            if (p0 + i * kSlices < pieces)
+            {
+                // A piece without keys is all 0; one of NaN scores has this maximum too, and stays NaN.
+                const float w = head[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(head[i][0] - best);
+                den = fmaf(w, head[i][1], den);
+                num += w * x[i];
+            }
+        }
     }
-    sliceNum[slice][channel] = num;
-    if (channel == 0)
+    sliceNum[slice][lane] = num;
+    if (lane == 0)
     {
+        sliceMax[slice] = top;
         sliceDen[slice] = den;
     }
     __syncthreads();
     if (slice == 0)
     {
+        float best = -INFINITY;
 #pragma unroll
-        for (uint32_t s = 1; s < kSlices; ++s)
+        for (uint32_t s = 0; s < kSlices; ++s)
         {
-            num += sliceNum[s][channel];
-            den += sliceDen[s];
+            best = fmaxf(best, sliceMax[s]);
         }
-        a.out[((static_cast<uint64_t>(query) * a.kvHeads + g) * a.group + h) * kHd + channel] =
-            den == 0.0f ? 0.0f : num / den;
+        num = float4v{};
+        den = 0.0f;
+#pragma unroll
+        for (uint32_t s = 0; s < kSlices; ++s)
+        {
+            const float w = sliceMax[s] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sliceMax[s] - best);
+            den = fmaf(w, sliceDen[s], den);
+            num += w * sliceNum[s][lane];
+        }
+        const float4v result = den == 0.0f ? float4v{} : num / den;
+        *reinterpret_cast<float4v*>(
+            a.out + ((static_cast<uint64_t>(cut.x) * a.kvHeads + cut.y) * a.group + h) * kHd + 4 * lane) = result;
     }
 }
 
@@ -665,25 +797,41 @@ bool AttentionShape(uint32_t queries, uint32_t heads, uint32_t kvHeads, uint32_t
            heads / kvHeads <= kMaxGroup && heads <= 1024 && (headDim == 64 || headDim == 128);
 }
 
-size_t TileSumBytes(uint32_t queries) { return (8 * (static_cast<size_t>(queries) + 1) + 15) & ~static_cast<size_t>(15); }
+/// The workspace's parts: the sums of batches that the workgroups do not sum themselves, the cuts, the
+/// partials.
+size_t TileSumBytes(uint32_t queries)
+{
+    return queries <= kScanQueries ? 0 : (4 * (static_cast<size_t>(queries) + 1) + 15) & ~static_cast<size_t>(15);
+}
+
+constexpr size_t kCutBytes = kSplitBlocks * sizeof(uint4);
 
 template <int kHd>
-hipError_t LaunchPagedAttention(hipStream_t s, const PagedAttentionArgs& a)
+hipError_t LaunchPagedAttention(hipStream_t s, PagedAttentionArgs a)
 {
     const uint64_t keys = std::min<uint64_t>(static_cast<uint64_t>(a.tablePages) << a.pageShift,
                                              a.window != 0 ? a.window : 0xFFFFFFFFull);
-    if (keys <= kWholeTiles * kTile)
+    const uint64_t units = static_cast<uint64_t>(a.queries) * a.kvHeads;
+    if (keys <= kWholeKeys || units * (keys / kTile + 2) > 0x7FFFFFFFull)
     {
-        hipLaunchKernelGGL((PagedAttentionKernel<kHd, false>), dim3(a.queries * a.kvHeads), dim3(kBlock), 0, s, a);
+        hipLaunchKernelGGL((PagedAttentionKernel<kHd, false>), dim3(static_cast<uint32_t>(units)), dim3(kBlock), 0, s, a);
         return hipGetLastError();
     }
     if (a.queries > kScanQueries)
     {
         hipLaunchKernelGGL(PagedTileSumsKernel, dim3(1), dim3(1024), 0, s, a);
     }
-    const uint32_t blocks = SplitBlocks(kHd);
-    hipLaunchKernelGGL((PagedAttentionKernel<kHd, true>), dim3(blocks), dim3(kBlock), 0, s, a);
-    hipLaunchKernelGGL(PagedAttentionMergeKernel<kHd>, dim3(blocks - 1, a.group), dim3(kBlock), 0, s, a, blocks);
+    a.cutsByUnit = units < kSplitBlocks ? 1 : 0;
+    const uint32_t joins = a.cutsByUnit != 0 ? static_cast<uint32_t>(units) : kSplitBlocks - 1;
+    hipLaunchKernelGGL((PagedAttentionKernel<kHd, true>), dim3(kSplitBlocks), dim3(kBlock), 0, s, a);
+    if (joins * a.group <= 256)
+    {
+        hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, 512>), dim3(joins, a.group), dim3(512), 0, s, a);
+    }
+    else
+    {
+        hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, 256>), dim3(joins, a.group), dim3(256), 0, s, a);
+    }
     return hipGetLastError();
 }
 }  // namespace
@@ -698,7 +846,8 @@ extern "C" size_t muyo_paged_attention_decode_f16kv_workspace_bytes(uint32_t que
     {
         return 0;
     }
-    return TileSumBytes(queries) + sizeof(float) * 2 * SplitBlocks(head_dim) * (heads / kv_heads) * (head_dim + 4);
+    return TileSumBytes(queries) + kCutBytes +
+           sizeof(float) * 2 * kSplitBlocks * (heads / kv_heads) * (head_dim + 4);
 }
 
 extern "C" int muyo_paged_attention_decode_f16kv(const float* q, const void* kcache, const void* vcache, float* out,
@@ -756,8 +905,10 @@ extern "C" int muyo_paged_attention_decode_f16kv(const float* q, const void* kca
                          0,
                          window,
                          scale,
-                         static_cast<uint64_t*>(workspace),
-                         reinterpret_cast<float*>(static_cast<char*>(workspace) + TileSumBytes(queries))};
+                         static_cast<uint32_t*>(workspace),
+                         reinterpret_cast<uint4*>(static_cast<char*>(workspace) + TileSumBytes(queries)),
+                         0,
+                         reinterpret_cast<float*>(static_cast<char*>(workspace) + TileSumBytes(queries) + kCutBytes)};
     while ((1u << a.pageShift) < page_size)
     {
         ++a.pageShift;

@@ -431,6 +431,7 @@ def test_attention_pages_and_windows(mh, gpu, size, window):
 @pytest.mark.parametrize("hd, positions", [
     (128, [20000]), (64, [20011]), (64, [32767]), (128, [3000, 1, 9000, 0, 150]),
     (64, [700] * 200), (128, list(range(0, 640, 5))),
+    (64, [2000, 5] * 512), (64, [0, 40, 1300, 7, -1] * 250), (128, [9] * 1500 + [4000]),
 ])
 def test_attention_long_and_many(mh, gpu, hd, positions):
     rng = np.random.default_rng(len(positions))
