@@ -1,9 +1,9 @@
 // Log probabilities of given tokens, their ranks, the entropy and the most likely tokens of rows of
 // logits.
 //
-// With m the row's largest logit, s = sum e^(x - m) and t = sum e^(x - m) (x - m): a token's log
-// probability is x - m - log s and the row's entropy log s - t / s. Parts of a row join exactly: over a
-// larger maximum m' = m - d, s becomes s e^d and t becomes (t + d s) e^d (d <= 0).
+// With m the row's largest logit, y = (x - m) log2 e, s = sum 2^y and t = sum 2^y y, a token's log
+// probability is (x - m) - ln s and the row's entropy ln s - ln 2 t / s. Parts of a row join exactly: over
+// a larger m, with d = (m - larger) log2 e, s becomes s 2^d and t becomes (t + d s) 2^d.
 #include <algorithm>
 #include <cmath>
 
@@ -15,12 +15,15 @@ namespace
 {
 constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / kWave;
-constexpr int kQuads = 8;                           // 16-byte loads of a lane's batch
+constexpr int kQuads = 4;                           // 16-byte loads of a lane's batch
 constexpr uint32_t kBatch = kWave * 4 * kQuads;     // logits a wave takes at a time
+constexpr int kFewLanes = 4;                        // looked at one by one
 constexpr uint32_t kMaxTop = 64;                    // a lane of a wave each
 constexpr uint32_t kMaxParts = 64;                  // workgroups of a row
-constexpr uint32_t kTargetBlocks = 2048;            // workgroups wanted of a call: eight for each of 256 CUs
+constexpr uint32_t kBlocksAtOnce = 1280;            // workgroups that 256 CUs run at once
+constexpr uint64_t kOnceBytes = 256ull << 20;       // logits that no cache holds: read without caching them
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct LogprobArgs
 {
@@ -79,85 +82,148 @@ struct Sums
 /// `x` over the maximum `m` (at least its own).
 __device__ __forceinline__ void Rebase(Sums& x, float m)
 {
-    // Differences of the type's lowest value or of -inf: their weight is 0, and 0 times them shall be 0. (NaN
-    // stays in s.)
-    const float d = x.m == m ? 0.0f : fmaxf(x.m - m, -1e4f);
-    const float f = exp2f(d * kLog2e);
+    // Differences to the type's lowest value overflow: the weight is 0, and 0 times them shall be 0. (A
+    // part without logits above -inf has sums of 0, and NaN stays in s.)
+    const float d = x.m == m || x.m == -INFINITY ? 0.0f : fmaxf((x.m - m) * kLog2e, -1e4f);
+    const float f = exp2f(d);
     x.t = (x.t + d * x.s) * f;
     x.s *= f;
     x.m = m;
 }
 
-/// One row's answers from its sums and the keys of its first `top` tokens. By the calling threads,
-/// `thread` of `threads`.
-__device__ __forceinline__ void WriteRow(const LogprobArgs& a, uint32_t row, const Sums& x, const uint64_t* best,
-                                         uint32_t thread, uint32_t threads)
+/// The given token of a row, and its logit.
+struct Given
+{
+    bool is;
+    uint32_t token;
+    float logit;
+};
+
+__device__ __forceinline__ Given GivenOf(const LogprobArgs& a, uint32_t row)
+{
+    const int32_t token = a.tokens != nullptr ? a.tokens[row] : -1;
+    Given g;
+    g.is = token >= 0 && static_cast<uint32_t>(token) < a.vocab;
+    g.token = static_cast<uint32_t>(token);
+    g.logit = g.is ? a.logits[row * a.stride + g.token] : INFINITY;
+    return g;
+}
+
+/// One row's answers from its sums and the keys of its first `top` tokens.
+__device__ __forceinline__ void WriteRow(const LogprobArgs& a, uint32_t row, const Sums& x, const Given& given,
+                                         const uint64_t* best)
 {
     const bool empty = x.s == 0.0f;  // no logit above -inf
     const float logSum = empty ? 0.0f : logf(x.s);
-    for (uint32_t k = thread; k < a.top; k += threads)
+    for (uint32_t k = threadIdx.x; k < a.top; k += kBlock)
     {
         const uint64_t at = static_cast<uint64_t>(row) * a.top + k;
         a.topIds[at] = static_cast<int32_t>(~static_cast<uint32_t>(best[k]));
         a.topLogprobs[at] = empty ? -INFINITY : KeyValue(best[k]) - x.m - logSum;
     }
-    if (thread == 0)
+    if (threadIdx.x == 0)
     {
-        const int32_t token = a.tokens != nullptr ? a.tokens[row] : -1;
-        const bool given = token >= 0 && static_cast<uint32_t>(token) < a.vocab;
         if (a.logprobs != nullptr)
         {
-            a.logprobs[row] =
-                !given || empty ? -INFINITY : a.logits[row * a.stride + static_cast<uint32_t>(token)] - x.m - logSum;
+            a.logprobs[row] = !given.is || empty ? -INFINITY : given.logit - x.m - logSum;
         }
         if (a.ranks != nullptr)
         {
-            a.ranks[row] = given ? static_cast<int32_t>(x.above) : -1;
+            a.ranks[row] = given.is ? static_cast<int32_t>(x.above) : -1;
         }
         if (a.entropy != nullptr)
         {
-            a.entropy[row] = empty ? 0.0f : logSum - x.t / x.s;
+            a.entropy[row] = empty ? 0.0f : logSum - kLn2 * (x.t / x.s);
         }
     }
 }
 
 /// The `top` largest of keys[0..count) (different ones, in LDS), into best[0..top) in falling order: a
-/// key's place is the number of keys above it.
-__device__ __forceinline__ void RankKeys(const uint64_t* keys, uint32_t count, uint32_t top, uint64_t* best)
+/// key's place is the number of keys above it. Up to 256 keys are counted against by four threads each (64
+/// keys), two or one; `places` has room for 256.
+__device__ __forceinline__ void RankKeys(const uint64_t* keys, uint32_t count, uint32_t top, uint64_t* best,
+                                         uint32_t* places)
 {
-    for (uint32_t i = threadIdx.x; i < count; i += blockDim.x)
+    if (count <= kBlock)
+    {
+        const uint32_t span = count <= 64 ? 64 : count <= 128 ? 128 : 256;
+        const uint32_t i = threadIdx.x & (span - 1);
+        places[threadIdx.x] = 0;
+        __syncthreads();
+        const uint64_t key = i < count ? keys[i] : 0;
+        uint32_t above = 0;
+#pragma unroll 4
+        for (uint32_t j = threadIdx.x / span; j < count; j += kBlock / span)
+        {
+            above += keys[j] > key ? 1u : 0u;
+        }
+        if (i < count)
+        {
+            atomicAdd(places + i, above);
+        }
+        __syncthreads();
+        if (threadIdx.x < count && places[threadIdx.x] < top)
+        {
+            best[places[threadIdx.x]] = key;
+        }
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < count; i += kBlock)
     {
         const uint64_t key = keys[i];
-        uint32_t place = 0;
-#pragma unroll 8
+        uint32_t above = 0;
+#pragma unroll 4
         for (uint32_t j = 0; j < count; ++j)
         {
-            place += keys[j] > key ? 1u : 0u;
+            above += keys[j] > key ? 1u : 0u;
         }
-        if (place < top)
+        if (above < top)
         {
-            best[place] = key;
+            best[above] = key;
         }
     }
 }
 
-/// One pass over the row: a wave takes batches of 2048 logits into registers, the next one on its way
-/// meanwhile, and each lane keeps the sums of its own.
+/// A value that `high` reaches in lanes that count for `top` together, `each` apiece (0: fewer do): the
+/// largest one of 16 bits.
+__device__ __forceinline__ uint32_t LowerBound(uint32_t high, uint32_t each, uint32_t top)
+{
+    uint32_t bound = 0;
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit > 1u << 15; bit >>= 1)
+    {
+        bound = CountLanes(high >= (bound | bit)) * each >= top ? bound | bit : bound;
+    }
+    return bound;
+}
+
+/// One pass over the row: a wave takes batches of kBatch logits into registers and each lane keeps the sums
+/// of its own.
 ///
 /// The first `top` tokens: the wave's best so far lie in order across its lanes (lane i has the i-th), and
 /// a batch is looked through only if some lane's largest logit reaches the last of them. Then a lower bound
 /// of the batch's own `top`-th is found first, by bisection: a value that the largest ones of `top` lanes
-/// reach. What reaches both bounds, a few more than `top` in the first batch and hardly any later, is
-/// inserted one by one. Equal logits are told apart by their index in the key, so nothing overflows.
+/// reach. Few lanes reach both bounds in a later batch: their logits are looked at lane by lane. In the first
+/// batch the candidates, a few more than `top`, are gathered and ranked (a candidate's place is the number
+/// of those above it). What is left (more than 64 candidates) is inserted one by one. Equal logits are told
+/// apart by their index in the key, so nothing overflows.
 ///
 /// The rank is counted on the way: the tokens before a given one have a larger logit, or the same at
 /// a lower index, which is a different comparison on each side of its batch.
+///
+/// That batch, and batches to be looked through, go through LDS: the registers are free for the next
+/// batch at once, and loops over their logits need not be unrolled (most workgroups run such code once
+/// or twice, and its instructions would come from memory).
 template <bool kOnce>
-__global__ __launch_bounds__(kBlock, 3) void TokenLogprobsKernel(LogprobArgs a)
+__global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
 {
     __shared__ Sums waveSums[kWaves];
-    __shared__ uint64_t waveKeys[kWaves * kMaxTop];
+    __shared__ uint32_t waveHeld[kWaves];
+    __shared__ uint64_t waveKeys[kWaves * kWave];
     __shared__ uint64_t best[kMaxTop];
+    __shared__ uint32_t places[kBlock];
+    __shared__ float4v staged[kWaves][kQuads][kWave];
+    __shared__ uint64_t candidates[kWaves][kWave];
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t row = blockIdx.x / a.parts;
@@ -170,18 +236,18 @@ __global__ __launch_bounds__(kBlock, 3) void TokenLogprobsKernel(LogprobArgs a)
     const uint32_t stride = a.parts * kWaves;
 
     // A batch's logits, and a bit for each that is the row's (the others are -inf).
-    float4v next[kQuads];
-    uint32_t nextThere = ~0u;
+    float4v v[kQuads];
+    uint32_t there = ~0u;
     auto request = [&](uint32_t batch) {
         const uint64_t first = static_cast<uint64_t>(batch) * kBatch;
-        nextThere = ~0u;
+        there = ~0u;
         if (first >= lead && first + kBatch <= span)
         {
             const float4v* from = reinterpret_cast<const float4v*>(x - lead + first) + lane;
 #pragma unroll
             for (int j = 0; j < kQuads; ++j)
             {
-                next[j] = kOnce ? __builtin_nontemporal_load(from + j * kWave) : from[j * kWave];
+                v[j] = kOnce ? __builtin_nontemporal_load(from + j * kWave) : from[j * kWave];
             }
             return;
         }
@@ -192,9 +258,9 @@ __global__ __launch_bounds__(kBlock, 3) void TokenLogprobsKernel(LogprobArgs a)
             for (int c = 0; c < 4; ++c)
             {
                 const uint64_t at = first + 4 * (j * kWave + lane) + c;
-                const bool there = at >= lead && at < span;
-                next[j][c] = there ? x[at - lead] : -INFINITY;
-                nextThere = there ? nextThere : nextThere & ~(1u << (4 * j + c));
+                const bool is = at >= lead && at < span;
+                v[j][c] = is ? x[at - lead] : -INFINITY;
+                there = is ? there : there & ~(1u << (4 * j + c));
             }
         }
     };
@@ -204,30 +270,23 @@ __global__ __launch_bounds__(kBlock, 3) void TokenLogprobsKernel(LogprobArgs a)
     {
         request(batch);
     }
-    const int32_t token = a.tokens != nullptr ? a.tokens[row] : -1;
-    const bool given = token >= 0 && static_cast<uint32_t>(token) < a.vocab;
-    const float own = given ? x[token] : INFINITY;
-    const uint64_t ownKey = given ? OrderKey(own, static_cast<uint32_t>(token)) : ~0ull;
-    const bool plain = own > -INFINITY;  // not -inf, not NaN
-    const float below = nextafterf(own, -INFINITY);
+    const Given given = GivenOf(a, row);
+    const uint64_t ownKey = given.is ? OrderKey(given.logit, given.token) : ~0ull;
+    const bool plain = given.logit > -INFINITY;  // not -inf, not NaN
+    const float below = nextafterf(given.logit, -INFINITY);
 
     Sums sums{-INFINITY, 0.0f, 0.0f, 0};
+    uint32_t above = 0;      // the wave's
     uint64_t mine = 0;       // lane i: the i-th best so far
     uint64_t least = 0;      // the last of the first `top`
+    auto insert = [&](uint64_t one) {
+        const uint32_t place = CountLanes(mine > one);
+        const uint64_t left = __shfl_up(static_cast<unsigned long long>(mine), 1);
+        mine = lane < place ? mine : lane == place ? one : left;
+        least = KeyOfLane(mine, a.top - 1);
+    };
     for (; batch < batches; batch += stride)
     {
-        float4v v[kQuads];
-        const uint32_t there = nextThere;
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j)
-        {
-            v[j] = next[j];
-        }
-        if (batch + stride < batches)
-        {
-            request(batch + stride);
-        }
-
         float largest = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kQuads; ++j)
@@ -239,112 +298,192 @@ __global__ __launch_bounds__(kBlock, 3) void TokenLogprobsKernel(LogprobArgs a)
             Rebase(sums, largest);
         }
         const float base = sums.m == -INFINITY ? 0.0f : sums.m;
-        float s[4] = {}, t[4] = {};
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j)
         {
+            float s[4] = {}, t[4] = {};
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int j = 0; j < kQuads; ++j)
             {
-                const float d = v[j][c] - base;
-                const float e = __builtin_amdgcn_exp2f(d * kLog2e);
-                s[c] += e;
-                t[c] = fmaf(e, fmaxf(d, -1e4f), t[c]);  // 0 times -inf would be NaN
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                {
+                    const float y = (v[j][c] - base) * kLog2e;
+                    const float e = __builtin_amdgcn_exp2f(y);
+                    s[c] += e;
+                    t[c] = fmaf(e, y, t[c]);
+                }
             }
+            float more = (t[0] + t[1]) + (t[2] + t[3]);
+            if (__any(more != more))
+            {
+                // 0 times the -inf of a masked logit. (NaN logits stay in s.)
+                more = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kQuads; ++j)
+                {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                    {
+                        const float y = (v[j][c] - base) * kLog2e;
+                        more = fmaf(__builtin_amdgcn_exp2f(y), fmaxf(y, -1e4f), more);
+                    }
+                }
+            }
+            sums.s += (s[0] + s[1]) + (s[2] + s[3]);
+            sums.t += more;
         }
-        sums.s += (s[0] + s[1]) + (s[2] + s[3]);
-        sums.t += (t[0] + t[1]) + (t[2] + t[3]);
 
         // Index of v[j][c]: at0 + 256 j + c.
-        const uint32_t at0 = static_cast<uint32_t>(static_cast<uint64_t>(batch) * kBatch - lead) + 4 * lane;
-        if (given)
+        const int64_t begin = static_cast<int64_t>(batch) * kBatch - lead;
+        const uint32_t at0 = static_cast<uint32_t>(begin) + 4 * lane;
+        const bool after = begin > given.token;
+        const bool before = begin + kBatch <= given.token;
+        const bool single = given.is && !(plain && (after || before));
+        if (given.is && !single)
         {
-            const bool after = static_cast<int64_t>(batch) * kBatch - lead > token;
-            const bool before = static_cast<int64_t>(batch) * kBatch - lead + kBatch <= token;
-            if (plain && (after || before))
-            {
-                const float over = after ? own : below;
+            const float over = after ? given.logit : below;
 #pragma unroll
-                for (int j = 0; j < kQuads; ++j)
-                {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                    {
-                        sums.above += v[j][c] > over ? 1u : 0u;
-                    }
-                }
-            }
-            else
+            for (int j = 0; j < kQuads; ++j)
             {
 #pragma unroll
-                for (int j = 0; j < kQuads; ++j)
+                for (int c = 0; c < 4; ++c)
                 {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                    {
-                        const bool is = (there >> (4 * j + c) & 1u) != 0;
-                        sums.above += is && OrderKey(v[j][c], at0 + 256 * j + c) > ownKey ? 1u : 0u;
-                    }
+                    above += CountLanes(v[j][c] > over);
                 }
             }
         }
-
-        if (a.top > 0)
+        const uint32_t last = static_cast<uint32_t>(least >> 32);
+        // A lane of NaN, or of none of the row's logits, has no -inf: its key may be lower than `largest` says.
+        const uint32_t is = there;
+        const bool odd = __any(is != ~0u || sums.s != sums.s);
+        const bool look = a.top > 0 && (odd || __any(OrderBits(largest) >= last));
+        if (single || look)
         {
-            uint32_t high = OrderBits(largest);
-            if (__any(there != ~0u || sums.s != sums.s))
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
             {
-                // Of a lane with NaN, or without logits: not that of the -inf that `largest` begins with.
-                high = 0;
-#pragma unroll
-                for (int j = 0; j < kQuads; ++j)
-                {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                    {
-                        high = (there >> (4 * j + c) & 1u) != 0 ? max(high, OrderBits(v[j][c])) : high;
-                    }
-                }
+                staged[wave][j][lane] = v[j];
             }
-            uint32_t floor = static_cast<uint32_t>(least >> 32);
-            const uint32_t reach = CountLanes(high >= floor);
-            if (reach != 0)
-            {
-                if (reach >= a.top)
-                {
-                    uint32_t bound = 0;
+        }
+        if (batch + stride < batches)
+        {
+            request(batch + stride);
+        }
+        if (!single && !look)
+        {
+            continue;
+        }
+        if (single || odd)
+        {
+            uint32_t high = 0;
 #pragma unroll 1
-                    for (uint32_t bit = 1u << 31; bit > 1u << 11; bit >>= 1)
-                    {
-                        bound = CountLanes(high >= (bound | bit)) >= a.top ? bound | bit : bound;
-                    }
-                    floor = max(floor, bound);
-                }
+            for (int j = 0; j < kQuads; ++j)
+            {
+                const float4v x4 = staged[wave][j][lane];
 #pragma unroll
-                for (int j = 0; j < kQuads; ++j)
+                for (int c = 0; c < 4; ++c)
                 {
+                    const uint64_t key = (is >> (4 * j + c) & 1u) != 0 ? OrderKey(x4[c], at0 + 256 * j + c) : 0;
+                    sums.above += single && key > ownKey ? 1u : 0u;
+                    high = max(high, static_cast<uint32_t>(key >> 32));
+                }
+            }
+            largest = KeyValue(static_cast<uint64_t>(high) << 32);
+        }
+        if (!look)
+        {
+            continue;
+        }
+        const uint32_t high = OrderBits(largest);
+        uint32_t floor = last;
+        if (CountLanes(high >= floor) >= a.top)
+        {
+            floor = max(floor, LowerBound(high, 1, a.top));
+        }
+        // The wave's LDS operations complete in order; the fences keep the compiler's order too.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        uint64_t lanes = __ballot(high >= floor);
+        uint32_t found = kWave + 1;
+        if (__popcll(lanes) > kFewLanes && KeyOfLane(mine, 0) == 0)
+        {
+            uint32_t take = 0;  // a bit for each of the lane's candidates
+#pragma unroll 1
+            for (int j = 0; j < kQuads; ++j)
+            {
+                const float4v x4 = staged[wave][j][lane];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                    {
-                        const uint32_t bits = OrderBits(v[j][c]);
-                        const bool is = bits >= floor && (there >> (4 * j + c) & 1u) != 0;
-                        const uint64_t key = (static_cast<uint64_t>(bits) << 32) | ~(at0 + 256 * j + c);
-                        uint64_t mask = __ballot(is && key > least);
-                        while (mask != 0)
-                        {
-                            const uint32_t from = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(mask)) - 1);
-                            const uint64_t one = KeyOfLane(key, from);
-                            const uint32_t place = CountLanes(mine > one);
-                            const uint64_t left = __shfl_up(static_cast<unsigned long long>(mine), 1);
-                            mine = lane < place ? mine : lane == place ? one : left;
-                            least = KeyOfLane(mine, a.top - 1);
-                            mask &= mask - 1;
-                            mask &= __ballot(key > least);
-                        }
-                    }
+                for (int c = 0; c < 4; ++c)
+                {
+                    take |= OrderBits(x4[c]) >= floor ? 1u << (4 * j + c) : 0u;
+                }
+            }
+            take &= is;
+            found = 0;
+            for (uint64_t mask = __ballot(take != 0); mask != 0; mask = __ballot(take != 0))
+            {
+                const uint32_t place =
+                    found + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+                if (take != 0 && place < kWave)
+                {
+                    const uint32_t e = static_cast<uint32_t>(__ffs(static_cast<int>(take)) - 1);
+                    candidates[wave][place] = OrderKey(staged[wave][e / 4][lane][e % 4], at0 + 256 * (e / 4) + e % 4);
+                }
+                take &= take - 1;
+                found += static_cast<uint32_t>(__popcll(mask));
+            }
+        }
+        if (found <= kWave)
+        {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const uint64_t key = lane < found ? candidates[wave][lane] : 0;
+            mine = key;
+            if (batch + stride >= batches)
+            {
+                continue;  // the workgroup ranks them
+            }
+            uint32_t place = 0;
+#pragma unroll 4
+            for (uint32_t i = 0; i < found; ++i)
+            {
+                place += KeyOfLane(key, i) > key ? 1u : 0u;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (lane < found)
+            {
+                candidates[wave][place] = key;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            mine = lane < found ? candidates[wave][lane] : 0;
+            least = KeyOfLane(mine, a.top - 1);
+        }
+        else
+        {
+            // Lane l looks at the l-th of their values.
+            while (lanes != 0)
+            {
+                const uint32_t from = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(lanes)) - 1);
+                lanes &= lanes - 1;
+                const uint32_t j = lane / 4 % kQuads;
+                const float value = staged[wave][j][from][lane % 4];
+                const uint32_t theirs = __builtin_amdgcn_readlane(is, from);
+                const uint64_t key = OrderKey(value, static_cast<uint32_t>(begin) + 4 * from + 256 * j + lane % 4);
+                const bool take = lane < 4 * kQuads && (theirs >> lane & 1u) != 0 &&
+                                  static_cast<uint32_t>(key >> 32) >= floor;
+                uint64_t mask = __ballot(take && key > least);
+                while (mask != 0)
+                {
+                    insert(KeyOfLane(key, static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(mask)) - 1)));
+                    mask &= mask - 1;
+                    mask &= __ballot(key > least);
                 }
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 
     // Lanes, then waves.
@@ -357,19 +496,28 @@ __global__ __launch_bounds__(kBlock, 3) void TokenLogprobsKernel(LogprobArgs a)
     {
         sums.above += __shfl_xor(sums.above, step);
     }
+    sums.above += above;
+    const uint32_t held = CountLanes(mine != 0);
     if (lane == 0)
     {
         waveSums[wave] = sums;
-    }
-    if (lane < a.top)
-    {
-        waveKeys[wave * a.top + lane] = mine;
+        waveHeld[wave] = held;
     }
     if (wave == 0)
     {
         best[lane] = 0;  // a part may have fewer tokens
     }
     __syncthreads();
+    uint32_t keys = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w)
+    {
+        if (w == wave && lane < held)
+        {
+            waveKeys[keys + lane] = mine;  // none of them is 0, and they come first
+        }
+        keys += waveHeld[w];
+    }
     float most = waveSums[0].m;
 #pragma unroll
     for (int w = 1; w < kWaves; ++w)
@@ -386,11 +534,15 @@ __global__ __launch_bounds__(kBlock, 3) void TokenLogprobsKernel(LogprobArgs a)
         all.t += one.t;
         all.above += one.above;
     }
-    RankKeys(waveKeys, kWaves * a.top, a.top, best);
-    __syncthreads();
+    if (a.top > 0)
+    {
+        __syncthreads();
+        RankKeys(waveKeys, keys, a.top, best, places);
+        __syncthreads();
+    }
     if (a.parts == 1)
     {
-        WriteRow(a, row, all, best, threadIdx.x, kBlock);
+        WriteRow(a, row, all, given, best);
         return;
     }
     if (threadIdx.x == 0)
@@ -409,13 +561,28 @@ __global__ __launch_bounds__(kBlock) void TokenLogprobsJoinKernel(LogprobArgs a)
 {
     __shared__ uint64_t held[kMaxParts * kMaxTop];
     __shared__ uint64_t best[kMaxTop];
+    __shared__ uint32_t places[kBlock];
     __shared__ uint32_t count;
     const uint32_t row = blockIdx.x;
     const uint32_t lane = threadIdx.x % kWave;
     const uint64_t first = static_cast<uint64_t>(row) * a.parts;
-    // Lane p of every wave has part p.
-    const float4 own = a.sums[first + min(lane, a.parts - 1)];
-    uint64_t floor = a.top > 0 ? a.keys[(first + min(lane, a.parts - 1)) * a.top + a.top - 1] : 0;
+    const Given given = GivenOf(a, row);
+    const uint32_t keys = a.parts * a.top;
+    uint64_t early[2];  // most calls' keys, on their way together with the sums
+#pragma unroll
+    for (uint32_t e = 0; e < 2; ++e)
+    {
+        const uint32_t i = e * kBlock + threadIdx.x;
+        early[e] = i < keys ? a.keys[first * a.top + i] : 0;
+    }
+    // Lane p of every wave has part p. Its `deep`-th key counts for `deep` keys: where the lanes with one that
+    // reaches a value have `top` together, that value is a lower bound too.
+    const uint32_t deep = a.top > 0 ? (a.top + a.parts - 1) / a.parts : 1;
+    const uint64_t part = first + min(lane, a.parts - 1);
+    const uint32_t reach =
+        a.top > 0 && lane < a.parts ? static_cast<uint32_t>(a.keys[part * a.top + deep - 1] >> 32) : 0;
+    const float4 own = a.sums[part];
+    uint64_t floor = a.top > 0 ? a.keys[part * a.top + a.top - 1] : 0;
     Sums sums{own.x, own.y, own.z, __float_as_uint(own.w)};
     if (lane >= a.parts)
     {
@@ -434,31 +601,47 @@ __global__ __launch_bounds__(kBlock) void TokenLogprobsJoinKernel(LogprobArgs a)
     }
     if (a.top > 0)
     {
+        const uint64_t lower = static_cast<uint64_t>(LowerBound(reach, deep, a.top)) << 32;
+        floor = floor > lower ? floor : lower;
         if (threadIdx.x == 0)
         {
             count = 0;
         }
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < a.parts * a.top; i += kBlock)
+        for (uint32_t i = threadIdx.x; i < keys; i += kBlock)
         {
-            const uint64_t key = a.keys[first * a.top + i];
+            const uint64_t key = i < kBlock ? early[0] : i < 2 * kBlock ? early[1] : a.keys[first * a.top + i];
             if (key >= floor)
             {
                 held[atomicAdd(&count, 1u)] = key;  // the order does not matter: keys are ranked
             }
         }
         __syncthreads();
-        RankKeys(held, count, a.top, best);
+        RankKeys(held, count, a.top, best, places);
         __syncthreads();
     }
-    WriteRow(a, row, sums, best, threadIdx.x, kBlock);
+    WriteRow(a, row, sums, given, best);
 }
 
-/// Workgroups of a row: enough for kTargetBlocks in all, a batch for each wave at least.
+/// Workgroups of a row: the fewest estimated batches after one another, when 1280 workgroups run at once (five on
+/// each of 256 CUs) and one of more than one round costs as much as three batches besides its own.
 uint32_t RowParts(uint32_t rows, uint32_t vocab)
 {
-    const uint32_t most = std::min(kMaxParts, CeilDiv(CeilDiv(static_cast<uint64_t>(vocab) + 3, kBatch), kWaves));
-    return std::max(1u, std::min(most, CeilDiv(kTargetBlocks, rows)));
+    const uint32_t batches = CeilDiv(static_cast<uint64_t>(vocab) + 3, kBatch);
+    const uint32_t most = std::min(kMaxParts, CeilDiv(batches, kWaves));
+    uint32_t best = 1;
+    uint64_t least = ~0ull;
+    for (uint32_t parts = 1; parts <= most; ++parts)
+    {
+        const uint64_t rounds = CeilDiv(static_cast<uint64_t>(rows) * parts, kBlocksAtOnce);
+        const uint64_t cost = rounds * (CeilDiv(batches, static_cast<uint64_t>(parts) * kWaves) + 3) + (parts > 1 ? 3 : 0);
+        if (cost < least)
+        {
+            least = cost;
+            best = parts;
+        }
+    }
+    return best;
 }
 }  // namespace
 }  // namespace muyo
@@ -513,7 +696,15 @@ extern "C" int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride,
     {
         return Fail(MUYO_E_RANGE, "%s: %u rows are too many for one launch", name, rows);
     }
-    hipLaunchKernelGGL(TokenLogprobsKernel<false>, dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, AsStream(stream), a);
+    const dim3 grid(static_cast<uint32_t>(blocks));
+    if (4ull * rows * vocab > kOnceBytes)
+    {
+        hipLaunchKernelGGL(TokenLogprobsKernel<true>, grid, dim3(kBlock), 0, AsStream(stream), a);
+    }
+    else
+    {
+        hipLaunchKernelGGL(TokenLogprobsKernel<false>, grid, dim3(kBlock), 0, AsStream(stream), a);
+    }
     if (parts > 1)
     {
         hipLaunchKernelGGL(TokenLogprobsJoinKernel, dim3(rows), dim3(kBlock), 0, AsStream(stream), a);

@@ -151,6 +151,23 @@ def test_masked_logits(mh, gpu, vocab):
     assert (got["tops"][4] == -np.inf).all() and np.array_equal(got["ids"][4], np.arange(20))
 
 
+def test_largest_and_smallest_logits(mh, gpu):
+    """Logits at the ends of the type's range, alone and beside ordinary ones."""
+    rng = np.random.default_rng(3)
+    big = np.finfo(np.float32).max
+    x = rng.normal(0, 2, (7, 3000)).astype(np.float32)
+    x[0, 100] = big
+    x[1, ::7] = big
+    x[2, :] = -big
+    x[2, 5] = -big * np.float32(0.999)
+    x[3] *= np.float32(1e-42)
+    x[4, 1:] = -big
+    x[5] = x[5] * np.float32(1e37)
+    x[6] = x[6] * np.float32(1e-3) + np.float32(2e5)
+    tokens = np.array([100, 1, 5, 7, 0, int(x[5].argmax()), 9])
+    check(run(mh, gpu, x, tokens, 20), x, tokens, 20)
+
+
 def test_logits_that_are_no_numbers(mh, gpu):
     """NaN or +inf in a row makes its log probabilities and entropy NaN, and only its; in the order NaN is
     last and +inf first."""
