@@ -70,6 +70,15 @@ __device__ __forceinline__ uint64_t KeyOfLane(uint64_t key, uint32_t lane)
     return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
+/// `key` of the lane before (wave_shr:1; lane 0 keeps its own).
+__device__ __forceinline__ uint64_t KeyOfLaneBefore(uint64_t key)
+{
+    const int lo = static_cast<int>(static_cast<uint32_t>(key));
+    const int hi = static_cast<int>(static_cast<uint32_t>(key >> 32));
+    return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(hi, hi, 0x138, 0xF, 0xF, false))) << 32) |
+           static_cast<uint32_t>(__builtin_amdgcn_update_dpp(lo, lo, 0x138, 0xF, 0xF, false));
+}
+
 __device__ __forceinline__ uint32_t CountLanes(bool is) { return static_cast<uint32_t>(__popcll(__ballot(is))); }
 
 /// The sums of a lane, a wave, a workgroup or a row.
@@ -203,10 +212,10 @@ __device__ __forceinline__ uint32_t LowerBound(uint32_t high, uint32_t each, uin
 /// The first `top` tokens: the wave's best so far lie in order across its lanes (lane i has the i-th), and
 /// a batch is looked through only if some lane's largest logit reaches the last of them. Then a lower bound
 /// of the batch's own `top`-th is found first, by bisection: a value that the largest ones of `top` lanes
-/// reach. Few lanes reach both bounds in a later batch: their logits are looked at lane by lane. In the first
-/// batch the candidates, a few more than `top`, are gathered and ranked (a candidate's place is the number
-/// of those above it). What is left (more than 64 candidates) is inserted one by one. Equal logits are told
-/// apart by their index in the key, so nothing overflows.
+/// reach. Few lanes reach both bounds in a later batch: their logits are looked at lane by lane and inserted
+/// one by one. In the first batches the candidates (a few more than `top` in the first) are gathered, with
+/// the best so far, and ranked: a candidate's place is the number of those above it. More than 64 are
+/// inserted too. Equal logits are told apart by their index in the key, so nothing overflows.
 ///
 /// The rank is counted on the way: the tokens before a given one have a larger logit, or the same at
 /// a lower index, which is a different comparison on each side of its batch.
@@ -281,7 +290,7 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
     uint64_t least = 0;      // the last of the first `top`
     auto insert = [&](uint64_t one) {
         const uint32_t place = CountLanes(mine > one);
-        const uint64_t left = __shfl_up(static_cast<unsigned long long>(mine), 1);
+        const uint64_t left = KeyOfLaneBefore(mine);
         mine = lane < place ? mine : lane == place ? one : left;
         least = KeyOfLane(mine, a.top - 1);
     };
@@ -404,7 +413,7 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
         __builtin_amdgcn_wave_barrier();
         uint64_t lanes = __ballot(high >= floor);
         uint32_t found = kWave + 1;
-        if (__popcll(lanes) > kFewLanes && KeyOfLane(mine, 0) == 0)
+        if (__popcll(lanes) > kFewLanes)
         {
             uint32_t take = 0;  // a bit for each of the lane's candidates
 #pragma unroll 1
@@ -432,6 +441,12 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
                 take &= take - 1;
                 found += static_cast<uint32_t>(__popcll(mask));
             }
+            const uint32_t kept = min(CountLanes(mine != 0), a.top);
+            if (found + kept <= kWave && lane < kept)
+            {
+                candidates[wave][found + lane] = mine;
+            }
+            found += kept;
         }
         if (found <= kWave)
         {
