@@ -15,6 +15,7 @@ namespace
 {
 constexpr uint32_t kMaxPlanSequences = 4096;
 constexpr uint32_t kMaxPlanTokens = 1u << 24;
+constexpr uint32_t kSmallPlan = 1024;  // sequences that workgroups of 256 threads plan
 
 struct PlanArgs
 {
@@ -279,6 +280,10 @@ hipError_t LaunchPlan(hipStream_t s, PlanArgs p, uint32_t blocks)
     {
         hipLaunchKernelGGL((PagedPlanKernel<256, 1>), dim3(blocks), dim3(256), 0, s, p);
     }
+    else if (p.sequences <= kSmallPlan)
+    {
+        hipLaunchKernelGGL((PagedPlanKernel<256, 4>), dim3(blocks), dim3(256), 0, s, p);
+    }
     else
     {
         hipLaunchKernelGGL((PagedPlanKernel<1024, 4>), dim3(blocks), dim3(1024), 0, s, p);
@@ -347,6 +352,84 @@ __device__ __forceinline__ uint16_t* AppendTarget(const AppendArgs& a, uint32_t 
     const uint32_t page = slot >> a.pageShift;
     const uint32_t row = slot & ((1u << a.pageShift) - 1);
     return cache + ((((static_cast<uint64_t>(page) * a.kvHeads + g) << a.pageShift) + row) * a.headDim);
+}
+
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+
+/// One thread per (token, row, eight values) for rotary dimensions that are multiples of 8: four pairs, or
+/// eight values behind the rotated ones, as two loads of 16 bytes and two stores (8 bytes of f16). v's
+/// values go the same way without the rotation.
+///
+/// What bounds it: memory. 8191 tokens of 28 / 4 heads of 128, 64 values rotated: 285 MB in 54 us, 5.3 TB/s,
+/// at the rate of a large copy (5.1); in pairs, by the kernel below, 109 us. Several rows a thread, so that
+/// an angle serves them all, measured the same there (two, three or four: 53 to 54 us) and slower for few
+/// tokens (253: 4.4 us with one, 5.2 with four), non-temporal loads 58 us: q was just written.
+template <bool kInterleaved>
+__global__ __launch_bounds__(256) void PagedAppendOctets(AppendArgs a)
+{
+    const uint32_t octets = a.headDim / 8;
+    const uint32_t rows = a.heads + 2 * a.kvHeads;
+    const uint32_t perToken = rows * octets;
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const uint64_t token = item / perToken;
+    if (token >= a.tokens)
+    {
+        return;
+    }
+    const uint32_t rest = static_cast<uint32_t>(item - token * perToken);
+    const uint32_t r = rest / octets;
+    const uint32_t o = rest - r * octets;
+    const int32_t position = a.positions[token];
+    const int32_t slot = a.slots[token];
+    const bool turned = 8 * o < a.rotary;
+    // Two quads of values: halves of four pairs, or one behind the other.
+    const uint32_t lo = turned && !kInterleaved ? 4 * o : 8 * o;
+    const uint32_t hi = turned && !kInterleaved ? 4 * o + a.rotary / 2 : 8 * o + 4;
+    const float* from = AppendSource(a, token, r);
+    const float4v x0 = *reinterpret_cast<const float4v*>(from + lo);
+    const float4v x1 = *reinterpret_cast<const float4v*>(from + hi);
+    const bool stored = slot >= 0 && static_cast<uint32_t>(slot) < a.slotCount;
+    if (position < 0 || (r >= a.heads && !stored))
+    {
+        return;
+    }
+    float4v y0 = x0;
+    float4v y1 = x1;
+    if (turned && r < a.heads + a.kvHeads)
+    {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+        {
+            float c, s;
+            PairAngle(a.turns[4 * o + e], position, a.magnitude, c, s);
+            float u, w;
+            if (kInterleaved)
+            {
+                Rotate((e < 2 ? x0 : x1)[e % 2 * 2], (e < 2 ? x0 : x1)[e % 2 * 2 + 1], c, s, u, w);
+                (e < 2 ? y0 : y1)[e % 2 * 2] = u;
+                (e < 2 ? y0 : y1)[e % 2 * 2 + 1] = w;
+            }
+            else
+            {
+                Rotate(x0[e], x1[e], c, s, u, w);
+                y0[e] = u;
+                y1[e] = w;
+            }
+        }
+    }
+    if (r < a.heads)
+    {
+        float* to = a.qOut + (token * a.heads + r) * a.headDim;
+        *reinterpret_cast<float4v*>(to + lo) = y0;
+        *reinterpret_cast<float4v*>(to + hi) = y1;
+    }
+    else
+    {
+        // The cache's type: half a step of f16, 2^-11 of the value.
+        uint16_t* to = AppendTarget(a, static_cast<uint32_t>(slot), r);
+        *reinterpret_cast<half4*>(to + lo) = __builtin_convertvector(y0, half4);
+        *reinterpret_cast<half4*>(to + hi) = __builtin_convertvector(y1, half4);
+    }
 }
 
 /// One thread per (token, row, pair of values): any even rotary dimension.
@@ -498,8 +581,12 @@ extern "C" int muyo_paged_plan(const int32_t* lengths, const int32_t* targets, u
     {
         ++p.pageShift;
     }
-    // Up to 2048 tokens one workgroup does everything; more of them share the lists.
-    const uint32_t blocks = std::min(256u, std::max(1u, CeilDiv(tokens, 2048)));
+    // A thread has one token (of a workgroup of 1024, two): its chain of loads (sequence, length, page) is what
+    // takes long. 131104 tokens of 256 sequences take 11.8 us at eight a thread, 7.2 at two, 6.5 at one. A
+    // list that one workgroup goes through twice is one launch still.
+    const uint32_t threads = sequences <= kSmallPlan ? 256 : 1024;
+    const uint32_t blocks =
+        tokens <= 2 * threads ? 1 : std::min(1024u, CeilDiv(tokens, threads == 256 ? threads : 2 * threads));
     if (blocks > 1 && inPlace)
     {
         // The state is overwritten only when every workgroup has read it.
@@ -665,12 +752,26 @@ extern "C" int muyo_paged_rope_append_f16kv(const float* q, const float* k, cons
     {
         ++a.pageShift;
     }
-    const uint64_t items = static_cast<uint64_t>(tokens) * (heads + 2 * kv_heads) * (head_dim / 2);
-    if (items > 256ull * 0x7FFFFFFFull)
+    const uint32_t rows = heads + 2 * kv_heads;
+    const bool octets = rotary_dim % 8 == 0;
+    const uint64_t items = static_cast<uint64_t>(tokens) * rows * (octets ? head_dim / 8 : head_dim / 2);
+    const uint64_t blocks = (items + 255) / 256;
+    if (blocks > 0x7FFFFFFFull)
     {
-        return Fail(MUYO_E_RANGE, "%s: %llu values are too many for one launch", name,
-                    static_cast<unsigned long long>(2 * items));
+        return Fail(MUYO_E_RANGE, "%s: %u tokens of %u rows are too many for one launch", name, tokens, rows);
     }
-    hipLaunchKernelGGL(PagedAppendPairs, dim3(CeilDiv(items, 256)), dim3(256), 0, AsStream(stream), a);
+    const dim3 grid(static_cast<uint32_t>(blocks));
+    if (octets && rope_layout == MUYO_ROPE_INTERLEAVED)
+    {
+        hipLaunchKernelGGL(PagedAppendOctets<true>, grid, dim3(256), 0, AsStream(stream), a);
+    }
+    else if (octets)
+    {
+        hipLaunchKernelGGL(PagedAppendOctets<false>, grid, dim3(256), 0, AsStream(stream), a);
+    }
+    else
+    {
+        hipLaunchKernelGGL(PagedAppendPairs, grid, dim3(256), 0, AsStream(stream), a);
+    }
     return LaunchStatus(name);
 }

@@ -128,6 +128,8 @@ PLANS = [
     ("scarce_pages", 100, 300, 16, 0.4, 0.1, 0.5, 100000),
     ("scarce_room", 100, 300, 16, 0.4, 0.1, 1.0, 2000),
     ("no_pages", 40, 200, 16, 0.2, 0.2, 0.0, 100000),
+    ("middle_1024", 1024, 60, 16, 0.2, 0.1, 0.9, 30000),
+    ("middle_1025", 1025, 60, 16, 0.2, 0.1, 1.0, 30000),
     ("many_4096", 4096, 40, 16, 0.1, 0.1, 0.9, 30000),
     ("page_1024", 9, 5000, 1024, 0.3, 0.0, 1.0, 50000),
 ]
