@@ -114,6 +114,19 @@ __device__ __forceinline__ uint32_t BlockSums(uint32_t v, uint32_t* waveSum, uin
     return v + before;
 }
 
+/// Inclusive sum over the wave's lanes: shifts inside rows of 16 lanes, then the last lanes of rows to the
+/// rows behind them.
+__device__ __forceinline__ uint32_t WaveSums(uint32_t v)
+{
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x111, 0xF, 0xF, false));  // row_shr:1
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x112, 0xF, 0xF, false));
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x114, 0xF, 0xF, false));
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x118, 0xF, 0xF, false));
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x142, 0xA, 0xF, false));  // row_bcast:15
+    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x143, 0xC, 0xF, false));  // row_bcast:31
+    return v;
+}
+
 /// The i with sums[i] <= at < sums[i + 1] (sums[0] = 0, at < sums[n]).
 __device__ __forceinline__ uint32_t OwnerOf(const uint32_t* sums, uint32_t n, uint32_t at)
 {
@@ -230,7 +243,25 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
     if constexpr (kSplit)
     {
         uint32_t total;
-        if (a.queries <= kScanQueries)
+        if (a.queries <= kWave)
+        {
+            // Every wave makes the sums, a query a lane.
+            KeyRange mine = RangeOf(a, min(lane, a.queries - 1));
+            mine.tiles = lane < a.queries ? mine.tiles : 0;
+            const uint32_t sum = WaveSums(mine.tiles);
+            total = __builtin_amdgcn_readlane(sum, kWave - 1);
+            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinTiles);
+            at = blockIdx.x * share;
+            const uint64_t has = __ballot((sum - mine.tiles) * a.kvHeads <= at && at < sum * a.kvHeads);
+            query = has != 0 ? static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(has)) - 1) : 0;
+            queryAt = __builtin_amdgcn_readlane(sum - mine.tiles, query) * a.kvHeads;
+            range.begin = __builtin_amdgcn_readlane(mine.begin, query);
+            range.end = __builtin_amdgcn_readlane(mine.end, query);
+            range.firstTile = __builtin_amdgcn_readlane(mine.firstTile, query);
+            range.tiles = __builtin_amdgcn_readlane(mine.tiles, query);
+            range.row = __builtin_amdgcn_readlane(mine.row, query);
+        }
+        else if (a.queries <= kScanQueries)
         {
             // Every workgroup makes the sums; the thread that has the share's first query says so.
             constexpr uint32_t kPer = kScanQueries / kBlock;
@@ -245,7 +276,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             }
             const uint32_t all = sum;
             sum = BlockSums<kBlock>(sum, waveSum, total) - all;
-            share = max((total * a.kvHeads + gridDim.x - 1) / gridDim.x, kMinTiles);
+            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinTiles);
             at = blockIdx.x * share;
 #pragma unroll
             for (uint32_t e = 0; e < kPer; ++e)
@@ -266,7 +297,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
         else
         {
             total = a.tileSums[a.queries];
-            share = max((total * a.kvHeads + gridDim.x - 1) / gridDim.x, kMinTiles);
+            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinTiles);
             at = blockIdx.x * share;
             query = OwnerOf(a.tileSums, a.queries, min(at / a.kvHeads, total - 1));
             queryAt = a.tileSums[query] * a.kvHeads;
