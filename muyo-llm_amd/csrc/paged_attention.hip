@@ -20,7 +20,8 @@ constexpr int kHalves = kTile / 16;       // matrix operands of 16 keys
 constexpr uint32_t kMaxGroup = 16;        // query heads per kv head: the columns of a matrix operation
 constexpr uint32_t kScanQueries = 1024;   // batches up to this many queries: each workgroup makes the sums itself
 constexpr uint32_t kWholeKeys = 1024;     // caches of at most this many keys are not split
-constexpr uint32_t kMinTiles = kWaves;    // a workgroup's share of the tiles: at least one a wave
+constexpr uint32_t kMinShare = kWaves;    // a share is at least a tile a wave
+constexpr uint32_t kSetupTiles = 8;       // what a share's change to another (query, kv head) costs, in tiles
 constexpr uint32_t kSplitBlocks = 512;    // workgroups of a split launch: two on each of 256 CUs
 
 /// *p for a p that is the same in the whole wave, of memory that nothing writes while the kernel runs: a
@@ -52,7 +53,7 @@ struct PagedAttentionArgs
     uint32_t pages, pageShift;
     uint32_t window;
     float scale;
-    uint32_t* tileSums;  // [queries + 1]: tiles of one kv head of the queries before
+    uint32_t* costSums;  // [queries + 1]: CostOf of one kv head of the queries before
     uint4* cuts;         // what to join: query, kv head, first share, pieces (0: nothing)
     uint32_t cutsByUnit; // cuts has an entry per (query, kv head); else one per share
     float* partials;     // [2 * shares][group][4 + headDim]: max (log2 units), sum, -, -, weighted values
@@ -85,6 +86,12 @@ __device__ __forceinline__ KeyRange RangeOf(const PagedAttentionArgs& a, uint32_
     r.tiles = r.row < a.sequences ? max((r.end + kTile - 1) / kTile - r.firstTile, 1u) : 0;
     return r;
 }
+
+/// What a (query, kv head) of `tiles` tiles counts in the shares. A change to it (its q, its first tile's
+/// round trips, joining the waves) takes 3 to 4 us, a tile of each wave about one: dealt out by tiles alone,
+/// shares of short sequences had up to four of them. 28 / 4 heads of 128, with a cost of 0, 4, 8 and 12 tiles:
+/// 64 sequences of 1 to 500 keys 27, 15.7, 14.4 and 15.2 us; 250 of 1 to 2000, most short, -, 41, 38 and 43.
+__host__ __device__ constexpr uint32_t CostOf(uint32_t tiles) { return tiles != 0 ? tiles + kSetupTiles : 0; }
 
 /// Inclusive sum over the workgroup's threads, in thread order; `total` is the last one's.
 template <int kThreads>
@@ -148,25 +155,25 @@ __device__ __forceinline__ uint32_t OwnerOf(const uint32_t* sums, uint32_t n, ui
 }
 
 /// The sums of batches of more than kScanQueries queries, by one workgroup before the others start.
-__global__ __launch_bounds__(1024) void PagedTileSumsKernel(PagedAttentionArgs a)
+__global__ __launch_bounds__(1024) void PagedCostSumsKernel(PagedAttentionArgs a)
 {
     __shared__ uint32_t waveSum[1024 / kWave];
     uint32_t before = 0;
     for (uint32_t first = 0; first < a.queries; first += 1024)
     {
         const uint32_t i = first + threadIdx.x;
-        const uint32_t tiles = i < a.queries ? RangeOf(a, i).tiles : 0;
+        const uint32_t cost = i < a.queries ? CostOf(RangeOf(a, i).tiles) : 0;
         uint32_t total;
-        const uint32_t sum = BlockSums<1024>(tiles, waveSum, total);
+        const uint32_t sum = BlockSums<1024>(cost, waveSum, total);
         if (i < a.queries)
         {
-            a.tileSums[i] = before + sum - tiles;
+            a.costSums[i] = before + sum - cost;
         }
         before += total;
     }
     if (threadIdx.x == 0)
     {
-        a.tileSums[a.queries] = before;
+        a.costSums[a.queries] = before;
     }
 }
 
@@ -198,15 +205,16 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// the accumulators is rare. Only tiles that reach over an end of the key range, or into a page that is
 /// not there, are masked: their scores to -inf, and their V rows to 0, since 0 * NaN would be NaN.
 ///
-/// kSplit: the tiles of all queries and kv heads in a row are dealt out in equal shares, whatever the
-/// sequences' lengths. A share may begin and end inside a (query, kv head); those pieces go to
+/// kSplit: the tiles of all queries and kv heads in a row, each with its setup's cost before it, are dealt
+/// out in equal shares, whatever the sequences' lengths. A share may begin and end inside a (query, kv head); those pieces go to
 /// `partials` (a share has at most one that does not begin its (query, kv head) and one that does) for
 /// PagedAttentionMergeKernel, which finds in `cuts` what to join. Otherwise a workgroup has one (query,
 /// kv head). Either way the workgroup's four waves take every fourth tile and join in LDS.
 ///
 /// What bounds it: the cache's arrival. 64 sequences of 1 to 16384 keys (28 / 4 heads of 128, pages of 16,
-/// 1.07 GB of K and V): 169 us, 6.3 TB/s, where the best streaming read here has 6.9; 14 / 2 heads of 64,
-/// 0.27 GB: 47 us, 5.7 TB/s. Past the caches' size, loads without the non-temporal hint took 190 us; a
+/// 1.07 GB of K and V): 168 us, 6.4 TB/s, where the best streaming read here has 6.9; 14 / 2 heads of 64,
+/// 0.27 GB: 45 us, 6.0 TB/s; one sequence of 32749 keys, 67 MB: 15.7 us, 4.3 TB/s, of which the way to the
+/// first tile and the joins take about five. Past the caches' size, loads without the non-temporal hint took 190 us; a
 /// split launch is for long caches, and loads K and V with it. Short ones are a chain of round trips
 /// (position, page, rows), 5 us: 8 or 16 waves a workgroup, tiles of 64 keys, and two or three tiles in
 /// flight at head_dim 64 all measured no better or worse.
@@ -235,10 +243,11 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
 
     uint32_t query, g;
     KeyRange range;
-    uint32_t at = 0;        // this share's next tile, in the row of all (the host keeps that below 2^32)
+    uint32_t at = 0;        // where this share goes on in the row of all costs (the host keeps that below 2^31)
     uint32_t stop = 0;
     uint32_t share = 0;
-    uint32_t queryAt = 0;   // the first tile of the query
+    uint32_t queryAt = 0;   // where the query begins there, and its kv head
+    uint32_t unitAt = 0;
     uint4 cut = make_uint4(0, 0, 0, 0);
     if constexpr (kSplit)
     {
@@ -248,13 +257,14 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             // Every wave makes the sums, a query a lane.
             KeyRange mine = RangeOf(a, min(lane, a.queries - 1));
             mine.tiles = lane < a.queries ? mine.tiles : 0;
-            const uint32_t sum = WaveSums(mine.tiles);
+            const uint32_t cost = CostOf(mine.tiles);
+            const uint32_t sum = WaveSums(cost);
             total = __builtin_amdgcn_readlane(sum, kWave - 1);
-            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinTiles);
+            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
             at = blockIdx.x * share;
-            const uint64_t has = __ballot((sum - mine.tiles) * a.kvHeads <= at && at < sum * a.kvHeads);
+            const uint64_t has = __ballot((sum - cost) * a.kvHeads <= at && at < sum * a.kvHeads);
             query = has != 0 ? static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(has)) - 1) : 0;
-            queryAt = __builtin_amdgcn_readlane(sum - mine.tiles, query) * a.kvHeads;
+            queryAt = __builtin_amdgcn_readlane(sum - cost, query) * a.kvHeads;
             range.begin = __builtin_amdgcn_readlane(mine.begin, query);
             range.end = __builtin_amdgcn_readlane(mine.end, query);
             range.firstTile = __builtin_amdgcn_readlane(mine.firstTile, query);
@@ -271,23 +281,25 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             for (uint32_t e = 0; e < kPer; ++e)
             {
                 const uint32_t i = threadIdx.x * kPer + e;
-                ranges[e] = i < a.queries ? RangeOf(a, i) : KeyRange{};
-                sum += ranges[e].tiles;
+                ranges[e] = RangeOf(a, min(i, a.queries - 1));  // no condition: all loads at once
+                ranges[e].tiles = i < a.queries ? ranges[e].tiles : 0;
+                sum += CostOf(ranges[e].tiles);
             }
             const uint32_t all = sum;
             sum = BlockSums<kBlock>(sum, waveSum, total) - all;
-            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinTiles);
+            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
             at = blockIdx.x * share;
 #pragma unroll
             for (uint32_t e = 0; e < kPer; ++e)
             {
-                if (sum * a.kvHeads <= at && at < (sum + ranges[e].tiles) * a.kvHeads)
+                const uint32_t i = threadIdx.x * kPer + e;
+                if (sum * a.kvHeads <= at && at < (sum + CostOf(ranges[e].tiles)) * a.kvHeads)
                 {
                     firstRange = ranges[e];
-                    firstAt[0] = threadIdx.x * kPer + e;
+                    firstAt[0] = i;
                     firstAt[1] = sum;
                 }
-                sum += ranges[e].tiles;
+                sum += CostOf(ranges[e].tiles);
             }
             __syncthreads();
             query = firstAt[0];
@@ -296,11 +308,11 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
         }
         else
         {
-            total = a.tileSums[a.queries];
-            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinTiles);
+            total = a.costSums[a.queries];
+            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
             at = blockIdx.x * share;
-            query = OwnerOf(a.tileSums, a.queries, min(at / a.kvHeads, total - 1));
-            queryAt = a.tileSums[query] * a.kvHeads;
+            query = OwnerOf(a.costSums, a.queries, min(at / a.kvHeads, total - 1));
+            queryAt = a.costSums[query] * a.kvHeads;
             range = RangeOf(a, query);
         }
         total *= a.kvHeads;
@@ -346,9 +358,18 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                 range = RangeOf(a, query);
                 continue;
             }
-            g = __builtin_amdgcn_readfirstlane((at - queryAt) / range.tiles);
-            tile0 = __builtin_amdgcn_readfirstlane(at - queryAt - g * range.tiles);
-            tile1 = __builtin_amdgcn_readfirstlane(min(range.tiles, tile0 + (stop - at)));
+            const uint32_t cost = CostOf(range.tiles);
+            g = __builtin_amdgcn_readfirstlane((at - queryAt) / cost);
+            unitAt = __builtin_amdgcn_readfirstlane(queryAt + g * cost);
+            const uint32_t from = __builtin_amdgcn_readfirstlane(at - unitAt);
+            const uint32_t to = __builtin_amdgcn_readfirstlane(min(cost, from + (stop - at)));
+            at = unitAt + to;
+            tile0 = from > kSetupTiles ? from - kSetupTiles : 0;
+            tile1 = to > kSetupTiles ? to - kSetupTiles : 0;
+            if (tile0 >= tile1)  // its setup alone: the tiles are the next share's
+            {
+                continue;
+            }
         }
         else if (range.tiles == 0)
         {
@@ -697,7 +718,8 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             __syncthreads();  // the next piece overwrites the results
             if (tile0 == 0)
             {
-                const uint32_t pieces = whole ? 0 : (at + range.tiles - 1) / share - blockIdx.x + 1;
+                const uint32_t last = (unitAt + CostOf(range.tiles) - 1) / share;
+                const uint32_t pieces = whole ? 0 : last - blockIdx.x + 1;
                 const uint4 join = make_uint4(query, g, blockIdx.x, pieces);
                 if (a.cutsByUnit == 0)
                 {
@@ -708,8 +730,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                     a.cuts[query * a.kvHeads + g] = join;
                 }
             }
-            at += tile1 - tile0;
-            if (at < stop && tile1 == range.tiles && g + 1 == a.kvHeads)
+            if (at < stop && g + 1 == a.kvHeads)
             {
                 queryAt = at;
                 ++query;
@@ -830,7 +851,7 @@ bool AttentionShape(uint32_t queries, uint32_t heads, uint32_t kvHeads, uint32_t
 
 /// The workspace's parts: the sums of batches that the workgroups do not sum themselves, the cuts, the
 /// partials.
-size_t TileSumBytes(uint32_t queries)
+size_t CostSumBytes(uint32_t queries)
 {
     return queries <= kScanQueries ? 0 : (4 * (static_cast<size_t>(queries) + 1) + 15) & ~static_cast<size_t>(15);
 }
@@ -843,14 +864,14 @@ hipError_t LaunchPagedAttention(hipStream_t s, PagedAttentionArgs a)
     const uint64_t keys = std::min<uint64_t>(static_cast<uint64_t>(a.tablePages) << a.pageShift,
                                              a.window != 0 ? a.window : 0xFFFFFFFFull);
     const uint64_t units = static_cast<uint64_t>(a.queries) * a.kvHeads;
-    if (keys <= kWholeKeys || units * (keys / kTile + 2) > 0x7FFFFFFFull)
+    if (keys <= kWholeKeys || units * (keys / kTile + 2 + kSetupTiles) > 0x7FFFFFFFull)
     {
         hipLaunchKernelGGL((PagedAttentionKernel<kHd, false>), dim3(static_cast<uint32_t>(units)), dim3(kBlock), 0, s, a);
         return hipGetLastError();
     }
     if (a.queries > kScanQueries)
     {
-        hipLaunchKernelGGL(PagedTileSumsKernel, dim3(1), dim3(1024), 0, s, a);
+        hipLaunchKernelGGL(PagedCostSumsKernel, dim3(1), dim3(1024), 0, s, a);
     }
     a.cutsByUnit = units < kSplitBlocks ? 1 : 0;
     const uint32_t joins = a.cutsByUnit != 0 ? static_cast<uint32_t>(units) : kSplitBlocks - 1;
@@ -877,7 +898,7 @@ extern "C" size_t muyo_paged_attention_decode_f16kv_workspace_bytes(uint32_t que
     {
         return 0;
     }
-    return TileSumBytes(queries) + kCutBytes +
+    return CostSumBytes(queries) + kCutBytes +
            sizeof(float) * 2 * kSplitBlocks * (heads / kv_heads) * (head_dim + 4);
 }
 
@@ -937,9 +958,9 @@ extern "C" int muyo_paged_attention_decode_f16kv(const float* q, const void* kca
                          window,
                          scale,
                          static_cast<uint32_t*>(workspace),
-                         reinterpret_cast<uint4*>(static_cast<char*>(workspace) + TileSumBytes(queries)),
+                         reinterpret_cast<uint4*>(static_cast<char*>(workspace) + CostSumBytes(queries)),
                          0,
-                         reinterpret_cast<float*>(static_cast<char*>(workspace) + TileSumBytes(queries) + kCutBytes)};
+                         reinterpret_cast<float*>(static_cast<char*>(workspace) + CostSumBytes(queries) + kCutBytes)};
     while ((1u << a.pageShift) < page_size)
     {
         ++a.pageShift;

@@ -443,6 +443,21 @@ def test_attention_long_and_many(mh, gpu, hd, positions):
     batch.check()
 
 
+@pytest.mark.parametrize("queries", [1, 5, 64, 65, 256, 300])
+@pytest.mark.parametrize("longest", [512, 513])
+def test_attention_of_short_sequences_in_wide_tables(mh, gpu, queries, longest):
+    """Tables of 4096 keys, sequences up to `longest`, padding among them, on either side of what is cut."""
+    rng = np.random.default_rng(queries + longest)
+    positions = rng.integers(0, longest, queries)
+    positions[0] = longest - 1
+    sequence = rng.permutation(queries)
+    if queries > 4:
+        sequence[3] = -1
+    batch = Attend(mh, gpu, rng, 14, 2, 64, 16, positions, width=256, sequence=sequence)
+    batch.poison_unseen()
+    batch.check()
+
+
 def test_attention_padding_empty_rows_and_bad_pages(mh, gpu):
     """Padding rows stay, rows without keys are 0, pages outside the cache and keys past the table are
     left out, and several queries may share a sequence."""
