@@ -727,9 +727,10 @@ extern "C" int muyo_paged_rope_append_f16kv(const float* q, const float* k, cons
         return Fail(MUYO_E_CONTRACT, "%s: token strides must be multiples of 4 that hold a token's heads", name);
     }
     if (!Aligned16(q) || !Aligned16(k) || !Aligned16(v) || !Aligned16(q_out) || !Aligned16(kcache) ||
-        !Aligned16(vcache) || (reinterpret_cast<uintptr_t>(turns) & 7u) != 0)
+        !Aligned16(vcache) || (reinterpret_cast<uintptr_t>(turns) & 7u) != 0 || !std::isfinite(magnitude))
     {
-        return Fail(MUYO_E_CONTRACT, "%s: q, k, v, q_out and the caches must be 16-byte aligned, turns 8-byte aligned",
+        return Fail(MUYO_E_CONTRACT, "%s: q, k, v, q_out and the caches must be 16-byte aligned, turns 8-byte aligned, "
+                                     "magnitude finite",
                     name);
     }
     const Range out{q_out, 4 * qdim * tokens, "q_out"};

@@ -102,6 +102,9 @@ SHAPES = [
     (1500, 5000, 10, 2.0, None, 0),
     (2100, 129, 2, 2.0, None, 0),
     (1, 600001, 7, 3.0, None, 0),
+    (70000, 40, 3, 2.0, 41, 1),
+    (3000, 1024, 64, 2.0, None, 0),
+    (2, 2000000, 33, 3.0, None, 2),
 ]
 
 

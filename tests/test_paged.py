@@ -67,6 +67,7 @@ REFUSALS = [
     ("paged_rope_append_f16kv", APPEND, dict(q=ctypes.c_void_p(8)), "MUYO_E_CONTRACT"),
     ("paged_rope_append_f16kv", APPEND, dict(kcache=ctypes.c_void_p((5 << 30) + 2)), "MUYO_E_CONTRACT"),
     ("paged_rope_append_f16kv", APPEND, dict(turns=ctypes.c_void_p(4)), "MUYO_E_CONTRACT"),
+    ("paged_rope_append_f16kv", APPEND, dict(magnitude=math.nan), "MUYO_E_CONTRACT"),
     ("paged_rope_append_f16kv", APPEND, dict(q_out=APPEND["k"]), "MUYO_E_CONTRACT"),
     ("paged_rope_append_f16kv", APPEND, dict(q_out=APPEND["q"], q_stride=1152), "MUYO_E_CONTRACT"),
     *[("paged_attention_decode_f16kv", ATTEND, {k: None}, "MUYO_E_NULL")
@@ -84,6 +85,8 @@ REFUSALS = [
     ("paged_attention_decode_f16kv", ATTEND, dict(pages=1 << 27), "MUYO_E_RANGE"),
     ("paged_attention_decode_f16kv", ATTEND, dict(q=ctypes.c_void_p(4)), "MUYO_E_CONTRACT"),
     ("paged_attention_decode_f16kv", ATTEND, dict(vcache=ctypes.c_void_p(8)), "MUYO_E_CONTRACT"),
+    ("paged_attention_decode_f16kv", ATTEND, dict(scale=math.inf), "MUYO_E_CONTRACT"),
+    ("paged_attention_decode_f16kv", ATTEND, dict(scale=math.nan), "MUYO_E_CONTRACT"),
     ("paged_attention_decode_f16kv", ATTEND, dict(workspace=None), "MUYO_E_CONTRACT"),
     ("paged_attention_decode_f16kv", ATTEND, dict(workspace=ctypes.c_void_p(8)), "MUYO_E_CONTRACT"),
     ("paged_attention_decode_f16kv", ATTEND, dict(workspace_bytes=15), "MUYO_E_CONTRACT"),
@@ -95,6 +98,7 @@ REFUSALS = [
     ("token_logprobs_f32", LOGPROBS, dict(vocab=0, row_stride=0, top=0), "MUYO_E_RANGE"),
     ("token_logprobs_f32", LOGPROBS, dict(top=65), "MUYO_E_RANGE"),
     ("token_logprobs_f32", LOGPROBS, dict(vocab=4), "MUYO_E_RANGE"),
+    ("token_logprobs_f32", LOGPROBS, dict(logits=ctypes.c_void_p(2)), "MUYO_E_CONTRACT"),
     ("token_logprobs_f32", LOGPROBS, dict(row_stride=999), "MUYO_E_CONTRACT"),
     ("token_logprobs_f32", LOGPROBS, dict(workspace=None), "MUYO_E_CONTRACT"),
     ("token_logprobs_f32", LOGPROBS, dict(workspace_bytes=0), "MUYO_E_CONTRACT"),

@@ -529,6 +529,85 @@ def test_attention_past_four_gigabytes_of_cache(mh, gpu):
     batch.compare(host(out))
 
 
+def test_attention_replayed_with_other_lengths(mh, gpu):
+    """A captured call whose positions, tables, q and padding change between replays, its workspace used by
+    calls of other shapes in between."""
+    torch, rng = gpu, np.random.default_rng(31)
+    heads, kv, hd, size, width, n = 28, 4, 128, 16, 200, 9
+    pages = n * width
+    batch = Attend(mh, gpu, rng, heads, kv, hd, size, np.full(n, width * size - 1), spare=0)
+    other = Attend(mh, gpu, rng, 14, 2, 64, 32, np.array([4000, 17, 900]))
+    out = torch.full((n, heads, hd), 9.0, device="cuda")
+    batch.call(out=out)
+    other.call()
+    assert other.nbytes <= batch.nbytes
+    other.space = batch.space
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch.call(where=True, out=out)
+    for replay in range(6):
+        batch.positions = rng.integers(0, width * size, n) if replay % 2 else rng.integers(0, 50, n)
+        batch.sequence = rng.permutation(n)
+        batch.sequence[replay % n] = -1
+        batch.tables = rng.permutation(pages).reshape(n, width)
+        batch.q = rng.normal(0, 2, batch.q.shape).astype(np.float32)
+        for d, value in zip((batch.d[0], batch.d[3], batch.d[4], batch.d[5]),
+                            (batch.q, batch.tables, batch.sequence, batch.positions)):
+            d.copy_(dev(torch, value.astype(np.float32 if value.dtype == np.float32 else np.int32)))
+        out.fill_(9.0)
+        other_out = other.call(where=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        batch.compare(host(out))
+        other.compare(host(other_out))
+
+
+def test_two_attentions_at_once(mh, gpu):
+    """Two streams, a workspace each."""
+    torch, rng = gpu, np.random.default_rng(32)
+    batches = [Attend(mh, gpu, rng, 28, 4, 128, 16, rng.integers(0, 6000, 12)),
+               Attend(mh, gpu, rng, 14, 2, 64, 64, rng.integers(0, 9000, 20))]
+    alone = [host(b.check()) for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    together = []
+    for _ in range(5):
+        for b, s in zip(batches, streams):
+            with torch.cuda.stream(s):
+                together.append(b.call(where=True))
+    torch.cuda.synchronize()
+    for i, out in enumerate(together):
+        assert np.array_equal(host(out).view(np.uint32), alone[i % 2].view(np.uint32)), i
+
+
+def test_attention_in_place_and_most_heads(mh, gpu):
+    """out may be q; 1024 heads of 64 kv heads, whole and split."""
+    torch, rng = gpu, np.random.default_rng(33)
+    for positions in ([5, 300], [1500, 3]):
+        batch = Attend(mh, gpu, rng, 1024, 64, 64, 16, np.array(positions))
+        batch.poison_unseen()
+        want = host(batch.check())
+        got = batch.call(where=True, out=batch.d[0].view(len(positions), 1024, 64))
+        torch.cuda.synchronize()
+        assert np.array_equal(host(got).view(np.uint32), want.view(np.uint32))
+
+
+def test_plan_of_the_longest_lists(mh, gpu):
+    """2^24 list entries, nearly all of them padding, and a long sequence that ends."""
+    rng = np.random.default_rng(34)
+    lengths, targets = np.array([100000, 3, 0]), np.array([0, 5, 40000])
+    tables, ring, pool = plan_state(rng, lengths, 7000, 16, 3000)
+    want = plan_reference(lengths, targets, tables, ring, pool, 16, 60000)
+    for in_place in (False, True):
+        got = run_plan(mh, gpu, lengths, targets, tables, ring, pool, 16, 1 << 24, in_place)
+        for key in want:
+            if key == "lists":
+                assert np.array_equal(got[key][:, :60000], want[key]) and (got[key][:, 60000:] == -1).all()
+            else:
+                assert np.array_equal(got[key], want[key]), key
+
+
 def test_a_steps_operators_in_one_graph(mh, gpu):
     """Plan, append, attention, a head's product and the log probabilities captured together, in place, and
     replayed: each replay is the next token of every sequence, against the same steps in 64 bits."""
