@@ -124,17 +124,23 @@ __device__ __forceinline__ uint32_t BlockSums(uint32_t v, uint32_t* waveSum, uin
     return v + before;
 }
 
+/// v plus that of the lane a DPP control names, in the given rows of 16 lanes; 0 from no lane.
+template <int kControl, int kRows>
+__device__ __forceinline__ uint32_t PlusLane(uint32_t v)
+{
+    return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kControl, kRows, 0xF, false));
+}
+
 /// Inclusive sum over the wave's lanes: shifts inside rows of 16 lanes, then the last lanes of rows to the
 /// rows behind them.
 __device__ __forceinline__ uint32_t WaveSums(uint32_t v)
 {
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x111, 0xF, 0xF, false));  // row_shr:1
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x112, 0xF, 0xF, false));
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x114, 0xF, 0xF, false));
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x118, 0xF, 0xF, false));
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x142, 0xA, 0xF, false));  // row_bcast:15
-    v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x143, 0xC, 0xF, false));  // row_bcast:31
-    return v;
+    v = PlusLane<0x111, 0xF>(v);  // row_shr:1
+    v = PlusLane<0x112, 0xF>(v);
+    v = PlusLane<0x114, 0xF>(v);
+    v = PlusLane<0x118, 0xF>(v);
+    v = PlusLane<0x142, 0xA>(v);     // row_bcast:15
+    return PlusLane<0x143, 0xC>(v);  // row_bcast:31
 }
 
 /// The i with sums[i] <= at < sums[i + 1] (sums[0] = 0, at < sums[n]).
@@ -209,10 +215,11 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// not there, are masked: their scores to -inf, and their V rows to 0, since 0 * NaN would be NaN.
 ///
 /// kSplit: the tiles of all queries and kv heads in a row, each with its setup's cost before it, are dealt
-/// out in equal shares, whatever the sequences' lengths. A share may begin and end inside a (query, kv head); those pieces go to
-/// `partials` (a share has at most one that does not begin its (query, kv head) and one that does) for
-/// PagedAttentionMergeKernel, which finds in `cuts` what to join. Otherwise a workgroup has one (query,
-/// kv head). Either way the workgroup's four waves take every fourth tile and join in LDS.
+/// out in equal shares, whatever the sequences' lengths. A share may begin and end inside a (query, kv
+/// head); those pieces go to `partials` (a share has at most one that does not begin its (query, kv head)
+/// and one that does) for PagedAttentionMergeKernel, which finds in `cuts` what to join. Otherwise a
+/// workgroup has one (query, kv head). Either way the workgroup's four waves take every fourth tile and join
+/// in LDS.
 ///
 /// What bounds it: the cache's arrival. 64 sequences of 1 to 16384 keys (28 / 4 heads of 128, pages of 16,
 /// 1.07 GB of K and V): 168 us, 6.4 TB/s, where the best streaming read here has 6.9; 14 / 2 heads of 64,
@@ -236,7 +243,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
     __shared__ float waveTotal[kWaves][kMaxGroup];
     __shared__ uint32_t waveSum[kWaves];
     __shared__ KeyRange firstRange;
-    __shared__ uint32_t firstAt[2];  // the share's first query, and the tiles before it
+    __shared__ uint32_t firstAt[2];  // the share's first query, and the costs before it
 
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -332,8 +339,8 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
     }
     else
     {
-        query = blockIdx.x / a.kvHeads;
-        g = blockIdx.x % a.kvHeads;
+        query = blockIdx.y;
+        g = blockIdx.x;
         range = RangeOf(a, query);
     }
 
@@ -869,7 +876,7 @@ hipError_t LaunchPagedAttention(hipStream_t s, PagedAttentionArgs a)
     const uint64_t units = static_cast<uint64_t>(a.queries) * a.kvHeads;
     if (keys <= kWholeKeys || units * (keys / kTile + 2 + kSetupTiles) > 0x7FFFFFFFull)
     {
-        hipLaunchKernelGGL((PagedAttentionKernel<kHd, false>), dim3(static_cast<uint32_t>(units)), dim3(kBlock), 0, s, a);
+        hipLaunchKernelGGL((PagedAttentionKernel<kHd, false>), dim3(a.kvHeads, a.queries), dim3(kBlock), 0, s, a);
         return hipGetLastError();
     }
     if (a.queries > kScanQueries)

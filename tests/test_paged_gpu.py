@@ -593,6 +593,29 @@ def test_attention_in_place_and_most_heads(mh, gpu):
         assert np.array_equal(host(got).view(np.uint32), want.view(np.uint32))
 
 
+def test_attention_of_more_heads_than_a_launch_has_workgroups_in_a_row(mh, gpu):
+    """16400 queries of 1024 kv heads: 2^24 + 16384 (query, kv head), 256 threads each. One key is visible, so a
+    head's output is that key's value."""
+    torch = gpu
+    queries, heads, hd = 16400, 1024, 64
+    keys = torch.randn(heads, 16, hd, device="cuda").half()
+    values = torch.randn(heads, 16, hd, device="cuda").half()
+    q = torch.randn(1, heads, hd, device="cuda").expand(queries, heads, hd).contiguous()
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    zeros = torch.zeros(queries, dtype=torch.int32, device="cuda")
+    lib = mh.load()
+    need = lib.muyo_paged_attention_decode_f16kv_workspace_bytes(queries, heads, heads, hd)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    mh.check(lib.muyo_paged_attention_decode_f16kv(
+        q.data_ptr(), keys.data_ptr(), values.data_ptr(), q.data_ptr(), table.data_ptr(), 1, 1, zeros.data_ptr(),
+        zeros.data_ptr(), queries, heads, heads, hd, 1, 16, 0, 0.125, work.data_ptr(), need, stream(torch)))
+    torch.cuda.synchronize()
+    want = values[:, 0].float()
+    # The weight of the only key cancels but for its low plane's rounding (2^-25, u / 2), the sum with the high
+    # plane's product (u), the reciprocal and the product with it (u / 2 to u each).
+    assert ((q - want).abs() <= 4 * U * want.abs()).all()
+
+
 def test_plan_of_the_longest_lists(mh, gpu):
     """2^24 list entries, nearly all of them padding, and a long sequence that ends."""
     rng = np.random.default_rng(34)
