@@ -542,7 +542,9 @@ int muyo_sample_f32(float* logits, uint32_t vocab, const int32_t* history, uint3
  *   - its length and target are in 0..table_pages * page_size,
  *   - its new tokens fit in `tokens` behind those asked for by the sequences before it, and
  *   - it needs no new page, or its pages are there behind those needed by the sequences before it;
- * otherwise it stays as it is, with granted[b] = lengths[b] and no tokens. On return
+ * otherwise it stays as it is, with granted[b] = lengths[b] and no tokens. (One behind more new tokens
+ * than `tokens` stays too when it asks for none or fewer: end sequences in a step whose list holds all.)
+ * On return
  *   granted[b]              the lengths after the step
  *   pool_out                the ring's first place and number of free pages after the step
  *   tables                  new pages entered from column ceil(length / page_size) on; the rest as it was
@@ -602,7 +604,8 @@ int muyo_rope_frequencies(double base, uint32_t rotary_dim, const MuyoRopeScalin
  * slots. q, k and v are f32 [tokens][heads * head_dim] with token strides of their own (in values,
  * multiples of 4), so that they may be parts of stacked projection rows; q_out may be q where its
  * stride is heads * head_dim. turns is device memory as muyo_rope_frequencies fills it.
- * head_dim % 8 == 0 up to 1024, rotary_dim even. A token with a position below 0 is padding: its row
+ * head_dim % 8 == 0 up to 1024, rotary_dim even; tokens * (heads + 2 kv_heads) * head_dim at most
+ * 2^34 where rotary_dim % 8 == 0, else 2^32. A token with a position below 0 is padding: its row
  * of q_out and the caches stay as they were. One with a slot outside the cache is not appended. The
  * slots of one call are distinct (as the plan makes them); the rows of a slot given twice are
  * undefined. */
@@ -617,11 +620,11 @@ int muyo_paged_rope_append_f16kv(const float* q, const float* k, const float* v,
  * the sequence in row query_sequence[i] of tables, sees keys j <= positions[i], the last `window` of them
  * where window > 0. For every head h (kv head h / (heads / kv_heads)):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h].k[j]) * v[j]
- * q and out are f32 [queries][heads * head_dim], and may be the same. A query without keys (a position below 0) gives 0. A
- * query whose sequence is outside 0..sequences - 1 is padding: its row of out stays as it was. Keys past
- * table_pages * page_size, or in pages with an id outside the cache, are left out. Queries may share a
- * sequence (several new tokens of one). Which keys a workgroup takes depends on the whole batch, so a
- * query's last bits may too; the same call gives the same bits.
+ * q and out are f32 [queries][heads * head_dim], and may be the same. A query without keys (a position
+ * below 0) gives 0. A query whose sequence is outside 0..sequences - 1 is padding: its row of out stays
+ * as it was. Keys past table_pages * page_size, or in pages with an id outside the cache, are left out.
+ * Queries may share a sequence (several new tokens of one). Which keys a workgroup takes depends on the
+ * whole batch, so a query's last bits may too; the same call gives the same bits.
  * K and V rows that a query sees are finite; the others may hold anything.
  * head_dim 64 or 128, at most 16 heads per kv head, 1024 heads, 65535 queries, scale finite.
  * `workspace` is caller-owned device memory (16-byte aligned) of at least
@@ -644,8 +647,8 @@ int muyo_paged_attention_decode_f16kv(const float* q, const void* kcache, const 
  * logprobs, ranks and entropy may each be NULL (tokens too, without the first two), top 0..64 and at
  * most vocab. A token outside the vocabulary has logprob -inf and rank -1. Logits of -inf have
  * probability 0; a row of nothing else has logprobs -inf and entropy 0. A NaN or +inf among a row's
- * logits makes its logprobs and entropy NaN; in the order NaN is last. `workspace` as above, of at least
- * muyo_token_logprobs_workspace_bytes(...) bytes. */
+ * logits makes its logprobs and entropy NaN; in the order NaN is last. Fewer than 2^24 rows. `workspace`
+ * as above, of at least muyo_token_logprobs_workspace_bytes(...) bytes. */
 size_t muyo_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top); /* 0: unsupported */
 int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
                             const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropy, uint32_t top,

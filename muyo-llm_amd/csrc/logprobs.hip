@@ -21,6 +21,7 @@ constexpr int kFewLanes = 4;                        // looked at one by one
 constexpr uint32_t kMaxTop = 64;                    // a lane of a wave each
 constexpr uint32_t kMaxParts = 64;                  // workgroups of a row
 constexpr uint32_t kBlocksAtOnce = 1280;            // workgroups that 256 CUs run at once
+constexpr uint32_t kMaxRows = (1u << 24) - 1;       // a launch has fewer than 2^32 threads
 constexpr uint64_t kOnceBytes = 256ull << 20;       // logits that no cache holds: read without caching them
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -75,8 +76,9 @@ __device__ __forceinline__ uint64_t KeyOfLaneBefore(uint64_t key)
 {
     const int lo = static_cast<int>(static_cast<uint32_t>(key));
     const int hi = static_cast<int>(static_cast<uint32_t>(key >> 32));
-    return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(hi, hi, 0x138, 0xF, 0xF, false))) << 32) |
-           static_cast<uint32_t>(__builtin_amdgcn_update_dpp(lo, lo, 0x138, 0xF, 0xF, false));
+    const uint32_t high = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(hi, hi, 0x138, 0xF, 0xF, false));
+    const uint32_t low = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(lo, lo, 0x138, 0xF, 0xF, false));
+    return (static_cast<uint64_t>(high) << 32) | low;
 }
 
 __device__ __forceinline__ uint32_t CountLanes(bool is) { return static_cast<uint32_t>(__popcll(__ballot(is))); }
@@ -645,8 +647,9 @@ __global__ __launch_bounds__(kBlock) void TokenLogprobsJoinKernel(LogprobArgs a)
     WriteRow(a, row, sums, given, best);
 }
 
-/// Workgroups of a row: the fewest estimated batches after one another, when 1280 workgroups run at once (five on
-/// each of 256 CUs) and one of more than one round costs as much as three batches besides its own.
+/// Workgroups of a row: the fewest estimated batches after one another, when 1280 workgroups run at once
+/// (five on each of 256 CUs), each round of them costs as much as three batches besides its own, and so
+/// does the join.
 uint32_t RowParts(uint32_t rows, uint32_t vocab)
 {
     const uint32_t batches = CeilDiv(static_cast<uint64_t>(vocab) + 3, kBatch);
@@ -656,7 +659,8 @@ uint32_t RowParts(uint32_t rows, uint32_t vocab)
     for (uint32_t parts = 1; parts <= most; ++parts)
     {
         const uint64_t rounds = CeilDiv(static_cast<uint64_t>(rows) * parts, kBlocksAtOnce);
-        const uint64_t cost = rounds * (CeilDiv(batches, static_cast<uint64_t>(parts) * kWaves) + 3) + (parts > 1 ? 3 : 0);
+        const uint64_t after = CeilDiv(batches, static_cast<uint64_t>(parts) * kWaves);
+        const uint64_t cost = rounds * (after + 3) + (parts > 1 ? 3 : 0);
         if (cost < least)
         {
             least = cost;
@@ -672,7 +676,7 @@ using namespace muyo;
 
 extern "C" size_t muyo_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top)
 {
-    if (rows == 0 || vocab == 0 || vocab > 0x7FFFFFFFu || top > kMaxTop || top > vocab)
+    if (rows == 0 || rows > kMaxRows || vocab == 0 || vocab > 0x7FFFFFFFu || top > kMaxTop || top > vocab)
     {
         return 0;
     }
@@ -695,8 +699,9 @@ extern "C" int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride,
     const size_t need = muyo_token_logprobs_workspace_bytes(rows, vocab, top);
     if (need == 0)
     {
-        return Fail(MUYO_E_RANGE, "%s: needs rows >= 1, 1 <= vocab < 2^31, top <= %u and top <= vocab (got %u, %u, %u)",
-                    name, kMaxTop, rows, vocab, top);
+        return Fail(MUYO_E_RANGE, "%s: needs 1..%u rows, 1 <= vocab < 2^31, top <= %u and top <= vocab (got %u, "
+                                  "%u, %u)",
+                    name, kMaxRows, kMaxTop, rows, vocab, top);
     }
     if (row_stride < vocab || (reinterpret_cast<uintptr_t>(logits) & 3u) != 0)
     {
@@ -714,9 +719,9 @@ extern "C" int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride,
                   entropy, top,        top_ids, top_logprobs, parts, sums,
                   reinterpret_cast<uint64_t*>(sums + static_cast<size_t>(rows) * parts)};
     const uint64_t blocks = static_cast<uint64_t>(rows) * parts;
-    if (blocks > 0x7FFFFFFFull)
+    if (blocks > kMaxRows)
     {
-        return Fail(MUYO_E_RANGE, "%s: %u rows are too many for one launch", name, rows);
+        return Fail(MUYO_E_RANGE, "%s: %u rows of %u are too many for one call", name, rows, vocab);
     }
     const dim3 grid(static_cast<uint32_t>(blocks));
     if (4ull * rows * vocab > kOnceBytes)

@@ -719,6 +719,14 @@ extern "C" int muyo_paged_rope_append_f16kv(const float* q, const float* k, cons
                                         "that, and a known rope_layout (got %u, %u, %u)",
                     name, head_dim, rotary_dim, rope_layout);
     }
+    const uint32_t rows = heads + 2 * kv_heads;
+    const bool octets = rotary_dim % 8 == 0;
+    const uint64_t items = static_cast<uint64_t>(tokens) * rows * (octets ? head_dim / 8 : head_dim / 2);
+    if (items > 1ull << 31)  // a launch has fewer than 2^32 threads
+    {
+        return Fail(MUYO_E_RANGE, "%s: %u tokens of %u heads of %u values are too many for one call", name, tokens,
+                    rows, head_dim);
+    }
     const uint64_t qdim = static_cast<uint64_t>(heads) * head_dim;
     const uint64_t kdim = static_cast<uint64_t>(kv_heads) * head_dim;
     if (q_stride < qdim || k_stride < kdim || v_stride < kdim || q_stride % 4 != 0 || k_stride % 4 != 0 ||
@@ -733,6 +741,11 @@ extern "C" int muyo_paged_rope_append_f16kv(const float* q, const float* k, cons
                                      "magnitude finite",
                     name);
     }
+    const uint64_t cacheBytes = 2 * kdim * pages * page_size;
+    if (Overlap({kcache, cacheBytes, "kcache"}, {vcache, cacheBytes, "vcache"}))
+    {
+        return Fail(MUYO_E_CONTRACT, "%s: kcache overlaps vcache", name);
+    }
     const Range out{q_out, 4 * qdim * tokens, "q_out"};
     const Range in[] = {{q, 4 * (q_stride * (tokens - 1) + qdim), "q"},
                         {k, 4 * (k_stride * (tokens - 1) + kdim), "k"},
@@ -740,28 +753,20 @@ extern "C" int muyo_paged_rope_append_f16kv(const float* q, const float* k, cons
     for (const Range& r : in)
     {
         // In place over a dense q each thread writes what it alone has read.
-        const bool inPlace = r.at == q_out && r.at == q && q_stride == qdim;
+        const bool inPlace = &r == in && q == q_out && q_stride == qdim;
         if (!inPlace && Overlap(out, r))
         {
             return Fail(MUYO_E_CONTRACT, "%s: q_out overlaps %s", name, r.name);
         }
     }
-    AppendArgs a{q,      k,         v,      q_stride, k_stride,         v_stride,   q_out, static_cast<uint16_t*>(kcache),
+    AppendArgs a{q, k, v, q_stride, k_stride, v_stride, q_out, static_cast<uint16_t*>(kcache),
                  static_cast<uint16_t*>(vcache), positions, slots, tokens, heads, kv_heads, head_dim, 0,
                  pages * page_size, rope_layout, rotary_dim, turns, magnitude};
     while ((1u << a.pageShift) < page_size)
     {
         ++a.pageShift;
     }
-    const uint32_t rows = heads + 2 * kv_heads;
-    const bool octets = rotary_dim % 8 == 0;
-    const uint64_t items = static_cast<uint64_t>(tokens) * rows * (octets ? head_dim / 8 : head_dim / 2);
-    const uint64_t blocks = (items + 255) / 256;
-    if (blocks > 0x7FFFFFFFull)
-    {
-        return Fail(MUYO_E_RANGE, "%s: %u tokens of %u rows are too many for one launch", name, tokens, rows);
-    }
-    const dim3 grid(static_cast<uint32_t>(blocks));
+    const dim3 grid(static_cast<uint32_t>((items + 255) / 256));
     if (octets && rope_layout == MUYO_ROPE_INTERLEAVED)
     {
         hipLaunchKernelGGL(PagedAppendOctets<true>, grid, dim3(256), 0, AsStream(stream), a);

@@ -68,6 +68,10 @@ REFUSALS = [
     ("paged_rope_append_f16kv", APPEND, dict(kcache=ctypes.c_void_p((5 << 30) + 2)), "MUYO_E_CONTRACT"),
     ("paged_rope_append_f16kv", APPEND, dict(turns=ctypes.c_void_p(4)), "MUYO_E_CONTRACT"),
     ("paged_rope_append_f16kv", APPEND, dict(magnitude=math.nan), "MUYO_E_CONTRACT"),
+    ("paged_rope_append_f16kv", APPEND, dict(vcache=APPEND["kcache"]), "MUYO_E_CONTRACT"),
+    ("paged_rope_append_f16kv", APPEND, dict(q_out=APPEND["q"], k=APPEND["q"]), "MUYO_E_CONTRACT"),
+    ("paged_rope_append_f16kv", APPEND, dict(tokens=1 << 24, q_out=APPEND["q"]), "MUYO_E_RANGE"),
+    ("paged_rope_append_f16kv", APPEND, dict(tokens=1 << 22, rotary_dim=60, q_out=APPEND["q"]), "MUYO_E_RANGE"),
     ("paged_rope_append_f16kv", APPEND, dict(q_out=APPEND["k"]), "MUYO_E_CONTRACT"),
     ("paged_rope_append_f16kv", APPEND, dict(q_out=APPEND["q"], q_stride=1152), "MUYO_E_CONTRACT"),
     *[("paged_attention_decode_f16kv", ATTEND, {k: None}, "MUYO_E_NULL")
@@ -95,6 +99,9 @@ REFUSALS = [
     ("token_logprobs_f32", LOGPROBS, dict(top_ids=None), "MUYO_E_NULL"),
     ("token_logprobs_f32", LOGPROBS, dict(top_logprobs=None), "MUYO_E_NULL"),
     ("token_logprobs_f32", LOGPROBS, dict(rows=0), "MUYO_E_RANGE"),
+    ("token_logprobs_f32", LOGPROBS, dict(rows=1 << 24), "MUYO_E_RANGE"),
+    ("token_logprobs_f32", LOGPROBS, dict(rows=(1 << 24) - 1, vocab=0x7FFFFFFF, row_stride=0x7FFFFFFF,
+                                          workspace_bytes=1 << 62), "MUYO_E_RANGE"),
     ("token_logprobs_f32", LOGPROBS, dict(vocab=0, row_stride=0, top=0), "MUYO_E_RANGE"),
     ("token_logprobs_f32", LOGPROBS, dict(top=65), "MUYO_E_RANGE"),
     ("token_logprobs_f32", LOGPROBS, dict(vocab=4), "MUYO_E_RANGE"),
