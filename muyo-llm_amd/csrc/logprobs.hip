@@ -17,10 +17,13 @@ constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / kWave;
 constexpr int kQuads = 4;                           // 16-byte loads of a lane's batch
 constexpr uint32_t kBatch = kWave * 4 * kQuads;     // logits a wave takes at a time
+constexpr int kKept = 3;                            // batches with its largest logits that a lane knows
+constexpr uint32_t kTooMany = 1u << 20;             // candidates
 constexpr int kFewLanes = 4;                        // looked at one by one
 constexpr uint32_t kMaxTop = 64;                    // a lane of a wave each
 constexpr uint32_t kMaxParts = 64;                  // workgroups of a row
-constexpr uint32_t kBlocksAtOnce = 1280;            // workgroups that 256 CUs run at once
+constexpr int kPerCu = 5;                           // workgroups of a CU
+constexpr uint32_t kBlocksAtOnce = 256 * kPerCu;    // workgroups that 256 CUs run at once
 constexpr uint32_t kMaxRows = (1u << 24) - 1;       // a launch has fewer than 2^32 threads
 constexpr uint64_t kOnceBytes = 256ull << 20;       // logits that no cache holds: read without caching them
 constexpr float kLog2e = 1.4426950408889634f;
@@ -208,219 +211,134 @@ __device__ __forceinline__ uint32_t LowerBound(uint32_t high, uint32_t each, uin
     return bound;
 }
 
-/// One pass over the row: a wave takes batches of kBatch logits into registers and each lane keeps the sums
-/// of its own.
-///
-/// The first `top` tokens: the wave's best so far lie in order across its lanes (lane i has the i-th), and
-/// a batch is looked through only if some lane's largest logit reaches the last of them. Then a lower bound
-/// of the batch's own `top`-th is found first, by bisection: a value that the largest ones of `top` lanes
-/// reach. Few lanes reach both bounds in a later batch: their logits are looked at lane by lane and inserted
-/// one by one. In the first batches the candidates (a few more than `top` in the first) are gathered, with
-/// the best so far, and ranked: a candidate's place is the number of those above it. More than 64 are
-/// inserted too. Equal logits are told apart by their index in the key, so nothing overflows.
-///
-/// The rank is counted on the way: the tokens before a given one have a larger logit, or the same at
-/// a lower index, which is a different comparison on each side of its batch.
-///
-/// That batch, and batches to be looked through, go through LDS: the registers are free for the next
-/// batch at once, and loops over their logits need not be unrolled (most workgroups run such code once
-/// or twice, and its instructions would come from memory).
-///
-/// What bounds it: for many rows, the logits' arrival. 1000 rows of 151936, 608 MB: 99 us, 6.1 TB/s, where the
-/// best streaming read here has 6.9; read without the non-temporal hint (they fit no cache) 114 us. For
-/// few rows, the chain of a wave's batch, 6 us of round trips, bisection and ranking: one row with 20
-/// alternatives takes 7.6 us and 4.4 for the join, 61 rows with 5 16.3 and 4.0, 300 rows with 20, whose
-/// vector units are busy with candidates, 59 and 5. Batches of 2048 logits, whose registers leave three
-/// workgroups a CU, took 10.8, 16.9 and 57 us, and 107 for the 1000 rows.
-template <bool kOnce>
-__global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
+/// The row's values begin `lead` values into a 16-byte load, and end at `span`.
+struct RowSpan
 {
-    __shared__ Sums waveSums[kWaves];
-    __shared__ uint32_t waveHeld[kWaves];
-    __shared__ uint64_t waveKeys[kWaves * kWave];
-    __shared__ uint64_t best[kMaxTop];
-    __shared__ uint32_t places[kBlock];
-    __shared__ float4v staged[kWaves][kQuads][kWave];
-    __shared__ uint64_t candidates[kWaves][kWave];
+    const float* x;
+    uint32_t lead, span;
+};
+
+__device__ __forceinline__ RowSpan SpanOf(const LogprobArgs& a, uint32_t row)
+{
+    RowSpan s;
+    s.x = a.logits + row * a.stride;
+    s.lead = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(s.x) / 4 % 4);
+    s.span = s.lead + a.vocab;
+    return s;
+}
+
+/// The lane's kQuads * 4 values of a batch, with a bit of `there` for each that is the row's.
+template <bool kOnce>
+__device__ __forceinline__ void LoadBatch(const RowSpan& s, uint32_t batch, uint32_t lane, float4v (&v)[kQuads],
+                                          uint32_t& there)
+{
+    there = ~0u;
+    const uint32_t first = batch * kBatch;
+    if (first >= s.lead && first + kBatch <= s.span)
+    {
+        const float4v* from = reinterpret_cast<const float4v*>(s.x - s.lead + first) + lane;
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j)
+        {
+            v[j] = kOnce ? __builtin_nontemporal_load(from + j * kWave) : from[j * kWave];
+        }
+        return;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kQuads; ++j)
+    {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c)
+        {
+            const uint32_t at = first + 4 * (j * kWave + lane) + c;
+            const bool is = at >= s.lead && at < s.span;
+            v[j][c] = is ? s.x[at - s.lead] : -INFINITY;
+            there = is ? there : there & ~(1u << (4 * j + c));
+        }
+    }
+}
+
+/// What a workgroup needs to find the first tokens of its part.
+struct TopSpace
+{
+    __attribute__((aligned(16))) uint32_t places[kBlock];
+    uint32_t bound;
+    uint32_t found;
+    uint32_t waveHeld[kWaves];
+    uint64_t keys[kWaves * kWave];
+    uint64_t best[kMaxTop];
+    float4v staged[kWaves][kQuads][kWave];
+    uint64_t candidates[kWaves][kWave];
+};
+
+/// The first a.top tokens of a part, for any number of logits that reach `floor`: wave by wave, batch by
+/// batch (from the wave's first, `stride` apart).
+///
+/// A wave's best so far lie in order across its lanes (lane i has the i-th). Few lanes of a batch reach the
+/// last of them: their logits are looked at lane by lane and inserted one by one. Otherwise a lower bound
+/// of the batch's own `top`-th is found first, by bisection: a value that the largest ones of `top` lanes
+/// reach. The candidates (a few more than `top`) are gathered, with the best so far, and ranked: a candidate's
+/// place is the number of those above it. More than 64 are inserted too. Equal logits are told apart by
+/// their index in the key, so nothing overflows. The batch goes through LDS: the registers are free for
+/// the next one at once, and loops over its logits need not be unrolled.
+__device__ __forceinline__ void TopByWaves(const LogprobArgs& a, const RowSpan& s, uint32_t batch, uint32_t batches,
+                                           uint32_t stride, uint32_t floorBits, TopSpace& space)
+{
+    const uint64_t floorKey = static_cast<uint64_t>(floorBits) << 32;
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t row = blockIdx.x / a.parts;
-    const uint32_t part = blockIdx.x - row * a.parts;
-    const float* x = a.logits + row * a.stride;
-    // Loads are 16-byte aligned: the row begins `lead` values into the first.
-    const uint32_t lead = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) / 4 % 4);
-    const uint64_t span = static_cast<uint64_t>(lead) + a.vocab;
-    const uint32_t batches = static_cast<uint32_t>((span + kBatch - 1) / kBatch);
-    const uint32_t stride = a.parts * kWaves;
-
-    // A batch's logits, and a bit for each that is the row's (the others are -inf).
     float4v v[kQuads];
-    uint32_t there = ~0u;
-    auto request = [&](uint32_t batch) {
-        const uint64_t first = static_cast<uint64_t>(batch) * kBatch;
-        there = ~0u;
-        if (first >= lead && first + kBatch <= span)
-        {
-            const float4v* from = reinterpret_cast<const float4v*>(x - lead + first) + lane;
-#pragma unroll
-            for (int j = 0; j < kQuads; ++j)
-            {
-                v[j] = kOnce ? __builtin_nontemporal_load(from + j * kWave) : from[j * kWave];
-            }
-            return;
-        }
+    uint32_t there = 0;
+    uint64_t mine = 0;          // lane i: the i-th best so far
+    uint64_t least = floorKey;  // the last of the first `top`, or what they reach
+    auto lastOf = [&]() {
+        const uint64_t last = KeyOfLane(mine, a.top - 1);
+        return last > floorKey ? last : floorKey;
+    };
+    if (batch < batches)
+    {
+        LoadBatch<false>(s, batch, lane, v, there);
+    }
+    for (; batch < batches; batch += stride)
+    {
+        const uint32_t at0 = batch * kBatch - s.lead;  // index of v[j][c]: at0 + 256 j + 4 lane + c
+        const uint32_t is = there;
+        uint32_t high = 0;
 #pragma unroll
         for (int j = 0; j < kQuads; ++j)
         {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
             {
-                const uint64_t at = first + 4 * (j * kWave + lane) + c;
-                const bool is = at >= lead && at < span;
-                v[j][c] = is ? x[at - lead] : -INFINITY;
-                there = is ? there : there & ~(1u << (4 * j + c));
+                high = max(high, (is >> (4 * j + c) & 1u) != 0 ? OrderBits(v[j][c]) : 0u);
             }
         }
-    };
-
-    uint32_t batch = part * kWaves + wave;
-    if (batch < batches)
-    {
-        request(batch);
-    }
-    const Given given = GivenOf(a, row);
-    const uint64_t ownKey = given.is ? OrderKey(given.logit, given.token) : ~0ull;
-    const bool plain = given.logit > -INFINITY;  // not -inf, not NaN
-    const float below = nextafterf(given.logit, -INFINITY);
-
-    Sums sums{-INFINITY, 0.0f, 0.0f, 0};
-    uint32_t above = 0;      // the wave's
-    uint64_t mine = 0;       // lane i: the i-th best so far
-    uint64_t least = 0;      // the last of the first `top`
-    auto insert = [&](uint64_t one) {
-        const uint32_t place = CountLanes(mine > one);
-        const uint64_t left = KeyOfLaneBefore(mine);
-        mine = lane < place ? mine : lane == place ? one : left;
-        least = KeyOfLane(mine, a.top - 1);
-    };
-    for (; batch < batches; batch += stride)
-    {
-        float largest = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j)
+        uint32_t floor = static_cast<uint32_t>(least >> 32);
+        const bool any = is != 0;
+        if (CountLanes(any && high >= floor) >= a.top)
         {
-            largest = fmaxf(largest, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
+            floor = max(floor, LowerBound(high, 1, a.top));
         }
-        if (largest > sums.m)
-        {
-            Rebase(sums, largest);
-        }
-        const float base = sums.m == -INFINITY ? 0.0f : sums.m;
-        {
-            float s[4] = {}, t[4] = {};
-#pragma unroll
-            for (int j = 0; j < kQuads; ++j)
-            {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                {
-                    const float y = (v[j][c] - base) * kLog2e;
-                    const float e = __builtin_amdgcn_exp2f(y);
-                    s[c] += e;
-                    t[c] = fmaf(e, y, t[c]);
-                }
-            }
-            float more = (t[0] + t[1]) + (t[2] + t[3]);
-            if (__any(more != more))
-            {
-                // 0 times the -inf of a masked logit. (NaN logits stay in s.)
-                more = 0.0f;
-#pragma unroll
-                for (int j = 0; j < kQuads; ++j)
-                {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                    {
-                        const float y = (v[j][c] - base) * kLog2e;
-                        more = fmaf(__builtin_amdgcn_exp2f(y), fmaxf(y, -1e4f), more);
-                    }
-                }
-            }
-            sums.s += (s[0] + s[1]) + (s[2] + s[3]);
-            sums.t += more;
-        }
-
-        // Index of v[j][c]: at0 + 256 j + c.
-        const int64_t begin = static_cast<int64_t>(batch) * kBatch - lead;
-        const uint32_t at0 = static_cast<uint32_t>(begin) + 4 * lane;
-        const bool after = begin > given.token;
-        const bool before = begin + kBatch <= given.token;
-        const bool single = given.is && !(plain && (after || before));
-        if (given.is && !single)
-        {
-            const float over = after ? given.logit : below;
-#pragma unroll
-            for (int j = 0; j < kQuads; ++j)
-            {
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                {
-                    above += CountLanes(v[j][c] > over);
-                }
-            }
-        }
-        const uint32_t last = static_cast<uint32_t>(least >> 32);
-        // A lane of NaN, or of none of the row's logits, has no -inf: its key may be lower than `largest` says.
-        const uint32_t is = there;
-        const bool odd = __any(is != ~0u || sums.s != sums.s);
-        const bool look = a.top > 0 && (odd || __any(OrderBits(largest) >= last));
-        if (single || look)
+        uint64_t lanes = __ballot(any && high >= floor);
+        if (lanes != 0)
         {
 #pragma unroll
             for (int j = 0; j < kQuads; ++j)
             {
-                staged[wave][j][lane] = v[j];
+                space.staged[wave][j][lane] = v[j];
             }
         }
         if (batch + stride < batches)
         {
-            request(batch + stride);
+            LoadBatch<false>(s, batch + stride, lane, v, there);
         }
-        if (!single && !look)
+        if (lanes == 0)
         {
             continue;
-        }
-        if (single || odd)
-        {
-            uint32_t high = 0;
-#pragma unroll 1
-            for (int j = 0; j < kQuads; ++j)
-            {
-                const float4v x4 = staged[wave][j][lane];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                {
-                    const uint64_t key = (is >> (4 * j + c) & 1u) != 0 ? OrderKey(x4[c], at0 + 256 * j + c) : 0;
-                    sums.above += single && key > ownKey ? 1u : 0u;
-                    high = max(high, static_cast<uint32_t>(key >> 32));
-                }
-            }
-            largest = KeyValue(static_cast<uint64_t>(high) << 32);
-        }
-        if (!look)
-        {
-            continue;
-        }
-        const uint32_t high = OrderBits(largest);
-        uint32_t floor = last;
-        if (CountLanes(high >= floor) >= a.top)
-        {
-            floor = max(floor, LowerBound(high, 1, a.top));
         }
         // The wave's LDS operations complete in order; the fences keep the compiler's order too.
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        uint64_t lanes = __ballot(high >= floor);
         uint32_t found = kWave + 1;
         if (__popcll(lanes) > kFewLanes)
         {
@@ -428,7 +346,7 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
 #pragma unroll 1
             for (int j = 0; j < kQuads; ++j)
             {
-                const float4v x4 = staged[wave][j][lane];
+                const float4v x4 = space.staged[wave][j][lane];
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                 {
@@ -445,7 +363,8 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
                 if (take != 0 && place < kWave)
                 {
                     const uint32_t e = static_cast<uint32_t>(__ffs(static_cast<int>(take)) - 1);
-                    candidates[wave][place] = OrderKey(staged[wave][e / 4][lane][e % 4], at0 + 256 * (e / 4) + e % 4);
+                    space.candidates[wave][place] = OrderKey(space.staged[wave][e / 4][lane][e % 4],
+                                                             at0 + 256 * (e / 4) + 4 * lane + e % 4);
                 }
                 take &= take - 1;
                 found += static_cast<uint32_t>(__popcll(mask));
@@ -453,7 +372,7 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
             const uint32_t kept = min(CountLanes(mine != 0), a.top);
             if (found + kept <= kWave && lane < kept)
             {
-                candidates[wave][found + lane] = mine;
+                space.candidates[wave][found + lane] = mine;
             }
             found += kept;
         }
@@ -461,7 +380,7 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
         {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            const uint64_t key = lane < found ? candidates[wave][lane] : 0;
+            const uint64_t key = lane < found ? space.candidates[wave][lane] : 0;
             mine = key;
             if (batch + stride >= batches)
             {
@@ -477,12 +396,12 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
             __builtin_amdgcn_wave_barrier();
             if (lane < found)
             {
-                candidates[wave][place] = key;
+                space.candidates[wave][place] = key;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            mine = lane < found ? candidates[wave][lane] : 0;
-            least = KeyOfLane(mine, a.top - 1);
+            mine = lane < found ? space.candidates[wave][lane] : 0;
+            least = lastOf();
         }
         else
         {
@@ -492,15 +411,20 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
                 const uint32_t from = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(lanes)) - 1);
                 lanes &= lanes - 1;
                 const uint32_t j = lane / 4 % kQuads;
-                const float value = staged[wave][j][from][lane % 4];
+                const float value = space.staged[wave][j][from][lane % 4];
                 const uint32_t theirs = __builtin_amdgcn_readlane(is, from);
-                const uint64_t key = OrderKey(value, static_cast<uint32_t>(begin) + 4 * from + 256 * j + lane % 4);
+                const uint64_t key = OrderKey(value, at0 + 256 * j + 4 * from + lane % 4);
                 const bool take = lane < 4 * kQuads && (theirs >> lane & 1u) != 0 &&
                                   static_cast<uint32_t>(key >> 32) >= floor;
                 uint64_t mask = __ballot(take && key > least);
                 while (mask != 0)
                 {
-                    insert(KeyOfLane(key, static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(mask)) - 1)));
+                    const uint64_t one =
+                        KeyOfLane(key, static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(mask)) - 1));
+                    const uint32_t place = CountLanes(mine > one);
+                    const uint64_t left = KeyOfLaneBefore(mine);
+                    mine = lane < place ? mine : lane == place ? one : left;
+                    least = lastOf();
                     mask &= mask - 1;
                     mask &= __ballot(key > least);
                 }
@@ -510,26 +434,10 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
         __builtin_amdgcn_wave_barrier();
     }
 
-    // Lanes, then waves.
-    const float top = GroupMax<kWave>(sums.m);
-    Rebase(sums, top);
-    sums.s = GroupSum<kWave>(sums.s);
-    sums.t = GroupSum<kWave>(sums.t);
-#pragma unroll
-    for (int step = 1; step < kWave; step *= 2)
-    {
-        sums.above += __shfl_xor(sums.above, step);
-    }
-    sums.above += above;
     const uint32_t held = CountLanes(mine != 0);
     if (lane == 0)
     {
-        waveSums[wave] = sums;
-        waveHeld[wave] = held;
-    }
-    if (wave == 0)
-    {
-        best[lane] = 0;  // a part may have fewer tokens
+        space.waveHeld[wave] = held;
     }
     __syncthreads();
     uint32_t keys = 0;
@@ -538,10 +446,325 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
     {
         if (w == wave && lane < held)
         {
-            waveKeys[keys + lane] = mine;  // none of them is 0, and they come first
+            space.keys[keys + lane] = mine;  // none of them is 0, and they come first
         }
-        keys += waveHeld[w];
+        keys += space.waveHeld[w];
     }
+    __syncthreads();
+    RankKeys(space.keys, keys, a.top, space.best, space.places);
+    __syncthreads();
+}
+
+/// A lane's batches with its largest logits: the largest of each, in falling order, and which of the wave's
+/// batches it is. Of the others only the largest logit is kept.
+struct LaneBatches
+{
+    float most[kKept + 1];
+    uint32_t nth[kKept];
+
+    __device__ __forceinline__ void Clear()
+    {
+#pragma unroll
+        for (int i = 0; i < kKept; ++i)
+        {
+            most[i] = -INFINITY;
+            nth[i] = 0;
+        }
+        most[kKept] = -INFINITY;
+    }
+
+    __device__ __forceinline__ void Add(float largest, uint32_t which)
+    {
+        if (!__any(largest > most[kKept - 1]))
+        {
+            most[kKept] = fmaxf(most[kKept], largest);
+            return;
+        }
+        most[kKept] = largest > most[kKept - 1] ? most[kKept - 1] : fmaxf(most[kKept], largest);
+#pragma unroll
+        for (int i = kKept - 1; i > 0; --i)
+        {
+            const bool here = largest > most[i];
+            const bool before = largest > most[i - 1];
+            most[i] = before ? most[i - 1] : here ? largest : most[i];
+            nth[i] = before ? nth[i - 1] : here ? which : nth[i];
+        }
+        const bool first = largest > most[0];
+        most[0] = first ? largest : most[0];
+        nth[0] = first ? which : nth[0];
+    }
+
+    __device__ __forceinline__ void Drop()
+    {
+#pragma unroll
+        for (int i = 0; i + 1 < kKept; ++i)
+        {
+            most[i] = most[i + 1];
+            nth[i] = nth[i + 1];
+        }
+        most[kKept - 1] = -INFINITY;
+    }
+};
+
+/// The first a.top tokens of a workgroup's part into space.best, in order (0 behind the last).
+///
+/// The a.top-th of the 256 threads' largest logits is a lower bound of the part's a.top-th. Threads look again
+/// at those of their batches that reach it, mostly one of a few threads (the last one is in v still), and what
+/// reaches it, a few more than a.top logits, is gathered and ranked. Where that does not do (a thread has more
+/// such batches than it knows, or there are more than 256 such logits, or fewer threads than a.top have any)
+/// the waves go through the part once more.
+__device__ __forceinline__ void TopOfPart(const LogprobArgs& a, const RowSpan& s, uint32_t firstBatch, uint32_t batches,
+                                          uint32_t stride, float4v (&v)[kQuads], uint32_t there, LaneBatches& own,
+                                          TopSpace& space)
+{
+    const uint32_t lane = threadIdx.x % kWave;
+    space.places[threadIdx.x] = own.most[0] > -INFINITY ? OrderBits(own.most[0]) : 0;  // -inf: NaN, or none
+    if (threadIdx.x < kMaxTop)
+    {
+        space.best[threadIdx.x] = 0;
+    }
+    __syncthreads();
+    if (threadIdx.x < kWave)
+    {
+        // Four threads' a lane. The bound's upper 16 bits are enough. (In every wave at once it would keep the
+        // scalar unit, which a CU's waves share, busy for 2 us.)
+        const uint4 four = *reinterpret_cast<const uint4*>(space.places + 4 * lane);
+        uint32_t bound = 0;
+#pragma unroll 1
+        for (uint32_t bit = 1u << 31; bit > 1u << 15; bit >>= 1)
+        {
+            const uint32_t next = bound | bit;
+            const uint32_t reach = CountLanes(four.x >= next) + CountLanes(four.y >= next) +
+                                   CountLanes(four.z >= next) + CountLanes(four.w >= next);
+            bound = reach >= a.top ? next : bound;
+        }
+        if (lane == 0)
+        {
+            space.bound = bound;
+            space.found = 0;
+        }
+    }
+    __syncthreads();
+    const uint32_t floor = __builtin_amdgcn_readfirstlane(space.bound);
+    if (floor == 0 || OrderBits(own.most[kKept]) >= floor)
+    {
+        space.found = kTooMany;
+    }
+    else
+    {
+        uint32_t held = (batches - 1 - firstBatch) / stride;
+        while (OrderBits(own.most[0]) >= floor)
+        {
+            const uint32_t batch = firstBatch + own.nth[0] * stride;
+            if (own.nth[0] != held)
+            {
+                LoadBatch<false>(s, batch, lane, v, there);
+            }
+            held = ~0u;
+            own.Drop();
+            uint32_t take = there;
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
+            {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                {
+                    take = OrderBits(v[j][c]) >= floor ? take : take & ~(1u << (4 * j + c));
+                }
+            }
+            take &= (1u << 4 * kQuads) - 1;
+            while (take != 0)
+            {
+                const uint32_t e = static_cast<uint32_t>(__ffs(static_cast<int>(take)) - 1);
+                take &= take - 1;
+                float value = v[0][0];
+#pragma unroll
+                for (uint32_t i = 1; i < 4 * kQuads; ++i)
+                {
+                    value = e == i ? v[i / 4][i % 4] : value;
+                }
+                const uint32_t place = atomicAdd(&space.found, 1u);
+                if (place < kBlock)
+                {
+                    // The order does not matter: they are ranked.
+                    space.keys[place] = OrderKey(value, batch * kBatch - s.lead + 256 * (e / 4) + 4 * lane + e % 4);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t found = space.found;
+    __syncthreads();
+    if (found <= kBlock)
+    {
+        RankKeys(space.keys, found, a.top, space.best, space.places);
+        __syncthreads();
+        return;
+    }
+    TopByWaves(a, s, firstBatch, batches, stride, floor, space);
+}
+
+/// One pass over the row: a wave takes batches of kBatch logits into registers, and each lane keeps the sums
+/// of its own, and which of its batches have its largest logits: enough to find the part's first `top` tokens
+/// when all of it has been read.
+///
+/// The rank is counted on the way: the tokens before a given one have a larger logit, or the same at
+/// a lower index, which is a different comparison on each side of its batch. That batch itself goes through
+/// LDS, so that the loop over its logits need not be unrolled (one wave of a row runs it, and its instructions
+/// come from memory).
+///
+/// What bounds it: for many rows, the logits' arrival. 1000 rows of 151936, 608 MB: 98 us, 6.2 TB/s, where the
+/// best streaming read here has 6.9; read without the non-temporal hint (they fit no cache) 111 us. For
+/// few rows, a chain: the batches' round trips, then two barriers and a bisection to the bound, another round
+/// trip and the ranking. One row with 20 alternatives takes 8.2 us and 4.3 for the join (4.5 of the first
+/// without alternatives), 61 rows with 5 14.4 and 4.0 (10.1), 300 rows with 20 42 and 5 (36). Looking for
+/// candidates in every batch as it comes took 7.7, 16.3 and 59 us; knowing only the largest logit of
+/// each batch, and reading those that reach the bound whole, 7.4, 15.9 and 49; keeping two batches a
+/// lane instead of three, and so going through more parts again, 48 for the last.
+template <bool kOnce>
+__global__ __launch_bounds__(kBlock, kPerCu) void TokenLogprobsKernel(LogprobArgs a)
+{
+    __shared__ Sums waveSums[kWaves];
+    __shared__ TopSpace space;
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t row = blockIdx.x / a.parts;
+    const uint32_t part = blockIdx.x - row * a.parts;
+    const RowSpan s = SpanOf(a, row);
+    const uint32_t stride = a.parts * kWaves;
+
+    float4v v[kQuads];
+    uint32_t there = ~0u;  // a bit for each that is the row's (the others are -inf)
+    const uint32_t batches = (s.span + kBatch - 1) / kBatch;
+    const uint32_t firstBatch = part * kWaves + wave;
+    if (firstBatch < batches)
+    {
+        LoadBatch<kOnce>(s, firstBatch, lane, v, there);
+    }
+    const Given given = GivenOf(a, row);
+    const uint64_t ownKey = given.is ? OrderKey(given.logit, given.token) : ~0ull;
+    const bool plain = given.logit > -INFINITY;  // not -inf, not NaN
+    const float below = nextafterf(given.logit, -INFINITY);
+
+    Sums sums{-INFINITY, 0.0f, 0.0f, 0};
+    uint32_t above = 0;     // the wave's
+    LaneBatches own;
+    own.Clear();
+    uint32_t nth = 0;
+    for (uint32_t batch = firstBatch; batch < batches; batch += stride, ++nth)
+    {
+        float largest = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j)
+        {
+            largest = fmaxf(largest, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
+        }
+        if (largest > sums.m)
+        {
+            Rebase(sums, largest);
+        }
+        const float base = sums.m == -INFINITY ? 0.0f : sums.m;
+        {
+            float es[4] = {}, ts[4] = {};
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
+            {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                {
+                    const float y = (v[j][c] - base) * kLog2e;
+                    const float e = __builtin_amdgcn_exp2f(y);
+                    es[c] += e;
+                    ts[c] = fmaf(e, y, ts[c]);
+                }
+            }
+            float more = (ts[0] + ts[1]) + (ts[2] + ts[3]);
+            if (__any(more != more))
+            {
+                // 0 times the -inf of a masked logit. (NaN logits stay in s.)
+                more = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kQuads; ++j)
+                {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                    {
+                        const float y = (v[j][c] - base) * kLog2e;
+                        more = fmaf(__builtin_amdgcn_exp2f(y), fmaxf(y, -1e4f), more);
+                    }
+                }
+            }
+            sums.s += (es[0] + es[1]) + (es[2] + es[3]);
+            sums.t += more;
+        }
+
+        // Index of v[j][c]: begin + 256 j + 4 lane + c.
+        const int64_t begin = static_cast<int64_t>(batch) * kBatch - s.lead;
+        const bool after = begin > given.token;
+        const bool before = begin + kBatch <= given.token;
+        const bool single = given.is && !(plain && (after || before));
+        if (given.is && !single)
+        {
+            const float over = after ? given.logit : below;
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
+            {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                {
+                    above += CountLanes(v[j][c] > over);
+                }
+            }
+        }
+        if (a.top > 0)
+        {
+            own.Add(largest, nth);
+        }
+        const uint32_t is = there;
+        if (single)
+        {
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
+            {
+                space.staged[wave][j][lane] = v[j];
+            }
+        }
+        if (batch + stride < batches)
+        {
+            LoadBatch<kOnce>(s, batch + stride, lane, v, there);
+        }
+        if (single)
+        {
+            const uint32_t at = static_cast<uint32_t>(begin) + 4 * lane;
+#pragma unroll 1
+            for (int j = 0; j < kQuads; ++j)
+            {
+                const float4v x4 = space.staged[wave][j][lane];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                {
+                    const bool counts = (is >> (4 * j + c) & 1u) != 0 && OrderKey(x4[c], at + 256 * j + c) > ownKey;
+                    sums.above += counts ? 1u : 0u;
+                }
+            }
+        }
+    }
+
+    // Lanes, then waves.
+    Rebase(sums, GroupMax<kWave>(sums.m));
+    sums.s = GroupSum<kWave>(sums.s);
+    sums.t = GroupSum<kWave>(sums.t);
+#pragma unroll
+    for (int step = 1; step < kWave; step *= 2)
+    {
+        sums.above += __shfl_xor(sums.above, step);
+    }
+    sums.above += above;
+    if (lane == 0)
+    {
+        waveSums[wave] = sums;
+    }
+    __syncthreads();
     float most = waveSums[0].m;
 #pragma unroll
     for (int w = 1; w < kWaves; ++w)
@@ -560,13 +783,11 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
     }
     if (a.top > 0)
     {
-        __syncthreads();
-        RankKeys(waveKeys, keys, a.top, best, places);
-        __syncthreads();
+        TopOfPart(a, s, firstBatch, batches, stride, v, there, own, space);
     }
     if (a.parts == 1)
     {
-        WriteRow(a, row, all, given, best);
+        WriteRow(a, row, all, given, space.best);
         return;
     }
     if (threadIdx.x == 0)
@@ -575,7 +796,7 @@ __global__ __launch_bounds__(kBlock, 5) void TokenLogprobsKernel(LogprobArgs a)
     }
     for (uint32_t k = threadIdx.x; k < a.top; k += kBlock)
     {
-        a.keys[static_cast<uint64_t>(blockIdx.x) * a.top + k] = best[k];
+        a.keys[static_cast<uint64_t>(blockIdx.x) * a.top + k] = space.best[k];
     }
 }
 

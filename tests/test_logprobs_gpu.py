@@ -133,6 +133,34 @@ def test_equal_logits_go_by_index(mh, gpu, rows, vocab):
     check(run(mh, gpu, rising, [0, 0], 64), rising, [0, 0], 64)
 
 
+@pytest.mark.parametrize("rows", [1, 61, 300, 1100])
+def test_first_tokens_close_together_and_far_apart(mh, gpu, rows):
+    """The first tokens in a stretch that one thread or one wave reads, spread so that one thread's loads have
+    them all, and tied in numbers past any list of candidates."""
+    vocab = 151936
+    rng = np.random.default_rng(rows)
+    x = np.repeat(rng.normal(0, 1, (1, vocab)).astype(np.float32), rows, 0)
+    for row in range(rows):
+        kind = row % 6 if rows > 1 else 1
+        if kind == 0:
+            x[row, 70000:70064] += 20
+        elif kind == 1:
+            x[row, 5::1024] += 20                     # a lane of every wave
+        elif kind == 2:
+            x[row, 4096:5120] = 20                    # more equal ones than are ranked at once
+        elif kind == 3:
+            x[row, rng.integers(0, vocab, 3000)] = 20
+        elif kind == 4:
+            x[row, -40:] = 20 - np.arange(40) % 7
+        else:
+            x[row, 8192 + 3::16384] = 30 + np.arange(len(x[row, 8192 + 3::16384]))
+    tokens = rng.integers(0, vocab, rows)
+    tokens[0] = 70001
+    got = run(mh, gpu, x, tokens, 20)
+    some = np.unique(np.concatenate([np.arange(min(rows, 12)), rng.integers(0, rows, 12)]))
+    check({k: v[some] for k, v in got.items()}, x[some], tokens[some], 20)
+
+
 @pytest.mark.parametrize("vocab", [100, 9001, 151936])
 def test_masked_logits(mh, gpu, vocab):
     """-inf and the type's lowest value among the logits, a row with one token left, a row with none."""
