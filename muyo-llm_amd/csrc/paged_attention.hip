@@ -672,7 +672,8 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
         }
         // A wave without keys has nothing to add: its weight is 0, not that of -inf - -inf.
         const float factor = runMax == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - top);
-        float* const acc = reinterpret_cast<float*>(mine);  // [16 heads][kHd]
+        // [16 heads][kHd], 16-byte chunks permuted by the head: eight heads' writes go to different banks.
+        float* const acc = reinterpret_cast<float*>(mine);
         if (column < a.group)
         {
 #pragma unroll
@@ -680,7 +681,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             {
                 // NaN scores leave the maximum at -inf and NaN in the sums: they are kept.
                 const float4v x = runMax == -INFINITY && runSum == 0.0f ? float4v{} : o[c] * factor;
-                *reinterpret_cast<float4v*>(acc + column * kHd + 16 * c + 4 * quad) = x;
+                *reinterpret_cast<float4v*>(acc + column * kHd + 4 * ((4 * c + quad) ^ (column & 7u))) = x;
             }
         }
         __syncthreads();
@@ -698,7 +699,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
 #pragma unroll
             for (int w = 0; w < kWaves; ++w)
             {
-                num += *reinterpret_cast<const float4v*>(lds + w * kWaveBytes + 16 * i);
+                num += *reinterpret_cast<const float4v*>(lds + w * kWaveBytes + 16 * (i ^ (h & 7u)));
                 const float share = waveTotal[w][h];
                 den += waveMax[w][h] == -INFINITY ? share * 0.0f
                                                   : share * __builtin_amdgcn_exp2f(waveMax[w][h] - best);
