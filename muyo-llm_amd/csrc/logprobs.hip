@@ -271,190 +271,6 @@ struct TopSpace
     uint64_t candidates[kWaves][kWave];
 };
 
-/// The first a.top tokens of a part, for any number of logits that reach `floor`: wave by wave, batch by
-/// batch (from the wave's first, `stride` apart).
-///
-/// A wave's best so far lie in order across its lanes (lane i has the i-th). Few lanes of a batch reach the
-/// last of them: their logits are looked at lane by lane and inserted one by one. Otherwise a lower bound
-/// of the batch's own `top`-th is found first, by bisection: a value that the largest ones of `top` lanes
-/// reach. The candidates (a few more than `top`) are gathered, with the best so far, and ranked: a candidate's
-/// place is the number of those above it. More than 64 are inserted too. Equal logits are told apart by
-/// their index in the key, so nothing overflows. The batch goes through LDS: the registers are free for
-/// the next one at once, and loops over its logits need not be unrolled.
-__device__ __forceinline__ void TopByWaves(const LogprobArgs& a, const RowSpan& s, uint32_t batch, uint32_t batches,
-                                           uint32_t stride, uint32_t floorBits, TopSpace& space)
-{
-    const uint64_t floorKey = static_cast<uint64_t>(floorBits) << 32;
-    const uint32_t lane = threadIdx.x % kWave;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    float4v v[kQuads];
-    uint32_t there = 0;
-    uint64_t mine = 0;          // lane i: the i-th best so far
-    uint64_t least = floorKey;  // the last of the first `top`, or what they reach
-    auto lastOf = [&]() {
-        const uint64_t last = KeyOfLane(mine, a.top - 1);
-        return last > floorKey ? last : floorKey;
-    };
-    if (batch < batches)
-    {
-        LoadBatch<false>(s, batch, lane, v, there);
-    }
-    for (; batch < batches; batch += stride)
-    {
-        const uint32_t at0 = batch * kBatch - s.lead;  // index of v[j][c]: at0 + 256 j + 4 lane + c
-        const uint32_t is = there;
-        uint32_t high = 0;
-#pragma unroll
-        for (int j = 0; j < kQuads; ++j)
-        {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-            {
-                high = max(high, (is >> (4 * j + c) & 1u) != 0 ? OrderBits(v[j][c]) : 0u);
-            }
-        }
-        uint32_t floor = static_cast<uint32_t>(least >> 32);
-        const bool any = is != 0;
-        if (CountLanes(any && high >= floor) >= a.top)
-        {
-            floor = max(floor, LowerBound(high, 1, a.top));
-        }
-        uint64_t lanes = __ballot(any && high >= floor);
-        if (lanes != 0)
-        {
-#pragma unroll
-            for (int j = 0; j < kQuads; ++j)
-            {
-                space.staged[wave][j][lane] = v[j];
-            }
-        }
-        if (batch + stride < batches)
-        {
-            LoadBatch<false>(s, batch + stride, lane, v, there);
-        }
-        if (lanes == 0)
-        {
-            continue;
-        }
-        // The wave's LDS operations complete in order; the fences keep the compiler's order too.
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        uint32_t found = kWave + 1;
-        if (__popcll(lanes) > kFewLanes)
-        {
-            uint32_t take = 0;  // a bit for each of the lane's candidates
-#pragma unroll 1
-            for (int j = 0; j < kQuads; ++j)
-            {
-                const float4v x4 = space.staged[wave][j][lane];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                {
-                    take |= OrderBits(x4[c]) >= floor ? 1u << (4 * j + c) : 0u;
-                }
-            }
-            take &= is;
-            found = 0;
-            for (uint64_t mask = __ballot(take != 0); mask != 0; mask = __ballot(take != 0))
-            {
-                const uint32_t place =
-                    found + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
-                                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
-                if (take != 0 && place < kWave)
-                {
-                    const uint32_t e = static_cast<uint32_t>(__ffs(static_cast<int>(take)) - 1);
-                    space.candidates[wave][place] = OrderKey(space.staged[wave][e / 4][lane][e % 4],
-                                                             at0 + 256 * (e / 4) + 4 * lane + e % 4);
-                }
-                take &= take - 1;
-                found += static_cast<uint32_t>(__popcll(mask));
-            }
-            const uint32_t kept = min(CountLanes(mine != 0), a.top);
-            if (found + kept <= kWave && lane < kept)
-            {
-                space.candidates[wave][found + lane] = mine;
-            }
-            found += kept;
-        }
-        if (found <= kWave)
-        {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            const uint64_t key = lane < found ? space.candidates[wave][lane] : 0;
-            mine = key;
-            if (batch + stride >= batches)
-            {
-                continue;  // the workgroup ranks them
-            }
-            uint32_t place = 0;
-#pragma unroll 4
-            for (uint32_t i = 0; i < found; ++i)
-            {
-                place += KeyOfLane(key, i) > key ? 1u : 0u;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if (lane < found)
-            {
-                space.candidates[wave][place] = key;
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            mine = lane < found ? space.candidates[wave][lane] : 0;
-            least = lastOf();
-        }
-        else
-        {
-            // Lane l looks at the l-th of their values.
-            while (lanes != 0)
-            {
-                const uint32_t from = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(lanes)) - 1);
-                lanes &= lanes - 1;
-                const uint32_t j = lane / 4 % kQuads;
-                const float value = space.staged[wave][j][from][lane % 4];
-                const uint32_t theirs = __builtin_amdgcn_readlane(is, from);
-                const uint64_t key = OrderKey(value, at0 + 256 * j + 4 * from + lane % 4);
-                const bool take = lane < 4 * kQuads && (theirs >> lane & 1u) != 0 &&
-                                  static_cast<uint32_t>(key >> 32) >= floor;
-                uint64_t mask = __ballot(take && key > least);
-                while (mask != 0)
-                {
-                    const uint64_t one =
-                        KeyOfLane(key, static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(mask)) - 1));
-                    const uint32_t place = CountLanes(mine > one);
-                    const uint64_t left = KeyOfLaneBefore(mine);
-                    mine = lane < place ? mine : lane == place ? one : left;
-                    least = lastOf();
-                    mask &= mask - 1;
-                    mask &= __ballot(key > least);
-                }
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    }
-
-    const uint32_t held = CountLanes(mine != 0);
-    if (lane == 0)
-    {
-        space.waveHeld[wave] = held;
-    }
-    __syncthreads();
-    uint32_t keys = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w)
-    {
-        if (w == wave && lane < held)
-        {
-            space.keys[keys + lane] = mine;  // none of them is 0, and they come first
-        }
-        keys += space.waveHeld[w];
-    }
-    __syncthreads();
-    RankKeys(space.keys, keys, a.top, space.best, space.places);
-    __syncthreads();
-}
-
 /// A lane's batches with its largest logits: the largest of each, in falling order, and which of the wave's
 /// batches it is. Of the others only the largest logit is kept.
 struct LaneBatches
@@ -506,6 +322,227 @@ struct LaneBatches
     }
 };
 
+/// The first a.top tokens of a part, for any number of logits that reach `floor`: wave by wave, batch by
+/// batch (from the wave's first, `stride` apart).
+///
+/// A wave's best so far lie in order across its lanes (lane i has the i-th). Few lanes of a batch reach the
+/// last of them: their logits are looked at lane by lane and inserted one by one. Otherwise a lower bound
+/// of the batch's own `top`-th is found first, by bisection: a value that the largest ones of `top` lanes
+/// reach. The candidates (a few more than `top`) are gathered, with the best so far, and ranked: a candidate's
+/// place is the number of those above it. More than 64 are inserted too. Equal logits are told apart by
+/// their index in the key, so nothing overflows. The batch goes through LDS: the registers are free for
+/// the next one at once, and loops over its logits need not be unrolled. Batches that no lane knows to
+/// reach the last are left out: of a row with few logits above -inf, or of equal ones, most (300 rows with ten
+/// above -inf and 20 alternatives: 67 us, 202 through all batches, where ordinary rows take 42).
+__device__ __forceinline__ void TopByWaves(const LogprobArgs& a, const RowSpan& s, uint32_t firstBatch,
+                                           uint32_t batches, uint32_t stride, uint32_t floorBits,
+                                           const LaneBatches& own, TopSpace& space)
+{
+    const uint64_t floorKey = static_cast<uint64_t>(floorBits) << 32;
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    float4v v[kQuads];
+    uint32_t there = 0;
+    uint64_t mine = 0;          // lane i: the i-th best so far
+    uint64_t least = floorKey;  // the last of the first `top`, or what they reach
+    auto lastOf = [&]() {
+        const uint64_t last = KeyOfLane(mine, a.top - 1);
+        return last > floorKey ? last : floorKey;
+    };
+    // What counts in a batch: the last's value too while it is a bound, and more than the last's once that is one of
+    // the wave's own, as the batches rise in index.
+    auto floorOf = [&]() { return static_cast<uint32_t>(least >> 32) + (static_cast<uint32_t>(least) != 0 ? 1u : 0u); };
+    uint32_t most[kKept + 1];
+#pragma unroll
+    for (int i = 0; i <= kKept; ++i)
+    {
+        most[i] = OrderBits(own.most[i]);
+    }
+    const uint32_t count = firstBatch < batches ? (batches - 1 - firstBatch) / stride + 1 : 0;
+    auto after = [&](uint32_t nth) {
+        const uint32_t floor = floorOf();
+        while (++nth < count)
+        {
+            bool reaches = most[kKept] >= floor;
+#pragma unroll
+            for (int i = 0; i < kKept; ++i)
+            {
+                reaches = reaches || (own.nth[i] == nth && most[i] >= floor);
+            }
+            if (__any(reaches))
+            {
+                break;
+            }
+        }
+        return nth;
+    };
+    if (count != 0)
+    {
+        LoadBatch<false>(s, firstBatch, lane, v, there);
+    }
+    uint32_t following;
+    for (uint32_t nth = 0; nth < count; nth = following)
+    {
+        const uint32_t batch = firstBatch + nth * stride;
+        const uint32_t at0 = batch * kBatch - s.lead;  // index of v[j][c]: at0 + 256 j + 4 lane + c
+        const uint32_t is = there;
+        uint32_t high = 0;
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j)
+        {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+            {
+                high = max(high, (is >> (4 * j + c) & 1u) != 0 ? OrderBits(v[j][c]) : 0u);
+            }
+        }
+        uint32_t floor = floorOf();
+        const bool any = is != 0;
+        if (CountLanes(any && high >= floor) >= a.top)
+        {
+            floor = max(floor, LowerBound(high, 1, a.top));
+        }
+        uint64_t lanes = __ballot(any && high >= floor);
+        if (lanes != 0)
+        {
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
+            {
+                space.staged[wave][j][lane] = v[j];
+            }
+        }
+        following = after(nth);
+        if (following < count)
+        {
+            LoadBatch<false>(s, firstBatch + following * stride, lane, v, there);
+        }
+        if (lanes == 0)
+        {
+            continue;
+        }
+        // The wave's LDS operations complete in order; the fences keep the compiler's order too.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        uint32_t found = kWave + 1;
+        if (__popcll(lanes) > kFewLanes)
+        {
+            uint32_t take = 0;  // a bit for each of the lane's candidates
+#pragma unroll 1
+            for (int j = 0; j < kQuads; ++j)
+            {
+                const float4v x4 = space.staged[wave][j][lane];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                {
+                    take |= OrderBits(x4[c]) >= floor ? 1u << (4 * j + c) : 0u;
+                }
+            }
+            take &= is;
+            found = 0;
+            for (uint64_t mask = __ballot(take != 0); mask != 0; mask = __ballot(take != 0))
+            {
+                const uint32_t place =
+                    found + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+                if (take != 0 && place < kWave)
+                {
+                    const uint32_t e = static_cast<uint32_t>(__ffs(static_cast<int>(take)) - 1);
+                    space.candidates[wave][place] = OrderKey(space.staged[wave][e / 4][lane][e % 4],
+                                                             at0 + 256 * (e / 4) + 4 * lane + e % 4);
+                }
+                take &= take - 1;
+                found += static_cast<uint32_t>(__popcll(mask));
+            }
+            const uint32_t kept = min(CountLanes(mine != 0), a.top);
+            if (found + kept <= kWave && lane < kept)
+            {
+                space.candidates[wave][found + lane] = mine;
+            }
+            found += kept;
+        }
+        if (found <= kWave)
+        {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const uint64_t key = lane < found ? space.candidates[wave][lane] : 0;
+            mine = key;
+            if (following >= count)
+            {
+                continue;  // the workgroup ranks them
+            }
+            uint32_t place = 0;
+#pragma unroll 4
+            for (uint32_t i = 0; i < found; ++i)
+            {
+                place += KeyOfLane(key, i) > key ? 1u : 0u;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (lane < found)
+            {
+                space.candidates[wave][place] = key;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            mine = lane < found ? space.candidates[wave][lane] : 0;
+            least = lastOf();
+        }
+        else
+        {
+            // Lane l looks at the l-th of their values. `best` is above any of its own's keys.
+            const uint32_t index = at0 + 4 * lane;
+            const uint64_t best =
+                (static_cast<uint64_t>(high) << 32) | ~(static_cast<int32_t>(index) < 0 ? 0u : index);
+            while (lanes != 0)
+            {
+                const uint32_t from = static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(lanes)) - 1);
+                lanes &= lanes - 1;
+                const uint32_t j = lane / 4 % kQuads;
+                const float value = space.staged[wave][j][from][lane % 4];
+                const uint32_t theirs = __builtin_amdgcn_readlane(is, from);
+                const uint64_t key = OrderKey(value, at0 + 256 * j + 4 * from + lane % 4);
+                const bool take = lane < 4 * kQuads && (theirs >> lane & 1u) != 0 &&
+                                  static_cast<uint32_t>(key >> 32) >= floor;
+                uint64_t mask = __ballot(take && key > least);
+                while (mask != 0)
+                {
+                    const uint64_t one =
+                        KeyOfLane(key, static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(mask)) - 1));
+                    const uint32_t place = CountLanes(mine > one);
+                    const uint64_t left = KeyOfLaneBefore(mine);
+                    mine = lane < place ? mine : lane == place ? one : left;
+                    least = lastOf();
+                    mask &= mask - 1;
+                    mask &= __ballot(key > least);
+                }
+                lanes &= __ballot(best > least);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    const uint32_t held = CountLanes(mine != 0);
+    if (lane == 0)
+    {
+        space.waveHeld[wave] = held;
+    }
+    __syncthreads();
+    uint32_t keys = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w)
+    {
+        if (w == wave && lane < held)
+        {
+            space.keys[keys + lane] = mine;  // none of them is 0, and they come first
+        }
+        keys += space.waveHeld[w];
+    }
+    __syncthreads();
+    RankKeys(space.keys, keys, a.top, space.best, space.places);
+    __syncthreads();
+}
+
 /// The first a.top tokens of a workgroup's part into space.best, in order (0 behind the last).
 ///
 /// The a.top-th of the 256 threads' largest logits is a lower bound of the part's a.top-th. Threads look again
@@ -514,7 +551,7 @@ struct LaneBatches
 /// such batches than it knows, or there are more than 256 such logits, or fewer threads than a.top have any)
 /// the waves go through the part once more.
 __device__ __forceinline__ void TopOfPart(const LogprobArgs& a, const RowSpan& s, uint32_t firstBatch, uint32_t batches,
-                                          uint32_t stride, float4v (&v)[kQuads], uint32_t there, LaneBatches& own,
+                                          uint32_t stride, float4v (&v)[kQuads], uint32_t there, const LaneBatches& own,
                                           TopSpace& space)
 {
     const uint32_t lane = threadIdx.x % kWave;
@@ -553,15 +590,16 @@ __device__ __forceinline__ void TopOfPart(const LogprobArgs& a, const RowSpan& s
     else
     {
         uint32_t held = (batches - 1 - firstBatch) / stride;
-        while (OrderBits(own.most[0]) >= floor)
+        LaneBatches left = own;
+        while (OrderBits(left.most[0]) >= floor)
         {
-            const uint32_t batch = firstBatch + own.nth[0] * stride;
-            if (own.nth[0] != held)
+            const uint32_t batch = firstBatch + left.nth[0] * stride;
+            if (left.nth[0] != held)
             {
                 LoadBatch<false>(s, batch, lane, v, there);
             }
             held = ~0u;
-            own.Drop();
+            left.Drop();
             uint32_t take = there;
 #pragma unroll
             for (int j = 0; j < kQuads; ++j)
@@ -601,7 +639,7 @@ __device__ __forceinline__ void TopOfPart(const LogprobArgs& a, const RowSpan& s
         __syncthreads();
         return;
     }
-    TopByWaves(a, s, firstBatch, batches, stride, floor, space);
+    TopByWaves(a, s, firstBatch, batches, stride, floor, own, space);
 }
 
 /// One pass over the row: a wave takes batches of kBatch logits into registers, and each lane keeps the sums

@@ -161,6 +161,26 @@ def test_first_tokens_close_together_and_far_apart(mh, gpu, rows):
     check({k: v[some] for k, v in got.items()}, x[some], tokens[some], 20)
 
 
+@pytest.mark.parametrize("rows, vocab, top", [(1, 151936, 20), (61, 152064, 5), (300, 151936, 20), (1100, 40000, 64)])
+def test_few_tokens_left_by_a_mask(mh, gpu, rows, vocab, top):
+    """Ten tokens allowed, anywhere or in one stretch, the others -inf or the lowest value; and logits rounded to
+    8 bits, with their ties."""
+    rng = np.random.default_rng(rows + top)
+    x = rng.normal(0, 3, (rows, vocab)).astype(np.float32)
+    bits = x[::4].view(np.uint32)
+    x[::4] = ((bits + 0x8000) & 0xFFFF0000).view(np.float32)
+    for row in range(rows):
+        if row % 4 != 0:
+            at = rng.integers(0, vocab, 10) if row % 2 else 5000 + np.arange(10)
+            keep = x[row, at]
+            x[row] = -np.inf if row % 4 != 3 else np.finfo(np.float32).min
+            x[row, at] = keep
+    tokens = rng.integers(0, vocab, rows)
+    got = run(mh, gpu, x, tokens, top)
+    some = np.unique(np.concatenate([np.arange(min(rows, 12)), rng.integers(0, rows, 12)]))
+    check({k: v[some] for k, v in got.items()}, x[some], tokens[some], top)
+
+
 @pytest.mark.parametrize("vocab", [100, 9001, 151936])
 def test_masked_logits(mh, gpu, vocab):
     """-inf and the type's lowest value among the logits, a row with one token left, a row with none."""
