@@ -620,11 +620,12 @@ int muyo_paged_rope_append_f16kv(const float* q, const float* k, const float* v,
  * the sequence in row query_sequence[i] of tables, sees keys j <= positions[i], the last `window` of them
  * where window > 0. For every head h (kv head h / (heads / kv_heads)):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h].k[j]) * v[j]
- * q and out are f32 [queries][heads * head_dim], and may be the same. A query without keys (a position
- * below 0) gives 0. A query whose sequence is outside 0..sequences - 1 is padding: its row of out stays
- * as it was. Keys past table_pages * page_size, or in pages with an id outside the cache, are left out.
- * Queries may share a sequence (several new tokens of one). Which keys a workgroup takes depends on the
- * whole batch, so a query's last bits may too; the same call gives the same bits.
+ * q and out are f32 [queries][heads * head_dim], and may be the same; out overlaps
+ * nothing else. A query without keys (a position below 0) gives 0. A query whose sequence is outside
+ * 0..sequences - 1 is padding: its row of out stays as it was. Keys past table_pages * page_size, or
+ * in pages with an id outside the cache, are left out. Queries may share a sequence (several new tokens
+ * of one). Which keys a workgroup takes depends on the whole batch, so a query's last bits may too; the
+ * same call gives the same bits.
  * K and V rows that a query sees are finite; the others may hold anything.
  * head_dim 64 or 128, at most 16 heads per kv head, 1024 heads, 65535 queries, scale finite.
  * `workspace` is caller-owned device memory (16-byte aligned) of at least

@@ -484,21 +484,6 @@ int Launched(hipError_t status, const char* name)
 {
     return status == hipSuccess ? MUYO_OK : HipStatus(status, name);
 }
-
-/// One buffer of a call, for the overlap check.
-struct Range
-{
-    const void* at;
-    uint64_t bytes;
-    const char* name;
-};
-
-bool Overlap(const Range& a, const Range& b)
-{
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at);
-    const uintptr_t y = reinterpret_cast<uintptr_t>(b.at);
-    return x < y + b.bytes && y < x + a.bytes;
-}
 }  // namespace
 
 int CheckPages(const char* name, uint32_t pages, uint32_t pageSize)

@@ -11,4 +11,19 @@ constexpr uint32_t kMaxPageSize = 1024;
 /// MUYO_OK for a power-of-two page size in kMinPageSize..kMaxPageSize and fewer than 2^31 slots,
 /// else the failure's status.
 int CheckPages(const char* name, uint32_t pages, uint32_t pageSize);
+
+/// One buffer of a call, for the overlap check.
+struct Range
+{
+    const void* at;
+    uint64_t bytes;
+    const char* name;
+};
+
+inline bool Overlap(const Range& a, const Range& b)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at);
+    const uintptr_t y = reinterpret_cast<uintptr_t>(b.at);
+    return x < y + b.bytes && y < x + a.bytes;
+}
 }  // namespace muyo

@@ -952,6 +952,21 @@ extern "C" int muyo_paged_attention_decode_f16kv(const float* q, const void* kca
         return Fail(MUYO_E_CONTRACT, "%s: needs a 16-byte aligned workspace of %zu bytes (got %llu)", name, need,
                     static_cast<unsigned long long>(workspace_bytes));
     }
+    const Range output{out, 4ull * queries * heads * head_dim, "out"};
+    const uint64_t cacheBytes = 2ull * pages * page_size * kv_heads * head_dim;
+    const Range inputs[] = {{q, output.bytes, "q"},
+                            {kcache, cacheBytes, "kcache"},
+                            {vcache, cacheBytes, "vcache"},
+                            {workspace, need, "workspace"}};
+    for (const Range& r : inputs)
+    {
+        // In place a workgroup has read its (query, kv head)'s q when it writes its output there, and one that
+        // is cut is written by the join.
+        if (!(&r == inputs && q == out) && Overlap(output, r))
+        {
+            return Fail(MUYO_E_CONTRACT, "%s: out overlaps %s", name, r.name);
+        }
+    }
     PagedAttentionArgs a{q,
                          static_cast<const uint16_t*>(kcache),
                          static_cast<const uint16_t*>(vcache),

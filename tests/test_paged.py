@@ -94,6 +94,10 @@ REFUSALS = [
     ("paged_attention_decode_f16kv", ATTEND, dict(workspace=None), "MUYO_E_CONTRACT"),
     ("paged_attention_decode_f16kv", ATTEND, dict(workspace=ctypes.c_void_p(8)), "MUYO_E_CONTRACT"),
     ("paged_attention_decode_f16kv", ATTEND, dict(workspace_bytes=15), "MUYO_E_CONTRACT"),
+    ("paged_attention_decode_f16kv", ATTEND, dict(out=ctypes.c_void_p(ATTEND["q"].value + 3584)), "MUYO_E_CONTRACT"),
+    ("paged_attention_decode_f16kv", ATTEND, dict(out=ATTEND["kcache"]), "MUYO_E_CONTRACT"),
+    ("paged_attention_decode_f16kv", ATTEND, dict(out=ATTEND["vcache"]), "MUYO_E_CONTRACT"),
+    ("paged_attention_decode_f16kv", ATTEND, dict(out=ATTEND["workspace"]), "MUYO_E_CONTRACT"),
     ("token_logprobs_f32", LOGPROBS, dict(logits=None), "MUYO_E_NULL"),
     ("token_logprobs_f32", LOGPROBS, dict(tokens=None), "MUYO_E_NULL"),
     ("token_logprobs_f32", LOGPROBS, dict(top_ids=None), "MUYO_E_NULL"),
