@@ -26,6 +26,11 @@ constexpr uint32_t kWholeKeys = 1024;
 constexpr uint32_t kMinShare = kWaves;    // a share is at least a tile a wave
 constexpr uint32_t kSetupTiles = 8;       // what a share's change to another (query, kv head) costs, in tiles
 constexpr uint32_t kSplitBlocks = 512;    // workgroups of a split launch: two on each of 256 CUs
+// Softmax weights are held in two planes of f16, which ends at 2^16: the weight of the maximum is 2^kWeightBias, and
+// 2^15 when a later one has run kLag binary orders ahead.
+constexpr float kLag = 4.0f;
+constexpr float kWeightBias = 15.0f - kLag;
+constexpr float kLowScale = 2048.0f;      // of the low plane: what 11 bits of the high one leave, in f16's range again
 
 /// *p for a p that is the same in the whole wave, of memory that nothing writes while the kernel runs: a
 /// scalar load. (Through a vector register the wait for it would also be one for every load before it:
@@ -210,8 +215,16 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// f16 products are exact in f32 and the sums are f32 throughout; the planes keep what one f16 operand
 /// would lose (1e-4 of the result).
 ///
-/// Weights are relative to `shift`, which follows the maximum only once that is 2^8 past it: rescaling
-/// the accumulators is rare. Only tiles that reach over an end of the key range, or into a page that is
+/// Weights are relative to `shift`, which follows the maximum only once that is 2^kLag past it: rescaling
+/// the accumulators is rare. Where one key has most of the weight and a small value row, the result is that of
+/// the small weights, so these need their bits too: f16 has 11 down to 2^-14, and the low plane, times
+/// kLowScale in accumulators of its own, the next 11. A weight keeps 22 bits down to 2^-25 of the largest
+/// (17 nats), and 2^-47 of the largest below. (With a key 20 nats above the others and a value row of 0, both planes
+/// in the same accumulators lose 3e-4 of the result, and a third of it with weights of at most 1.) The
+/// accumulators cost no time for long caches (64 sequences of 1 to 16384 keys 167.5 us, without 167.3) and
+/// 0.1 us for short ones.
+///
+/// Only tiles that reach over an end of the key range, or into a page that is
 /// not there, are masked: their scores to -inf, and their V rows to 0, since 0 * NaN would be NaN.
 ///
 /// kSplit: the tiles of all queries and kv heads in a row, each with its setup's cost before it, are dealt
@@ -459,11 +472,12 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             __builtin_amdgcn_sched_barrier(0);
         };
 
-        float4v o[kChannels];
+        float4v o[kChannels], oLow[kChannels];  // from the weights' planes; oLow times kLowScale
 #pragma unroll
         for (int c = 0; c < kChannels; ++c)
         {
             o[c] = float4v{};
+            oLow[c] = float4v{};
         }
         float runMax = -INFINITY;  // of the raw scores
         float shift = 0.0f;        // in log2 units
@@ -601,7 +615,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             tileMax = fmaxf(tileMax, PartnerLane<16>(tileMax));
             tileMax = fmaxf(tileMax, PartnerLane<32>(tileMax));
             const float top = tileMax * scaleLog2;
-            const bool rises = tileMax != -INFINITY && (runMax == -INFINITY || top > shift + 8.0f);
+            const bool rises = tileMax != -INFINITY && (runMax == -INFINITY || top > shift + kLag);
             if (__any(rises))
             {
                 const float newShift = rises ? top : shift;
@@ -614,6 +628,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                 for (int c = 0; c < kChannels; ++c)
                 {
                     o[c] *= factor;
+                    oLow[c] *= factor;
                 }
             }
             half8 phi[kHalves / 2], plo[kHalves / 2];
@@ -625,10 +640,10 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                 {
-                    p[r] = __builtin_amdgcn_exp2f(fmaf(score[half][r], scaleLog2, -shift));
+                    p[r] = __builtin_amdgcn_exp2f(fmaf(score[half][r], scaleLog2, kWeightBias - shift));
                     const _Float16 hi = static_cast<_Float16>(p[r]);
                     phi[half / 2][4 * (half % 2) + r] = hi;
-                    plo[half / 2][4 * (half % 2) + r] = static_cast<_Float16>(p[r] - static_cast<float>(hi));
+                    plo[half / 2][4 * (half % 2) + r] = static_cast<_Float16>(kLowScale * (p[r] - static_cast<float>(hi)));
                 }
                 sum += (p[0] + p[1]) + (p[2] + p[3]);
             }
@@ -647,7 +662,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                         half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                    (__attribute__((address_space(3))) short4v*)(from + 16 * 2 * kHd)));
                     const half8 vt = __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, plo[pair], o[c], 0, 0, 0);
+                    oLow[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, plo[pair], oLow[c], 0, 0, 0);
                     o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, phi[pair], o[c], 0, 0, 0);
                 }
             }
@@ -680,7 +695,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             for (int c = 0; c < kChannels; ++c)
             {
                 // NaN scores leave the maximum at -inf and NaN in the sums: they are kept.
-                const float4v x = runMax == -INFINITY && runSum == 0.0f ? float4v{} : o[c] * factor;
+                const float4v x = runMax == -INFINITY && runSum == 0.0f ? float4v{} : (o[c] + oLow[c] * (1.0f / kLowScale)) * factor;
                 *reinterpret_cast<float4v*>(acc + column * kHd + 4 * ((4 * c + quad) ^ (column & 7u))) = x;
             }
         }

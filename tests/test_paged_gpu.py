@@ -731,3 +731,52 @@ def test_a_steps_operators_in_one_graph(mh, gpu):
         assert np.array_equal(host(best_ids), order[:, :top])
         assert np.array_equal(host(ranks), np.argsort(order, 1)[np.arange(n + 1), tokens])
     assert lengths.tolist() == [20, 35, 36, 60, 119]
+
+
+def with_sinks(batch, rng, nats, value, last=False):
+    """Key 0 (or the last one) of each sequence scores `nats[i]` for every head of its query i, the others as
+    they were, a standard deviation of 2 about 0; its value row is `value` times one of theirs."""
+    heads, kv, hd, size = batch.shape
+    for i, (b, p) in enumerate(zip(batch.sequence, batch.positions)):
+        key = int(p) if last else 0
+        at = batch.tables[b, key // size], slice(None), key % size
+        for g, q in enumerate(batch.q[i].astype(np.float64).reshape(kv, heads // kv, hd)):
+            batch.caches[0][at][g] = np.linalg.pinv(q) @ np.full(heads // kv, nats[i] / batch.scale)
+        batch.caches[1][at] = rng.normal(0, value, (kv, hd))
+
+
+SINKS = [
+    # heads, kv_heads, head_dim, page_size, keys: whole, cut, and (300 queries) several to a workgroup
+    (14, 2, 64, 16, [302] * 8),
+    (28, 4, 128, 16, [300, 1000] * 4),
+    (14, 2, 64, 64, [16384] * 8),
+    (28, 4, 128, 64, [16384, 4096] * 4),
+    (14, 2, 64, 16, [1500] * 300),
+    (4, 4, 128, 16, [1100] * 300),
+    (16, 1, 128, 32, [5000] * 4),
+]
+
+
+@pytest.mark.parametrize("value, last, spread", [(0.0, False, 1.0), (0.0, False, 0.1), (0.01, False, 1.0),
+                                                 (0.01, False, 0.1), (1.0, False, 1.0), (0.0, True, 1.0)])
+@pytest.mark.parametrize("heads, kv, hd, size, keys", SINKS, ids=["-".join(map(str, (*s[:4], s[4][0], len(s[4]))))
+                                                                 for s in SINKS])
+def test_attention_with_a_key_that_has_most_of_the_weight(mh, gpu, heads, kv, hd, size, keys, value, last,
+                                                          spread):
+    """One key 8 to 20 nats above the mean of the others, which differ much or little, with a value row that is 0,
+    small or ordinary: the output is that of the many small weights. A score of S is off by some 4 u S, as
+    above, where 10 was taken for S; a sink's own S is larger, and its error is one of the sum of weights."""
+    rng = np.random.default_rng(hd + len(keys) + keys[0])
+    nats = np.resize(np.array([20.0, 8.0, 17.0, 14.0, 12.0, 0.0]), len(keys))
+    batch = Attend(mh, gpu, rng, heads, kv, hd, size, np.array(keys) - 1)
+    batch.caches[0] *= np.float16(spread)
+    with_sinks(batch, rng, nats, value, last)
+    out = batch.call()
+    gpu.cuda.synchronize()
+    got, some = host(out), np.unique(np.concatenate([np.arange(8) % len(keys), rng.integers(0, len(keys), 16)]))
+    worst = 0.0
+    for i in some:
+        want = attend64(batch.q[i], *batch.caches, batch.tables[batch.sequence[i]], keys[i] - 1, 0, batch.scale)
+        off = np.linalg.norm(got[i] - want) / np.linalg.norm(want)
+        worst = max(worst, off / max(1.0, nats[i] / 10))
+    assert worst <= ATTENTION_RTOL, worst
