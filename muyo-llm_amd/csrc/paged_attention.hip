@@ -204,8 +204,8 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// (v_mfma_f32_16x16x32_f16: D = A.B with lane l supplying A[l % 16][8 (l / 16) .. +8] and
 /// B[8 (l / 16) .. +8][l % 16], receiving D[4 (l / 16) + r][l % 16]). Per tile a wave
 ///   - takes K rows straight from memory as A operands (of 16 keys each) and forms S^T (keys x heads) =
-///     K . q^T, q in registers as two planes of f16 (hi + lo: 22 bits, of q over its largest value's
-///     power of two);
+///     K . q^T, q in registers as two planes of f16 (hi + lo, of q times the power of two that takes the head's
+///     largest value to 2^13 .. 2^14: 22 bits down to 2^-17 of that value, and 2^-39 of it below);
 ///   - passes the V rows through its own part of LDS, to read them back transposed
 ///     (ds_read_b64_tr_b16: 16 lanes give 4 rows of 16 channels, each gets a channel of 4 rows);
 ///   - requests the next tile's K and V into the registers that are now free;
@@ -487,8 +487,8 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
         request(min(tile0 + wave, tile1 - 1), pagesOf(min(tile0 + wave, tile1 - 1)));
         Pages next = pagesOf(min(tile0 + wave + kWaves, tile1 - 1));  // of the next tile to request
 
-        // The group's heads as columns; columns past it are 0. Planes of q / 2^e with 2^e above the head's
-        // largest value: f16 then holds any q.
+        // The group's heads as columns; columns past it are 0. Planes of q / 2^e, whose largest value is below 2^14:
+        // f16 then holds any q, and its small values with their bits where K makes them count.
         half8 qhi[kSteps], qlo[kSteps];
         float scaleLog2;
         {
@@ -509,6 +509,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             {
                 (void)frexpf(largest, &e);
             }
+            e -= 14;
             // A negative scale turns q's sign, and 0 clears q, so that scores are scaled by a positive number.
             const float sign = column >= a.group || a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
             scaleLog2 = a.scale == 0.0f ? 1.0f : fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e), 0x1p-126f);
@@ -519,9 +520,8 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                 for (int c = 0; c < 8; ++c)
                 {
                     const float x = column >= a.group ? 0.0f : ldexpf(qv[s][c / 4][c % 4], -e) * sign;
-                    const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);  // 11 bits: exact in f16
-                    qhi[s][c] = static_cast<_Float16>(hi);
-                    qlo[s][c] = static_cast<_Float16>(x - hi);
+                    qhi[s][c] = static_cast<_Float16>(x);
+                    qlo[s][c] = static_cast<_Float16>(x - static_cast<float>(qhi[s][c]));
                 }
             }
         }

@@ -780,3 +780,16 @@ def test_attention_with_a_key_that_has_most_of_the_weight(mh, gpu, heads, kv, hd
         off = np.linalg.norm(got[i] - want) / np.linalg.norm(want)
         worst = max(worst, off / max(1.0, nats[i] / 10))
     assert worst <= ATTENTION_RTOL, worst
+
+
+@pytest.mark.parametrize("heads, kv, hd, positions", [(14, 2, 64, [0, 40, 300]), (28, 4, 128, [700, 1000]),
+                                                      (14, 2, 64, [5000, 7]), (28, 4, 128, [3000, 16383])])
+@pytest.mark.parametrize("ratio", [300.0, 1e4, 1e5])
+def test_attention_with_one_large_component_of_q(mh, gpu, heads, kv, hd, positions, ratio):
+    """A component of q far above the others meets a component of K that is 0: the scores are those of the others,
+    with their own roundings."""
+    rng = np.random.default_rng(hd)
+    batch = Attend(mh, gpu, rng, heads, kv, hd, 16, np.array(positions))
+    batch.q[..., 5] *= ratio
+    batch.caches[0][..., 5] = 0
+    batch.check()
