@@ -64,7 +64,7 @@ struct PagedAttentionArgs
     uint32_t* costSums;  // [queries + 1]: CostOf of one kv head of the queries before
     uint4* cuts;         // what to join: query, kv head, first share, pieces (0: nothing)
     uint32_t cutsByUnit; // cuts has an entry per (query, kv head); else one per share
-    float* partials;     // [2 * shares][group][4 + headDim]: max (log2 units), sum, -, -, weighted values
+    float* partials;     // [2 * shares][group][4 + headDim]: base, sum, a score's log2 units, -, weighted values
 };
 
 /// The keys begin..end - 1 that a query sees, and the tiles they lie in. A query without any has one
@@ -215,8 +215,10 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// f16 products are exact in f32 and the sums are f32 throughout; the planes keep what one f16 operand
 /// would lose (1e-4 of the result).
 ///
-/// Weights are relative to `shift`, which follows the maximum only once that is 2^kLag past it: rescaling
-/// the accumulators is rare. Where one key has most of the weight and a small value row, the result is that of
+/// Weights are relative to `base`, a raw score that follows the maximum only once that is 2^kLag past it: rescaling
+/// the accumulators is rare. They are made of differences of raw scores, in the joins too, so that those of scaled
+/// scores of any size are 1 where scores are equal (scaled scores past 2^29 are rounded by more than f16 holds, and
+/// weights of them were infinite or 0). Where one key has most of the weight and a small value row, the result is that of
 /// the small weights, so these need their bits too: f16 has 11 down to 2^-14, and the low plane, times
 /// kLowScale in accumulators of its own, the next 11. A weight keeps 22 bits down to 2^-25 of the largest
 /// (17 nats), and 2^-47 of the largest below. (With a key 20 nats above the others and a value row of 0, both planes
@@ -252,8 +254,9 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
     constexpr uint32_t kWaveBytes = kTile * 2 * kHd;  // V of a tile; later O^T of 16 heads in f32
     static_assert(kWaveBytes >= kMaxGroup * kHd * 4, "O^T fits where V was");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaves * kWaveBytes];
-    __shared__ float waveMax[kWaves][kMaxGroup];
+    __shared__ float waveBase[kWaves][kMaxGroup];
     __shared__ float waveTotal[kWaves][kMaxGroup];
+    __shared__ float headScale[kMaxGroup];  // scaleLog2
     __shared__ uint32_t waveSum[kWaves];
     __shared__ KeyRange firstRange;
     __shared__ uint32_t firstAt[2];  // the share's first query, and the costs before it
@@ -479,9 +482,8 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             o[c] = float4v{};
             oLow[c] = float4v{};
         }
-        float runMax = -INFINITY;  // of the raw scores
-        float shift = 0.0f;        // in log2 units
-        float runSum = 0.0f;       // of this lane's keys
+        float base = -INFINITY;  // the raw score that weights are relative to; -inf: none yet
+        float runSum = 0.0f;     // of this lane's keys
         // A wave without a tile requests the last one and leaves it: a request under a condition would make
         // the wait for q one for everything.
         request(min(tile0 + wave, tile1 - 1), pagesOf(min(tile0 + wave, tile1 - 1)));
@@ -512,7 +514,9 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             e -= 14;
             // A negative scale turns q's sign, and 0 clears q, so that scores are scaled by a positive number.
             const float sign = column >= a.group || a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
-            scaleLog2 = a.scale == 0.0f ? 1.0f : fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e), 0x1p-126f);
+            // Finite and above 0: no difference of raw scores makes a NaN of it.
+            scaleLog2 = a.scale == 0.0f ? 1.0f
+                                        : fminf(fmaxf(ldexpf(fabsf(a.scale), e) * kLog2e, 0x1p-126f), 0x1.fffffep127f);
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
             {
@@ -614,15 +618,13 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             }
             tileMax = fmaxf(tileMax, PartnerLane<16>(tileMax));
             tileMax = fmaxf(tileMax, PartnerLane<32>(tileMax));
-            const float top = tileMax * scaleLog2;
-            const bool rises = tileMax != -INFINITY && (runMax == -INFINITY || top > shift + kLag);
+            const bool rises =
+                tileMax != -INFINITY && (base == -INFINITY || (tileMax - base) * scaleLog2 > kLag);
             if (__any(rises))
             {
-                const float newShift = rises ? top : shift;
                 const float factor =
-                    rises ? (runMax == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - newShift)) : 1.0f;
-                runMax = rises ? tileMax : runMax;
-                shift = newShift;
+                    rises ? (base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((base - tileMax) * scaleLog2)) : 1.0f;
+                base = rises ? tileMax : base;
                 runSum *= factor;
 #pragma unroll
                 for (int c = 0; c < kChannels; ++c)
@@ -632,6 +634,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                 }
             }
             half8 phi[kHalves / 2], plo[kHalves / 2];
+            const float from = base == -INFINITY ? 0.0f : base;  // without keys so far every score is -inf
             float sum = 0.0f;
 #pragma unroll
             for (int half = 0; half < kHalves; ++half)
@@ -640,7 +643,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                 {
-                    p[r] = __builtin_amdgcn_exp2f(fmaf(score[half][r], scaleLog2, kWeightBias - shift));
+                    p[r] = __builtin_amdgcn_exp2f(fmaf(score[half][r] - from, scaleLog2, kWeightBias));
                     const _Float16 hi = static_cast<_Float16>(p[r]);
                     phi[half / 2][4 * (half % 2) + r] = hi;
                     plo[half / 2][4 * (half % 2) + r] = static_cast<_Float16>(kLowScale * (p[r] - static_cast<float>(hi)));
@@ -654,13 +657,13 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
 #pragma unroll
                 for (int pair = 0; pair < kHalves / 2; ++pair)
                 {
-                    uint8_t* from = mine + ((readAt ^ (32u * c)) + pair * 32 * 2 * kHd);
+                    uint8_t* row = mine + ((readAt ^ (32u * c)) + pair * 32 * 2 * kHd);
                     const half4 first = __builtin_bit_cast(
                         half4,
-                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)from));
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)row));
                     const half4 second = __builtin_bit_cast(
                         half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                   (__attribute__((address_space(3))) short4v*)(from + 16 * 2 * kHd)));
+                                   (__attribute__((address_space(3))) short4v*)(row + 16 * 2 * kHd)));
                     const half8 vt = __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7);
                     oLow[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, plo[pair], oLow[c], 0, 0, 0);
                     o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, phi[pair], o[c], 0, 0, 0);
@@ -675,18 +678,22 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
         runSum += PartnerLane<32>(runSum);
         if (quad == 0)
         {
-            waveMax[wave][column] = runMax == -INFINITY ? -INFINITY : shift;
-            waveTotal[wave][column] = runSum;
+            waveBase[wave][column] = base;
+            headScale[column] = scaleLog2;  // the same in every wave
         }
         __syncthreads();
-        float top = waveMax[0][column];
+        float top = waveBase[0][column];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w)
         {
-            top = fmaxf(top, waveMax[w][column]);
+            top = fmaxf(top, waveBase[w][column]);
         }
         // A wave without keys has nothing to add: its weight is 0, not that of -inf - -inf.
-        const float factor = runMax == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - top);
+        const float factor = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((base - top) * scaleLog2);
+        if (quad == 0)
+        {
+            waveTotal[wave][column] = runSum * factor;
+        }
         // [16 heads][kHd], 16-byte chunks permuted by the head: eight heads' writes go to different banks.
         float* const acc = reinterpret_cast<float*>(mine);
         if (column < a.group)
@@ -694,8 +701,9 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
 #pragma unroll
             for (int c = 0; c < kChannels; ++c)
             {
-                // NaN scores leave the maximum at -inf and NaN in the sums: they are kept.
-                const float4v x = runMax == -INFINITY && runSum == 0.0f ? float4v{} : (o[c] + oLow[c] * (1.0f / kLowScale)) * factor;
+                // NaN scores leave the base at -inf and NaN in the sums: they are kept.
+                const float4v x = base == -INFINITY && runSum == 0.0f ? float4v{}
+                                                                      : (o[c] + oLow[c] * (1.0f / kLowScale)) * factor;
                 *reinterpret_cast<float4v*>(acc + column * kHd + 4 * ((4 * c + quad) ^ (column & 7u))) = x;
             }
         }
@@ -703,21 +711,13 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
         for (uint32_t i = threadIdx.x; i < a.group * kHd / 4; i += kBlock)
         {
             const uint32_t h = i / (kHd / 4);
-            float best = waveMax[0][h];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w)
-            {
-                best = fmaxf(best, waveMax[w][h]);
-            }
             float4v num = float4v{};
             float den = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w)
             {
                 num += *reinterpret_cast<const float4v*>(lds + w * kWaveBytes + 16 * (i ^ (h & 7u)));
-                const float share = waveTotal[w][h];
-                den += waveMax[w][h] == -INFINITY ? share * 0.0f
-                                                  : share * __builtin_amdgcn_exp2f(waveMax[w][h] - best);
+                den += waveTotal[w][h];
             }
             const uint32_t channel = 4 * (i % (kHd / 4));
             if (!kSplit || whole)
@@ -734,8 +734,15 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                 *reinterpret_cast<float4v*>(slot + 4 + channel) = num;
                 if (channel == 0)
                 {
+                    float best = waveBase[0][h];
+#pragma unroll
+                    for (int w = 1; w < kWaves; ++w)
+                    {
+                        best = fmaxf(best, waveBase[w][h]);
+                    }
                     slot[0] = best;
                     slot[1] = den;
+                    slot[2] = headScale[h];
                 }
             }
         }
@@ -776,7 +783,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
 /// Joins the pieces of a (query, kv head) that shares cut: blockIdx.x goes over those, or over the shares,
 /// whichever are fewer (a share's end cuts at most one that begins in it). A workgroup per head,
 /// kHd / 4 lanes over the channels of a piece, and kThreads / (kHd / 4) pieces side by side in slices,
-/// kDeep of each in flight. A slice's sums are relative to its own running maximum, so that nothing waits for
+/// kDeep of each in flight. A slice's sums are relative to its own running base, so that nothing waits for
 /// a first pass over the maxima. The order is fixed.
 ///
 /// 256 threads have 32 pieces of 128 channels in flight, 512 have 128: one sequence of 32749 keys (28 / 4
@@ -789,7 +796,7 @@ __global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAtten
     constexpr uint32_t kSlices = kThreads / kLanes;
     constexpr uint32_t kDeep = kThreads / 64;
     __shared__ float4v sliceNum[kSlices][kLanes];
-    __shared__ float sliceMax[kSlices];
+    __shared__ float sliceBase[kSlices];
     __shared__ float sliceDen[kSlices];
     const uint4 cut = a.cuts[blockIdx.x];
     const uint32_t pieces = cut.w;
@@ -803,6 +810,7 @@ __global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAtten
     const uint32_t slice = threadIdx.x / kLanes;
     float top = -INFINITY;
     float den = 0.0f;
+    float scaleLog2 = 1.0f;  // the head's, in every piece
     float4v num = float4v{};
     for (uint32_t p0 = slice; p0 < pieces; p0 += kDeep * kSlices)
     {
@@ -823,7 +831,8 @@ __global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAtten
         {
             best = p0 + i * kSlices < pieces ? fmaxf(best, head[i][0]) : best;
         }
-        const float factor = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - best);
+        scaleLog2 = head[0][2];
+        const float factor = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top - best) * scaleLog2);
         top = best;
         den *= factor;
         num *= factor;
@@ -832,8 +841,8 @@ __global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAtten
         {
             if (p0 + i * kSlices < pieces)
             {
-                // A piece without keys is all 0; one of NaN scores has this maximum too, and stays NaN.
-                const float w = head[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(head[i][0] - best);
+                // A piece without keys is all 0; one of NaN scores has this base too, and stays NaN.
+                const float w = head[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((head[i][0] - best) * scaleLog2);
                 den = fmaf(w, head[i][1], den);
                 num += w * x[i];
             }
@@ -842,7 +851,7 @@ __global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAtten
     sliceNum[slice][lane] = num;
     if (lane == 0)
     {
-        sliceMax[slice] = top;
+        sliceBase[slice] = top;
         sliceDen[slice] = den;
     }
     __syncthreads();
@@ -852,14 +861,14 @@ __global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAtten
 #pragma unroll
         for (uint32_t s = 0; s < kSlices; ++s)
         {
-            best = fmaxf(best, sliceMax[s]);
+            best = fmaxf(best, sliceBase[s]);
         }
         num = float4v{};
         den = 0.0f;
 #pragma unroll
         for (uint32_t s = 0; s < kSlices; ++s)
         {
-            const float w = sliceMax[s] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sliceMax[s] - best);
+            const float w = sliceBase[s] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((sliceBase[s] - best) * scaleLog2);
             den = fmaf(w, sliceDen[s], den);
             num += w * sliceNum[s][lane];
         }

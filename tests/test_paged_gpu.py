@@ -793,3 +793,25 @@ def test_attention_with_one_large_component_of_q(mh, gpu, heads, kv, hd, positio
     batch.q[..., 5] *= ratio
     batch.caches[0][..., 5] = 0
     batch.check()
+
+
+@pytest.mark.parametrize("heads, kv, hd, positions", [(14, 2, 64, [0, 33, 500]), (28, 4, 128, [900, 1023]),
+                                                      (14, 2, 64, [3000, 40, 20000]), (28, 4, 128, [16383, 1100])])
+@pytest.mark.parametrize("q_std, scale", [(2.0, 1e9), (2.0, -1e12), (2.0, 1e30), (2.0, 3e38), (1e20, 1e25),
+                                          (1e-20, 1e38)])
+def test_attention_of_scores_far_past_any_exponent(mh, gpu, heads, kv, hd, positions, q_std, scale):
+    """Scaled scores from 1e10 on: the largest one's value is the output, exactly but for the reciprocal of the sum
+    and the product with it; and keys that are all the same share the weight."""
+    rng = np.random.default_rng(hd + len(positions))
+    batch = Attend(mh, gpu, rng, heads, kv, hd, 64, np.array(positions), q_std=q_std)
+    batch.scale = scale
+    for i, p in enumerate(positions):  # no close second: a score's roundings are some 2^-20 of these
+        keys = np.arange(p + 1)
+        k = batch.caches[0][batch.tables[i, keys // 64], :, keys % 64].astype(np.float64)
+        scores = np.sort(np.einsum("hd,khd->hk", batch.q[i] / q_std, np.repeat(k, heads // kv, 1)) * np.sign(scale), 1)
+        if p:
+            small = (scores[:, -1] - scores[:, -2]) < 1e-4 * scores[:, -1]
+            assert not small.any()
+    batch.check(rtol=4 * U)
+    batch.caches[0][:] = batch.caches[0][:1, :, :1]
+    batch.check()
