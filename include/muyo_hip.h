@@ -603,7 +603,8 @@ int muyo_rope_frequencies(double base, uint32_t rotary_dim, const MuyoRopeScalin
  * the rest of a head stays. q goes to q_out [tokens][heads * head_dim] (f32), k and v as fp16 into their
  * slots. q, k and v are f32 [tokens][heads * head_dim] with token strides of their own (in values,
  * multiples of 4), so that they may be parts of stacked projection rows; q_out may be q where its
- * stride is heads * head_dim. turns is device memory as muyo_rope_frequencies fills it.
+ * stride is heads * head_dim, and what is written (q_out and the caches) overlaps nothing else. turns is
+ * device memory as muyo_rope_frequencies fills it.
  * head_dim % 8 == 0 up to 1024, rotary_dim even; tokens * (heads + 2 kv_heads) * head_dim at most
  * 2^34 where rotary_dim % 8 == 0, else 2^32. A token with a position below 0 is padding: its row
  * of q_out and the caches stay as they were. One with a slot outside the cache is not appended. The

@@ -727,11 +727,41 @@ extern "C" int muyo_paged_rope_append_f16kv(const float* q, const float* k, cons
                     name);
     }
     const uint64_t cacheBytes = 2 * kdim * pages * page_size;
-    if (Overlap({kcache, cacheBytes, "kcache"}, {vcache, cacheBytes, "vcache"}))
+    const Range written[] = {{kcache, cacheBytes, "kcache"},
+                             {vcache, cacheBytes, "vcache"},
+                             {q_out, 4 * qdim * tokens, "q_out"}};
+    const Range lists[] = {{positions, 4ull * tokens, "positions"},
+                           {slots, 4ull * tokens, "slots"},
+                           {turns, 4ull * rotary_dim, "turns"}};
+    const Rows sources[] = {{q, 4 * qdim, 4 * q_stride, tokens, "q"},
+                            {k, 4 * kdim, 4 * k_stride, tokens, "k"},
+                            {v, 4 * kdim, 4 * v_stride, tokens, "v"}};
+    for (int i = 0; i < 3; ++i)
     {
-        return Fail(MUYO_E_CONTRACT, "%s: kcache overlaps vcache", name);
+        const Range& w = written[i];
+        for (int j = i + 1; j < 3; ++j)
+        {
+            if (Overlap(w, written[j]))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, written[j].name);
+            }
+        }
+        for (const Range& r : lists)
+        {
+            if (Overlap(w, r))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, r.name);
+            }
+        }
+        for (const Rows& r : sources)
+        {
+            if (i < 2 && Overlap(w, r))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, r.name);
+            }
+        }
     }
-    const Range out{q_out, 4 * qdim * tokens, "q_out"};
+    const Range& out = written[2];
     const Range in[] = {{q, 4 * (q_stride * (tokens - 1) + qdim), "q"},
                         {k, 4 * (k_stride * (tokens - 1) + kdim), "k"},
                         {v, 4 * (v_stride * (tokens - 1) + kdim), "v"}};

@@ -226,3 +226,38 @@ def test_rope_frequencies_unknown_kind_and_nulls(mh):
     assert lib.muyo_rope_frequencies(1e6, 64, None, None, turns.ctypes.data, None) == mh.MUYO_E_NULL
     with pytest.raises(ValueError):
         mh.rope_frequencies(1e6, 64, pair_divisors=np.ones(31))
+
+
+# ------------------------------------------------------------------------------------------------
+# Buffers that a call writes and others that it uses: no two of them may share a byte.
+
+
+def moved(pointer, nbytes):
+    return ctypes.c_void_p(pointer.value + nbytes)
+
+
+APPEND_BYTES = dict(kcache=2 * 2 * 64 * 64 * 16, vcache=2 * 2 * 64 * 64 * 16, q_out=4 * 896 * 3, positions=12,
+                    slots=12, turns=256)
+
+
+@pytest.mark.parametrize("written, other", [(w, o) for w in ("q_out", "kcache", "vcache")
+                                            for o in ("q_out", "kcache", "vcache", "positions", "slots", "turns")
+                                            if w != o])
+def test_append_refuses_written_buffers_over_others(mh, written, other):
+    """At the other's beginning, over its last 16 bytes, and ending inside it."""
+    call = mh.load().muyo_paged_rope_append_f16kv
+    for at in (0, (APPEND_BYTES[other] - 1) // 16 * 16, 16 - APPEND_BYTES[written]):
+        change = {written: moved(APPEND[other], at)}
+        assert call(*{**APPEND, **change}.values()) == mh.MUYO_E_CONTRACT, at
+        assert b"overlaps" in mh.load().muyo_last_error()
+
+
+@pytest.mark.parametrize("source, width", [("q", 896), ("k", 128), ("v", 128)])
+@pytest.mark.parametrize("cache", ["kcache", "vcache"])
+def test_append_refuses_caches_over_the_rows_that_it_reads(mh, source, width, cache):
+    """Over a row's beginning, its last 16 bytes, and the last row, where rows are far apart."""
+    call, stride = mh.load().muyo_paged_rope_append_f16kv, 1 << 20
+    for at in (0, 4 * width - 16, 8 * stride + 4 * width - 16, 4 * stride + 16 - APPEND_BYTES[cache]):
+        change = {source + "_stride": stride, cache: moved(APPEND[source], at)}
+        assert call(*{**APPEND, **change}.values()) == mh.MUYO_E_CONTRACT, at
+        assert b"overlaps " + source.encode() in mh.load().muyo_last_error()
