@@ -621,7 +621,7 @@ int muyo_paged_rope_append_f16kv(const float* q, const float* k, const float* v,
  * the sequence in row query_sequence[i] of tables, sees keys j <= positions[i], the last `window` of them
  * where window > 0. For every head h (kv head h / (heads / kv_heads)):
  *   out[i][h] = sum_j softmax_j(scale * q[i][h].k[j]) * v[j]
- * q and out are f32 [queries][heads * head_dim], and may be the same; out overlaps
+ * q and out are f32 [queries][heads * head_dim], and may be the same; out and the workspace overlap
  * nothing else. A query without keys (a position below 0) gives 0. A query whose sequence is outside
  * 0..sequences - 1 is padding: its row of out stays as it was. Keys past table_pages * page_size, or
  * in pages with an id outside the cache, are left out. Queries may share a sequence (several new tokens

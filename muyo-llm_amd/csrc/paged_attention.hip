@@ -976,19 +976,30 @@ extern "C" int muyo_paged_attention_decode_f16kv(const float* q, const void* kca
         return Fail(MUYO_E_CONTRACT, "%s: needs a 16-byte aligned workspace of %zu bytes (got %llu)", name, need,
                     static_cast<unsigned long long>(workspace_bytes));
     }
-    const Range output{out, 4ull * queries * heads * head_dim, "out"};
+    const uint64_t rowsBytes = 4ull * queries * heads * head_dim;
     const uint64_t cacheBytes = 2ull * pages * page_size * kv_heads * head_dim;
-    const Range inputs[] = {{q, output.bytes, "q"},
+    // The positions, sequences and tables are read again while other workgroups write.
+    const Range ranges[] = {{out, rowsBytes, "out"},
+                            {workspace, need, "workspace"},
+                            {q, rowsBytes, "q"},
                             {kcache, cacheBytes, "kcache"},
                             {vcache, cacheBytes, "vcache"},
-                            {workspace, need, "workspace"}};
-    for (const Range& r : inputs)
+                            {tables, 4ull * sequences * table_pages, "tables"},
+                            {query_sequence, 4ull * queries, "query_sequence"},
+                            {positions, 4ull * queries, "positions"}};
+    constexpr int kOutputs = 2;
+    constexpr int kRanges = static_cast<int>(sizeof ranges / sizeof ranges[0]);
+    for (int i = 0; i < kOutputs; ++i)
     {
-        // In place a workgroup has read its (query, kv head)'s q when it writes its output there, and one that
-        // is cut is written by the join.
-        if (!(&r == inputs && q == out) && Overlap(output, r))
+        for (int j = i + 1; j < kRanges; ++j)
         {
-            return Fail(MUYO_E_CONTRACT, "%s: out overlaps %s", name, r.name);
+            // In place a workgroup has read its (query, kv head)'s q when it writes its output there, and one that
+            // is cut is written by the join.
+            const bool inPlace = i == 0 && j == kOutputs && q == out;
+            if (!inPlace && Overlap(ranges[i], ranges[j]))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, ranges[i].name, ranges[j].name);
+            }
         }
     }
     PagedAttentionArgs a{q,

@@ -261,3 +261,21 @@ def test_append_refuses_caches_over_the_rows_that_it_reads(mh, source, width, ca
         change = {source + "_stride": stride, cache: moved(APPEND[source], at)}
         assert call(*{**APPEND, **change}.values()) == mh.MUYO_E_CONTRACT, at
         assert b"overlaps " + source.encode() in mh.load().muyo_last_error()
+
+
+ATTEND_BYTES = dict(out=4 * 3 * 896, q=4 * 3 * 896, kcache=2 * 2 * 64 * 64 * 16, vcache=2 * 2 * 64 * 64 * 16,
+                    tables=4 * 3 * 8, query_sequence=12, positions=12)
+
+
+@pytest.mark.parametrize("written, other", [(w, o) for w in ("out", "workspace")
+                                            for o in ("out", "q", "kcache", "vcache", "tables", "query_sequence",
+                                                      "positions") if w != o])
+def test_attention_refuses_written_buffers_over_others(mh, written, other):
+    """At the other's beginning (out over q may be there), over its last 16 bytes, and ending inside it."""
+    lib = mh.load()
+    call = lib.muyo_paged_attention_decode_f16kv
+    own = dict(ATTEND_BYTES, workspace=lib.muyo_paged_attention_decode_f16kv_workspace_bytes(3, 14, 2, 64))[written]
+    for at in (0, (ATTEND_BYTES[other] - 1) // 16 * 16, 16 - own // 16 * 16):
+        if (written, other, at) != ("out", "q", 0):
+            assert call(*{**ATTEND, written: moved(ATTEND[other], at)}.values()) == mh.MUYO_E_CONTRACT, at
+            assert b"overlaps" in lib.muyo_last_error()
