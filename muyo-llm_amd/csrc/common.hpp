@@ -45,6 +45,40 @@ inline hipStream_t AsStream(void* stream) { return static_cast<hipStream_t>(stre
 
 inline bool Aligned16(const void* pointer) { return (reinterpret_cast<uintptr_t>(pointer) & 15u) == 0; }
 
+/// One buffer of a call, for the overlap check.
+struct Range
+{
+    const void* at;
+    uint64_t bytes;
+    const char* name;
+};
+
+inline bool Overlap(const Range& a, const Range& b)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at);
+    const uintptr_t y = reinterpret_cast<uintptr_t>(b.at);
+    return x < y + b.bytes && y < x + a.bytes;
+}
+
+/// A call's rows of `bytes` each, `stride` bytes apart: other buffers may lie between them.
+struct Rows
+{
+    const void* at;
+    uint64_t bytes;
+    uint64_t stride;
+    uint64_t count;
+    const char* name;
+};
+
+inline bool Overlap(const Range& a, const Rows& b)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at);
+    const uintptr_t y = reinterpret_cast<uintptr_t>(b.at);
+    // The first row that ends behind the range's begin: it overlaps, or none does.
+    const uint64_t row = x < y + b.bytes ? 0 : (x - y - b.bytes) / b.stride + 1;
+    return row < b.count && y + row * b.stride < x + a.bytes;
+}
+
 inline uint32_t CeilDiv(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1) / b); }
 
 /// ggml's fastdiv magic for divisor d: (mulhi(n, mp) + n) >> L == n / d for every 32-bit n

@@ -982,6 +982,35 @@ extern "C" int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride,
     {
         return Fail(MUYO_E_RANGE, "%s: %u rows of %u are too many for one call", name, rows, vocab);
     }
+    const Range ranges[] = {{logprobs, 4ull * rows, "logprobs"},
+                            {ranks, 4ull * rows, "ranks"},
+                            {entropy, 4ull * rows, "entropy"},
+                            {top_ids, 4ull * rows * top, "top_ids"},
+                            {top_logprobs, 4ull * rows * top, "top_logprobs"},
+                            {workspace, need, "workspace"},
+                            {tokens, 4ull * rows, "tokens"}};
+    constexpr int kOutputs = 6;
+    const Rows read{logits, 4ull * vocab, 4 * std::min<uint64_t>(row_stride, 1ull << 60), rows, "logits"};
+    for (int i = 0; i < kOutputs; ++i)
+    {
+        const Range& w = ranges[i];
+        if (w.at == nullptr || w.bytes == 0)
+        {
+            continue;
+        }
+        // The join reads a row's given token and its logit again when other rows' results are written.
+        if (Overlap(w, read))
+        {
+            return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, read.name);
+        }
+        for (int j = i + 1; j <= kOutputs; ++j)
+        {
+            if (ranges[j].at != nullptr && ranges[j].bytes != 0 && Overlap(w, ranges[j]))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, ranges[j].name);
+            }
+        }
+    }
     const dim3 grid(static_cast<uint32_t>(blocks));
     if (4ull * rows * vocab > kOnceBytes)
     {

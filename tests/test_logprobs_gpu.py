@@ -315,3 +315,27 @@ def test_logprobs_past_four_gigabytes_of_rows(mh, gpu):
     torch.cuda.synchronize()
     check(dict(logprobs=host(out)[0], entropy=host(out)[1], ranks=host(ranks), ids=host(ids), tops=host(tops)), values,
           [1, 2, 3], 2)
+
+
+def test_results_between_rows_of_logits(mh, gpu):
+    """Rows of a wider buffer whose further columns hold the results and the workspace of the call."""
+    torch, lib = gpu, mh.load()
+    rows, vocab, top = 3, 20001, 4
+    size = lib.muyo_token_logprobs_workspace_bytes(rows, vocab, top)
+    stride = vocab + 3 + size // 4 + 64
+    stride += -stride % 4
+    rng = np.random.default_rng(12)
+    x, given = rng.normal(0, 2, (rows, vocab)).astype(np.float32), rng.integers(0, vocab, rows)
+    buffer = torch.zeros((rows, stride), device="cuda")
+    buffer[:, :vocab] = torch.from_numpy(x).cuda()
+    tokens = torch.from_numpy(given.astype(np.int32)).cuda()
+    gaps = [buffer.data_ptr() + 4 * (r * stride + vocab) for r in range(rows)]
+    mh.check(lib.muyo_token_logprobs_f32(
+        buffer.data_ptr(), stride, rows, vocab, tokens.data_ptr(), gaps[0], gaps[0] + 12, gaps[0] + 24, top, gaps[2],
+        gaps[2] + 48, gaps[1] + 12, size, torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    got = host(buffer)
+    assert np.array_equal(got[:, :vocab], x)
+    first, last = got[0, vocab:vocab + 9], got[2, vocab:vocab + 24]
+    check(dict(logprobs=first[:3], ranks=first[3:6].view(np.int32), entropy=first[6:9],
+               ids=last[:12].view(np.int32).reshape(rows, top), tops=last[12:].reshape(rows, top)), x, given, top)

@@ -279,3 +279,27 @@ def test_attention_refuses_written_buffers_over_others(mh, written, other):
         if (written, other, at) != ("out", "q", 0):
             assert call(*{**ATTEND, written: moved(ATTEND[other], at)}.values()) == mh.MUYO_E_CONTRACT, at
             assert b"overlaps" in lib.muyo_last_error()
+
+
+LOGPROB_BYTES = dict(logits=4 * 3 * 1000, tokens=12, logprobs=12, ranks=12, entropy=12, top_ids=60, top_logprobs=60)
+
+
+@pytest.mark.parametrize("written, other", [(w, o) for w in ("logprobs", "ranks", "entropy", "top_ids", "top_logprobs",
+                                                             "workspace")
+                                            for o in LOGPROB_BYTES if w != o])
+def test_logprobs_refuse_written_buffers_over_others(mh, written, other):
+    """At the other's beginning, over its last 16 bytes, and ending inside it."""
+    lib = mh.load()
+    own = dict(LOGPROB_BYTES, workspace=lib.muyo_token_logprobs_workspace_bytes(3, 1000, 5))[written]
+    for at in (0, (LOGPROB_BYTES[other] - 1) // 16 * 16, 16 - max(16, own // 16 * 16)):
+        change = {written: moved(LOGPROBS[other], at)}
+        assert lib.muyo_token_logprobs_f32(*{**LOGPROBS, **change}.values()) == mh.MUYO_E_CONTRACT, at
+        assert b"overlaps" in lib.muyo_last_error()
+
+
+@pytest.mark.parametrize("at", [4 * 999, 4 * (1 << 20), 8 * (1 << 20) + 3996, 4 * (1 << 20) - 56])
+def test_logprobs_refuse_outputs_over_rows_far_apart(mh, at):
+    """A row's last logit, another's first, the last row's last, and an output that ends in a row."""
+    change = dict(row_stride=1 << 20, top_ids=moved(LOGPROBS["logits"], at))
+    assert mh.load().muyo_token_logprobs_f32(*{**LOGPROBS, **change}.values()) == mh.MUYO_E_CONTRACT
+    assert b"top_ids overlaps logits" in mh.load().muyo_last_error()
