@@ -576,7 +576,7 @@ enum
     MUYO_ROPE_SCALING_BASE = 2,   /* the base times factor^(d / (d - 2)): the slowest pair turns 1 / factor as fast */
     MUYO_ROPE_SCALING_YARN = 3,   /* pairs that turn over `high` times in trainedContext keep their speed, under `low`
                                      times turn 1 / factor as fast, a ramp over the pairs between; the rotated
-                                     values times attnFactor * (1 + ln(factor) / 10). The ramp of
+                                     values times attnFactor * (1 + ln(factor) / 10), above 0. The ramp of
                                      muyo_rope_neox_f32 with extFactor 1 (rope_funcs.glsl:17-35) */
     MUYO_ROPE_SCALING_WAVELENGTH = 4 /* the same ends, a ramp over the turns between */
 };
@@ -586,7 +586,7 @@ typedef struct MuyoRopeScaling
     uint32_t kind; /* MUYO_ROPE_SCALING_* */
     float factor;
     float low;  /* turns in the trained context (usually 1) */
-    float high; /* (usually 32 for YaRN, 4 by wavelength) */
+    float high; /* (usually 32 for YaRN, 4 by wavelength); at least low, by wavelength above it */
     float attnFactor; /* YaRN only (usually 1) */
     uint32_t trainedContext;
 } MuyoRopeScaling;

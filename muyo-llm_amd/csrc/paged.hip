@@ -616,10 +616,10 @@ extern "C" int muyo_rope_frequencies(double base, uint32_t rotary_dim, const Muy
     float scale = 1.0f;
     if (kind == MUYO_ROPE_SCALING_YARN)
     {
-        if (scaling->trainedContext == 0 || !(scaling->high > 0.0f) || !(scaling->low > 0.0f) ||
-            !std::isfinite(scaling->high) || !std::isfinite(scaling->low) || !std::isfinite(scaling->attnFactor))
+        if (scaling->trainedContext == 0 || !(scaling->low > 0.0f) || !(scaling->high >= scaling->low) ||
+            !std::isfinite(scaling->high))
         {
-            return Fail(MUYO_E_CONTRACT, "%s: YaRN needs trainedContext, low and high above 0", name);
+            return Fail(MUYO_E_CONTRACT, "%s: YaRN needs trainedContext and 0 < low <= high", name);
         }
         // The pairs that turn `high` and `low` times in the trained context bound the ramp.
         auto pairOf = [&](double turning) {
@@ -628,6 +628,12 @@ extern "C" int muyo_rope_frequencies(double base, uint32_t rotary_dim, const Muy
         low = std::max(0.0, std::floor(pairOf(scaling->high)));
         high = std::min(rotary_dim - 1.0, std::ceil(pairOf(scaling->low)));
         scale = static_cast<float>(scaling->attnFactor * (1.0 + 0.1 * std::log(factor)));
+        if (!(scale > 0.0f) || !std::isfinite(scale))
+        {
+            return Fail(MUYO_E_CONTRACT, "%s: YaRN's magnitude attnFactor * (1 + ln(factor) / 10) must be finite and "
+                                         "above 0",
+                        name);
+        }
     }
     if (kind == MUYO_ROPE_SCALING_WAVELENGTH &&
         (scaling->trainedContext == 0 || !(scaling->low > 0.0f) || !(scaling->high > scaling->low) ||

@@ -303,3 +303,25 @@ def test_logprobs_refuse_outputs_over_rows_far_apart(mh, at):
     change = dict(row_stride=1 << 20, top_ids=moved(LOGPROBS["logits"], at))
     assert mh.load().muyo_token_logprobs_f32(*{**LOGPROBS, **change}.values()) == mh.MUYO_E_CONTRACT
     assert b"top_ids overlaps logits" in mh.load().muyo_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(low=32.0, high=1.0), dict(low=33.0), dict(factor=1e-5), dict(factor=4e-5),
+                                    dict(attn_factor=0.0), dict(attn_factor=-1.0)],
+                         ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()))
+def test_rope_frequencies_yarn_without_a_ramp_or_magnitude(mh, change):
+    """Ends in the wrong order, and factors whose 1 + ln(factor) / 10 (with attn_factor) is not above 0."""
+    with pytest.raises(mh.MuyoError) as error:
+        mh.rope_frequencies(1e6, 64, "YARN", **{**dict(factor=4.0, trained_context=4096), **change})
+    assert error.value.status == mh.MUYO_E_CONTRACT
+
+
+def test_rope_frequencies_yarn_at_the_ends_of_what_is_taken(mh):
+    """low = high: pairs on one side keep their speed, on the other turn 1 / factor as fast, but for one on the border
+    (its place is rounded down for one end and up for the other). A factor just above e^-10 has a magnitude."""
+    turns, _ = mh.rope_frequencies(1e6, 64, "YARN", factor=4.0, low=8.0, high=8.0, trained_context=4096)
+    plain = np.array(plain_turns(1e6, 64))
+    border = 64 * math.log(4096 / (8 * 2 * math.pi)) / (2 * math.log(1e6))
+    j = np.arange(32)
+    np.testing.assert_allclose(turns, np.where(j <= border, plain, plain / 4), rtol=1e-14)
+    _, magnitude = mh.rope_frequencies(1e6, 64, "YARN", factor=5e-5, trained_context=4096)
+    assert magnitude == np.float32(1 + 0.1 * math.log(np.float32(5e-5))) and 0 < magnitude < 0.01
