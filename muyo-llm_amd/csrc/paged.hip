@@ -651,6 +651,10 @@ extern "C" int muyo_rope_frequencies(double base, uint32_t rotary_dim, const Muy
     if (kind == MUYO_ROPE_SCALING_BASE)
     {
         base *= std::pow(factor, rotary_dim / (rotary_dim - 2.0));
+        if (!std::isfinite(base))
+        {
+            return Fail(MUYO_E_CONTRACT, "%s: the stretched base is not finite", name);
+        }
     }
     for (uint32_t j = 0; j < rotary_dim / 2; ++j)
     {

@@ -325,3 +325,9 @@ def test_rope_frequencies_yarn_at_the_ends_of_what_is_taken(mh):
     np.testing.assert_allclose(turns, np.where(j <= border, plain, plain / 4), rtol=1e-14)
     _, magnitude = mh.rope_frequencies(1e6, 64, "YARN", factor=5e-5, trained_context=4096)
     assert magnitude == np.float32(1 + 0.1 * math.log(np.float32(5e-5))) and 0 < magnitude < 0.01
+
+
+def test_rope_frequencies_of_a_base_stretched_past_any_number(mh):
+    with pytest.raises(mh.MuyoError) as error:
+        mh.rope_frequencies(1e300, 4, "BASE", factor=1e30)
+    assert error.value.status == mh.MUYO_E_CONTRACT
