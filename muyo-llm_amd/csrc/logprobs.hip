@@ -332,8 +332,8 @@ struct LaneBatches
 /// place is the number of those above it. More than 64 are inserted too. Equal logits are told apart by
 /// their index in the key, so nothing overflows. The batch goes through LDS: the registers are free for
 /// the next one at once, and loops over its logits need not be unrolled. Batches that no lane knows to
-/// reach the last are left out: of a row with few logits above -inf, or of equal ones, most (300 rows with ten
-/// above -inf and 20 alternatives: 67 us, 202 through all batches, where ordinary rows take 42).
+/// reach the last are left out: of a row with few logits above -inf, or of equal ones, most (a call on 300 rows with
+/// ten above -inf and 20 alternatives: 66 us, 202 through all batches, where one on ordinary rows takes 49).
 __device__ __forceinline__ void TopByWaves(const LogprobArgs& a, const RowSpan& s, uint32_t firstBatch,
                                            uint32_t batches, uint32_t stride, uint32_t floorBits,
                                            const LaneBatches& own, TopSpace& space)

@@ -226,8 +226,8 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// accumulators cost no time for long caches (64 sequences of 1 to 16384 keys 167.5 us, without 167.3) and
 /// 0.1 us for short ones.
 ///
-/// Only tiles that reach over an end of the key range, or into a page that is
-/// not there, are masked: their scores to -inf, and their V rows to 0, since 0 * NaN would be NaN.
+/// Only tiles that reach over an end of the key range, or into a page that is not there, are masked: their scores to
+/// -inf, and their V rows to 0, since 0 * NaN would be NaN.
 ///
 /// kSplit: the tiles of all queries and kv heads in a row, each with its setup's cost before it, are dealt
 /// out in equal shares, whatever the sequences' lengths. A share may begin and end inside a (query, kv
@@ -238,10 +238,10 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 ///
 /// What bounds it: the cache's arrival. 64 sequences of 1 to 16384 keys (28 / 4 heads of 128, pages of 16,
 /// 1.07 GB of K and V): 168 us, 6.4 TB/s, where the best streaming read here has 6.9; 14 / 2 heads of 64,
-/// 0.27 GB: 45 us, 6.0 TB/s; one sequence of 32749 keys, 67 MB: 15.7 us, 4.3 TB/s, of which the way to the
+/// 0.27 GB: 45 us, 6.0 TB/s; one sequence of 32749 keys, 67 MB: 16 us, 4.2 TB/s, of which the way to the
 /// first tile and the joins take about five. Past the caches' size, loads without the non-temporal hint took 190 us; a
 /// split launch is for long caches, and loads K and V with it. Short ones are a chain of round trips
-/// (position, page, rows), 5 us: 8 or 16 waves a workgroup, tiles of 64 keys, and two or three tiles in
+/// (position, page, rows), 5.2 us: 8 or 16 waves a workgroup, tiles of 64 keys, and two or three tiles in
 /// flight at head_dim 64 all measured no better or worse.
 template <int kHd, bool kSplit>
 __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void PagedAttentionKernel(PagedAttentionArgs a)
