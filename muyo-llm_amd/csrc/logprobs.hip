@@ -651,7 +651,7 @@ __device__ __forceinline__ void TopOfPart(const LogprobArgs& a, const RowSpan& s
 /// LDS, so that the loop over its logits need not be unrolled (one wave of a row runs it, and its instructions
 /// come from memory).
 ///
-/// What bounds it: for many rows, the logits' arrival. 1000 rows of 151936, 608 MB: 98 us, 6.2 TB/s, where the
+/// What bounds it: for many rows, the logits' arrival. 1000 rows of 151936, 608 MB: 96 to 100 us, 6.2 TB/s, where the
 /// best streaming read here has 6.9; read without the non-temporal hint (they fit no cache) 111 us. For
 /// few rows, a chain: the batches' round trips, then two barriers and a bisection to the bound, another round
 /// trip and the ranking. One row with 20 alternatives takes 8.2 us and 4.3 for the join (4.5 of the first
