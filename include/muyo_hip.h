@@ -650,7 +650,8 @@ int muyo_paged_attention_decode_f16kv(const float* q, const void* kcache, const 
  * most vocab. A token outside the vocabulary has logprob -inf and rank -1. Logits of -inf have
  * probability 0; a row of nothing else has logprobs -inf and entropy 0. A NaN or +inf among a row's
  * logits makes its logprobs and entropy NaN; in the order NaN is last. Fewer than 2^24 rows. What is
- * written overlaps nothing else (it may lie between rows of logits). `workspace` as above, of at least muyo_token_logprobs_workspace_bytes(...) bytes. */
+ * written overlaps nothing else (it may lie between rows of logits). `workspace` as above, of at least
+ * muyo_token_logprobs_workspace_bytes(...) bytes. */
 size_t muyo_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top); /* 0: unsupported */
 int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
                             const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropy, uint32_t top,

@@ -205,7 +205,7 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// B[8 (l / 16) .. +8][l % 16], receiving D[4 (l / 16) + r][l % 16]). Per tile a wave
 ///   - takes K rows straight from memory as A operands (of 16 keys each) and forms S^T (keys x heads) =
 ///     K . q^T, q in registers as two planes of f16 (hi + lo, of q times the power of two that takes the head's
-///     largest value to 2^13 .. 2^14: 22 bits down to 2^-17 of that value, and 2^-39 of it below);
+///     largest value to 2^13 .. 2^14: 22 bits down to 2^-16 of that value, and 2^-38 of it below);
 ///   - passes the V rows through its own part of LDS, to read them back transposed
 ///     (ds_read_b64_tr_b16: 16 lanes give 4 rows of 16 channels, each gets a channel of 4 rows);
 ///   - requests the next tile's K and V into the registers that are now free;
@@ -218,8 +218,8 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// Weights are relative to `base`, a raw score that follows the maximum only once that is 2^kLag past it: rescaling
 /// the accumulators is rare. They are made of differences of raw scores, in the joins too, so that those of scaled
 /// scores of any size are 1 where scores are equal (scaled scores past 2^29 are rounded by more than f16 holds, and
-/// weights of them were infinite or 0). Where one key has most of the weight and a small value row, the result is that of
-/// the small weights, so these need their bits too: f16 has 11 down to 2^-14, and the low plane, times
+/// weights of them were infinite or 0). Where one key has most of the weight and a small value row, the result is
+/// that of the small weights, so these need their bits too: f16 has 11 down to 2^-14, and the low plane, times
 /// kLowScale in accumulators of its own, the next 11. A weight keeps 22 bits down to 2^-25 of the largest
 /// (17 nats), and 2^-47 of the largest below. (With a key 20 nats above the others and a value row of 0, both planes
 /// in the same accumulators lose 3e-4 of the result, and a third of it with weights of at most 1.) The
@@ -646,7 +646,8 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                     p[r] = __builtin_amdgcn_exp2f(fmaf(score[half][r] - from, scaleLog2, kWeightBias));
                     const _Float16 hi = static_cast<_Float16>(p[r]);
                     phi[half / 2][4 * (half % 2) + r] = hi;
-                    plo[half / 2][4 * (half % 2) + r] = static_cast<_Float16>(kLowScale * (p[r] - static_cast<float>(hi)));
+                    plo[half / 2][4 * (half % 2) + r] =
+                        static_cast<_Float16>(kLowScale * (p[r] - static_cast<float>(hi)));
                 }
                 sum += (p[0] + p[1]) + (p[2] + p[3]);
             }
