@@ -641,6 +641,40 @@ int muyo_paged_attention_decode_f16kv(const float* q, const void* kcache, const 
                                       uint32_t page_size, uint32_t window, float scale, void* workspace,
                                       uint64_t workspace_bytes, void* stream);
 
+/* A cache of half the bytes: kcache and vcache are [pages][kv_heads][page_size][head_dim] 8-bit codes, kscales and
+ * vscales [pages][kv_heads][page_size] f32, and a value is scale * code. The codes are whole numbers of
+ * -127..127, or e4m3 (four bits of exponent, three of fraction, up to 448). */
+enum
+{
+    MUYO_KV_INT8 = 0,
+    MUYO_KV_E4M3 = 1
+};
+
+/* muyo_paged_rope_append_f16kv into such a cache. A row y of a kv head (k rotated, or v) is stored with
+ *   scale = max|y| / 127 (int8) or / 448 (e4m3), rounded to f32, codes = y / scale, rounded to the nearest (even)
+ * from 64 bits, k's rotation included. A row of zeros has scale 0, as has one too small for f32 to hold its scale;
+ * one with an infinity or a NaN has scale NaN and codes 0. head_dim 64 or 128; else as above. Caches and scales are
+ * 16-byte aligned and overlap nothing else. */
+int muyo_paged_rope_append_q8kv(const float* q, const float* k, const float* v, uint64_t q_stride, uint64_t k_stride,
+                                uint64_t v_stride, float* q_out, void* kcache, void* vcache, float* kscales,
+                                float* vscales, const int32_t* positions, const int32_t* slots, uint32_t tokens,
+                                uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t pages,
+                                uint32_t page_size, uint32_t format, uint32_t rope_layout, uint32_t rotary_dim,
+                                const double* turns, float magnitude, void* stream);
+
+/* muyo_paged_attention_decode_f16kv over such a cache, of the values as they are stored:
+ *   out[i][h] = sum_j softmax_j(scale * kscale_j * (q[i][h].kcode[j])) * vscale_j * vcode[j]
+ * Rows and scales that a query sees are finite; the others may hold anything. The rest, the workspace too, as
+ * above. */
+size_t muyo_paged_attention_decode_q8kv_workspace_bytes(uint32_t queries, uint32_t heads, uint32_t kv_heads,
+                                                        uint32_t head_dim); /* 0: unsupported shape */
+int muyo_paged_attention_decode_q8kv(const float* q, const void* kcache, const void* vcache, const float* kscales,
+                                     const float* vscales, float* out, const int32_t* tables, uint32_t sequences,
+                                     uint32_t table_pages, const int32_t* query_sequence, const int32_t* positions,
+                                     uint32_t queries, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                     uint32_t pages, uint32_t page_size, uint32_t format, uint32_t window, float scale,
+                                     void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* Of each row of logits [rows][vocab] (f32, `row_stride` values apart), with p = softmax(row):
  *   logprobs[r]     ln p of tokens[r]
  *   ranks[r]        tokens before tokens[r] in the order of falling logits, equal ones by rising index

@@ -8,6 +8,7 @@
 
 #include "common.hpp"
 #include "paged.hpp"
+#include "paged_rope.hpp"
 
 namespace muyo
 {
@@ -314,24 +315,6 @@ struct AppendArgs
     float magnitude;
 };
 
-/// cos and sin of the angle 2 pi (position * turns), times the magnitude. Far positions turn a pair
-/// many times over, and only the fraction of a turn counts: the product and the fraction are in 64
-/// bits (in 32, position 100000 would leave two digits less), cos and sin of the fraction in 32.
-__device__ __forceinline__ void PairAngle(double turns, int32_t position, float magnitude, float& c, float& s)
-{
-    const double t = static_cast<double>(position) * turns;
-    float sn, cs;
-    sincospif(static_cast<float>(2.0 * (t - rint(t))), &sn, &cs);
-    c = cs * magnitude;
-    s = sn * magnitude;
-}
-
-__device__ __forceinline__ void Rotate(float x0, float x1, float c, float s, float& y0, float& y1)
-{
-    y0 = fmaf(x0, c, -(x1 * s));
-    y1 = fmaf(x0, s, x1 * c);
-}
-
 /// Row r of a token: a head of q, then of k, then of v.
 __device__ __forceinline__ const float* AppendSource(const AppendArgs& a, uint64_t token, uint32_t r)
 {
@@ -497,6 +480,107 @@ int CheckPages(const char* name, uint32_t pages, uint32_t pageSize)
     {
         return Fail(MUYO_E_RANGE, "%s: needs 1 <= pages and pages * page_size < 2^31 (got %u pages of %u)", name, pages,
                     pageSize);
+    }
+    return MUYO_OK;
+}
+
+int CheckAppend(const char* name, const AppendCall& c, const Range* caches, int cacheCount)
+{
+    bool missing = c.q == nullptr || c.k == nullptr || c.v == nullptr || c.qOut == nullptr ||
+                   c.positions == nullptr || c.slots == nullptr || c.turns == nullptr;
+    for (int i = 0; i < cacheCount; ++i)
+    {
+        missing = missing || caches[i].at == nullptr;
+    }
+    if (missing)
+    {
+        return Fail(MUYO_E_NULL, "%s: every buffer is required", name);
+    }
+    const int checked = CheckPages(name, c.pages, c.pageSize);
+    if (checked != MUYO_OK)
+    {
+        return checked;
+    }
+    if (c.tokens == 0 || c.tokens > kMaxPlanTokens || c.heads == 0 || c.kvHeads == 0 || c.heads > 1024 ||
+        c.kvHeads > 1024)
+    {
+        return Fail(MUYO_E_RANGE, "%s: takes 1..%u tokens, 1..1024 heads and kv_heads (got %u, %u and %u)", name,
+                    kMaxPlanTokens, c.tokens, c.heads, c.kvHeads);
+    }
+    if (c.headDim == 0 || c.headDim % 8 != 0 || c.headDim > 1024 || c.rotary < 2 || c.rotary % 2 != 0 ||
+        c.rotary > c.headDim || c.layout > MUYO_ROPE_INTERLEAVED)
+    {
+        return Fail(MUYO_E_UNSUPPORTED, "%s: needs head_dim a multiple of 8 up to 1024, an even rotary_dim of at most "
+                                        "that, and a known rope_layout (got %u, %u, %u)",
+                    name, c.headDim, c.rotary, c.layout);
+    }
+    if (c.threads > 1ull << 31)  // a launch has fewer than 2^32 threads
+    {
+        return Fail(MUYO_E_RANGE, "%s: %u tokens of %u heads of %u values are too many for one call", name, c.tokens,
+                    c.heads + 2 * c.kvHeads, c.headDim);
+    }
+    const uint64_t qdim = static_cast<uint64_t>(c.heads) * c.headDim;
+    const uint64_t kdim = static_cast<uint64_t>(c.kvHeads) * c.headDim;
+    if (c.qStride < qdim || c.kStride < kdim || c.vStride < kdim || c.qStride % 4 != 0 || c.kStride % 4 != 0 ||
+        c.vStride % 4 != 0 || c.qStride > 0xFFFFFFFFull || c.kStride > 0xFFFFFFFFull || c.vStride > 0xFFFFFFFFull)
+    {
+        return Fail(MUYO_E_CONTRACT, "%s: token strides must be multiples of 4 that hold a token's heads", name);
+    }
+    bool aligned = Aligned16(c.q) && Aligned16(c.k) && Aligned16(c.v) && Aligned16(c.qOut);
+    for (int i = 0; i < cacheCount; ++i)
+    {
+        aligned = aligned && Aligned16(caches[i].at);
+    }
+    if (!aligned || (reinterpret_cast<uintptr_t>(c.turns) & 7u) != 0 || !std::isfinite(c.magnitude))
+    {
+        return Fail(MUYO_E_CONTRACT, "%s: q, k, v, q_out and the caches must be 16-byte aligned, turns 8-byte aligned, "
+                                     "magnitude finite",
+                    name);
+    }
+    const Range out{c.qOut, 4 * qdim * c.tokens, "q_out"};
+    const Range lists[] = {{c.positions, 4ull * c.tokens, "positions"},
+                           {c.slots, 4ull * c.tokens, "slots"},
+                           {c.turns, 4ull * c.rotary, "turns"}};
+    const Rows sources[] = {{c.q, 4 * qdim, 4 * c.qStride, c.tokens, "q"},
+                            {c.k, 4 * kdim, 4 * c.kStride, c.tokens, "k"},
+                            {c.v, 4 * kdim, 4 * c.vStride, c.tokens, "v"}};
+    for (int i = 0; i <= cacheCount; ++i)
+    {
+        const Range& w = i < cacheCount ? caches[i] : out;
+        for (int j = i + 1; j <= cacheCount; ++j)
+        {
+            const Range& other = j < cacheCount ? caches[j] : out;
+            if (Overlap(w, other))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, other.name);
+            }
+        }
+        for (const Range& r : lists)
+        {
+            if (Overlap(w, r))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, r.name);
+            }
+        }
+        for (const Rows& r : sources)
+        {
+            if (i < cacheCount && Overlap(w, r))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, r.name);
+            }
+        }
+    }
+    const Range in[] = {{c.q, 4 * (c.qStride * (c.tokens - 1) + qdim), "q"},
+                        {c.k, 4 * (c.kStride * (c.tokens - 1) + kdim), "k"},
+                        {c.v, 4 * (c.vStride * (c.tokens - 1) + kdim), "v"}};
+    for (const Range& r : in)
+    {
+        // In place over a dense q each thread writes what it alone has read.
+        const bool inPlace = &r == in && c.q == c.qOut && c.qStride == qdim;
+        if (!inPlace && Overlap(out, r))
+        {
+            return Fail(MUYO_E_CONTRACT, "%s: q_out overlaps %s", name, r.name);
+        }
     }
     return MUYO_OK;
 }
@@ -692,97 +776,17 @@ extern "C" int muyo_paged_rope_append_f16kv(const float* q, const float* k, cons
                                             uint32_t rotary_dim, const double* turns, float magnitude, void* stream)
 {
     const char* name = "paged_rope_append_f16kv";
-    if (q == nullptr || k == nullptr || v == nullptr || q_out == nullptr || kcache == nullptr || vcache == nullptr ||
-        positions == nullptr || slots == nullptr || turns == nullptr)
-    {
-        return Fail(MUYO_E_NULL, "%s: every buffer is required", name);
-    }
-    const int checked = CheckPages(name, pages, page_size);
+    const uint64_t cacheBytes = 2ull * kv_heads * head_dim * pages * page_size;
+    const Range caches[] = {{kcache, cacheBytes, "kcache"}, {vcache, cacheBytes, "vcache"}};
+    const bool octets = rotary_dim % 8 == 0;
+    const uint64_t items =
+        static_cast<uint64_t>(tokens) * (heads + 2ull * kv_heads) * (octets ? head_dim / 8 : head_dim / 2);
+    const AppendCall call{q,     k,     v,        q_stride, k_stride, v_stride,  q_out,       positions,  slots, tokens,
+                          heads, kv_heads, head_dim, pages, page_size, rope_layout, rotary_dim, turns, magnitude, items};
+    const int checked = CheckAppend(name, call, caches, 2);
     if (checked != MUYO_OK)
     {
         return checked;
-    }
-    if (tokens == 0 || tokens > kMaxPlanTokens || heads == 0 || kv_heads == 0 || heads > 1024 || kv_heads > 1024)
-    {
-        return Fail(MUYO_E_RANGE, "%s: takes 1..%u tokens, 1..1024 heads and kv_heads (got %u, %u and %u)", name,
-                    kMaxPlanTokens, tokens, heads, kv_heads);
-    }
-    if (head_dim == 0 || head_dim % 8 != 0 || head_dim > 1024 || rotary_dim < 2 || rotary_dim % 2 != 0 ||
-        rotary_dim > head_dim || rope_layout > MUYO_ROPE_INTERLEAVED)
-    {
-        return Fail(MUYO_E_UNSUPPORTED, "%s: needs head_dim a multiple of 8 up to 1024, an even rotary_dim of at most "
-                                        "that, and a known rope_layout (got %u, %u, %u)",
-                    name, head_dim, rotary_dim, rope_layout);
-    }
-    const uint32_t rows = heads + 2 * kv_heads;
-    const bool octets = rotary_dim % 8 == 0;
-    const uint64_t items = static_cast<uint64_t>(tokens) * rows * (octets ? head_dim / 8 : head_dim / 2);
-    if (items > 1ull << 31)  // a launch has fewer than 2^32 threads
-    {
-        return Fail(MUYO_E_RANGE, "%s: %u tokens of %u heads of %u values are too many for one call", name, tokens,
-                    rows, head_dim);
-    }
-    const uint64_t qdim = static_cast<uint64_t>(heads) * head_dim;
-    const uint64_t kdim = static_cast<uint64_t>(kv_heads) * head_dim;
-    if (q_stride < qdim || k_stride < kdim || v_stride < kdim || q_stride % 4 != 0 || k_stride % 4 != 0 ||
-        v_stride % 4 != 0 || q_stride > 0xFFFFFFFFull || k_stride > 0xFFFFFFFFull || v_stride > 0xFFFFFFFFull)
-    {
-        return Fail(MUYO_E_CONTRACT, "%s: token strides must be multiples of 4 that hold a token's heads", name);
-    }
-    if (!Aligned16(q) || !Aligned16(k) || !Aligned16(v) || !Aligned16(q_out) || !Aligned16(kcache) ||
-        !Aligned16(vcache) || (reinterpret_cast<uintptr_t>(turns) & 7u) != 0 || !std::isfinite(magnitude))
-    {
-        return Fail(MUYO_E_CONTRACT, "%s: q, k, v, q_out and the caches must be 16-byte aligned, turns 8-byte aligned, "
-                                     "magnitude finite",
-                    name);
-    }
-    const uint64_t cacheBytes = 2 * kdim * pages * page_size;
-    const Range written[] = {{kcache, cacheBytes, "kcache"},
-                             {vcache, cacheBytes, "vcache"},
-                             {q_out, 4 * qdim * tokens, "q_out"}};
-    const Range lists[] = {{positions, 4ull * tokens, "positions"},
-                           {slots, 4ull * tokens, "slots"},
-                           {turns, 4ull * rotary_dim, "turns"}};
-    const Rows sources[] = {{q, 4 * qdim, 4 * q_stride, tokens, "q"},
-                            {k, 4 * kdim, 4 * k_stride, tokens, "k"},
-                            {v, 4 * kdim, 4 * v_stride, tokens, "v"}};
-    for (int i = 0; i < 3; ++i)
-    {
-        const Range& w = written[i];
-        for (int j = i + 1; j < 3; ++j)
-        {
-            if (Overlap(w, written[j]))
-            {
-                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, written[j].name);
-            }
-        }
-        for (const Range& r : lists)
-        {
-            if (Overlap(w, r))
-            {
-                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, r.name);
-            }
-        }
-        for (const Rows& r : sources)
-        {
-            if (i < 2 && Overlap(w, r))
-            {
-                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w.name, r.name);
-            }
-        }
-    }
-    const Range& out = written[2];
-    const Range in[] = {{q, 4 * (q_stride * (tokens - 1) + qdim), "q"},
-                        {k, 4 * (k_stride * (tokens - 1) + kdim), "k"},
-                        {v, 4 * (v_stride * (tokens - 1) + kdim), "v"}};
-    for (const Range& r : in)
-    {
-        // In place over a dense q each thread writes what it alone has read.
-        const bool inPlace = &r == in && q == q_out && q_stride == qdim;
-        if (!inPlace && Overlap(out, r))
-        {
-            return Fail(MUYO_E_CONTRACT, "%s: q_out overlaps %s", name, r.name);
-        }
     }
     AppendArgs a{q, k, v, q_stride, k_stride, v_stride, q_out, static_cast<uint16_t*>(kcache),
                  static_cast<uint16_t*>(vcache), positions, slots, tokens, heads, kv_heads, head_dim, 0,

@@ -1,9 +1,7 @@
 // Attention of single tokens over a paged fp16 cache, many sequences of any lengths in one call.
-#include <algorithm>
 #include <cmath>
 
-#include "common.hpp"
-#include "paged.hpp"
+#include "paged_attention_core.hpp"
 
 namespace muyo
 {
@@ -12,183 +10,24 @@ namespace
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 
-constexpr int kBlock = 256;
-constexpr int kWaves = kBlock / kWave;
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kTile = 32;            // keys of a tile: what a wave takes at a time
 constexpr int kHalves = kTile / 16;       // matrix operands of 16 keys
-constexpr uint32_t kMaxGroup = 16;        // query heads per kv head: the columns of a matrix operation
-constexpr uint32_t kScanQueries = 1024;   // batches up to this many queries: each workgroup makes the sums itself
-// Tables or windows of at most this many keys are not split: 16 sequences of 1 to 1000 keys (28 / 4 heads of
-// 128) take 13.4 us whole, 9.8 and 3.8 for the join split; one of 1000 8.2, 6.7 and 4.4; 250 of 1 to 1000 at
-// 14 / 2 heads of 64 14.7, 17.9 and 4.9.
-constexpr uint32_t kWholeKeys = 1024;
-constexpr uint32_t kMinShare = kWaves;    // a share is at least a tile a wave
-constexpr uint32_t kSetupTiles = 8;       // what a share's change to another (query, kv head) costs, in tiles
-constexpr uint32_t kSplitBlocks = 512;    // workgroups of a split launch: two on each of 256 CUs
 // Softmax weights are held in two planes of f16, which ends at 2^16: the weight of the maximum is 2^kWeightBias, and
 // 2^15 when a later one has run kLag binary orders ahead.
 constexpr float kLag = 4.0f;
 constexpr float kWeightBias = 15.0f - kLag;
 constexpr float kLowScale = 2048.0f;      // of the low plane: what 11 bits of the high one leave, in f16's range again
 
-/// *p for a p that is the same in the whole wave, of memory that nothing writes while the kernel runs: a
-/// scalar load. (Through a vector register the wait for it would also be one for every load before it:
-/// that took a third longer.)
-__device__ __forceinline__ int32_t ScalarLoad(const int32_t* p)
+struct PagedAttentionF16Args : PagedAttentionArgs
 {
-    return *(const __attribute__((address_space(4))) int32_t*)reinterpret_cast<uintptr_t>(p);
-}
+    const uint16_t* kcache;
+    const uint16_t* vcache;
+};
 
 template <bool kOnce>
 __device__ __forceinline__ half8 LoadRow(const uint16_t* p)
 {
     return kOnce ? __builtin_nontemporal_load(reinterpret_cast<const half8*>(p)) : *reinterpret_cast<const half8*>(p);
-}
-
-struct PagedAttentionArgs
-{
-    const float* q;
-    const uint16_t* kcache;
-    const uint16_t* vcache;
-    float* out;
-    const int32_t* tables;
-    uint32_t sequences;
-    uint32_t tablePages;
-    const int32_t* querySequence;
-    const int32_t* positions;
-    uint32_t queries, group, kvHeads;
-    uint32_t pages, pageShift;
-    uint32_t window;
-    float scale;
-    uint32_t* costSums;  // [queries + 1]: CostOf of one kv head of the queries before
-    uint4* cuts;         // what to join: query, kv head, first share, pieces (0: nothing)
-    uint32_t cutsByUnit; // cuts has an entry per (query, kv head); else one per share
-    float* partials;     // [2 * shares][group][4 + headDim]: base, sum, a score's log2 units, -, weighted values
-};
-
-/// The keys begin..end - 1 that a query sees, and the tiles they lie in. A query without any has one
-/// tile of which it sees nothing (its output is 0), one without a sequence none.
-struct KeyRange
-{
-    uint32_t begin, end, firstTile, tiles;
-    uint32_t row;  // of the tables
-};
-
-__device__ __forceinline__ KeyRange RangeOf(const PagedAttentionArgs& a, uint32_t query)
-{
-    const int32_t row = a.querySequence[query];
-    const int32_t position = a.positions[query];
-    const uint32_t capacity = a.tablePages << a.pageShift;  // the host keeps it below 2^31
-    const uint32_t count = position < 0 ? 0 : static_cast<uint32_t>(position) + 1;
-    KeyRange r;
-    r.end = min(count, capacity);
-    r.begin = a.window != 0 && count > a.window ? count - a.window : 0;
-    if (r.begin >= r.end)
-    {
-        r.begin = 0;
-        r.end = 0;
-    }
-    r.firstTile = r.begin / kTile;
-    r.row = static_cast<uint32_t>(row);
-    r.tiles = r.row < a.sequences ? max((r.end + kTile - 1) / kTile - r.firstTile, 1u) : 0;
-    return r;
-}
-
-/// What a (query, kv head) of `tiles` tiles counts in the shares. A change to it (its q, its first tile's
-/// round trips, joining the waves) takes 3 to 4 us, a tile of each wave about one: dealt out by tiles alone,
-/// shares of short sequences had up to four of them. 28 / 4 heads of 128, with a cost of 0, 4, 8 and 12 tiles:
-/// 64 sequences of 1 to 500 keys 27, 15.7, 14.4 and 15.2 us; 250 of 1 to 2000, most short, -, 41, 38 and 43.
-__host__ __device__ constexpr uint32_t CostOf(uint32_t tiles) { return tiles != 0 ? tiles + kSetupTiles : 0; }
-
-/// Inclusive sum over the workgroup's threads, in thread order; `total` is the last one's.
-template <int kThreads>
-__device__ __forceinline__ uint32_t BlockSums(uint32_t v, uint32_t* waveSum, uint32_t& total)
-{
-    const uint32_t lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-    for (uint32_t step = 1; step < kWave; step *= 2)
-    {
-        const uint32_t other = __shfl_up(v, step);
-        v += lane >= step ? other : 0;
-    }
-    __syncthreads();
-    if (lane == kWave - 1)
-    {
-        waveSum[threadIdx.x / kWave] = v;
-    }
-    __syncthreads();
-    total = 0;
-    uint32_t before = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kThreads / kWave; ++w)
-    {
-        before += w < threadIdx.x / kWave ? waveSum[w] : 0;
-        total += waveSum[w];
-    }
-    return v + before;
-}
-
-/// v plus that of the lane a DPP control names, in the given rows of 16 lanes; 0 from no lane.
-template <int kControl, int kRows>
-__device__ __forceinline__ uint32_t PlusLane(uint32_t v)
-{
-    return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kControl, kRows, 0xF, false));
-}
-
-/// Inclusive sum over the wave's lanes: shifts inside rows of 16 lanes, then the last lanes of rows to the
-/// rows behind them.
-__device__ __forceinline__ uint32_t WaveSums(uint32_t v)
-{
-    v = PlusLane<0x111, 0xF>(v);  // row_shr:1
-    v = PlusLane<0x112, 0xF>(v);
-    v = PlusLane<0x114, 0xF>(v);
-    v = PlusLane<0x118, 0xF>(v);
-    v = PlusLane<0x142, 0xA>(v);     // row_bcast:15
-    return PlusLane<0x143, 0xC>(v);  // row_bcast:31
-}
-
-/// The i with sums[i] <= at < sums[i + 1] (sums[0] = 0, at < sums[n]).
-__device__ __forceinline__ uint32_t OwnerOf(const uint32_t* sums, uint32_t n, uint32_t at)
-{
-    uint32_t low = 0;
-    uint32_t high = n;
-    while (high - low > 1)
-    {
-        const uint32_t mid = (low + high) / 2;
-        if (sums[mid] <= at)
-        {
-            low = mid;
-        }
-        else
-        {
-            high = mid;
-        }
-    }
-    return low;
-}
-
-/// The sums of batches of more than kScanQueries queries, by one workgroup before the others start.
-__global__ __launch_bounds__(1024) void PagedCostSumsKernel(PagedAttentionArgs a)
-{
-    __shared__ uint32_t waveSum[1024 / kWave];
-    uint32_t before = 0;
-    for (uint32_t first = 0; first < a.queries; first += 1024)
-    {
-        const uint32_t i = first + threadIdx.x;
-        const uint32_t cost = i < a.queries ? CostOf(RangeOf(a, i).tiles) : 0;
-        uint32_t total;
-        const uint32_t sum = BlockSums<1024>(cost, waveSum, total);
-        if (i < a.queries)
-        {
-            a.costSums[i] = before + sum - cost;
-        }
-        before += total;
-    }
-    if (threadIdx.x == 0)
-    {
-        a.costSums[a.queries] = before;
-    }
 }
 
 /// LDS byte of 16-byte chunk `chunk` of V row `row`: chunks are permuted by the row so that the eight
@@ -243,8 +82,8 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 /// split launch is for long caches, and loads K and V with it. Short ones are a chain of round trips
 /// (position, page, rows), 5.2 us: 8 or 16 waves a workgroup, tiles of 64 keys, and two or three tiles in
 /// flight at head_dim 64 all measured no better or worse.
-template <int kHd, bool kSplit>
-__global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void PagedAttentionKernel(PagedAttentionArgs a)
+template <int kHd, bool kSplit, bool kStats>
+__global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void PagedAttentionKernel(PagedAttentionF16Args a)
 {
     constexpr int kSteps = kHd / 32;               // matrix operations over a head's channels
     constexpr int kChannels = kHd / 16;            // 16-channel blocks of the output
@@ -257,9 +96,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
     __shared__ float waveBase[kWaves][kMaxGroup];
     __shared__ float waveTotal[kWaves][kMaxGroup];
     __shared__ float headScale[kMaxGroup];  // scaleLog2
-    __shared__ uint32_t waveSum[kWaves];
-    __shared__ KeyRange firstRange;
-    __shared__ uint32_t firstAt[2];  // the share's first query, and the costs before it
+    __shared__ ShareSpace space;
 
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -277,73 +114,11 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
     uint4 cut = make_uint4(0, 0, 0, 0);
     if constexpr (kSplit)
     {
-        uint32_t total;
-        if (a.queries <= kWave)
-        {
-            // Every wave makes the sums, a query a lane.
-            KeyRange mine = RangeOf(a, min(lane, a.queries - 1));
-            mine.tiles = lane < a.queries ? mine.tiles : 0;
-            const uint32_t cost = CostOf(mine.tiles);
-            const uint32_t sum = WaveSums(cost);
-            total = __builtin_amdgcn_readlane(sum, kWave - 1);
-            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
-            at = blockIdx.x * share;
-            const uint64_t has = __ballot((sum - cost) * a.kvHeads <= at && at < sum * a.kvHeads);
-            query = has != 0 ? static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(has)) - 1) : 0;
-            queryAt = __builtin_amdgcn_readlane(sum - cost, query) * a.kvHeads;
-            range.begin = __builtin_amdgcn_readlane(mine.begin, query);
-            range.end = __builtin_amdgcn_readlane(mine.end, query);
-            range.firstTile = __builtin_amdgcn_readlane(mine.firstTile, query);
-            range.tiles = __builtin_amdgcn_readlane(mine.tiles, query);
-            range.row = __builtin_amdgcn_readlane(mine.row, query);
-        }
-        else if (a.queries <= kScanQueries)
-        {
-            // Every workgroup makes the sums; the thread that has the share's first query says so.
-            constexpr uint32_t kPer = kScanQueries / kBlock;
-            KeyRange ranges[kPer];
-            uint32_t sum = 0;
-#pragma unroll
-            for (uint32_t e = 0; e < kPer; ++e)
-            {
-                const uint32_t i = threadIdx.x * kPer + e;
-                ranges[e] = RangeOf(a, min(i, a.queries - 1));  // no condition: all loads at once
-                ranges[e].tiles = i < a.queries ? ranges[e].tiles : 0;
-                sum += CostOf(ranges[e].tiles);
-            }
-            const uint32_t all = sum;
-            sum = BlockSums<kBlock>(sum, waveSum, total) - all;
-            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
-            at = blockIdx.x * share;
-#pragma unroll
-            for (uint32_t e = 0; e < kPer; ++e)
-            {
-                const uint32_t i = threadIdx.x * kPer + e;
-                if (sum * a.kvHeads <= at && at < (sum + CostOf(ranges[e].tiles)) * a.kvHeads)
-                {
-                    firstRange = ranges[e];
-                    firstAt[0] = i;
-                    firstAt[1] = sum;
-                }
-                sum += CostOf(ranges[e].tiles);
-            }
-            __syncthreads();
-            query = firstAt[0];
-            queryAt = firstAt[1] * a.kvHeads;
-            range = firstRange;
-        }
-        else
-        {
-            total = a.costSums[a.queries];
-            share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
-            at = blockIdx.x * share;
-            query = OwnerOf(a.costSums, a.queries, min(at / a.kvHeads, total - 1));
-            queryAt = a.costSums[query] * a.kvHeads;
-            range = RangeOf(a, query);
-        }
-        total *= a.kvHeads;
-        stop = min(at + share, total);
-        if (at >= total)
+        const Share first = FirstShare<kTile>(a, lane, space);
+        share = first.share;
+        at = first.at;
+        stop = first.stop;
+        if (at >= stop)
         {
             if (a.cutsByUnit == 0 && threadIdx.x == 0)
             {
@@ -351,13 +126,16 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             }
             return;
         }
+        query = first.query;
+        queryAt = first.queryAt;
+        range = first.range;
         g = 0;
     }
     else
     {
         query = blockIdx.y;
         g = blockIdx.x;
-        range = RangeOf(a, query);
+        range = RangeOf<kTile>(a, query);
     }
 
     uint8_t* const mine = lds + wave * kWaveBytes;
@@ -381,17 +159,17 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             if (range.tiles == 0)  // padding
             {
                 ++query;
-                range = RangeOf(a, query);
+                range = RangeOf<kTile>(a, query);
                 continue;
             }
-            const uint32_t cost = CostOf(range.tiles);
+            const uint32_t cost = CostOf<kTile>(range.tiles);
             g = __builtin_amdgcn_readfirstlane((at - queryAt) / cost);
             unitAt = __builtin_amdgcn_readfirstlane(queryAt + g * cost);
             const uint32_t from = __builtin_amdgcn_readfirstlane(at - unitAt);
             const uint32_t to = __builtin_amdgcn_readfirstlane(min(cost, from + (stop - at)));
             at = unitAt + to;
-            tile0 = from > kSetupTiles ? from - kSetupTiles : 0;
-            tile1 = to > kSetupTiles ? to - kSetupTiles : 0;
+            tile0 = from > kSetupTiles<kTile> ? from - kSetupTiles<kTile> : 0;
+            tile1 = to > kSetupTiles<kTile> ? to - kSetupTiles<kTile> : 0;
             if (tile0 >= tile1)  // its setup alone: the tiles are the next share's
             {
                 continue;
@@ -709,6 +487,15 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             }
         }
         __syncthreads();
+        auto bestOf = [&](uint32_t h) {
+            float best = waveBase[0][h];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w)
+            {
+                best = fmaxf(best, waveBase[w][h]);
+            }
+            return best;
+        };
         for (uint32_t i = threadIdx.x; i < a.group * kHd / 4; i += kBlock)
         {
             const uint32_t h = i / (kHd / 4);
@@ -725,8 +512,12 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             {
                 const float inv = 1.0f / den;
                 const float4v x = den == 0.0f ? float4v{} : num * inv;
-                *reinterpret_cast<float4v*>(
-                    a.out + ((static_cast<uint64_t>(query) * a.kvHeads + g) * a.group + h) * kHd + channel) = x;
+                const uint64_t head = (static_cast<uint64_t>(query) * a.kvHeads + g) * a.group + h;
+                *reinterpret_cast<float4v*>(a.out + head * kHd + channel) = x;
+                if (kStats && channel == 0)
+                {
+                    a.stats[head] = make_float4(bestOf(h), den, headScale[h], 0.0f);
+                }
             }
             else
             {
@@ -735,13 +526,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
                 *reinterpret_cast<float4v*>(slot + 4 + channel) = num;
                 if (channel == 0)
                 {
-                    float best = waveBase[0][h];
-#pragma unroll
-                    for (int w = 1; w < kWaves; ++w)
-                    {
-                        best = fmaxf(best, waveBase[w][h]);
-                    }
-                    slot[0] = best;
+                    slot[0] = bestOf(h);
                     slot[1] = den;
                     slot[2] = headScale[h];
                 }
@@ -752,7 +537,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             __syncthreads();  // the next piece overwrites the results
             if (tile0 == 0)
             {
-                const uint32_t last = (unitAt + CostOf(range.tiles) - 1) / share;
+                const uint32_t last = (unitAt + CostOf<kTile>(range.tiles) - 1) / share;
                 const uint32_t pieces = whole ? 0 : last - blockIdx.x + 1;
                 const uint4 join = make_uint4(query, g, blockIdx.x, pieces);
                 if (a.cutsByUnit == 0)
@@ -768,7 +553,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
             {
                 queryAt = at;
                 ++query;
-                range = RangeOf(a, query);
+                range = RangeOf<kTile>(a, query);
             }
         }
     } while (kSplit && at < stop);
@@ -780,149 +565,80 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
         }
     }
 }
+}  // namespace
 
-/// Joins the pieces of a (query, kv head) that shares cut: blockIdx.x goes over those, or over the shares,
-/// whichever are fewer (a share's end cuts at most one that begins in it). A workgroup per head,
-/// kHd / 4 lanes over the channels of a piece, and kThreads / (kHd / 4) pieces side by side in slices,
-/// kDeep of each in flight. A slice's sums are relative to its own running base, so that nothing waits for
-/// a first pass over the maxima. The order is fixed.
-///
-/// 256 threads have 32 pieces of 128 channels in flight, 512 have 128: one sequence of 32749 keys (28 / 4
-/// heads, 28 workgroups of 128 pieces) takes 4.9 us with 512 threads and 7.6 with 256; 64 sequences (1792
-/// workgroups, most with three pieces) take 8.4 us with 512, whose waves start no faster, and 4.7 with 256.
-template <int kHd, int kThreads>
-__global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAttentionArgs a)
+int CheckAttention(const char* name, const AttentionCall& c, const Range* more, int moreCount, int aligned)
 {
-    constexpr uint32_t kLanes = kHd / 4;
-    constexpr uint32_t kSlices = kThreads / kLanes;
-    constexpr uint32_t kDeep = kThreads / 64;
-    __shared__ float4v sliceNum[kSlices][kLanes];
-    __shared__ float sliceBase[kSlices];
-    __shared__ float sliceDen[kSlices];
-    const uint4 cut = a.cuts[blockIdx.x];
-    const uint32_t pieces = cut.w;
-    // By unit, padding has no entry.
-    if ((a.cutsByUnit != 0 && RangeOf(a, blockIdx.x / a.kvHeads).tiles == 0) || pieces == 0)
+    bool missing = c.q == nullptr || c.out == nullptr || c.tables == nullptr || c.querySequence == nullptr ||
+                   c.positions == nullptr;
+    bool wide = Aligned16(c.q) && Aligned16(c.out);
+    for (int i = 0; i < moreCount; ++i)
     {
-        return;
+        missing = missing || more[i].at == nullptr;
+        wide = wide && (i >= aligned || Aligned16(more[i].at));
     }
-    const uint32_t h = blockIdx.y;
-    const uint32_t lane = threadIdx.x % kLanes;
-    const uint32_t slice = threadIdx.x / kLanes;
-    float top = -INFINITY;
-    float den = 0.0f;
-    float scaleLog2 = 1.0f;  // the head's, in every piece
-    float4v num = float4v{};
-    for (uint32_t p0 = slice; p0 < pieces; p0 += kDeep * kSlices)
+    if (missing)
     {
-        float4v head[kDeep], x[kDeep];
-        float best = top;
-#pragma unroll
-        for (uint32_t i = 0; i < kDeep; ++i)
+        return Fail(MUYO_E_NULL, "%s: every buffer is required", name);
+    }
+    const int checked = CheckPages(name, c.pages, c.pageSize);
+    if (checked != MUYO_OK)
+    {
+        return checked;
+    }
+    if (!AttentionShape(c.queries, c.heads, c.kvHeads, c.headDim))
+    {
+        return Fail(MUYO_E_UNSUPPORTED, "%s: needs 1..65535 queries, heads %% kv_heads == 0, at most 16 heads per kv "
+                                        "head and 1024 in all, head_dim 64 or 128",
+                    name);
+    }
+    if (c.sequences == 0 || c.tablePages == 0 || static_cast<uint64_t>(c.tablePages) * c.pageSize > 0x7FFFFFFFull)
+    {
+        return Fail(MUYO_E_RANGE, "%s: needs sequences >= 1 and table_pages * page_size in 1..2^31 - 1", name);
+    }
+    if (!wide || !std::isfinite(c.scale))
+    {
+        return Fail(MUYO_E_CONTRACT, "%s: q, out and the caches must be 16-byte aligned, and scale finite", name);
+    }
+    if (c.workspace == nullptr || !Aligned16(c.workspace) || c.workspaceBytes < c.need)
+    {
+        return Fail(MUYO_E_CONTRACT, "%s: needs a 16-byte aligned workspace of %llu bytes (got %llu)", name,
+                    static_cast<unsigned long long>(c.need), static_cast<unsigned long long>(c.workspaceBytes));
+    }
+    const uint64_t rowsBytes = 4ull * c.queries * c.heads * c.headDim;
+    const Range out{c.out, rowsBytes, "out"};
+    const Range space{c.workspace, c.need, "workspace"};
+    // The positions, sequences and tables are read again while other workgroups write.
+    const Range lists[] = {{c.q, rowsBytes, "q"},
+                           {c.tables, 4ull * c.sequences * c.tablePages, "tables"},
+                           {c.querySequence, 4ull * c.queries, "query_sequence"},
+                           {c.positions, 4ull * c.queries, "positions"}};
+    if (Overlap(out, space))
+    {
+        return Fail(MUYO_E_CONTRACT, "%s: out overlaps workspace", name);
+    }
+    for (const Range* w : {&out, &space})
+    {
+        for (const Range& r : lists)
         {
-            // Piece 0 begins the (query, kv head), the others are their shares' first.
-            const uint32_t p = min(p0 + i * kSlices, pieces - 1);
-            const float* from = a.partials + (static_cast<uint64_t>(2 * (cut.z + p) + (p == 0 ? 1 : 0)) * a.group +
-                                              h) * (kHd + 4);
-            head[i] = *reinterpret_cast<const float4v*>(from);
-            x[i] = *reinterpret_cast<const float4v*>(from + 4 + 4 * lane);
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < kDeep; ++i)
-        {
-            best = p0 + i * kSlices < pieces ? fmaxf(best, head[i][0]) : best;
-        }
-        scaleLog2 = head[0][2];
-        const float factor = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((top - best) * scaleLog2);
-        top = best;
-        den *= factor;
-        num *= factor;
-#pragma unroll
-        for (uint32_t i = 0; i < kDeep; ++i)
-        {
-            if (p0 + i * kSlices < pieces)
+            // In place a workgroup has read its (query, kv head)'s q when it writes its output there, and one that
+            // is cut is written by the join.
+            const bool inPlace = w == &out && &r == lists && c.q == c.out;
+            if (!inPlace && Overlap(*w, r))
             {
-                // A piece without keys is all 0; one of NaN scores has this base too, and stays NaN.
-                const float w = head[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((head[i][0] - best) * scaleLog2);
-                den = fmaf(w, head[i][1], den);
-                num += w * x[i];
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w->name, r.name);
+            }
+        }
+        for (int i = 0; i < moreCount; ++i)
+        {
+            if (Overlap(*w, more[i]))
+            {
+                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, w->name, more[i].name);
             }
         }
     }
-    sliceNum[slice][lane] = num;
-    if (lane == 0)
-    {
-        sliceBase[slice] = top;
-        sliceDen[slice] = den;
-    }
-    __syncthreads();
-    if (slice == 0)
-    {
-        float best = -INFINITY;
-#pragma unroll
-        for (uint32_t s = 0; s < kSlices; ++s)
-        {
-            best = fmaxf(best, sliceBase[s]);
-        }
-        num = float4v{};
-        den = 0.0f;
-#pragma unroll
-        for (uint32_t s = 0; s < kSlices; ++s)
-        {
-            const float w = sliceBase[s] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((sliceBase[s] - best) * scaleLog2);
-            den = fmaf(w, sliceDen[s], den);
-            num += w * sliceNum[s][lane];
-        }
-        const float4v result = den == 0.0f ? float4v{} : num / den;
-        *reinterpret_cast<float4v*>(
-            a.out + ((static_cast<uint64_t>(cut.x) * a.kvHeads + cut.y) * a.group + h) * kHd + 4 * lane) = result;
-    }
+    return MUYO_OK;
 }
-
-bool AttentionShape(uint32_t queries, uint32_t heads, uint32_t kvHeads, uint32_t headDim)
-{
-    return queries >= 1 && queries <= 65535 && kvHeads >= 1 && heads >= 1 && heads % kvHeads == 0 &&
-           heads / kvHeads <= kMaxGroup && heads <= 1024 && (headDim == 64 || headDim == 128);
-}
-
-/// The workspace's parts: the sums of batches that the workgroups do not sum themselves, the cuts, the
-/// partials.
-size_t CostSumBytes(uint32_t queries)
-{
-    return queries <= kScanQueries ? 0 : (4 * (static_cast<size_t>(queries) + 1) + 15) & ~static_cast<size_t>(15);
-}
-
-constexpr size_t kCutBytes = kSplitBlocks * sizeof(uint4);
-
-template <int kHd>
-hipError_t LaunchPagedAttention(hipStream_t s, PagedAttentionArgs a)
-{
-    const uint64_t keys = std::min<uint64_t>(static_cast<uint64_t>(a.tablePages) << a.pageShift,
-                                             a.window != 0 ? a.window : 0xFFFFFFFFull);
-    const uint64_t units = static_cast<uint64_t>(a.queries) * a.kvHeads;
-    if (keys <= kWholeKeys || units * (keys / kTile + 2 + kSetupTiles) > 0x7FFFFFFFull)
-    {
-        hipLaunchKernelGGL((PagedAttentionKernel<kHd, false>), dim3(a.kvHeads, a.queries), dim3(kBlock), 0, s, a);
-        return hipGetLastError();
-    }
-    if (a.queries > kScanQueries)
-    {
-        hipLaunchKernelGGL(PagedCostSumsKernel, dim3(1), dim3(1024), 0, s, a);
-    }
-    a.cutsByUnit = units < kSplitBlocks ? 1 : 0;
-    const uint32_t joins = a.cutsByUnit != 0 ? static_cast<uint32_t>(units) : kSplitBlocks - 1;
-    hipLaunchKernelGGL((PagedAttentionKernel<kHd, true>), dim3(kSplitBlocks), dim3(kBlock), 0, s, a);
-    if (joins * a.group <= 256)
-    {
-        hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, 512>), dim3(joins, a.group), dim3(512), 0, s, a);
-    }
-    else
-    {
-        hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, 256>), dim3(joins, a.group), dim3(256), 0, s, a);
-    }
-    return hipGetLastError();
-}
-}  // namespace
 }  // namespace muyo
 
 using namespace muyo;
@@ -934,8 +650,7 @@ extern "C" size_t muyo_paged_attention_decode_f16kv_workspace_bytes(uint32_t que
     {
         return 0;
     }
-    return CostSumBytes(queries) + kCutBytes +
-           sizeof(float) * 2 * kSplitBlocks * (heads / kv_heads) * (head_dim + 4);
+    return DecodeWorkspaceBytes(queries, heads, kv_heads, head_dim);
 }
 
 extern "C" int muyo_paged_attention_decode_f16kv(const float* q, const void* kcache, const void* vcache, float* out,
@@ -947,87 +662,25 @@ extern "C" int muyo_paged_attention_decode_f16kv(const float* q, const void* kca
                                                  uint64_t workspace_bytes, void* stream)
 {
     const char* name = "paged_attention_decode_f16kv";
-    if (q == nullptr || kcache == nullptr || vcache == nullptr || out == nullptr || tables == nullptr ||
-        query_sequence == nullptr || positions == nullptr)
-    {
-        return Fail(MUYO_E_NULL, "%s: every buffer is required", name);
-    }
-    const int checked = CheckPages(name, pages, page_size);
+    const uint64_t cacheBytes = 2ull * pages * page_size * kv_heads * head_dim;
+    const Range caches[] = {{kcache, cacheBytes, "kcache"}, {vcache, cacheBytes, "vcache"}};
+    const AttentionCall call{q,       out,      tables,   sequences, table_pages, query_sequence, positions, queries, heads,
+                             kv_heads, head_dim, pages, page_size, scale, workspace, workspace_bytes,
+                             muyo_paged_attention_decode_f16kv_workspace_bytes(queries, heads, kv_heads, head_dim)};
+    const int checked = CheckAttention(name, call, caches, 2, 2);
     if (checked != MUYO_OK)
     {
         return checked;
     }
-    if (!AttentionShape(queries, heads, kv_heads, head_dim))
-    {
-        return Fail(MUYO_E_UNSUPPORTED, "%s: needs 1..65535 queries, heads %% kv_heads == 0, at most 16 heads per kv "
-                                        "head and 1024 in all, head_dim 64 or 128",
-                    name);
-    }
-    if (sequences == 0 || table_pages == 0 || static_cast<uint64_t>(table_pages) * page_size > 0x7FFFFFFFull)
-    {
-        return Fail(MUYO_E_RANGE, "%s: needs sequences >= 1 and table_pages * page_size in 1..2^31 - 1", name);
-    }
-    if (!Aligned16(q) || !Aligned16(kcache) || !Aligned16(vcache) || !Aligned16(out) || !std::isfinite(scale))
-    {
-        return Fail(MUYO_E_CONTRACT, "%s: q, out and the caches must be 16-byte aligned, and scale finite", name);
-    }
-    const size_t need = muyo_paged_attention_decode_f16kv_workspace_bytes(queries, heads, kv_heads, head_dim);
-    if (workspace == nullptr || !Aligned16(workspace) || workspace_bytes < need)
-    {
-        return Fail(MUYO_E_CONTRACT, "%s: needs a 16-byte aligned workspace of %zu bytes (got %llu)", name, need,
-                    static_cast<unsigned long long>(workspace_bytes));
-    }
-    const uint64_t rowsBytes = 4ull * queries * heads * head_dim;
-    const uint64_t cacheBytes = 2ull * pages * page_size * kv_heads * head_dim;
-    // The positions, sequences and tables are read again while other workgroups write.
-    const Range ranges[] = {{out, rowsBytes, "out"},
-                            {workspace, need, "workspace"},
-                            {q, rowsBytes, "q"},
-                            {kcache, cacheBytes, "kcache"},
-                            {vcache, cacheBytes, "vcache"},
-                            {tables, 4ull * sequences * table_pages, "tables"},
-                            {query_sequence, 4ull * queries, "query_sequence"},
-                            {positions, 4ull * queries, "positions"}};
-    constexpr int kOutputs = 2;
-    constexpr int kRanges = static_cast<int>(sizeof ranges / sizeof ranges[0]);
-    for (int i = 0; i < kOutputs; ++i)
-    {
-        for (int j = i + 1; j < kRanges; ++j)
-        {
-            // In place a workgroup has read its (query, kv head)'s q when it writes its output there, and one that
-            // is cut is written by the join.
-            const bool inPlace = i == 0 && j == kOutputs && q == out;
-            if (!inPlace && Overlap(ranges[i], ranges[j]))
-            {
-                return Fail(MUYO_E_CONTRACT, "%s: %s overlaps %s", name, ranges[i].name, ranges[j].name);
-            }
-        }
-    }
-    PagedAttentionArgs a{q,
-                         static_cast<const uint16_t*>(kcache),
-                         static_cast<const uint16_t*>(vcache),
-                         out,
-                         tables,
-                         sequences,
-                         table_pages,
-                         query_sequence,
-                         positions,
-                         queries,
-                         heads / kv_heads,
-                         kv_heads,
-                         pages,
-                         0,
-                         window,
-                         scale,
-                         static_cast<uint32_t*>(workspace),
-                         reinterpret_cast<uint4*>(static_cast<char*>(workspace) + CostSumBytes(queries)),
-                         0,
-                         reinterpret_cast<float*>(static_cast<char*>(workspace) + CostSumBytes(queries) + kCutBytes)};
-    while ((1u << a.pageShift) < page_size)
-    {
-        ++a.pageShift;
-    }
-    const hipError_t launched = head_dim == 64 ? LaunchPagedAttention<64>(AsStream(stream), a)
-                                               : LaunchPagedAttention<128>(AsStream(stream), a);
+    PagedAttentionF16Args a{};
+    FillAttentionArgs(a, call, window);
+    a.kcache = static_cast<const uint16_t*>(kcache);
+    a.vcache = static_cast<const uint16_t*>(vcache);
+    const hipError_t launched =
+        head_dim == 64 ? LaunchPagedAttention<64, kTile, false>(AsStream(stream), a, PagedAttentionKernel<64, false, false>,
+                                                                PagedAttentionKernel<64, true, false>)
+                       : LaunchPagedAttention<128, kTile, false>(AsStream(stream), a,
+                                                                 PagedAttentionKernel<128, false, false>,
+                                                                 PagedAttentionKernel<128, true, false>);
     return launched == hipSuccess ? MUYO_OK : HipStatus(launched, name);
 }

@@ -117,6 +117,7 @@ class MuyoRopeScaling(ctypes.Structure):
 
 
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+KV_INT8, KV_E4M3 = 0, 1
 ROPE_SCALING = dict(NONE=0, LINEAR=1, BASE=2, YARN=3, WAVELENGTH=4)
 
 
@@ -231,6 +232,11 @@ _SIGNATURES = {
     "muyo_paged_attention_decode_f16kv_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32, u32]),
     "muyo_paged_attention_decode_f16kv": (ctypes.c_int, [vp, vp, vp, vp, vp, u32, u32, vp, vp, u32, u32, u32, u32, u32,
                                                          u32, u32, f32, vp, u64, vp]),
+    "muyo_paged_rope_append_q8kv": (ctypes.c_int, [vp, vp, vp, u64, u64, u64, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32,
+                                                   u32, u32, u32, u32, u32, u32, vp, f32, vp]),
+    "muyo_paged_attention_decode_q8kv_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32, u32]),
+    "muyo_paged_attention_decode_q8kv": (ctypes.c_int, [vp, vp, vp, vp, vp, vp, vp, u32, u32, vp, vp, u32, u32, u32, u32,
+                                                        u32, u32, u32, u32, f32, vp, u64, vp]),
     "muyo_token_logprobs_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32]),
     "muyo_token_logprobs_f32": (ctypes.c_int, [vp, u64, u32, u32, vp, vp, vp, vp, u32, vp, vp, vp, u64, vp]),
     "muyo_fill_normal_f16": (ctypes.c_int, [vp, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_double, ctypes.c_double, vp]),
