@@ -11,9 +11,9 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kTile = 64;       // keys of a tile: as many bytes of K and V as 32 of f16
+constexpr uint32_t kTile = 32;       // keys of a tile
 constexpr int kParts = kTile / 16;   // matrix operands of 16 keys
-constexpr int kPlanes = 3;           // of 8 bits: what f32 holds
+constexpr int kPlanes = 3;           // of weights, 8 bits each: what f32 holds
 constexpr float kLag = 4.0f;         // binary orders that a weight may be above 1
 
 struct PagedAttentionQ8Args : PagedAttentionArgs
@@ -36,35 +36,66 @@ __device__ __forceinline__ uint32_t UpperHalves(float first, float second)
     return __builtin_amdgcn_perm(__float_as_uint(second), __float_as_uint(first), 0x07060302u);
 }
 
-/// Four codes as bf16, which holds each: whole numbers of 7 bits, or 4 bits and an exponent.
+/// Eight codes as bf16, which holds each: whole numbers of 7 bits, or 4 bits and an exponent.
 template <int kFormat>
-__device__ __forceinline__ uint2 Widen(uint32_t codes)
+__device__ __forceinline__ bf8 ToBf16(uint32_t lo, uint32_t hi)
 {
-    if constexpr (kFormat == MUYO_KV_INT8)
-    {
-        float x[4];
+    uint4v words;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-        {
-            x[e] = static_cast<float>(static_cast<int8_t>(codes >> (8 * e)));
-        }
-        return make_uint2(UpperHalves(x[0], x[1]), UpperHalves(x[2], x[3]));
-    }
-    else
+    for (int i = 0; i < 2; ++i)
     {
-        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-        const bf2 first = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false);
-        const bf2 second = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true);
-        return make_uint2(__builtin_bit_cast(uint32_t, first), __builtin_bit_cast(uint32_t, second));
+        const uint32_t codes = i == 0 ? lo : hi;
+        if constexpr (kFormat == MUYO_KV_INT8)
+        {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                x[e] = static_cast<float>(static_cast<int8_t>(codes >> (8 * e)));
+            }
+            words[2 * i] = UpperHalves(x[0], x[1]);
+            words[2 * i + 1] = UpperHalves(x[2], x[3]);
+        }
+        else
+        {
+            words[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false));
+            words[2 * i + 1] =
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true));
+        }
     }
+    return __builtin_bit_cast(bf8, words);
 }
 
+/// Eight codes as f16, which holds each too.
 template <int kFormat>
-__device__ __forceinline__ bf8 WidenEight(uint32_t lo, uint32_t hi)
+__device__ __forceinline__ half8 ToF16(uint32_t lo, uint32_t hi)
 {
-    const uint2 a = Widen<kFormat>(lo);
-    const uint2 b = Widen<kFormat>(hi);
-    return __builtin_bit_cast(bf8, uint4v{a.x, a.y, b.x, b.y});
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    uint4v words;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+    {
+        const uint32_t codes = i == 0 ? lo : hi;
+        if constexpr (kFormat == MUYO_KV_INT8)
+        {
+            // 128 above the code, below f16's upper byte of 1024: 1152 above it.
+            const uint32_t above = codes ^ 0x80808080u;
+            const half2v by = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+            const half2v first =
+                __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, above, 0x04010400u)) + by;
+            const half2v second =
+                __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, above, 0x04030402u)) + by;
+            words[2 * i] = __builtin_bit_cast(uint32_t, first);
+            words[2 * i + 1] = __builtin_bit_cast(uint32_t, second);
+        }
+        else
+        {
+            words[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, false));
+            words[2 * i + 1] =
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, true));
+        }
+    }
+    return __builtin_bit_cast(half8, words);
 }
 
 /// Planes of eight f32, each the first 8 bits of what the ones before leave: together exactly the value.
@@ -113,7 +144,7 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 ///     each of the fp16 cache's two; the cache's arrival hides them.
 ///   - scores are raw, q (taken to 1 .. 2 by a power of two) times code times scale, and weights 2^kLag at most.
 template <int kHd, int kFormat, bool kSplit>
-__global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttentionQ8Args a)
+__global__ __launch_bounds__(kBlock, kHd == 64 ? 3 : 2) void PagedAttentionQ8Kernel(PagedAttentionQ8Args a)
 {
     constexpr int kSteps = kHd / 32;             // matrix operations over a head's channels
     constexpr int kChunksK = kHd / 64;           // 16-byte loads of a lane from a K row
@@ -124,6 +155,7 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
     constexpr uint32_t kWaveBytes = kTile * 2 * kHd;  // V of a tile; later O^T of 16 heads in f32
     static_assert(kWaveBytes >= kMaxGroup * kHd * 4, "O^T fits where V was");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaves * kWaveBytes];
+    __shared__ __attribute__((aligned(16))) float waveScales[kWaves][2 * kTile];  // of a tile: K's, V's
     __shared__ float waveBase[kWaves][kMaxGroup];
     __shared__ float waveTotal[kWaves][kMaxGroup];
     __shared__ float headScale[kMaxGroup];  // scaleLog2
@@ -170,6 +202,7 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
     }
 
     uint8_t* const mine = lds + wave * kWaveBytes;
+    float* const scales = waveScales[wave];
     const uint32_t readAt = ValueAt<kHd>(4 * quad + column / 4, column % 4 / 2) + column % 2 * 8;
     do
     {
@@ -237,6 +270,7 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
         // range, and so masked.
         auto pagesOf = [&](uint32_t tile) {
             Pages ids;
+            tile = min(tile, tile1 - 1);
 #pragma unroll
             for (uint32_t part = 0; part < kParts; ++part)
             {
@@ -249,44 +283,49 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
         {
             Pages pages;
             uint4v k[kParts][kChunksK];
-            float4v kscale[kParts];
+            float scale;  // of K's row lane % 32, or of V's in the wave's upper half
             uint4v v[kParts][kPartLoads];
-            float4v vscale[kParts];
         };
-        Tile now;
+        Tile even, odd;  // two tiles are on their way
         // A tile's K, then its V: loads complete in order, and the scores wait only for K. Pages outside the
-        // cache are read as page 0, whose rows are then masked.
-        auto request = [&](uint32_t tile, const Pages& pages) {
+        // cache are read as page 0, whose rows are then masked. Tiles past the last are requests for one row of it:
+        // a request under a condition would make the waits for the other tile ones for everything.
+        auto request = [&](Tile& now, uint32_t tile, const Pages& pages) {
+            const uint32_t lanes = tile < tile1 ? ~0u : 0u;
+            tile = min(tile, tile1 - 1);
             now.pages = pages;
             uint64_t base[kParts];
 #pragma unroll
             for (uint32_t part = 0; part < kParts; ++part)
             {
-                const uint32_t page = pages.of[part] < a.pages ? pages.of[part] : 0;
+                const uint32_t page = now.pages.of[part] < a.pages ? now.pages.of[part] : 0;
                 const uint32_t row = ((range.firstTile + tile) * kTile + 16 * part) & (pageSize - 1);
                 base[part] = ((static_cast<uint64_t>(page) * a.kvHeads + g) << a.pageShift) + row;
             }
+            const uint32_t keyAt = (column * kHd + 16 * quad) & lanes;
+            const uint32_t valueAt = (lane * 16) & lanes;
 #pragma unroll
             for (uint32_t part = 0; part < kParts; ++part)
             {
 #pragma unroll
                 for (int i = 0; i < kChunksK; ++i)
                 {
-                    now.k[part][i] =
-                        LoadOnce<kSplit, uint4v>(a.kcache + base[part] * kHd + (column * kHd + 16 * quad) + 64 * i);
+                    now.k[part][i] = LoadOnce<kSplit, uint4v>(a.kcache + base[part] * kHd + keyAt + 64 * i);
                 }
-                now.kscale[part] = LoadOnce<kSplit, float4v>(a.kscales + base[part] + 4 * quad);
             }
+            static_assert(kTile == 32 && kParts == 2, "a lane for each scale");
+            const uint64_t first = base[0];
+            const uint64_t second = base[1];
+            now.scale = LoadOnce<kSplit, float>((lane < 32 ? a.kscales : a.vscales) +
+                                                (quad % 2 == 0 ? first : second) + column);
 #pragma unroll
             for (uint32_t part = 0; part < kParts; ++part)
             {
 #pragma unroll
                 for (int j = 0; j < kPartLoads; ++j)
                 {
-                    now.v[part][j] =
-                        LoadOnce<kSplit, uint4v>(a.vcache + base[part] * kHd + lane * 16 + j * kRows * kHd);
+                    now.v[part][j] = LoadOnce<kSplit, uint4v>(a.vcache + base[part] * kHd + valueAt + j * kRows * kHd);
                 }
-                now.vscale[part] = LoadOnce<kSplit, float4v>(a.vscales + base[part] + 4 * quad);
             }
             __builtin_amdgcn_sched_barrier(0);
         };
@@ -299,14 +338,16 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
         }
         float base = -INFINITY;  // the raw score that weights are relative to; -inf: none yet
         float runSum = 0.0f;     // of this lane's keys
-        // A wave without a tile requests the last one and leaves it: a request under a condition would make
-        // the wait for q one for everything.
-        request(min(tile0 + wave, tile1 - 1), pagesOf(min(tile0 + wave, tile1 - 1)));
-        Pages next = pagesOf(min(tile0 + wave + kWaves, tile1 - 1));  // of the next tile to request
+        {
+            const Pages first = pagesOf(tile0 + wave);
+            const Pages second = pagesOf(tile0 + wave + kWaves);
+            request(even, tile0 + wave, first);
+            request(odd, tile0 + wave + kWaves, second);
+        }
 
-        // The group's heads as columns; columns past it are 0. q over the power of two below its largest value:
-        // products with codes stay far from f32's end.
-        bf8 qp[kSteps][kPlanes];
+        // The group's heads as columns; columns past it are 0. Planes of q / 2^e, whose largest value is below 2^14:
+        // f16 then holds any q, and its small values with their bits where K makes them count.
+        half8 qhi[kSteps], qlo[kSteps];
         float scaleLog2;
         {
             float largest = 0.0f;
@@ -326,7 +367,7 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
             {
                 (void)frexpf(largest, &e);
             }
-            e -= 1;
+            e -= 14;
             // A negative scale turns q's sign, and 0 clears q, so that scores are scaled by a positive number.
             const float sign = column >= a.group || a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
             // Finite and above 0: no difference of raw scores makes a NaN of it.
@@ -335,35 +376,40 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)
             {
-                float x[8];
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                 {
-                    x[c] = column >= a.group ? 0.0f : ldexpf(qv[s][c / 4][c % 4], -e) * sign;
+                    const float x = column >= a.group ? 0.0f : ldexpf(qv[s][c / 4][c % 4], -e) * sign;
+                    qhi[s][c] = static_cast<_Float16>(x);
+                    qlo[s][c] = static_cast<_Float16>(x - static_cast<float>(qhi[s][c]));
                 }
-                Split(x, qp[s]);
             }
         }
 
-        for (uint32_t tile = tile0 + wave; tile < tile1; tile += kWaves)
-        {
-            const Pages afterNext = pagesOf(min(tile + 2 * kWaves, tile1 - 1));
+        auto take = [&](Tile& now, uint32_t tile) {
+            const Pages next = pagesOf(tile + 2 * kWaves);  // on their way while the scores are made
+            __builtin_amdgcn_sched_barrier(0);
             float4v score[kParts];
 #pragma unroll
             for (int part = 0; part < kParts; ++part)
             {
                 score[part] = float4v{};
+            }
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s)
+            for (int s = 0; s < kSteps; ++s)
+            {
+                half8 k[kParts];
+#pragma unroll
+                for (int part = 0; part < kParts; ++part)
                 {
-                    const bf8 k = WidenEight<kFormat>(now.k[part][s / 2][2 * (s % 2)], now.k[part][s / 2][2 * (s % 2) + 1]);
-#pragma unroll
-                    for (int p = kPlanes - 1; p >= 0; --p)
-                    {
-                        score[part] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qp[s][p], score[part], 0, 0, 0);
-                    }
+                    k[part] = ToF16<kFormat>(now.k[part][s / 2][2 * (s % 2)], now.k[part][s / 2][2 * (s % 2) + 1]);
+                    score[part] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[part], qlo[s], score[part], 0, 0, 0);
                 }
-                score[part] *= now.kscale[part];
+#pragma unroll
+                for (int part = 0; part < kParts; ++part)
+                {
+                    score[part] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[part], qhi[s], score[part], 0, 0, 0);
+                }
             }
             const uint32_t key0 = (range.firstTile + tile) * kTile;
             bool inside = key0 >= range.begin && key0 + kTile <= range.end;
@@ -371,6 +417,22 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
             for (uint32_t part = 0; part < kParts; ++part)
             {
                 inside = inside && now.pages.of[part] < a.pages;
+            }
+            if (!inside && lane >= 32)
+            {
+                const uint32_t key = key0 + lane % 32;
+                const bool first = now.pages.of[0] < a.pages;
+                const bool second = now.pages.of[1] < a.pages;
+                const bool there = quad % 2 == 0 ? first : second;
+                now.scale = there && key >= range.begin && key < range.end ? now.scale : 0.0f;
+            }
+            scales[lane] = now.scale;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+            {
+                score[part] *= *reinterpret_cast<const float4v*>(scales + 16 * part + 4 * quad);
             }
             if (!inside)
             {
@@ -394,35 +456,28 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
                         if (!there || key < range.begin || key >= range.end)
                         {
                             score[part][r] = -INFINITY;
-                            now.vscale[part][r] = 0.0f;
                         }
                     }
                 }
             }
-            float4v vscale[kParts];
 #pragma unroll
             for (uint32_t part = 0; part < kParts; ++part)
             {
-                vscale[part] = now.vscale[part];
 #pragma unroll
                 for (int j = 0; j < kPartLoads; ++j)
                 {
                     const uint32_t row = 16 * part + j * kRows + lane / kLanesV;
                     const uint32_t chunk = 2 * (lane % kLanesV);
                     const uint4v codes = now.v[part][j];
-                    *reinterpret_cast<bf8*>(mine + ValueAt<kHd>(row, chunk)) = WidenEight<kFormat>(codes[0], codes[1]);
+                    *reinterpret_cast<bf8*>(mine + ValueAt<kHd>(row, chunk)) = ToBf16<kFormat>(codes[0], codes[1]);
                     *reinterpret_cast<bf8*>(mine + ValueAt<kHd>(row, chunk + 1)) =
-                        WidenEight<kFormat>(codes[2], codes[3]);
+                        ToBf16<kFormat>(codes[2], codes[3]);
                 }
             }
             // The wave's LDS operations complete in order; this keeps the compiler's order too.
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            if (tile + kWaves < tile1)
-            {
-                request(tile + kWaves, next);
-                next = afterNext;
-            }
+            request(now, tile + 2 * kWaves, next);
 
             float tileMax = -INFINITY;
 #pragma unroll
@@ -458,11 +513,13 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
                 for (int part = 0; part < 2; ++part)
                 {
                     float4v p;
+                    const float4v vscale =
+                        *reinterpret_cast<const float4v*>(scales + 32 + 16 * (2 * pair + part) + 4 * quad);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                     {
                         p[r] = __builtin_amdgcn_exp2f((score[2 * pair + part][r] - from) * scaleLog2);
-                        scaled[4 * part + r] = p[r] * vscale[2 * pair + part][r];
+                        scaled[4 * part + r] = p[r] * vscale[r];
                     }
                     sum += (p[0] + p[1]) + (p[2] + p[3]);
                 }
@@ -490,6 +547,17 @@ __global__ __launch_bounds__(kBlock, 2) void PagedAttentionQ8Kernel(PagedAttenti
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
+        };
+        uint32_t tile = tile0 + wave;
+        // In pairs: a way out between them would meet the way round, where the compiler then waits for both.
+        for (; tile + kWaves < tile1; tile += 2 * kWaves)
+        {
+            take(even, tile);
+            take(odd, tile + kWaves);
+        }
+        if (tile < tile1)
+        {
+            take(even, tile);
         }
 
         // The four waves' results meet in LDS.
