@@ -149,6 +149,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 3 : 2) void PagedAttentionQ8Ker
     constexpr int kSteps = kHd / 32;             // matrix operations over a head's channels
     constexpr int kChunksK = kHd / 64;           // 16-byte loads of a lane from a K row
     constexpr int kChannels = kHd / 16;          // 16-channel blocks of the output
+    constexpr int kAtOnce = 4;                   // of them
     constexpr uint32_t kLanesV = kHd / 16;       // lanes of a V row
     constexpr uint32_t kRows = kWave / kLanesV;  // V rows of one load of the wave
     constexpr int kPartLoads = 16 / kRows;       // V loads of 16 keys
@@ -478,6 +479,22 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 3 : 2) void PagedAttentionQ8Ker
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             request(now, tile + 2 * kWaves, next);
+            // V of some channels, transposed; the first are on their way while the weights are made.
+            auto valuesOf = [&](int group, bf8 (&vt)[kAtOnce]) {
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i)
+                {
+                    uint8_t* row = mine + (readAt ^ (32u * (group * kAtOnce + i)));
+                    const short4v first = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) short4v*)row);
+                    const short4v second = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) short4v*)(row + 16 * 2 * kHd));
+                    vt[i] = __builtin_bit_cast(bf8, __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+            };
+            bf8 vt[kAtOnce];
+            valuesOf(0, vt);
+            __builtin_amdgcn_sched_barrier(0);
 
             float tileMax = -INFINITY;
 #pragma unroll
@@ -502,47 +519,49 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 3 : 2) void PagedAttentionQ8Ker
                     o[c] *= factor;
                 }
             }
-            bf8 weights[kParts / 2][kPlanes];
+            bf8 weights[kPlanes];
             const float from = base == -INFINITY ? 0.0f : base;  // without keys so far every score is -inf
             float sum = 0.0f;
+            float scaled[8];
 #pragma unroll
-            for (int pair = 0; pair < kParts / 2; ++pair)
+            for (int part = 0; part < kParts; ++part)
             {
-                float scaled[8];
+                float4v p;
+                const float4v vscale = *reinterpret_cast<const float4v*>(scales + 32 + 16 * part + 4 * quad);
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+                for (int r = 0; r < 4; ++r)
                 {
-                    float4v p;
-                    const float4v vscale =
-                        *reinterpret_cast<const float4v*>(scales + 32 + 16 * (2 * pair + part) + 4 * quad);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                    {
-                        p[r] = __builtin_amdgcn_exp2f((score[2 * pair + part][r] - from) * scaleLog2);
-                        scaled[4 * part + r] = p[r] * vscale[r];
-                    }
-                    sum += (p[0] + p[1]) + (p[2] + p[3]);
+                    p[r] = __builtin_amdgcn_exp2f((score[part][r] - from) * scaleLog2);
+                    scaled[4 * part + r] = p[r] * vscale[r];
                 }
-                Split(scaled, weights[pair]);
+                sum += (p[0] + p[1]) + (p[2] + p[3]);
             }
+            Split(scaled, weights);
             runSum += sum;
+            // A group's planes in turn over its channels: sums that do not wait for one another.
 #pragma unroll
-            for (int c = 0; c < kChannels; ++c)
+            for (int group = 0; group < kChannels / kAtOnce; ++group)
             {
-#pragma unroll
-                for (int pair = 0; pair < kParts / 2; ++pair)
+                bf8 later[kAtOnce];
+                if (group + 1 < kChannels / kAtOnce)
                 {
-                    uint8_t* row = mine + ((readAt ^ (32u * c)) + pair * 32 * 2 * kHd);
-                    const short4v first = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) short4v*)row);
-                    const short4v second = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) short4v*)(row + 16 * 2 * kHd));
-                    const bf8 vt = __builtin_bit_cast(bf8, __builtin_shufflevector(first, second, 0, 1, 2, 3, 4, 5, 6, 7));
+                    valuesOf(group + 1, later);
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int p = kPlanes - 1; p >= 0; --p)
+                for (int p = kPlanes - 1; p >= 0; --p)
+                {
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i)
                     {
-                        o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, weights[pair][p], o[c], 0, 0, 0);
+                        const int c = group * kAtOnce + i;
+                        o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt[i], weights[p], o[c], 0, 0, 0);
                     }
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i)
+                {
+                    vt[i] = later[i];
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
