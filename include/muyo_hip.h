@@ -692,6 +692,28 @@ int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride, uint32_t r
                             int32_t* top_ids, float* top_logprobs, void* workspace, uint64_t workspace_bytes,
                             void* stream);
 
+/* The next token of each row of logits [rows][vocab] (f32, `row_stride` values apart) by the row's own settings, from
+ * one given random number of [0, 1). With the order of falling logits, equal ones by rising index, and weights
+ * w = exp((x - max) / temperatures[r]), the tokens kept are, in that order,
+ *   the first top_ks[r] (all where that is below 1), and of these
+ *   the fewest first ones that have at least top_ps[r] of their weight (all where that is 1 or more), and of these
+ *   those with w >= min_ps[r] (all where that is 0 or less); always the first.
+ * tokens[r] is the first of those kept, by rising index, up to which they have more than randoms[r] of the weight
+ * of all kept; logprobs[r] (may be NULL) the log of its share of that. A temperature that is not above 0 takes the
+ * order's first token (logprob 0). A NULL array is a setting that is off (temperatures: 1). Weights and their sums
+ * are good to some 2^-39, and weights under 2^-60 of the largest are 0.
+ * A logit of -inf or NaN is never taken, one of +inf counts as the largest finite one. A row of nothing else
+ * than the former has token -1 and logprob -inf. Numbers below 0 (and NaN) count as 0, from 1 on take the
+ * last token kept. At most 2^24 logits a row, and fewer than 2^22 rows. tokens, logprobs and the workspace
+ * overlap nothing else (they may lie between rows of logits). `workspace` as above, of at least
+ * muyo_sample_rows_workspace_bytes(...) bytes. The single row that a chat samples, with its repetition penalty and
+ * its own generator, is muyo_sample_f32's. */
+size_t muyo_sample_rows_workspace_bytes(uint32_t rows, uint32_t vocab); /* 0: unsupported */
+int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
+                         const float* temperatures, const int32_t* top_ks, const float* top_ps, const float* min_ps,
+                         const double* randoms, int32_t* tokens, float* logprobs, void* workspace,
+                         uint64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Synthetic-input helpers (portable seeded generator; bit-identical on host and device).
  *   word(seed, i)   = mix64(mix64(seed) + i)            mix64 = SplitMix64's finaliser

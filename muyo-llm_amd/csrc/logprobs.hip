@@ -7,7 +7,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "common.hpp"
+#include "logit_order.hpp"
 
 namespace muyo
 {
@@ -45,26 +45,6 @@ struct LogprobArgs
     float4* sums;     // [rows][parts]: m, s, t, tokens before the given one (bits)
     uint64_t* keys;   // [rows][parts][top]
 };
-
-/// The order's upper word: rises with the value. -0 counts as +0, NaN comes before -inf.
-__device__ __forceinline__ uint32_t OrderBits(float v)
-{
-    const uint32_t u = __float_as_uint(v + 0.0f);
-    const uint32_t ordered = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
-    return v != v ? 0u : ordered;
-}
-
-/// A 64-bit key whose descending order is (value descending, index ascending). 0 is below every key.
-__device__ __forceinline__ uint64_t OrderKey(float v, uint32_t index)
-{
-    return (static_cast<uint64_t>(OrderBits(v)) << 32) | static_cast<uint64_t>(~index);
-}
-
-__device__ __forceinline__ float KeyValue(uint64_t key)
-{
-    const uint32_t o = static_cast<uint32_t>(key >> 32);
-    return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);  // 0 is a NaN
-}
 
 /// `key` of lane `lane` (the same in every lane), in every lane.
 __device__ __forceinline__ uint64_t KeyOfLane(uint64_t key, uint32_t lane)

@@ -239,6 +239,8 @@ _SIGNATURES = {
                                                         u32, u32, u32, u32, f32, vp, u64, vp]),
     "muyo_token_logprobs_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32]),
     "muyo_token_logprobs_f32": (ctypes.c_int, [vp, u64, u32, u32, vp, vp, vp, vp, u32, vp, vp, vp, u64, vp]),
+    "muyo_sample_rows_workspace_bytes": (ctypes.c_size_t, [u32, u32]),
+    "muyo_sample_rows_f32": (ctypes.c_int, [vp, u64, u32, u32, vp, vp, vp, vp, vp, vp, vp, vp, u64, vp]),
     "muyo_fill_normal_f16": (ctypes.c_int, [vp, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_double, ctypes.c_double, vp]),
     "muyo_fill_normal_f32": (ctypes.c_int, [vp, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_double, ctypes.c_double, vp]),
     "muyo_fill_uniform_f32": (ctypes.c_int, [vp, ctypes.c_uint64, ctypes.c_uint64, vp]),
