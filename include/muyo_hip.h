@@ -701,7 +701,7 @@ int muyo_token_logprobs_f32(const float* logits, uint64_t row_stride, uint32_t r
  * tokens[r] is the first of those kept, by rising index, up to which they have more than randoms[r] of the weight
  * of all kept; logprobs[r] (may be NULL) the log of its share of that. A temperature that is not above 0 takes the
  * order's first token (logprob 0). A NULL array is a setting that is off (temperatures: 1). Weights and their sums
- * are good to some 2^-39, and weights under 2^-60 of the largest are 0.
+ * are good to some 2^-39, and weights under 2^-50 of the largest may count as 0.
  * A logit of -inf or NaN is never taken, one of +inf counts as the largest finite one. A row of nothing else
  * than the former has token -1 and logprob -inf. Numbers below 0 (and NaN) count as 0, from 1 on take the
  * last token kept. At most 2^24 logits a row, and fewer than 2^22 rows. tokens, logprobs and the workspace

@@ -3,7 +3,9 @@
 // A logit x has a place on a grid of eighths of an octave of weight, y = x 8 log2(e) / temperature = g + f, g whole
 // and f within half a step of 0: its weight is 2^(g / 8) 2^(f / 8). The second factor, near 1, is held as a whole
 // number of 2^-38, so that the mass of all logits in the same step is an exact sum in any order, and weights of
-// different steps meet as 64-bit floating-point numbers in a fixed order: the same call gives the same bits.
+// different steps meet as 64-bit floating-point numbers in a fixed order: the same call gives the same bits. Sums in
+// 32 bits would not do: a number lands on another token where the sums before it are off, which of 151936 tokens of
+// similar weight one row in ten would see.
 #include <algorithm>
 #include <cmath>
 
@@ -17,27 +19,30 @@ constexpr int kBlock = 256;                    // threads that count a part of a
 constexpr int kWaves = kBlock / kWave;
 constexpr int kSteps = 512;                    // of the grid, from the row's largest logit down: 64 octaves
 constexpr int kSlack = 8;                      // steps above the largest logit so far
-constexpr int kLoads = 16;                     // of a lane at a time
-constexpr uint32_t kBatch = kWave * kLoads;    // logits a wave takes at a time
+constexpr int kQuads = 4;                      // 16-byte loads of a lane's batch
+constexpr uint32_t kBatch = kWave * 4 * kQuads;  // logits a wave takes at a time
 constexpr int kPickBlock = 1024;               // threads that decide a row
 constexpr int kPickWaves = kPickBlock / kWave;
 constexpr int kPickLoads = 8;
 constexpr uint32_t kGroup = kWave * kPickLoads;  // logits of a sum on the way to the token
-constexpr uint32_t kListed = 4096;             // logits of a step that are listed
+constexpr uint32_t kListed = 4096;             // logits that are listed
+constexpr int32_t kListedK = 2048;             // a top-k up to which listing the tokens is likely to do
+constexpr uint32_t kDigits = 256;
+constexpr uint32_t kFew = kWave;               // candidates that a wave looks at one by one
 constexpr uint32_t kMaxParts = 64;             // workgroups of a row
 constexpr uint32_t kMaxRows = (1u << 22) - 1;  // a launch has fewer than 2^32 threads
 constexpr uint32_t kMaxVocab = 1u << 24;       // masses of so many logits fit in 63 bits
 constexpr uint32_t kBlocksAtOnce = 256 * 6;    // workgroups that 256 CUs run at once
 constexpr double kLog2e = 1.44269504088896340736;
-constexpr double kLn2 = 0.69314718055994530942;
-constexpr double kUnit = 0x1p-38;              // of a mass
+constexpr double kFar = 0x1p48;                // places whose rounding errors are not within half a step
+constexpr double kFixed = 0x1p50;              // units of the top step's weight, for sums of listed logits
 
 /// What a part of a row says besides its counts.
 struct PartHead
 {
     double top;    // the grid's place of its first step, -inf: it has none
     float most;    // its largest logit
-    uint32_t at;   // the first place of that
+    uint32_t at;   // the first place of that, of a greedy row
 };
 
 struct SampleArgs
@@ -58,15 +63,30 @@ struct SampleArgs
     uint32_t* counts;    // [rows][parts][kSteps]
 };
 
-/// A logit as it counts: -inf for NaN, the largest finite one for +inf.
-__device__ __forceinline__ float Counted(float x) { return x == x ? fminf(x, 0x1.fffffep127f) : -INFINITY; }
+/// What a row asks for.
+struct RowMode
+{
+    double perUnit;  // steps of the grid per unit of a logit; below 0: the largest logit is taken
+    int32_t topK;    // 0: all
+    bool counted;    // logits of a step are counted, for top-k
+    bool weighed;    // their masses are summed; where few tokens are kept at most, these are listed instead
+};
 
-/// Steps of the grid per unit of a logit, 0 for a greedy row.
-__device__ __forceinline__ double StepsPerUnit(const SampleArgs& a, uint32_t row)
+__device__ __forceinline__ RowMode ModeOf(const SampleArgs& a, uint32_t row)
 {
     const float t = a.temperatures != nullptr ? a.temperatures[row] : 1.0f;
-    return t > 0.0f ? 8.0 * kLog2e / static_cast<double>(t) : -1.0;
+    RowMode mode;
+    // Above 0 also where the temperature is infinite, so that a logit of -inf is as far away as elsewhere.
+    mode.perUnit = t > 0.0f ? fmax(8.0 * kLog2e / static_cast<double>(t), 1e-290) : -1.0;
+    mode.topK = a.topKs != nullptr ? max(a.topKs[row], 0) : 0;
+    mode.counted = mode.topK > 0;
+    mode.weighed = mode.topK == 0 || mode.topK > kListedK;
+    return mode;
 }
+
+/// A logit as it counts: -inf for NaN (the larger of a NaN and a number is the number), the largest finite one for
+/// +inf.
+__device__ __forceinline__ float Counted(float x) { return fminf(fmaxf(x, -INFINITY), 0x1.fffffep127f); }
 
 /// A logit's place on the grid.
 struct Place
@@ -75,7 +95,9 @@ struct Place
     double rest;  // from its middle
 };
 
-/// The same bits wherever it is computed: nothing is contracted.
+/// The same bits wherever it is computed: nothing is contracted. kBounded: also right past kFar, where steps are
+/// whole numbers apart and `rest` would be a rounding error of any size.
+template <bool kBounded = true>
 __device__ __forceinline__ Place PlaceOf(float x, double perUnit)
 {
 #pragma clang fp contract(off)
@@ -85,35 +107,59 @@ __device__ __forceinline__ Place PlaceOf(float x, double perUnit)
     const double left = fma(y, perUnit, -p);
     Place at;
     at.step = rint(p);
-    // Places past 2^50 are whole steps apart, if they differ at all.
-    at.rest = fmin(fmax((p - at.step) + left, -0.75), 0.75);
+    at.rest = (p - at.step) + left;
+    if (kBounded)
+    {
+        at.rest = fmin(fmax(at.rest, -0.75), 0.75);
+    }
     return at;
 }
 
-/// 2^(rest / 8) in units of 2^-38: a power series, whose next term is below 2^-49 (|rest / 8 ln 2| <= 0.065).
+/// 2^(rest / 8) in units of 2^-38, by a polynomial (the fit of least error over half a step each way: 2^-41.6), to
+/// a whole number by 2^52, whose bits then go.
 __device__ __forceinline__ uint64_t MassOf(double rest)
 {
-    const double z = rest * (kLn2 / 8.0);
-    double s = 1.0 / 5040.0;
-    s = fma(s, z, 1.0 / 720.0);
-    s = fma(s, z, 1.0 / 120.0);
-    s = fma(s, z, 1.0 / 24.0);
-    s = fma(s, z, 1.0 / 6.0);
-    s = fma(s, z, 0.5);
-    s = fma(s, z, 1.0);
-    s = fma(s, z, 1.0);
-    // Rounded to a whole number by 2^52, whose bits then go.
-    return static_cast<uint64_t>(__double_as_longlong(fma(s, 1.0 / kUnit, 0x1p52))) & 0xFFFFFFFFFFFFFull;
+    constexpr double kOne = 0x1p38;
+    double s = 4.069392558613428e-08 * kOne;
+    s = fma(s, rest, 2.3483963990465326e-06 * kOne);
+    s = fma(s, rest, 0.00010840646184941278 * kOne);
+    s = fma(s, rest, 0.0037535391505790455 * kOne);
+    s = fma(s, rest, 0.08664339757000515 * kOne);
+    s = fma(s, rest, 1.0000000000002864 * kOne + 0x1p52);
+    return static_cast<uint64_t>(__double_as_longlong(s)) & 0xFFFFFFFFFFFFFull;
 }
 
-/// The weight of a mass in the `d`-th step from the top, relative to that.
-__device__ __forceinline__ double WeightOf(uint64_t mass, uint32_t d)
+/// Weight of a unit of mass in step d, relative to the top's.
+__device__ __forceinline__ double UnitOf(uint32_t d) { return exp2(-38.0 - static_cast<double>(d) * 0.125); }
+
+template <bool kCount, bool kMass, bool kBounded>
+__device__ __forceinline__ void AddBatch(const float (&v)[4 * kQuads], double top, double perUnit, uint64_t* masses,
+                                         uint32_t* counts)
 {
-    return static_cast<double>(mass) * exp2(-38.0 - static_cast<double>(d) * 0.125);
+#pragma unroll
+    for (int i = 0; i < 4 * kQuads; ++i)
+    {
+        const Place place = PlaceOf<kBounded>(v[i], perUnit);
+        const double d = top - place.step;
+        if (d < kSteps)
+        {
+            const uint32_t step = static_cast<uint32_t>(d);
+            if (kMass)
+            {
+                atomicAdd(reinterpret_cast<unsigned long long*>(masses + step), MassOf(place.rest));
+            }
+            if (kCount)
+            {
+                atomicAdd(counts + step, 1u);
+            }
+        }
+    }
 }
 
 /// Counts the logits of a part of a row in steps of the grid, and their masses. A wave has counters of its own in
 /// LDS, from a step above the largest logit that it has met; a larger one moves them down, which is rare.
+///
+/// What bounds it: the arithmetic in 64 bits, some 22 operations a logit with its mass and 12 without.
 __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
 {
     __shared__ uint64_t massOf[kWaves][kSteps];
@@ -128,7 +174,8 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
     const uint32_t begin = part * a.partLength;
     const uint32_t end = min(begin + a.partLength, a.vocab);
     const float* const x = a.logits + row * a.stride;
-    const double perUnit = StepsPerUnit(a, row);
+    const RowMode mode = ModeOf(a, row);
+    const bool greedy = mode.perUnit < 0.0;
     uint64_t* const masses = massOf[wave];
     uint32_t* const counts = countOf[wave];
     for (int i = lane; i < kSteps; i += kWave)
@@ -137,36 +184,67 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
         counts[i] = 0;
     }
     double top = -INFINITY;
-    float most = -INFINITY;
+    float most = -INFINITY;  // of the wave; of a greedy row's lane
     uint32_t at = 0;
-    for (uint32_t first = begin + wave * kBatch; first < end; first += kWaves * kBatch)
+    // 16-byte loads from the last such address at or before the part's first logit; batches that reach over an end
+    // of the part go logit by logit.
+    const uint32_t before = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x + begin) / 4 % 4);
+    for (uint32_t first = wave * kBatch; first < end - begin + before; first += kWaves * kBatch)
     {
-        float v[kLoads];
-#pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i)
+        float v[4 * kQuads];
+        // A lane's logits: four in a row from each quad.
+        auto indexOf = [&](uint32_t i) { return begin - before + first + (i / 4 * kWave + lane) * 4 + i % 4; };
+        if (first >= before && first + kBatch <= end - begin + before)
         {
-            const uint32_t index = first + i * kWave + lane;
-            v[i] = x[min(index, end - 1)];
-        }
-        float batchMost = -INFINITY;
 #pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i)
-        {
-            const uint32_t index = first + i * kWave + lane;
-            v[i] = index < end ? Counted(v[i]) : -INFINITY;
-            batchMost = fmaxf(batchMost, v[i]);
-            if (v[i] > most)
+            for (uint32_t q = 0; q < kQuads; ++q)
             {
-                most = v[i];
-                at = index;
+                const float4v four = *reinterpret_cast<const float4v*>(x + indexOf(4 * q));
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                {
+                    v[4 * q + e] = Counted(four[e]);
+                }
             }
         }
+        else
+        {
+#pragma unroll
+            for (uint32_t i = 0; i < 4 * kQuads; ++i)
+            {
+                // Before the part's first logit the index wraps or is too small: both are left out.
+                const uint32_t index = indexOf(i);
+                const bool inside = index >= begin && index < end;
+                const float one = x[inside ? index : begin];
+                v[i] = inside ? Counted(one) : -INFINITY;
+            }
+        }
+        float batchMost = v[0];
+#pragma unroll
+        for (uint32_t i = 1; i < 4 * kQuads; ++i)
+        {
+            batchMost = fmaxf(batchMost, v[i]);
+        }
+        if (greedy)
+        {
+            if (batchMost > most)
+            {
+                most = batchMost;
+#pragma unroll
+                for (int i = 4 * kQuads - 1; i >= 0; --i)
+                {
+                    at = v[i] == batchMost ? indexOf(i) : at;
+                }
+            }
+            continue;
+        }
         batchMost = GroupMax<kWave>(batchMost);
-        if (perUnit < 0.0 || batchMost == -INFINITY)
+        most = fmaxf(most, batchMost);
+        if (batchMost == -INFINITY)
         {
             continue;
         }
-        const double highest = PlaceOf(batchMost, perUnit).step;
+        const double highest = PlaceOf(batchMost, mode.perUnit).step;
         if (highest > top)
         {
             const double moved = highest + kSlack;
@@ -196,32 +274,40 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
             }
             top = moved;
         }
-#pragma unroll
-        for (uint32_t i = 0; i < kLoads; ++i)
+        if (!mode.weighed)
         {
-            const Place place = PlaceOf(v[i], perUnit);
-            const double d = top - place.step;
-            if (v[i] > -INFINITY && d < kSteps)
-            {
-                const uint32_t step = static_cast<uint32_t>(d);
-                atomicAdd(reinterpret_cast<unsigned long long*>(masses + step), MassOf(place.rest));
-                atomicAdd(counts + step, 1u);
-            }
+            AddBatch<true, false, false>(v, top, mode.perUnit, masses, counts);
+        }
+        else if (fabs(top) >= kFar)
+        {
+            AddBatch<true, true, true>(v, top, mode.perUnit, masses, counts);
+        }
+        else if (mode.counted)
+        {
+            AddBatch<true, true, false>(v, top, mode.perUnit, masses, counts);
+        }
+        else
+        {
+            AddBatch<false, true, false>(v, top, mode.perUnit, masses, counts);
         }
     }
-    // The wave's largest and its first place.
-    const float waveMost = GroupMax<kWave>(most);
-    uint32_t first = most == waveMost && most > -INFINITY ? at : ~0u;
-#pragma unroll
-    for (int step = 1; step < kWave; step *= 2)
+    if (greedy)
     {
-        first = min(first, static_cast<uint32_t>(__shfl_xor(first, step)));
+        // The wave's largest and its first place.
+        const float waveMost = GroupMax<kWave>(most);
+        at = most == waveMost && most > -INFINITY ? at : ~0u;
+#pragma unroll
+        for (int step = 1; step < kWave; step *= 2)
+        {
+            at = min(at, static_cast<uint32_t>(__shfl_xor(at, step)));
+        }
+        most = waveMost;
     }
     if (lane == 0)
     {
         topOf[wave] = top;
-        mostOf[wave] = waveMost;
-        atOf[wave] = first;
+        mostOf[wave] = most;
+        atOf[wave] = at;
     }
     __syncthreads();
     double partTop = topOf[0];
@@ -258,35 +344,28 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
                 count += countOf[w][from];
             }
         }
-        a.masses[slot * kSteps + i] = mass;
-        a.counts[slot * kSteps + i] = count;
+        if (mode.weighed)
+        {
+            a.masses[slot * kSteps + i] = mass;
+        }
+        if (mode.counted)
+        {
+            a.counts[slot * kSteps + i] = count;
+        }
     }
 }
 
-/// Inclusive sums over the workgroup's threads, in thread order.
 template <typename T>
-__device__ __forceinline__ T PickSums(T v, T* waveSum)
+__device__ __forceinline__ T WaveInclusive(T v)
 {
     const uint32_t lane = threadIdx.x % kWave;
-    const uint32_t wave = threadIdx.x / kWave;
 #pragma unroll
     for (int step = 1; step < kWave; step *= 2)
     {
         const T other = __shfl_up(v, step);
         v += lane >= static_cast<uint32_t>(step) ? other : T{};
     }
-    __syncthreads();
-    if (lane == kWave - 1)
-    {
-        waveSum[wave] = v;
-    }
-    __syncthreads();
-    T before{};
-    for (uint32_t w = 0; w < wave; ++w)
-    {
-        before += waveSum[w];
-    }
-    return before + v;
+    return v;
 }
 
 template <typename T>
@@ -300,32 +379,51 @@ __device__ __forceinline__ T WaveSum(T v)
     return v;
 }
 
-/// A key and the counts of those above it.
-struct Cut
-{
-    uint64_t key;    // what is kept of a step has at least this key
-    uint64_t mass;   // of what is kept
-};
-
 struct PickSpace
 {
     uint64_t keys[kListed];
-    uint64_t steps[kSteps];      // masses of a step, of digits; weights up to a step (as double)
-    uint32_t counts[kSteps];     // logits up to a step
-    uint32_t digitCounts[256];
+    double unit[kSteps];         // UnitOf
+    double upTo[kSteps];         // weights of the steps up to each
+    uint64_t masses[kSteps];
+    uint32_t counts[kSteps];     // logits up to each, or a bound of them
+    uint64_t digitMasses[kDigits];
+    uint32_t digitCounts[kDigits];
+    uint64_t fewKeys[kFew];
+    uint64_t fewMasses[kFew];
     double waveWeights[kPickWaves];
     uint32_t waveCounts[kPickWaves];
-    uint64_t waveMasses[kPickWaves];
     double groupWeights[kPickBlock];
     uint32_t partShift[kMaxParts];
-    uint64_t partMass[kMaxParts];
+    unsigned long long partMass[kMaxParts];
     double partWeight[kMaxParts];
-    uint64_t digitMasses[256];
-    uint32_t listed;
+    unsigned long long low, high, sum;
+    uint32_t listed, active, few;
     uint32_t stepK, stepP;
-    uint32_t last, lastAbove;  // a digit of the cut, and the logits above it
-    uint64_t lastMasses[2];    // above it, and its own
 };
+
+/// Inclusive sums of both over the first kSteps threads, in thread order.
+__device__ __forceinline__ void StepSums(uint32_t& count, double& weight, PickSpace& s)
+{
+    const uint32_t wave = threadIdx.x / kWave;
+    count = WaveInclusive(count);
+    weight = WaveInclusive(weight);
+    __syncthreads();
+    if (threadIdx.x % kWave == kWave - 1)
+    {
+        s.waveCounts[wave] = count;
+        s.waveWeights[wave] = weight;
+    }
+    __syncthreads();
+    uint32_t counts = 0;
+    double weights = 0.0;
+    for (uint32_t w = 0; w < min(wave, static_cast<uint32_t>(kSteps / kWave)); ++w)
+    {
+        counts += s.waveCounts[w];
+        weights += s.waveWeights[w];
+    }
+    count += counts;
+    weight += weights;
+}
 
 /// A row's grid and its threshold.
 struct RowGrid
@@ -342,121 +440,336 @@ __device__ __forceinline__ bool Reaches(const RowGrid& r, const Place& at)
     return (at.step - r.largest.step) + (at.rest - r.largest.rest) >= r.lowest;
 }
 
-/// Calls use(key, mass) for the logits of step d that reach min-p, by all threads (a barrier before and after is
-/// the caller's).
+/// Calls use(key, step, mass) for the row's logits in steps first..last, by all threads.
+///
+/// What bounds it: the row's arrival at one CU. A bound in f32, a little wide, keeps the 64-bit arithmetic to the
+/// logits near the steps.
 template <typename Use>
-__device__ __forceinline__ void ForStep(const RowGrid& r, uint32_t d, Use use)
+__device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, Use use)
 {
-    for (uint32_t first = 0; first < r.vocab; first += kPickBlock * kPickLoads)
+    const double wide = 0.5 + 1e-6 + 1e-9 * fabs(r.top);
+    const float low = __double2float_rd((r.top - last - wide) / r.perUnit);
+    const float high = __double2float_ru((r.top - first + wide) / r.perUnit);
+    auto look = [&](float v, uint32_t index) {
+        const float x = Counted(v);
+        if (x >= low && x <= high && x > -INFINITY)
+        {
+            const Place at = PlaceOf(x, r.perUnit);
+            const double d = r.top - at.step;
+            if (d >= first && d <= last)
+            {
+                use(OrderKey(x, index), static_cast<uint32_t>(d), MassOf(at.rest));
+            }
+        }
+    };
+    const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(r.x) / 4 % 4)) % 4u, r.vocab);
+    const uint32_t quads = (r.vocab - head) / 4;
+    const uint32_t tail = head + 4 * quads;
+    if (threadIdx.x < head)
     {
-        float v[kPickLoads];
+        look(r.x[threadIdx.x], threadIdx.x);
+    }
+    if (threadIdx.x < r.vocab - tail)
+    {
+        look(r.x[tail + threadIdx.x], tail + threadIdx.x);
+    }
+    for (uint32_t from = 0; from < quads; from += kPickBlock * kPickLoads)
+    {
+        float4v v[kPickLoads];
 #pragma unroll
         for (uint32_t i = 0; i < kPickLoads; ++i)
         {
-            v[i] = r.x[min(first + i * kPickBlock + threadIdx.x, r.vocab - 1)];
+            const uint32_t quad = min(from + i * kPickBlock + threadIdx.x, quads - 1);
+            v[i] = *reinterpret_cast<const float4v*>(r.x + head + 4 * quad);
         }
 #pragma unroll
         for (uint32_t i = 0; i < kPickLoads; ++i)
         {
-            const uint32_t index = first + i * kPickBlock + threadIdx.x;
-            const float x = Counted(v[i]);
-            const Place at = PlaceOf(x, r.perUnit);
-            if (index < r.vocab && x > -INFINITY && r.top - at.step == static_cast<double>(d) && Reaches(r, at))
+            const uint32_t quad = from + i * kPickBlock + threadIdx.x;
+            if (quad < quads)
             {
-                use(OrderKey(x, index), MassOf(at.rest));
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                {
+                    look(v[i][e], head + 4 * quad + e);
+                }
             }
         }
     }
 }
 
-/// The cut in step d: the first keys, `most` at most, and no more than it takes to have `limit` of mass (a key is
-/// kept where those above it have less). Digit by digit of the keys, from the highest: the digit in which the cut
-/// lies is found from counts and masses of all digits. Steps of up to kListed logits are listed first.
-__device__ Cut CutStep(const RowGrid& r, uint32_t d, uint32_t count, uint32_t most, double limit, PickSpace& s)
+/// Lists the keys of the logits in steps first..last (at most kListed, as the caller has seen).
+__device__ __forceinline__ void ListSteps(const RowGrid& r, uint32_t first, uint32_t last, PickSpace& s)
 {
-    const bool list = count <= kListed;
     __syncthreads();
-    if (list)
+    if (threadIdx.x == 0)
     {
+        s.listed = 0;
+    }
+    __syncthreads();
+    ForSteps(r, first, last, [&](uint64_t key, uint32_t, uint64_t) {
+        const uint32_t at = atomicAdd(&s.listed, 1u);
+        if (at < kListed)
+        {
+            s.keys[at] = key;
+        }
+    });
+    __syncthreads();
+}
+
+/// The last of what is kept, and the mass of all of it.
+struct Cut
+{
+    uint64_t key;
+    uint64_t mass;
+};
+
+/// Of `n` items in falling order of their keys (which differ), those that have fewer than `most` before them and
+/// less than `limit` of mass: the last one's key, and their mass. item(i, key, mass) says whether there is one.
+///
+/// Keys are taken apart into 256 equal ranges between the smallest and the largest, the range with the last one is
+/// found from counts and masses of all, and so on until a wave can look at the rest one by one.
+template <typename Item>
+__device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, uint64_t limit, PickSpace& s)
+{
+    const uint32_t lane = threadIdx.x % kWave;
+    uint64_t low = 0;
+    uint64_t high = ~0ull;
+    uint32_t above = 0;
+    uint64_t aboveMass = 0;
+    bool few = n <= kFew;
+    while (true)
+    {
+        __syncthreads();
         if (threadIdx.x == 0)
         {
-            s.listed = 0;
+            s.low = ~0ull;
+            s.high = 0;
+            s.active = 0;
+            s.few = 0;
         }
-        __syncthreads();
-        ForStep(r, d, [&](uint64_t key, uint64_t) { s.keys[atomicAdd(&s.listed, 1u)] = key; });
-        __syncthreads();
-    }
-    uint64_t prefix = 0;     // of the cut's key
-    uint64_t aboveMass = 0;  // of keys above those with the prefix
-    uint32_t above = 0;
-    for (int shift = 56; shift >= 0; shift -= 8)
-    {
-        for (uint32_t i = threadIdx.x; i < 256; i += kPickBlock)
+        for (uint32_t i = threadIdx.x; i < kDigits; i += kPickBlock)
         {
             s.digitCounts[i] = 0;
             s.digitMasses[i] = 0;
         }
-        if (threadIdx.x == 0)
+        __syncthreads();
+        if (!few)
         {
-            s.last = 0;
+            uint64_t least = ~0ull;
+            uint64_t largest = 0;
+            uint32_t count = 0;
+            for (uint32_t i = threadIdx.x; i < n; i += kPickBlock)
+            {
+                uint64_t key, mass;
+                if (item(i, key, mass) && key >= low && key <= high)
+                {
+                    least = least < key ? least : key;
+                    largest = largest > key ? largest : key;
+                    ++count;
+                }
+            }
+#pragma unroll
+            for (int step = 1; step < kWave; step *= 2)
+            {
+                const uint64_t l = __shfl_xor(static_cast<unsigned long long>(least), step);
+                const uint64_t h = __shfl_xor(static_cast<unsigned long long>(largest), step);
+                least = least < l ? least : l;
+                largest = largest > h ? largest : h;
+                count += __shfl_xor(count, step);
+            }
+            if (lane == 0 && count > 0)
+            {
+                atomicMin(&s.low, static_cast<unsigned long long>(least));
+                atomicMax(&s.high, static_cast<unsigned long long>(largest));
+                atomicAdd(&s.active, count);
+            }
+            __syncthreads();
+            low = s.low;
+            high = s.high;
+            if (s.active == 0)
+            {
+                return Cut{~0ull, aboveMass};
+            }
+            few = s.active <= kFew;
+        }
+        if (few)
+        {
+            for (uint32_t i = threadIdx.x; i < n; i += kPickBlock)
+            {
+                uint64_t key, mass;
+                if (item(i, key, mass) && key >= low && key <= high)
+                {
+                    const uint32_t at = atomicAdd(&s.few, 1u);
+                    s.fewKeys[at] = key;
+                    s.fewMasses[at] = mass;
+                }
+            }
+            __syncthreads();
+            // Every wave finds the same.
+            const uint32_t count = s.few;
+            const uint64_t key = lane < count ? s.fewKeys[lane] : 0;
+            const uint64_t mass = lane < count ? s.fewMasses[lane] : 0;
+            uint32_t before = above;
+            uint64_t massBefore = aboveMass;
+            for (uint32_t j = 0; j < count; ++j)
+            {
+                const bool is = s.fewKeys[j] > key;
+                before += is ? 1u : 0u;
+                massBefore += is ? s.fewMasses[j] : 0;
+            }
+            const bool kept = lane < count && before < most && massBefore < limit;
+            Cut last{kept ? key : ~0ull, kept ? massBefore + mass : aboveMass};
+#pragma unroll
+            for (int step = 1; step < kWave; step *= 2)
+            {
+                const uint64_t k = __shfl_xor(static_cast<unsigned long long>(last.key), step);
+                const uint64_t m = __shfl_xor(static_cast<unsigned long long>(last.mass), step);
+                last.mass = k < last.key ? m : last.mass;
+                last.key = k < last.key ? k : last.key;
+            }
+            return last;
+        }
+        const int bits = 64 - __clzll(static_cast<long long>(high - low));
+        const int shift = max(bits - 8, 0);
+        for (uint32_t i = threadIdx.x; i < n; i += kPickBlock)
+        {
+            uint64_t key, mass;
+            if (item(i, key, mass) && key >= low && key <= high)
+            {
+                const uint32_t digit = static_cast<uint32_t>((high - key) >> shift);
+                atomicAdd(&s.digitCounts[digit], 1u);
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.digitMasses[digit]), mass);
+            }
         }
         __syncthreads();
-        auto use = [&](uint64_t key, uint64_t mass) {
-            if (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
+        // Every wave finds the last range that begins before both limits, four of them a lane.
+        constexpr uint32_t kPer = kDigits / kWave;
+        uint32_t c[kPer];
+        uint64_t m[kPer];
+        uint32_t ofLane = 0;
+        uint64_t massOfLane = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < kPer; ++e)
+        {
+            c[e] = s.digitCounts[lane * kPer + e];
+            m[e] = s.digitMasses[lane * kPer + e];
+            ofLane += c[e];
+            massOfLane += m[e];
+        }
+        uint32_t before = above + WaveInclusive(ofLane) - ofLane;
+        uint64_t massBefore =
+            aboveMass + WaveInclusive(static_cast<unsigned long long>(massOfLane)) - massOfLane;
+        uint32_t which = ~0u;
+        uint32_t beforeIt = 0;
+        uint64_t massBeforeIt = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < kPer; ++e)
+        {
+            if (c[e] > 0 && before < most && massBefore < limit)
+            {
+                which = lane * kPer + e;
+                beforeIt = before;
+                massBeforeIt = massBefore;
+            }
+            before += c[e];
+            massBefore += m[e];
+        }
+        const uint64_t has = __ballot(which != ~0u);
+        if (has == 0)
+        {
+            return Cut{~0ull, aboveMass};
+        }
+        const int owner = 63 - __clzll(static_cast<long long>(has));
+        which = __shfl(which, owner);
+        above = __shfl(beforeIt, owner);
+        aboveMass = __shfl(static_cast<unsigned long long>(massBeforeIt), owner);
+        high -= static_cast<uint64_t>(which) << shift;
+        const uint64_t span = (1ull << shift) - 1;
+        low = high - low > span ? high - span : low;
+    }
+}
+
+/// The cut in a step of more logits than are listed: digit by digit of the keys, from the highest, with a pass over
+/// the row for each.
+__device__ Cut LastKeptOfRow(const RowGrid& r, uint32_t d, uint32_t most, uint64_t limit, PickSpace& s)
+{
+    uint64_t prefix = 0;
+    uint32_t above = 0;
+    uint64_t aboveMass = 0;
+    for (int shift = 56; shift >= 0; shift -= 8)
+    {
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < kDigits; i += kPickBlock)
+        {
+            s.digitCounts[i] = 0;
+            s.digitMasses[i] = 0;
+        }
+        __syncthreads();
+        ForSteps(r, d, d, [&](uint64_t key, uint32_t, uint64_t mass) {
+            if ((shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))) &&
+                Reaches(r, PlaceOf(KeyValue(key), r.perUnit)))
             {
                 const uint32_t digit = 255u - (static_cast<uint32_t>(key >> shift) & 255u);
                 atomicAdd(&s.digitCounts[digit], 1u);
                 atomicAdd(reinterpret_cast<unsigned long long*>(&s.digitMasses[digit]), mass);
             }
-        };
-        if (list)
+        });
+        __syncthreads();
+        uint32_t before = above;
+        uint64_t massBefore = aboveMass;
+        uint32_t which = ~0u;
+        uint64_t massOfIt = 0;
+        for (uint32_t digit = 0; digit < kDigits; ++digit)
         {
-            for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+            const uint32_t c = s.digitCounts[digit];
+            const uint64_t m = s.digitMasses[digit];
+            if (c > 0 && before < most && massBefore < limit)
             {
-                use(s.keys[i], MassOf(PlaceOf(KeyValue(s.keys[i]), r.perUnit).rest));
+                which = digit;
+                above = before;
+                aboveMass = massBefore;
+                massOfIt = m;
             }
+            before += c;
+            massBefore += m;
         }
-        else
-        {
-            ForStep(r, d, use);
-        }
-        __syncthreads();
-        // In falling order of digits; those of a key that is kept begin before both limits.
-        const uint32_t c = threadIdx.x < 256 ? s.digitCounts[threadIdx.x] : 0;
-        const uint64_t m = threadIdx.x < 256 ? s.digitMasses[threadIdx.x] : 0;
-        const uint32_t counts = above + PickSums(c, s.waveCounts) - c;
-        const uint64_t masses = aboveMass + PickSums(m, s.waveMasses) - m;
-        const bool begins = c > 0 && counts < most && static_cast<double>(masses) < limit;
-        if (begins)
-        {
-            atomicMax(&s.last, threadIdx.x + 1);  // the last digit of which something is kept
-        }
-        __syncthreads();
-        const uint32_t last = s.last;
-        if (last == 0)  // nothing in the step reaches min-p
+        if (which == ~0u)  // nothing in the step reaches min-p
         {
             return Cut{~0ull, aboveMass};
         }
-        if (threadIdx.x == last - 1)
-        {
-            s.lastAbove = counts;
-            s.lastMasses[0] = masses;
-            s.lastMasses[1] = m;
-        }
-        __syncthreads();
-        above = s.lastAbove;
-        aboveMass = s.lastMasses[0];
-        prefix |= static_cast<uint64_t>(256u - last) << shift;
+        prefix |= static_cast<uint64_t>(255u - which) << shift;
         if (shift == 0)
         {
-            aboveMass += s.lastMasses[1];  // keys differ: one
+            aboveMass += massOfIt;  // keys differ: one
         }
-        __syncthreads();
     }
     return Cut{prefix, aboveMass};
 }
 
-/// Decides a row: where the cuts lie in the steps' counts and masses, in which part the token lies, and which it is.
+/// The cut in step d, from the list where it has the step.
+__device__ __forceinline__ Cut CutStep(const RowGrid& r, uint32_t d, bool listed, uint32_t most, double limit,
+                                       PickSpace& s)
+{
+    const uint64_t below = limit < 0x1p63 ? static_cast<uint64_t>(ceil(limit)) : ~0ull;
+    if (!listed)
+    {
+        return LastKeptOfRow(r, d, most, below, s);
+    }
+    return LastKept(
+        s.listed,
+        [&](uint32_t i, uint64_t& key, uint64_t& mass) {
+            key = s.keys[i];
+            const Place at = PlaceOf(KeyValue(key), r.perUnit);
+            mass = MassOf(at.rest);
+            return r.top - at.step == static_cast<double>(d) && Reaches(r, at);
+        },
+        most, below, s);
+}
+
+/// Decides a row: where the cuts lie in the steps' counts and masses, and which token the number lands on. Where the
+/// logits of the steps down to the cut are few they are listed, in one pass over the row; else the step of the cut is,
+/// and the token is looked for in the part of the row that the parts' masses name.
 __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
 {
     __shared__ PickSpace s;
@@ -468,6 +781,10 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     // Every wave looks at the parts, a lane each.
     static_assert(kMaxParts == kWave, "a lane for each part");
     PartHead head = a.heads[slot + min(lane, a.parts - 1)];
+    const RowMode mode = ModeOf(a, row);
+    const float topP = a.topPs != nullptr ? a.topPs[row] : 1.0f;
+    const float minP = a.minPs != nullptr ? a.minPs[row] : 0.0f;
+    const double random = a.randoms[row];
     if (lane >= a.parts)
     {
         head = PartHead{-INFINITY, -INFINITY, ~0u};
@@ -481,8 +798,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         at = min(at, static_cast<uint32_t>(__shfl_xor(at, step)));
         top = fmax(top, __shfl_xor(top, step));
     }
-    const double perUnit = StepsPerUnit(a, row);
-    if (most == -INFINITY || perUnit < 0.0)
+    if (most == -INFINITY || mode.perUnit < 0.0)
     {
         if (threadIdx.x == 0)
         {
@@ -497,181 +813,316 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     RowGrid r;
     r.x = a.logits + row * a.stride;
     r.vocab = a.vocab;
-    r.perUnit = perUnit;
+    r.perUnit = mode.perUnit;
     r.top = top;
-    r.largest = PlaceOf(most, perUnit);
-    const float minP = a.minPs != nullptr ? a.minPs[row] : 0.0f;
-    r.lowest = minP > 0.0f ? 8.0 * log2(static_cast<double>(minP)) : -INFINITY;
-    if (threadIdx.x < kWave)
+    r.largest = PlaceOf(most, mode.perUnit);
+    r.lowest = -INFINITY;
+    const uint32_t d = threadIdx.x % kSteps;
+    if (wave == 0)
     {
         const double by = top - head.top;
         s.partShift[lane] = by < kSteps ? static_cast<uint32_t>(by) : kSteps;  // a part with nothing: all
         s.partMass[lane] = 0;
+        if (lane == 0)
+        {
+            s.stepK = kSteps - 1;
+            s.stepP = kSteps - 1;
+        }
+    }
+    if (threadIdx.x < kSteps)
+    {
+        s.unit[d] = UnitOf(d);
     }
     __syncthreads();
 
-    // The row's steps, and what they add up to.
-    const uint32_t d = threadIdx.x;
+    // The row's steps: half of the threads take every other part, several parts' on their way at a time.
+    static_assert(kPickBlock == 2 * kSteps, "two threads a step");
     uint64_t mass = 0;
     uint32_t count = 0;
-    if (d < kSteps)
     {
-        for (uint32_t p = 0; p < a.parts; ++p)
+        constexpr uint32_t kDeep = 16;
+        const uint32_t half = threadIdx.x / kSteps;
+        for (uint32_t p0 = half; p0 < a.parts; p0 += 2 * kDeep)
         {
-            const uint32_t shift = s.partShift[p];
-            if (d >= shift)
+            uint64_t m[kDeep];
+            uint32_t c[kDeep];
+#pragma unroll
+            for (uint32_t i = 0; i < kDeep; ++i)
             {
-                mass += a.masses[(slot + p) * kSteps + d - shift];
-                count += a.counts[(slot + p) * kSteps + d - shift];
+                const uint32_t p = min(p0 + 2 * i, a.parts - 1);
+                const uint32_t shift = s.partShift[p];
+                const uint64_t from = (slot + p) * kSteps + (d >= shift ? d - shift : 0);
+                const bool is = p0 + 2 * i < a.parts && d >= shift;
+                m[i] = is && mode.weighed ? a.masses[from] : 0;
+                c[i] = is && mode.counted ? a.counts[from] : 0;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kDeep; ++i)
+            {
+                mass += m[i];
+                count += c[i];
             }
         }
+        if (half == 1)
+        {
+            s.masses[d] = mass;
+            s.counts[d] = count;
+        }
+        __syncthreads();
+        mass = half == 0 ? mass + s.masses[d] : 0;
+        count = half == 0 ? count + s.counts[d] : 0;
     }
-    const double weight = WeightOf(mass, d);
-    const uint32_t counts = PickSums(count, s.waveCounts);
-    const double weights = PickSums(weight, s.waveWeights);
-    double* const upTo = reinterpret_cast<double*>(s.steps);
-    if (d < kSteps)
+    const bool mine = threadIdx.x < kSteps;
+    double weight = static_cast<double>(mass) * s.unit[d];
+    if (!mode.counted)
     {
-        s.counts[d] = counts;
-        upTo[d] = weights;
+        // A bound: a logit's mass is at least 2^(-1/16) of a unit's.
+        count = static_cast<uint32_t>(static_cast<double>(mass) * (0x1p-38 * 1.0443)) + (mass != 0 ? 1u : 0u);
     }
-    if (threadIdx.x == 0)
+    StepSums(count, weight, s);
+    if (mine)
     {
-        s.stepK = kSteps - 1;
-        s.stepP = kSteps - 1;
+        s.counts[d] = count;
+        s.upTo[d] = weight;
     }
     __syncthreads();
-    const uint32_t all = s.counts[kSteps - 1];
-    const int32_t topK = a.topKs != nullptr ? a.topKs[row] : 0;
-    const float topP = a.topPs != nullptr ? a.topPs[row] : 1.0f;
-    const uint32_t k = topK > 0 ? min(static_cast<uint32_t>(topK), all) : all;
     // The step in which the first k end.
-    if (d < kSteps && counts >= k)
+    uint32_t stepK = kSteps - 1;
+    uint32_t left = ~0u;  // of the first k in that step
+    bool wholeK = true;
+    if (mode.counted)
     {
-        atomicMin(&s.stepK, d);
+        const uint32_t k = min(static_cast<uint32_t>(mode.topK), s.counts[kSteps - 1]);
+        if (mine && count >= k)
+        {
+            atomicMin(&s.stepK, d);
+        }
+        __syncthreads();
+        stepK = s.stepK;
+        left = k - (stepK > 0 ? s.counts[stepK - 1] : 0);
+        wholeK = s.counts[stepK] == k;
     }
-    __syncthreads();
-    const uint32_t stepK = s.stepK;
-    const uint32_t beforeK = stepK > 0 ? s.counts[stepK - 1] : 0;
-    const bool wholeK = s.counts[stepK] == k;
+    // Steps that are listed: first..last.
+    uint32_t listFirst = 1;
+    uint32_t listLast = 0;
+    bool partsKnown = true;
+    if (!mode.weighed)
+    {
+        if (mine)
+        {
+            s.masses[d] = 0;
+        }
+        partsKnown = false;
+        if (s.counts[stepK] <= kListed)
+        {
+            ListSteps(r, 0, stepK, s);
+            listFirst = 0;
+            listLast = stepK;
+            for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+            {
+                const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[static_cast<uint32_t>(top - place.step)]),
+                          MassOf(place.rest));
+            }
+        }
+        else
+        {
+            __syncthreads();
+            ForSteps(r, 0, stepK, [&](uint64_t, uint32_t step, uint64_t one) {
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[step]), one);
+            });
+        }
+        __syncthreads();
+        uint32_t unused = 0;
+        weight = mine ? static_cast<double>(s.masses[d]) * s.unit[d] : 0.0;
+        StepSums(unused, weight, s);
+        if (mine)
+        {
+            s.upTo[d] = weight;
+        }
+        __syncthreads();
+    }
+    auto countOf = [&](uint32_t step) { return s.counts[step] - (step > 0 ? s.counts[step - 1] : 0); };
+    auto weightBefore = [&](uint32_t step) { return step > 0 ? s.upTo[step - 1] : 0.0; };
+    auto isListed = [&](uint32_t step) { return listFirst <= step && step <= listLast; };
+    // Lists a step if it is not and fits.
+    auto listStep = [&](uint32_t step) {
+        if (!isListed(step) && countOf(step) <= kListed)
+        {
+            ListSteps(r, step, step, s);
+            listFirst = step;
+            listLast = step;
+        }
+    };
     // The step in which top-p's share of their weight is reached.
     uint32_t stepP = kSteps;
     double share = INFINITY;
     if (topP < 1.0f)
     {
-        double ofK = upTo[stepK];
+        double ofK = s.upTo[stepK];
         if (!wholeK)
         {
-            RowGrid whole = r;
-            whole.lowest = -INFINITY;
-            const Cut cut = CutStep(whole, stepK, s.counts[stepK] - beforeK, k - beforeK, INFINITY, s);
-            ofK = (stepK > 0 ? upTo[stepK - 1] : 0.0) + WeightOf(cut.mass, stepK);
+            listStep(stepK);
+            ofK = weightBefore(stepK) +
+                  static_cast<double>(CutStep(r, stepK, isListed(stepK), left, INFINITY, s).mass) * s.unit[stepK];
         }
         share = static_cast<double>(topP) * ofK;
-        if (d <= stepK && counts > 0 && weights >= share)
+        if (mine && d <= stepK && weight > 0.0 && weight >= share)
         {
             atomicMin(&s.stepP, d);
         }
         __syncthreads();
         stepP = min(s.stepP, stepK);
     }
-    // The step in which min-p's bound lies.
+    // The step in which min-p's bound lies; the largest always reaches it.
     uint32_t stepM = kSteps;
     if (minP > 0.0f)
     {
-        const double by = top - rint(r.largest.step + r.largest.rest + r.lowest);
-        const double first = top - r.largest.step;
-        stepM = by < kSteps ? static_cast<uint32_t>(fmax(by, first)) : kSteps;
+        const double lowest = fmin(8.0 * log2(static_cast<double>(minP)), 0.0);
+        const double by = top - rint(r.largest.step + r.largest.rest + lowest);
+        stepM = by < kSteps ? static_cast<uint32_t>(fmax(by, top - r.largest.step)) : kSteps;
+        r.lowest = stepM <= min(stepK, stepP) ? lowest : -INFINITY;
+        left = minP > 1.0f ? 1u : left;
     }
     const uint32_t step = min(min(stepK, stepP), stepM);
-    const double before = step > 0 ? upTo[step - 1] : 0.0;
-    const uint32_t countBefore = step > 0 ? s.counts[step - 1] : 0;
-    Cut cut{0, 0};
     const bool whole = step != stepP && step != stepM && (step != stepK || wholeK);
-    double total = upTo[step];
+    const bool all = listFirst == 0 && step <= listLast ? true : s.counts[step] <= kListed;
+    if (all && !(listFirst == 0 && step <= listLast))
+    {
+        ListSteps(r, 0, step, s);
+        listFirst = 0;
+        listLast = step;
+    }
+    Cut cut{0, 0};
+    double total = s.upTo[step];
     if (!whole)
     {
-        const uint32_t left = step == stepK ? k - countBefore : ~0u;
+        listStep(step);
         // A share that is reached before this step's first, by a rounding, still keeps that one.
         const double limit =
-            step == stepP ? fmax((share - before) * exp2(38.0 + static_cast<double>(step) * 0.125), 0x1p-30) : INFINITY;
-        RowGrid bounded = r;
-        bounded.lowest = step == stepM ? r.lowest : -INFINITY;
-        // The first logit is always kept.
-        bounded.lowest = fmin(bounded.lowest, 0.0);
-        cut = CutStep(bounded, step, s.counts[step] - countBefore, minP > 1.0f ? min(left, 1u) : left, limit, s);
-        total = before + WeightOf(cut.mass, step);
+            step == stepP ? fmax((share - weightBefore(step)) / s.unit[step], 0x1p-30) : INFINITY;
+        cut = CutStep(r, step, isListed(step), step == stepK || minP > 1.0f ? left : ~0u, limit, s);
+        total = weightBefore(step) + static_cast<double>(cut.mass) * s.unit[step];
     }
+    const double number = random > 0.0 ? random : 0.0;
+    if (all)
+    {
+        // All that is kept is listed: weights as whole numbers, whose sums are exact, by falling ~index.
+        const double last = static_cast<double>(step);
+        auto item = [&](uint32_t i, uint64_t& key, uint64_t& fixed) {
+            const uint64_t of = s.keys[i];
+            const Place place = PlaceOf(KeyValue(of), r.perUnit);
+            const double dist = top - place.step;
+            const bool kept = dist < last || (dist == last && of >= cut.key);
+            key = of & 0xFFFFFFFFull;
+            fixed = kept ? static_cast<uint64_t>(rint(static_cast<double>(MassOf(place.rest)) *
+                                                      (s.unit[static_cast<uint32_t>(dist)] * kFixed)))
+                         : 0;
+            return kept && fixed != 0;
+        };
+        __syncthreads();
+        if (threadIdx.x == 0)
+        {
+            s.sum = 0;
+        }
+        __syncthreads();
+        uint64_t sum = 0;
+        for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+        {
+            uint64_t key, fixed;
+            sum += item(i, key, fixed) ? fixed : 0;
+        }
+        sum = WaveSum(static_cast<unsigned long long>(sum));
+        if (lane == 0)
+        {
+            atomicAdd(&s.sum, static_cast<unsigned long long>(sum));
+        }
+        __syncthreads();
+        // The first token whose sum is past the number's share is the last that begins at or before it.
+        const double reach = number * static_cast<double>(s.sum);
+        const uint64_t limit = reach < 0x1p63 ? static_cast<uint64_t>(floor(reach)) + 1 : ~0ull;
+        const Cut token = LastKept(s.listed, item, ~0u, limit, s);
+        for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+        {
+            if ((s.keys[i] & 0xFFFFFFFFull) == token.key)
+            {
+                a.tokens[row] = static_cast<int32_t>(~static_cast<uint32_t>(token.key));
+                if (a.logprobs != nullptr)
+                {
+                    const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
+                    const double of =
+                        static_cast<double>(MassOf(place.rest)) * s.unit[static_cast<uint32_t>(top - place.step)];
+                    a.logprobs[row] = static_cast<float>(log(of / total));
+                }
+            }
+        }
+        return;
+    }
+
     // Kept: the steps before, and of this one the keys from the cut on.
     auto weightAt = [&](float v, uint32_t index) {
         const float x = Counted(v);
-        const Place place = PlaceOf(x, perUnit);
+        const Place place = PlaceOf(x, r.perUnit);
         const double dist = top - place.step;
-        const bool kept = x > -INFINITY && (dist < static_cast<double>(step) ||
-                                            (dist == static_cast<double>(step) && OrderKey(x, index) >= cut.key));
-        return kept ? WeightOf(MassOf(place.rest), static_cast<uint32_t>(dist)) : 0.0;
+        const bool kept = dist < static_cast<double>(step) ||
+                          (dist == static_cast<double>(step) && OrderKey(x, index) >= cut.key);
+        return kept ? static_cast<double>(MassOf(place.rest)) * s.unit[static_cast<uint32_t>(dist)] : 0.0;
     };
-
-    // What each part has of it: the steps before from its counts, this one's kept logits by a look at them.
-    __syncthreads();
-    constexpr uint32_t kLanesOfPart = kPickBlock / kMaxParts;
+    const double reach = number * total;
+    uint32_t begin = 0;
+    uint32_t end = a.vocab;
+    double passed = 0.0;
+    if (partsKnown)
     {
-        const uint32_t p = threadIdx.x / kLanesOfPart;
-        double sum = 0.0;
-        if (p < a.parts)
+        // What each part has of it: the steps before from its masses, this one's kept logits by a look at them.
+        __syncthreads();
+        const uint32_t until = whole ? step + 1 : step;
+        for (uint32_t p = wave; p < a.parts; p += kPickWaves)
         {
             const uint32_t shift = s.partShift[p];
-            const uint32_t until = whole ? step + 1 : step;
-            for (uint32_t i = shift + threadIdx.x % kLanesOfPart; i < until; i += kLanesOfPart)
+            double sum = 0.0;
+            for (uint32_t i = shift + lane; i < until; i += kWave)
             {
-                sum += WeightOf(a.masses[(slot + p) * kSteps + i - shift], i);
+                sum += static_cast<double>(a.masses[(slot + p) * kSteps + i - shift]) * s.unit[i];
+            }
+            sum = WaveSum(sum);
+            if (lane == 0)
+            {
+                s.partWeight[p] = sum;
             }
         }
-#pragma unroll
-        for (uint32_t i = 1; i < kLanesOfPart; i *= 2)
+        if (!whole)
         {
-            sum += __shfl_xor(sum, i);
-        }
-        if (threadIdx.x % kLanesOfPart == 0)
-        {
-            s.partWeight[p] = sum;
-        }
-    }
-    __syncthreads();
-    if (!whole)
-    {
-        auto use = [&](uint64_t key, uint64_t ofKey) {
-            if (key >= cut.key)
+            auto use = [&](uint64_t key, uint64_t one) {
+                if (key >= cut.key)
+                {
+                    atomicAdd(&s.partMass[~static_cast<uint32_t>(key) / a.partLength],
+                              static_cast<unsigned long long>(one));
+                }
+            };
+            if (isListed(step))
             {
-                atomicAdd(reinterpret_cast<unsigned long long*>(&s.partMass[~static_cast<uint32_t>(key) / a.partLength]),
-                          ofKey);
+                for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+                {
+                    const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
+                    if (top - place.step == static_cast<double>(step))
+                    {
+                        use(s.keys[i], MassOf(place.rest));
+                    }
+                }
             }
-        };
-        if (s.counts[step] - countBefore <= kListed)
-        {
-            for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+            else
             {
-                use(s.keys[i], MassOf(PlaceOf(KeyValue(s.keys[i]), perUnit).rest));
+                ForSteps(r, step, step, [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
             }
         }
-        else
-        {
-            RowGrid bounded = r;
-            bounded.lowest = -INFINITY;
-            ForStep(bounded, step, use);
-        }
-    }
-    __syncthreads();
-    const double random = a.randoms[row];
-    const double reach = (random > 0.0 ? random : 0.0) * total;
-    // The first part that reaches past the number's share, else the last with anything kept.
-    uint32_t part = 0;
-    double passed = 0.0;
-    {
+        __syncthreads();
+        // The first part that reaches past the number's share, else the last with anything kept.
+        uint32_t part = 0;
         double upToPart = 0.0;
         for (uint32_t p = 0; p < a.parts; ++p)
         {
-            const double of = s.partWeight[p] + WeightOf(s.partMass[p], step);
+            const double of = s.partWeight[p] + static_cast<double>(s.partMass[p]) * s.unit[step];
             if (of > 0.0)
             {
                 part = p;
@@ -683,10 +1134,10 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                 }
             }
         }
+        begin = part * a.partLength;
+        end = min(begin + a.partLength, a.vocab);
     }
-    // Sums of its groups of logits, and the first group that reaches past it, else the last with anything kept.
-    const uint32_t begin = part * a.partLength;
-    const uint32_t end = min(begin + a.partLength, a.vocab);
+    // Sums of groups of logits, and the first group that reaches past it, else the last with anything kept.
     const uint32_t groups = (end - begin + kGroup - 1) / kGroup;
     uint32_t group = 0;
     double sum = passed;
@@ -741,27 +1192,21 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     {
         const uint32_t index = from + j * kWave + lane;
         const double own = index < end ? weightAt(r.x[index], index) : 0.0;
-        double sum = own;
-#pragma unroll
-        for (int i = 1; i < kWave; i *= 2)
-        {
-            const double other = __shfl_up(sum, i);
-            sum += lane >= static_cast<uint32_t>(i) ? other : 0.0;
-        }
+        const double upToOwn = WaveInclusive(own);
         const uint64_t kept = __ballot(own > 0.0);
-        const uint64_t past = __ballot(own > 0.0 && passed + sum > reach);
+        const uint64_t over = __ballot(own > 0.0 && passed + upToOwn > reach);
         if (kept != 0)
         {
-            const int which = past != 0 ? __ffsll(static_cast<unsigned long long>(past)) - 1
+            const int which = over != 0 ? __ffsll(static_cast<unsigned long long>(over)) - 1
                                         : 63 - __clzll(static_cast<long long>(kept));
             token = from + j * kWave + which;
             of = __shfl(own, which);
         }
-        if (past != 0)
+        if (over != 0)
         {
             break;
         }
-        passed += __shfl(sum, kWave - 1);
+        passed += __shfl(upToOwn, kWave - 1);
     }
     if (lane == 0)
     {
