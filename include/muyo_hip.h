@@ -641,6 +641,23 @@ int muyo_paged_attention_decode_f16kv(const float* q, const void* kcache, const 
                                       uint32_t page_size, uint32_t window, float scale, void* workspace,
                                       uint64_t workspace_bytes, void* stream);
 
+/* muyo_paged_attention_decode_f16kv for sequences that go on from the same first keys (a system prompt, a document):
+ * prefix[0] is the row of tables, prefix[1] the number, of keys that every query sees before its own, as if its
+ * sequence's pages began with that row's. Positions count a query's own keys: one below 0 leaves it the prefix
+ * alone. prefix is device data like the rest: without a row in 0..sequences - 1, or keys, there is none, and keys past
+ * table_pages * page_size, or in pages with an id outside the cache, are left out. The prefix is read once for
+ * 128 (query, head)s of a kv head, so many queries cost little more than one. No window; the rest, the workspace
+ * too, as above. (The prefix is a sequence of the plan like the others, which keeps its pages while it has a
+ * target; the tokens behind it have rope positions of its length plus their own.) */
+size_t muyo_paged_attention_prefix_f16kv_workspace_bytes(uint32_t queries, uint32_t heads, uint32_t kv_heads,
+                                                         uint32_t head_dim); /* 0: unsupported shape */
+int muyo_paged_attention_prefix_f16kv(const float* q, const void* kcache, const void* vcache, float* out,
+                                      const int32_t* tables, uint32_t sequences, uint32_t table_pages,
+                                      const int32_t* query_sequence, const int32_t* positions, uint32_t queries,
+                                      const int32_t* prefix, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                      uint32_t pages, uint32_t page_size, float scale, void* workspace,
+                                      uint64_t workspace_bytes, void* stream);
+
 /* A cache of half the bytes: kcache and vcache are [pages][kv_heads][page_size][head_dim] 8-bit codes, kscales and
  * vscales [pages][kv_heads][page_size] f32, and a value is scale * code. The codes are whole numbers of
  * -127..127, or e4m3 (four bits of exponent, three of fraction, up to 448). */

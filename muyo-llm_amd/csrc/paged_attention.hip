@@ -1,7 +1,7 @@
 // Attention of single tokens over a paged fp16 cache, many sequences of any lengths in one call.
 #include <cmath>
 
-#include "paged_attention_core.hpp"
+#include "paged_attention_f16.hpp"
 
 namespace muyo
 {
@@ -17,12 +17,6 @@ constexpr int kHalves = kTile / 16;       // matrix operands of 16 keys
 constexpr float kLag = 4.0f;
 constexpr float kWeightBias = 15.0f - kLag;
 constexpr float kLowScale = 2048.0f;      // of the low plane: what 11 bits of the high one leave, in f16's range again
-
-struct PagedAttentionF16Args : PagedAttentionArgs
-{
-    const uint16_t* kcache;
-    const uint16_t* vcache;
-};
 
 template <bool kOnce>
 __device__ __forceinline__ half8 LoadRow(const uint16_t* p)
@@ -566,6 +560,16 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void Page
     }
 }
 }  // namespace
+
+template <int kHd>
+hipError_t LaunchOwnKeys(hipStream_t s, const PagedAttentionF16Args& a)
+{
+    return LaunchPagedAttention<kHd, kTile, true>(s, a, PagedAttentionKernel<kHd, false, true>,
+                                                  PagedAttentionKernel<kHd, true, true>);
+}
+
+template hipError_t LaunchOwnKeys<64>(hipStream_t, const PagedAttentionF16Args&);
+template hipError_t LaunchOwnKeys<128>(hipStream_t, const PagedAttentionF16Args&);
 
 int CheckAttention(const char* name, const AttentionCall& c, const Range* more, int moreCount, int aligned)
 {

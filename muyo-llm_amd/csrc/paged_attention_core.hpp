@@ -9,6 +9,26 @@
 
 namespace muyo
 {
+struct PagedAttentionArgs
+{
+    const float* q;
+    float* out;
+    const int32_t* tables;
+    uint32_t sequences;
+    uint32_t tablePages;
+    const int32_t* querySequence;
+    const int32_t* positions;
+    uint32_t queries, group, kvHeads;
+    uint32_t pages, pageShift;
+    uint32_t window;
+    float scale;
+    uint32_t* costSums;  // [queries + 1]: CostOf of one kv head of the queries before
+    uint4* cuts;         // what to join: query, kv head, first share, pieces (0: nothing)
+    uint32_t cutsByUnit; // cuts has an entry per (query, kv head); else one per share
+    float4* stats;       // of kStats: base, sum, a score's log2 units, -, of each query's heads
+    float* partials;     // [2 * shares][group][4 + headDim]: base, sum, a score's log2 units, -, weighted values
+};
+
 /// The arguments that the attentions have in common.
 struct AttentionCall
 {
@@ -51,26 +71,6 @@ __device__ __forceinline__ int32_t ScalarLoad(const int32_t* p)
 {
     return *(const __attribute__((address_space(4))) int32_t*)reinterpret_cast<uintptr_t>(p);
 }
-
-struct PagedAttentionArgs
-{
-    const float* q;
-    float* out;
-    const int32_t* tables;
-    uint32_t sequences;
-    uint32_t tablePages;
-    const int32_t* querySequence;
-    const int32_t* positions;
-    uint32_t queries, group, kvHeads;
-    uint32_t pages, pageShift;
-    uint32_t window;
-    float scale;
-    uint32_t* costSums;  // [queries + 1]: CostOf of one kv head of the queries before
-    uint4* cuts;         // what to join: query, kv head, first share, pieces (0: nothing)
-    uint32_t cutsByUnit; // cuts has an entry per (query, kv head); else one per share
-    float4* stats;       // of kStats: base, sum, a score's log2 units, -, of each query's heads
-    float* partials;     // [2 * shares][group][4 + headDim]: base, sum, a score's log2 units, -, weighted values
-};
 
 /// The keys begin..end - 1 that a query sees, and the tiles they lie in. A query without any has one
 /// tile of which it sees nothing (its output is 0), one without a sequence none.

@@ -239,6 +239,9 @@ _SIGNATURES = {
                                                         u32, u32, u32, u32, f32, vp, u64, vp]),
     "muyo_token_logprobs_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32]),
     "muyo_token_logprobs_f32": (ctypes.c_int, [vp, u64, u32, u32, vp, vp, vp, vp, u32, vp, vp, vp, u64, vp]),
+    "muyo_paged_attention_prefix_f16kv_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32, u32]),
+    "muyo_paged_attention_prefix_f16kv": (ctypes.c_int, [vp, vp, vp, vp, vp, u32, u32, vp, vp, u32, vp, u32, u32, u32,
+                                                         u32, u32, f32, vp, u64, vp]),
     "muyo_sample_rows_workspace_bytes": (ctypes.c_size_t, [u32, u32]),
     "muyo_sample_rows_f32": (ctypes.c_int, [vp, u64, u32, u32, vp, vp, vp, vp, vp, vp, vp, vp, u64, vp]),
     "muyo_fill_normal_f16": (ctypes.c_int, [vp, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_double, ctypes.c_double, vp]),
