@@ -356,10 +356,13 @@ def test_attention_of_large_small_and_negative_scales(mh, gpu, form):
             batch.check(rtol=ATTENTION_RTOL * max(1.0, 4 * q_std * k_size * abs(scale)))
 
 
+HERE = [s for s in SINKS if len(s[4]) < 100] + [(4, 4, 128, 16, [1100] * 70)]
+
+
 @pytest.mark.parametrize("form", FORMATS)
 @pytest.mark.parametrize("value, last", [(0.0, False), (0.01, False), (1.0, False), (0.0, True)])
-@pytest.mark.parametrize("heads, kv, hd, size, keys", SINKS, ids=["-".join(map(str, (*s[:4], s[4][0], len(s[4]))))
-                                                                 for s in SINKS])
+@pytest.mark.parametrize("heads, kv, hd, size, keys", HERE, ids=["-".join(map(str, (*s[:4], s[4][0], len(s[4]))))
+                                                                for s in HERE])
 def test_attention_with_a_key_that_has_most_of_the_weight(mh, gpu, heads, kv, hd, size, keys, value, last, form):
     """One key up to 20 nats above the others with a value row that is 0, small or ordinary: the output is that
     of the many small weights. A score of S is off by some 4 u S, where 10 was taken for S."""
