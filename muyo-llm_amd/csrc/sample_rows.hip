@@ -21,10 +21,11 @@ constexpr int kSteps = 512;                    // of the grid, from the row's la
 constexpr int kSlack = 8;                      // steps above the largest logit so far
 constexpr int kQuads = 4;                      // 16-byte loads of a lane's batch
 constexpr uint32_t kBatch = kWave * 4 * kQuads;  // logits a wave takes at a time
-constexpr int kPickBlock = 1024;               // threads that decide a row
+constexpr int kPickBlock = 512;                // threads that decide a row
 constexpr int kPickWaves = kPickBlock / kWave;
 constexpr int kPickLoads = 8;
 constexpr uint32_t kGroup = kWave * kPickLoads;  // logits of a sum on the way to the token
+constexpr uint32_t kGroups = 1024;             // such sums at a time
 constexpr uint32_t kListed = 4096;             // logits that are listed
 constexpr int32_t kListedK = 2048;             // a top-k up to which listing the tokens is likely to do
 constexpr uint32_t kDigits = 256;
@@ -32,9 +33,10 @@ constexpr uint32_t kFew = kWave;               // candidates that a wave looks a
 constexpr uint32_t kMaxParts = 64;             // workgroups of a row
 constexpr uint32_t kMaxRows = (1u << 22) - 1;  // a launch has fewer than 2^32 threads
 constexpr uint32_t kMaxVocab = 1u << 24;       // masses of so many logits fit in 63 bits
-constexpr uint32_t kBlocksAtOnce = 256 * 6;    // workgroups that 256 CUs run at once
+constexpr uint32_t kCountBlocks = 2048;        // workgroups to aim at that count
 constexpr double kLog2e = 1.44269504088896340736;
-constexpr double kFar = 0x1p48;                // places whose rounding errors are not within half a step
+constexpr double kFar = 0x1p48;                // places past which steps are not whole numbers apart
+constexpr double kWhole = 0x1.8p52;            // added, the whole part's last 32 bits come last
 constexpr double kFixed = 0x1p50;              // units of the top step's weight, for sums of listed logits
 
 /// What a part of a row says besides its counts.
@@ -95,23 +97,18 @@ struct Place
     double rest;  // from its middle
 };
 
-/// The same bits wherever it is computed: nothing is contracted. kBounded: also right past kFar, where steps are
-/// whole numbers apart and `rest` would be a rounding error of any size.
-template <bool kBounded = true>
+/// The whole number next to y * perUnit, as its sum with kWhole: for products below 2^51.
+__device__ __forceinline__ double WholeOf(double y, double perUnit) { return fma(y, perUnit, kWhole); }
+
+/// The same bits wherever it is computed.
 __device__ __forceinline__ Place PlaceOf(float x, double perUnit)
 {
-#pragma clang fp contract(off)
-    // The product and what its rounding left out: differences of far places keep their bits.
+    // A product is rounded once, what is left of it too: differences of far places keep their bits.
     const double y = static_cast<double>(x);
-    const double p = y * perUnit;
-    const double left = fma(y, perUnit, -p);
     Place at;
-    at.step = rint(p);
-    at.rest = (p - at.step) + left;
-    if (kBounded)
-    {
-        at.rest = fmin(fmax(at.rest, -0.75), 0.75);
-    }
+    at.step = fabs(y * perUnit) < 0x1p50 ? WholeOf(y, perUnit) - kWhole : rint(y * perUnit);
+    // Far places are whole steps apart, if they differ at all, and have any remainder.
+    at.rest = fmin(fmax(fma(y, perUnit, -at.step), -0.75), 0.75);
     return at;
 }
 
@@ -119,34 +116,62 @@ __device__ __forceinline__ Place PlaceOf(float x, double perUnit)
 /// a whole number by 2^52, whose bits then go.
 __device__ __forceinline__ uint64_t MassOf(double rest)
 {
+    // As it stands: the compiler would take the form that overwrites its summand, and copy each constant first.
+    auto add = [](double x, double y, double z) {
+        double d;
+        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(x), "v"(y), "v"(z));
+        return d;
+    };
     constexpr double kOne = 0x1p38;
     double s = 4.069392558613428e-08 * kOne;
-    s = fma(s, rest, 2.3483963990465326e-06 * kOne);
-    s = fma(s, rest, 0.00010840646184941278 * kOne);
-    s = fma(s, rest, 0.0037535391505790455 * kOne);
-    s = fma(s, rest, 0.08664339757000515 * kOne);
-    s = fma(s, rest, 1.0000000000002864 * kOne + 0x1p52);
+    s = add(s, rest, 2.3483963990465326e-06 * kOne);
+    s = add(s, rest, 0.00010840646184941278 * kOne);
+    s = add(s, rest, 0.0037535391505790455 * kOne);
+    s = add(s, rest, 0.08664339757000515 * kOne);
+    s = add(s, rest, 1.0000000000002864 * kOne + 0x1p52);
     return static_cast<uint64_t>(__double_as_longlong(s)) & 0xFFFFFFFFFFFFFull;
 }
 
 /// Weight of a unit of mass in step d, relative to the top's.
 __device__ __forceinline__ double UnitOf(uint32_t d) { return exp2(-38.0 - static_cast<double>(d) * 0.125); }
 
-template <bool kCount, bool kMass, bool kBounded>
-__device__ __forceinline__ void AddBatch(const float (&v)[4 * kQuads], double top, double perUnit, uint64_t* masses,
-                                         uint32_t* counts)
+/// Adds a lane's logit to the counters of steps below `top`.
+__device__ __forceinline__ void AddOne(float v, double top, double perUnit, uint64_t* masses, uint32_t* counts)
 {
+    const float x = Counted(v);
+    const Place place = PlaceOf(x, perUnit);
+    const double d = top - place.step;
+    if (x > -INFINITY && d < kSteps)
+    {
+        const uint32_t step = static_cast<uint32_t>(d);
+        atomicAdd(reinterpret_cast<unsigned long long*>(masses + step), MassOf(place.rest));
+        atomicAdd(counts + step, 1u);
+    }
+}
+
+/// The same of a batch, for places below kFar, with fewer operations: a step is the last 32 bits of a place's sum with kWhole. Logits
+/// below `least`, past the last step, count as that, so that no place is far.
+template <bool kCount, bool kMass>
+__device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double top, float least, double perUnit,
+                                             uint64_t* masses, uint32_t* counts)
+{
+    const uint32_t topStep = static_cast<uint32_t>(__double_as_longlong(top + kWhole));
 #pragma unroll
     for (int i = 0; i < 4 * kQuads; ++i)
     {
-        const Place place = PlaceOf<kBounded>(v[i], perUnit);
-        const double d = top - place.step;
-        if (d < kSteps)
+        // The smaller of a signalling NaN and a number is a quiet NaN, the larger of that and a number the number.
+        float x;
+        asm("v_min_f32 %0, %1, %2" : "=v"(x) : "v"(v[i / 4][i % 4]), "v"(0x1.fffffep127f));
+        asm("v_max_f32 %0, %1, %2" : "=v"(x) : "v"(x), "v"(least));
+        const double y = static_cast<double>(x);
+        const double whole = WholeOf(y, perUnit);
+        const uint32_t step = topStep - static_cast<uint32_t>(__double_as_longlong(whole));
+        if (step < kSteps)
         {
-            const uint32_t step = static_cast<uint32_t>(d);
             if (kMass)
             {
-                atomicAdd(reinterpret_cast<unsigned long long*>(masses + step), MassOf(place.rest));
+                atomicAdd(reinterpret_cast<unsigned long long*>(masses + step),
+                          MassOf(fma(y, perUnit, -(whole - kWhole))));
             }
             if (kCount)
             {
@@ -159,7 +184,6 @@ __device__ __forceinline__ void AddBatch(const float (&v)[4 * kQuads], double to
 /// Counts the logits of a part of a row in steps of the grid, and their masses. A wave has counters of its own in
 /// LDS, from a step above the largest logit that it has met; a larger one moves them down, which is rare.
 ///
-/// What bounds it: the arithmetic in 64 bits, some 22 operations a logit with its mass and 12 without.
 __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
 {
     __shared__ uint64_t massOf[kWaves][kSteps];
@@ -184,47 +208,55 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
         counts[i] = 0;
     }
     double top = -INFINITY;
-    float most = -INFINITY;  // of the wave; of a greedy row's lane
+    float least = -INFINITY;  // past the last step, where places are near
+    bool near = false;
+    float most = -INFINITY;   // of the wave; of a greedy row's lane
     uint32_t at = 0;
     // 16-byte loads from the last such address at or before the part's first logit; batches that reach over an end
-    // of the part go logit by logit.
+    // of the part go logit by logit. A batch is on its way while the one before is counted.
     const uint32_t before = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x + begin) / 4 % 4);
-    for (uint32_t first = wave * kBatch; first < end - begin + before; first += kWaves * kBatch)
-    {
-        float v[4 * kQuads];
-        // A lane's logits: four in a row from each quad.
-        auto indexOf = [&](uint32_t i) { return begin - before + first + (i / 4 * kWave + lane) * 4 + i % 4; };
-        if (first >= before && first + kBatch <= end - begin + before)
+    const uint32_t length = end - begin + before;
+    // A lane's logits: four in a row from each quad.
+    auto indexOf = [&](uint32_t first, uint32_t i) { return begin - before + first + (i / 4 * kWave + lane) * 4 + i % 4; };
+    auto load = [&](uint32_t first, float4v (&v)[kQuads]) {
+        if (first >= before && first + kBatch <= length)
         {
 #pragma unroll
             for (uint32_t q = 0; q < kQuads; ++q)
             {
-                const float4v four = *reinterpret_cast<const float4v*>(x + indexOf(4 * q));
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e)
-                {
-                    v[4 * q + e] = Counted(four[e]);
-                }
+                v[q] = *reinterpret_cast<const float4v*>(x + indexOf(first, 4 * q));
             }
         }
-        else
+        else if (first < length)
         {
 #pragma unroll
             for (uint32_t i = 0; i < 4 * kQuads; ++i)
             {
                 // Before the part's first logit the index wraps or is too small: both are left out.
-                const uint32_t index = indexOf(i);
+                const uint32_t index = indexOf(first, i);
                 const bool inside = index >= begin && index < end;
                 const float one = x[inside ? index : begin];
-                v[i] = inside ? Counted(one) : -INFINITY;
+                v[i / 4][i % 4] = inside ? one : -INFINITY;
             }
         }
-        float batchMost = v[0];
+    };
+    float4v v[kQuads], next[kQuads];
+    load(wave * kBatch, next);
+    for (uint32_t first = wave * kBatch; first < length; first += kWaves * kBatch)
+    {
 #pragma unroll
-        for (uint32_t i = 1; i < 4 * kQuads; ++i)
+        for (int q = 0; q < kQuads; ++q)
         {
-            batchMost = fmaxf(batchMost, v[i]);
+            v[q] = next[q];
         }
+        load(first + kWaves * kBatch, next);
+        float batchMost = -INFINITY;
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * kQuads; ++i)
+        {
+            batchMost = fmaxf(batchMost, v[i / 4][i % 4]);
+        }
+        batchMost = fminf(batchMost, 0x1.fffffep127f);
         if (greedy)
         {
             if (batchMost > most)
@@ -233,7 +265,7 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
 #pragma unroll
                 for (int i = 4 * kQuads - 1; i >= 0; --i)
                 {
-                    at = v[i] == batchMost ? indexOf(i) : at;
+                    at = Counted(v[i / 4][i % 4]) == batchMost ? indexOf(first, i) : at;
                 }
             }
             continue;
@@ -273,22 +305,32 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
                 __builtin_amdgcn_wave_barrier();
             }
             top = moved;
+            const double bound = (top - (kSteps + 2)) / mode.perUnit;
+            least = static_cast<float>(bound);
+            // (At huge temperatures the bound is below all numbers, and does not tell -inf from them.)
+            near = fabs(top) < kFar && bound > -0x1p127;
         }
-        if (!mode.weighed)
+        if (!near)
         {
-            AddBatch<true, false, false>(v, top, mode.perUnit, masses, counts);
+#pragma unroll 1
+            for (uint32_t i = 0; i < 4 * kQuads; ++i)
+            {
+                const uint32_t index = indexOf(first, i);
+                const bool inside = index >= begin && index < end;
+                AddOne(inside ? x[index] : -INFINITY, top, mode.perUnit, masses, counts);
+            }
         }
-        else if (fabs(top) >= kFar)
+        else if (!mode.weighed)
         {
-            AddBatch<true, true, true>(v, top, mode.perUnit, masses, counts);
+            AddNearBatch<true, false>(v, top, least, mode.perUnit, masses, counts);
         }
         else if (mode.counted)
         {
-            AddBatch<true, true, false>(v, top, mode.perUnit, masses, counts);
+            AddNearBatch<true, true>(v, top, least, mode.perUnit, masses, counts);
         }
         else
         {
-            AddBatch<false, true, false>(v, top, mode.perUnit, masses, counts);
+            AddNearBatch<false, true>(v, top, least, mode.perUnit, masses, counts);
         }
     }
     if (greedy)
@@ -392,7 +434,7 @@ struct PickSpace
     uint64_t fewMasses[kFew];
     double waveWeights[kPickWaves];
     uint32_t waveCounts[kPickWaves];
-    double groupWeights[kPickBlock];
+    double groupWeights[kGroups];
     uint32_t partShift[kMaxParts];
     unsigned long long partMass[kMaxParts];
     double partWeight[kMaxParts];
@@ -401,7 +443,7 @@ struct PickSpace
     uint32_t stepK, stepP;
 };
 
-/// Inclusive sums of both over the first kSteps threads, in thread order.
+/// Inclusive sums of both over the threads, in their order.
 __device__ __forceinline__ void StepSums(uint32_t& count, double& weight, PickSpace& s)
 {
     const uint32_t wave = threadIdx.x / kWave;
@@ -416,7 +458,7 @@ __device__ __forceinline__ void StepSums(uint32_t& count, double& weight, PickSp
     __syncthreads();
     uint32_t counts = 0;
     double weights = 0.0;
-    for (uint32_t w = 0; w < min(wave, static_cast<uint32_t>(kSteps / kWave)); ++w)
+    for (uint32_t w = 0; w < wave; ++w)
     {
         counts += s.waveCounts[w];
         weights += s.waveWeights[w];
@@ -442,57 +484,80 @@ __device__ __forceinline__ bool Reaches(const RowGrid& r, const Place& at)
 
 /// Calls use(key, step, mass) for the row's logits in steps first..last, by all threads.
 ///
-/// What bounds it: the row's arrival at one CU. A bound in f32, a little wide, keeps the 64-bit arithmetic to the
-/// logits near the steps.
+/// What bounds it: the row's arrival at one CU. Bounds in f32, a little wide, tell which of a thread's 32 logits may be
+/// meant; those are placed one by one (a copy of that for each of them filled the instruction cache).
 template <typename Use>
 __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, Use use)
 {
     const double wide = 0.5 + 1e-6 + 1e-9 * fabs(r.top);
     const float low = __double2float_rd((r.top - last - wide) / r.perUnit);
     const float high = __double2float_ru((r.top - first + wide) / r.perUnit);
-    auto look = [&](float v, uint32_t index) {
-        const float x = Counted(v);
-        if (x >= low && x <= high && x > -INFINITY)
+    const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(r.x) / 4 % 4)) % 4u, r.vocab);
+    const uint32_t quads = (r.vocab - head) / 4;
+    const uint32_t edges = r.vocab - 4 * quads;  // before the first quad and behind the last
+    // +inf is not above `high`, which is rounded up, where it counts as f32's last number.
+    const float most = high >= 0x1.fffffep127f ? INFINITY : high;
+    constexpr uint32_t kAhead = 8;  // quads of a thread in a round; the next round's are on their way
+    float4v v[kAhead], next[kAhead];
+    auto load = [&](uint32_t from) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i)
         {
+            const uint32_t quad = min(from + i * kPickBlock + threadIdx.x, quads - 1);
+            next[i] = *reinterpret_cast<const float4v*>(r.x + head + 4 * quad);
+        }
+    };
+    if (quads > 0)
+    {
+        load(0);
+    }
+    // The first round is that of the edges.
+    uint32_t may = threadIdx.x < edges ? 1u : 0u;
+    bool edge = true;
+    const uint32_t edgeIndex = threadIdx.x < head ? threadIdx.x : threadIdx.x + 4 * quads;
+    v[0][0] = r.x[threadIdx.x < edges ? edgeIndex : 0];
+    uint32_t from = 0;
+    while (true)
+    {
+        while (may != 0)
+        {
+            const uint32_t bit = __ffs(static_cast<int>(may)) - 1;
+            may &= may - 1;
+            float logit = v[0][0];
+#pragma unroll
+            for (uint32_t i = 1; i < 4 * kAhead; ++i)
+            {
+                logit = bit == i ? v[i / 4][i % 4] : logit;
+            }
+            const uint32_t index = edge ? edgeIndex : head + 4 * (from + bit / 4 * kPickBlock + threadIdx.x) + bit % 4;
+            const float x = Counted(logit);
             const Place at = PlaceOf(x, r.perUnit);
             const double d = r.top - at.step;
-            if (d >= first && d <= last)
+            if (x > -INFINITY && d >= first && d <= last)
             {
                 use(OrderKey(x, index), static_cast<uint32_t>(d), MassOf(at.rest));
             }
         }
-    };
-    const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(r.x) / 4 % 4)) % 4u, r.vocab);
-    const uint32_t quads = (r.vocab - head) / 4;
-    const uint32_t tail = head + 4 * quads;
-    if (threadIdx.x < head)
-    {
-        look(r.x[threadIdx.x], threadIdx.x);
-    }
-    if (threadIdx.x < r.vocab - tail)
-    {
-        look(r.x[tail + threadIdx.x], tail + threadIdx.x);
-    }
-    for (uint32_t from = 0; from < quads; from += kPickBlock * kPickLoads)
-    {
-        float4v v[kPickLoads];
-#pragma unroll
-        for (uint32_t i = 0; i < kPickLoads; ++i)
+        from += edge ? 0 : kPickBlock * kAhead;
+        edge = false;
+        if (from >= quads)
         {
-            const uint32_t quad = min(from + i * kPickBlock + threadIdx.x, quads - 1);
-            v[i] = *reinterpret_cast<const float4v*>(r.x + head + 4 * quad);
+            break;
         }
 #pragma unroll
-        for (uint32_t i = 0; i < kPickLoads; ++i)
+        for (uint32_t i = 0; i < kAhead; ++i)
         {
-            const uint32_t quad = from + i * kPickBlock + threadIdx.x;
-            if (quad < quads)
-            {
+            v[i] = next[i];
+        }
+        load(from + kPickBlock * kAhead);
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e)
-                {
-                    look(v[i][e], head + 4 * quad + e);
-                }
+        for (uint32_t i = 0; i < kAhead; ++i)
+        {
+            const bool there = from + i * kPickBlock + threadIdx.x < quads;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+            {
+                may |= there && v[i][e] >= low && v[i][e] <= most ? 1u << (4 * i + e) : 0u;
             }
         }
     }
@@ -747,26 +812,6 @@ __device__ Cut LastKeptOfRow(const RowGrid& r, uint32_t d, uint32_t most, uint64
     return Cut{prefix, aboveMass};
 }
 
-/// The cut in step d, from the list where it has the step.
-__device__ __forceinline__ Cut CutStep(const RowGrid& r, uint32_t d, bool listed, uint32_t most, double limit,
-                                       PickSpace& s)
-{
-    const uint64_t below = limit < 0x1p63 ? static_cast<uint64_t>(ceil(limit)) : ~0ull;
-    if (!listed)
-    {
-        return LastKeptOfRow(r, d, most, below, s);
-    }
-    return LastKept(
-        s.listed,
-        [&](uint32_t i, uint64_t& key, uint64_t& mass) {
-            key = s.keys[i];
-            const Place at = PlaceOf(KeyValue(key), r.perUnit);
-            mass = MassOf(at.rest);
-            return r.top - at.step == static_cast<double>(d) && Reaches(r, at);
-        },
-        most, below, s);
-}
-
 /// Decides a row: where the cuts lie in the steps' counts and masses, and which token the number lands on. Where the
 /// logits of the steps down to the cut are few they are listed, in one pass over the row; else the step of the cut is,
 /// and the token is looked for in the part of the row that the parts' masses name.
@@ -784,22 +829,27 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     const RowMode mode = ModeOf(a, row);
     const float topP = a.topPs != nullptr ? a.topPs[row] : 1.0f;
     const float minP = a.minPs != nullptr ? a.minPs[row] : 0.0f;
-    const double random = a.randoms[row];
+    const double given = a.randoms[row];
+    const double number = given > 0.0 ? given : 0.0;
     if (lane >= a.parts)
     {
         head = PartHead{-INFINITY, -INFINITY, ~0u};
     }
     const float most = GroupMax<kWave>(head.most);
-    uint32_t at = head.most == most ? head.at : ~0u;
     double top = head.top;
 #pragma unroll
     for (int step = 1; step < kWave; step *= 2)
     {
-        at = min(at, static_cast<uint32_t>(__shfl_xor(at, step)));
         top = fmax(top, __shfl_xor(top, step));
     }
     if (most == -INFINITY || mode.perUnit < 0.0)
     {
+        uint32_t at = head.most == most ? head.at : ~0u;
+#pragma unroll
+        for (int step = 1; step < kWave; step *= 2)
+        {
+            at = min(at, static_cast<uint32_t>(__shfl_xor(at, step)));
+        }
         if (threadIdx.x == 0)
         {
             a.tokens[row] = most == -INFINITY ? -1 : static_cast<int32_t>(at);
@@ -817,7 +867,8 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     r.top = top;
     r.largest = PlaceOf(most, mode.perUnit);
     r.lowest = -INFINITY;
-    const uint32_t d = threadIdx.x % kSteps;
+    static_assert(kPickBlock == kSteps, "a thread a step");
+    const uint32_t d = threadIdx.x;
     if (wave == 0)
     {
         const double by = top - head.top;
@@ -829,50 +880,34 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
             s.stepP = kSteps - 1;
         }
     }
-    if (threadIdx.x < kSteps)
-    {
-        s.unit[d] = UnitOf(d);
-    }
+    s.unit[d] = UnitOf(d);
     __syncthreads();
 
-    // The row's steps: half of the threads take every other part, several parts' on their way at a time.
-    static_assert(kPickBlock == 2 * kSteps, "two threads a step");
+    // The row's steps, a thread each, several parts' on their way at a time.
     uint64_t mass = 0;
     uint32_t count = 0;
+    constexpr uint32_t kDeep = 20;
+    for (uint32_t p0 = 0; p0 < a.parts; p0 += kDeep)
     {
-        constexpr uint32_t kDeep = 16;
-        const uint32_t half = threadIdx.x / kSteps;
-        for (uint32_t p0 = half; p0 < a.parts; p0 += 2 * kDeep)
-        {
-            uint64_t m[kDeep];
-            uint32_t c[kDeep];
+        uint64_t m[kDeep];
+        uint32_t c[kDeep];
 #pragma unroll
-            for (uint32_t i = 0; i < kDeep; ++i)
-            {
-                const uint32_t p = min(p0 + 2 * i, a.parts - 1);
-                const uint32_t shift = s.partShift[p];
-                const uint64_t from = (slot + p) * kSteps + (d >= shift ? d - shift : 0);
-                const bool is = p0 + 2 * i < a.parts && d >= shift;
-                m[i] = is && mode.weighed ? a.masses[from] : 0;
-                c[i] = is && mode.counted ? a.counts[from] : 0;
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < kDeep; ++i)
-            {
-                mass += m[i];
-                count += c[i];
-            }
-        }
-        if (half == 1)
+        for (uint32_t i = 0; i < kDeep; ++i)
         {
-            s.masses[d] = mass;
-            s.counts[d] = count;
+            const uint32_t p = min(p0 + i, a.parts - 1);
+            const uint32_t shift = s.partShift[p];
+            const uint64_t from = (slot + p) * kSteps + (d >= shift ? d - shift : 0);
+            const bool is = p0 + i < a.parts && d >= shift;
+            m[i] = is && mode.weighed ? a.masses[from] : 0;
+            c[i] = is && mode.counted ? a.counts[from] : 0;
         }
-        __syncthreads();
-        mass = half == 0 ? mass + s.masses[d] : 0;
-        count = half == 0 ? count + s.counts[d] : 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kDeep; ++i)
+        {
+            mass += m[i];
+            count += c[i];
+        }
     }
-    const bool mine = threadIdx.x < kSteps;
     double weight = static_cast<double>(mass) * s.unit[d];
     if (!mode.counted)
     {
@@ -880,11 +915,8 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         count = static_cast<uint32_t>(static_cast<double>(mass) * (0x1p-38 * 1.0443)) + (mass != 0 ? 1u : 0u);
     }
     StepSums(count, weight, s);
-    if (mine)
-    {
-        s.counts[d] = count;
-        s.upTo[d] = weight;
-    }
+    s.counts[d] = count;
+    s.upTo[d] = weight;
     __syncthreads();
     // The step in which the first k end.
     uint32_t stepK = kSteps - 1;
@@ -893,327 +925,382 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     if (mode.counted)
     {
         const uint32_t k = min(static_cast<uint32_t>(mode.topK), s.counts[kSteps - 1]);
-        if (mine && count >= k)
+        if (count >= k && (d == 0 || s.counts[d - 1] < k))  // one thread
         {
-            atomicMin(&s.stepK, d);
+            s.stepK = d;
         }
         __syncthreads();
         stepK = s.stepK;
         left = k - (stepK > 0 ? s.counts[stepK - 1] : 0);
         wholeK = s.counts[stepK] == k;
     }
-    // Steps that are listed: first..last.
-    uint32_t listFirst = 1;
-    uint32_t listLast = 0;
-    bool partsKnown = true;
-    if (!mode.weighed)
+    auto countOf = [&](uint32_t step) { return s.counts[step] - (step > 0 ? s.counts[step - 1] : 0); };
+    auto weightBefore = [&](uint32_t step) { return step > 0 ? s.upTo[step - 1] : 0.0; };
+    if (mode.weighed == false && s.counts[stepK] > kListed)
     {
-        if (mine)
+        // Counted alone, and too many for the list after all: the masses by a pass of their own.
+        s.masses[d] = 0;
+        __syncthreads();
+        ForSteps(r, 0, stepK, [&](uint64_t, uint32_t step, uint64_t one) {
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[step]), one);
+        });
+    }
+
+    // In turn, where each is needed: the masses of a list that has all of the first k; the cut of these; the cut of
+    // all that is kept; and the token among what is listed.
+    enum Task
+    {
+        kMassesOfK,
+        kCutOfK,
+        kCutOfAll,
+        kToken
+    };
+    const bool narrow = topP < 1.0f;
+    Task task = !mode.weighed ? kMassesOfK : narrow && !wholeK ? kCutOfK : kCutOfAll;
+    uint32_t listFirst = 1;  // steps that are listed: none
+    uint32_t listLast = 0;
+    uint32_t step = 0;       // of the cut of all
+    bool whole = false;      // nothing of that step is cut off
+    bool all = false;        // all that is kept is listed
+    double ofK = 0.0;
+    double share = INFINITY;
+    double total = 0.0;
+    uint32_t stepP = kSteps;
+    Cut cut{0, 0};
+    Cut token{0, 0};
+    while (true)
+    {
+        uint32_t from = 1;  // to be listed
+        uint32_t to = 0;
+        if (task == kMassesOfK)
         {
-            s.masses[d] = 0;
+            to = s.counts[stepK] <= kListed ? stepK : 0;
+            from = s.counts[stepK] <= kListed ? 0 : 1;
         }
-        partsKnown = false;
-        if (s.counts[stepK] <= kListed)
+        else if (task == kCutOfK)
         {
-            ListSteps(r, 0, stepK, s);
-            listFirst = 0;
-            listLast = stepK;
+            to = countOf(stepK) <= kListed ? stepK : 0;
+            from = countOf(stepK) <= kListed ? stepK : 1;
+        }
+        else if (task == kCutOfAll)
+        {
+            if (narrow)
+            {
+                // The step in which top-p's share of the first k's weight is reached.
+                share = static_cast<double>(topP) * (wholeK ? s.upTo[stepK] : ofK);
+                auto reached = [&](double sum) { return sum > 0.0 && sum >= share; };
+                if (reached(weight) && (d == 0 || !reached(s.upTo[d - 1])))
+                {
+                    s.stepP = d;
+                }
+                __syncthreads();
+                stepP = min(s.stepP, stepK);
+            }
+            // The step in which min-p's bound lies; the largest always reaches it.
+            uint32_t stepM = kSteps;
+            if (minP > 0.0f)
+            {
+                const double lowest = fmin(8.0 * log2(static_cast<double>(minP)), 0.0);
+                const double by = top - rint(r.largest.step + r.largest.rest + lowest);
+                stepM = by < kSteps ? static_cast<uint32_t>(fmax(by, top - r.largest.step)) : kSteps;
+                r.lowest = stepM <= min(stepK, stepP) ? lowest : -INFINITY;
+            }
+            step = min(min(stepK, stepP), stepM);
+            whole = step != stepP && step != stepM && (step != stepK || wholeK);
+            const bool have = listFirst == 0 && step <= listLast;
+            all = have || s.counts[step] <= kListed;
+            if (!have && (all || (!whole && countOf(step) <= kListed)))
+            {
+                from = all ? 0 : step;
+                to = step;
+            }
+            total = s.upTo[step];
+        }
+        if (from <= to && !(listFirst <= from && to <= listLast))
+        {
+            ListSteps(r, from, to, s);
+            listFirst = from;
+            listLast = to;
+        }
+        if (task == kMassesOfK)
+        {
+            if (from <= to)
+            {
+                s.masses[d] = 0;
+                __syncthreads();
+                for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+                {
+                    const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[static_cast<uint32_t>(top - place.step)]),
+                              MassOf(place.rest));
+                }
+            }
+            __syncthreads();
+            uint32_t unused = 0;
+            weight = static_cast<double>(s.masses[d]) * s.unit[d];
+            StepSums(unused, weight, s);
+            s.upTo[d] = weight;
+            __syncthreads();
+            task = narrow && !wholeK ? kCutOfK : kCutOfAll;
+            continue;
+        }
+        // What is looked for: items of step `of` (or, for the token, all that are kept).
+        const uint32_t of = task == kCutOfK ? stepK : step;
+        uint32_t atMost = ~0u;
+        double limit = INFINITY;
+        bool needed = true;
+        if (task == kCutOfK)
+        {
+            atMost = left;
+        }
+        else if (task == kCutOfAll)
+        {
+            needed = !whole;
+            atMost = minP > 1.0f ? 1u : step == stepK ? left : ~0u;
+            // A share that is reached before this step's first, by a rounding, still keeps that one.
+            limit = step == stepP ? fmax((share - weightBefore(step)) / s.unit[step], 0x1p-30) : INFINITY;
+        }
+        auto item = [&](uint32_t i, uint64_t& key, uint64_t& ofKey) {
+            key = s.keys[i];
+            const Place place = PlaceOf(KeyValue(key), r.perUnit);
+            const uint32_t dist = static_cast<uint32_t>(top - place.step);
+            ofKey = MassOf(place.rest);
+            if (task != kToken)
+            {
+                return dist == of && Reaches(r, place);
+            }
+            // By falling ~index, weights as whole numbers, whose sums are exact.
+            const bool kept = dist < of || (dist == of && key >= cut.key);
+            ofKey = static_cast<uint64_t>(rint(static_cast<double>(ofKey) * (s.unit[dist] * kFixed)));
+            key &= 0xFFFFFFFFull;
+            return kept && ofKey != 0;
+        };
+        if (task == kToken)
+        {
+            __syncthreads();
+            if (threadIdx.x == 0)
+            {
+                s.sum = 0;
+            }
+            __syncthreads();
+            uint64_t sum = 0;
             for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
             {
-                const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
-                atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[static_cast<uint32_t>(top - place.step)]),
-                          MassOf(place.rest));
+                uint64_t key, fixed;
+                sum += item(i, key, fixed) ? fixed : 0;
             }
+            sum = WaveSum(static_cast<unsigned long long>(sum));
+            if (lane == 0 && sum != 0)
+            {
+                atomicAdd(&s.sum, static_cast<unsigned long long>(sum));
+            }
+            __syncthreads();
+            // The first token whose sum is past the number's share is the last that begins at or before it.
+            limit = floor(number * static_cast<double>(s.sum)) + 1.0;
+        }
+        Cut found{0, 0};
+        if (needed)
+        {
+            const uint64_t below = limit < 0x1p63 ? static_cast<uint64_t>(ceil(limit)) : ~0ull;
+            found = task == kToken || (listFirst <= of && of <= listLast) ? LastKept(s.listed, item, atMost, below, s)
+                                                                          : LastKeptOfRow(r, of, atMost, below, s);
+        }
+        if (task == kCutOfK)
+        {
+            ofK = weightBefore(stepK) + static_cast<double>(found.mass) * s.unit[stepK];
+            task = kCutOfAll;
+        }
+        else if (task == kCutOfAll)
+        {
+            cut = found;
+            total = whole ? total : weightBefore(step) + static_cast<double>(cut.mass) * s.unit[step];
+            if (!all)
+            {
+                break;
+            }
+            task = kToken;
         }
         else
         {
-            __syncthreads();
-            ForSteps(r, 0, stepK, [&](uint64_t, uint32_t step, uint64_t one) {
-                atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[step]), one);
-            });
+            token = found;
+            break;
         }
-        __syncthreads();
-        uint32_t unused = 0;
-        weight = mine ? static_cast<double>(s.masses[d]) * s.unit[d] : 0.0;
-        StepSums(unused, weight, s);
-        if (mine)
-        {
-            s.upTo[d] = weight;
-        }
-        __syncthreads();
     }
-    auto countOf = [&](uint32_t step) { return s.counts[step] - (step > 0 ? s.counts[step - 1] : 0); };
-    auto weightBefore = [&](uint32_t step) { return step > 0 ? s.upTo[step - 1] : 0.0; };
-    auto isListed = [&](uint32_t step) { return listFirst <= step && step <= listLast; };
-    // Lists a step if it is not and fits.
-    auto listStep = [&](uint32_t step) {
-        if (!isListed(step) && countOf(step) <= kListed)
-        {
-            ListSteps(r, step, step, s);
-            listFirst = step;
-            listLast = step;
-        }
-    };
-    // The step in which top-p's share of their weight is reached.
-    uint32_t stepP = kSteps;
-    double share = INFINITY;
-    if (topP < 1.0f)
-    {
-        double ofK = s.upTo[stepK];
-        if (!wholeK)
-        {
-            listStep(stepK);
-            ofK = weightBefore(stepK) +
-                  static_cast<double>(CutStep(r, stepK, isListed(stepK), left, INFINITY, s).mass) * s.unit[stepK];
-        }
-        share = static_cast<double>(topP) * ofK;
-        if (mine && d <= stepK && weight > 0.0 && weight >= share)
-        {
-            atomicMin(&s.stepP, d);
-        }
-        __syncthreads();
-        stepP = min(s.stepP, stepK);
-    }
-    // The step in which min-p's bound lies; the largest always reaches it.
-    uint32_t stepM = kSteps;
-    if (minP > 0.0f)
-    {
-        const double lowest = fmin(8.0 * log2(static_cast<double>(minP)), 0.0);
-        const double by = top - rint(r.largest.step + r.largest.rest + lowest);
-        stepM = by < kSteps ? static_cast<uint32_t>(fmax(by, top - r.largest.step)) : kSteps;
-        r.lowest = stepM <= min(stepK, stepP) ? lowest : -INFINITY;
-        left = minP > 1.0f ? 1u : left;
-    }
-    const uint32_t step = min(min(stepK, stepP), stepM);
-    const bool whole = step != stepP && step != stepM && (step != stepK || wholeK);
-    const bool all = listFirst == 0 && step <= listLast ? true : s.counts[step] <= kListed;
-    if (all && !(listFirst == 0 && step <= listLast))
-    {
-        ListSteps(r, 0, step, s);
-        listFirst = 0;
-        listLast = step;
-    }
-    Cut cut{0, 0};
-    double total = s.upTo[step];
-    if (!whole)
-    {
-        listStep(step);
-        // A share that is reached before this step's first, by a rounding, still keeps that one.
-        const double limit =
-            step == stepP ? fmax((share - weightBefore(step)) / s.unit[step], 0x1p-30) : INFINITY;
-        cut = CutStep(r, step, isListed(step), step == stepK || minP > 1.0f ? left : ~0u, limit, s);
-        total = weightBefore(step) + static_cast<double>(cut.mass) * s.unit[step];
-    }
-    const double number = random > 0.0 ? random : 0.0;
+
+    uint32_t index = ~static_cast<uint32_t>(token.key);
+    double ofToken = 0.0;  // its weight, in one thread
+    bool writes = false;
     if (all)
     {
-        // All that is kept is listed: weights as whole numbers, whose sums are exact, by falling ~index.
-        const double last = static_cast<double>(step);
-        auto item = [&](uint32_t i, uint64_t& key, uint64_t& fixed) {
-            const uint64_t of = s.keys[i];
-            const Place place = PlaceOf(KeyValue(of), r.perUnit);
-            const double dist = top - place.step;
-            const bool kept = dist < last || (dist == last && of >= cut.key);
-            key = of & 0xFFFFFFFFull;
-            fixed = kept ? static_cast<uint64_t>(rint(static_cast<double>(MassOf(place.rest)) *
-                                                      (s.unit[static_cast<uint32_t>(dist)] * kFixed)))
-                         : 0;
-            return kept && fixed != 0;
-        };
-        __syncthreads();
-        if (threadIdx.x == 0)
-        {
-            s.sum = 0;
-        }
-        __syncthreads();
-        uint64_t sum = 0;
-        for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
-        {
-            uint64_t key, fixed;
-            sum += item(i, key, fixed) ? fixed : 0;
-        }
-        sum = WaveSum(static_cast<unsigned long long>(sum));
-        if (lane == 0)
-        {
-            atomicAdd(&s.sum, static_cast<unsigned long long>(sum));
-        }
-        __syncthreads();
-        // The first token whose sum is past the number's share is the last that begins at or before it.
-        const double reach = number * static_cast<double>(s.sum);
-        const uint64_t limit = reach < 0x1p63 ? static_cast<uint64_t>(floor(reach)) + 1 : ~0ull;
-        const Cut token = LastKept(s.listed, item, ~0u, limit, s);
         for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
         {
             if ((s.keys[i] & 0xFFFFFFFFull) == token.key)
             {
-                a.tokens[row] = static_cast<int32_t>(~static_cast<uint32_t>(token.key));
-                if (a.logprobs != nullptr)
-                {
-                    const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
-                    const double of =
-                        static_cast<double>(MassOf(place.rest)) * s.unit[static_cast<uint32_t>(top - place.step)];
-                    a.logprobs[row] = static_cast<float>(log(of / total));
-                }
+                const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
+                ofToken = static_cast<double>(MassOf(place.rest)) * s.unit[static_cast<uint32_t>(top - place.step)];
+                writes = true;
             }
         }
-        return;
     }
-
-    // Kept: the steps before, and of this one the keys from the cut on.
-    auto weightAt = [&](float v, uint32_t index) {
-        const float x = Counted(v);
-        const Place place = PlaceOf(x, r.perUnit);
-        const double dist = top - place.step;
-        const bool kept = dist < static_cast<double>(step) ||
-                          (dist == static_cast<double>(step) && OrderKey(x, index) >= cut.key);
-        return kept ? static_cast<double>(MassOf(place.rest)) * s.unit[static_cast<uint32_t>(dist)] : 0.0;
-    };
-    const double reach = number * total;
-    uint32_t begin = 0;
-    uint32_t end = a.vocab;
-    double passed = 0.0;
-    if (partsKnown)
+    else
     {
-        // What each part has of it: the steps before from its masses, this one's kept logits by a look at them.
-        __syncthreads();
-        const uint32_t until = whole ? step + 1 : step;
-        for (uint32_t p = wave; p < a.parts; p += kPickWaves)
+        // Kept: the steps before, and of this one the keys from the cut on.
+        auto weightAt = [&](float v, uint32_t at) {
+            const float x = Counted(v);
+            const Place place = PlaceOf(x, r.perUnit);
+            const double dist = top - place.step;
+            const bool kept = dist < static_cast<double>(step) ||
+                              (dist == static_cast<double>(step) && OrderKey(x, at) >= cut.key);
+            return kept ? static_cast<double>(MassOf(place.rest)) * s.unit[static_cast<uint32_t>(dist)] : 0.0;
+        };
+        const double reach = number * total;
+        uint32_t begin = 0;
+        uint32_t end = a.vocab;
+        double passed = 0.0;
+        if (mode.weighed)
         {
-            const uint32_t shift = s.partShift[p];
-            double sum = 0.0;
-            for (uint32_t i = shift + lane; i < until; i += kWave)
+            // What each part has of it: the steps before from its masses, this one's kept logits by a look at them.
+            __syncthreads();
+            const uint32_t until = whole ? step + 1 : step;
+            for (uint32_t p = wave; p < a.parts; p += kPickWaves)
             {
-                sum += static_cast<double>(a.masses[(slot + p) * kSteps + i - shift]) * s.unit[i];
-            }
-            sum = WaveSum(sum);
-            if (lane == 0)
-            {
-                s.partWeight[p] = sum;
-            }
-        }
-        if (!whole)
-        {
-            auto use = [&](uint64_t key, uint64_t one) {
-                if (key >= cut.key)
+                const uint32_t shift = s.partShift[p];
+                double sum = 0.0;
+#pragma unroll 4
+                for (uint32_t i = shift + lane; i < until; i += kWave)
                 {
-                    atomicAdd(&s.partMass[~static_cast<uint32_t>(key) / a.partLength],
-                              static_cast<unsigned long long>(one));
+                    sum += static_cast<double>(a.masses[(slot + p) * kSteps + i - shift]) * s.unit[i];
                 }
-            };
-            if (isListed(step))
-            {
-                for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+                sum = WaveSum(sum);
+                if (lane == 0)
                 {
-                    const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
-                    if (top - place.step == static_cast<double>(step))
+                    s.partWeight[p] = sum;
+                }
+            }
+            if (!whole)
+            {
+                auto use = [&](uint64_t key, uint64_t one) {
+                    if (key >= cut.key)
                     {
-                        use(s.keys[i], MassOf(place.rest));
+                        atomicAdd(&s.partMass[~static_cast<uint32_t>(key) / a.partLength],
+                                  static_cast<unsigned long long>(one));
+                    }
+                };
+                if (listFirst <= step && step <= listLast)
+                {
+                    for (uint32_t i = threadIdx.x; i < s.listed; i += kPickBlock)
+                    {
+                        const Place place = PlaceOf(KeyValue(s.keys[i]), r.perUnit);
+                        if (top - place.step == static_cast<double>(step))
+                        {
+                            use(s.keys[i], MassOf(place.rest));
+                        }
+                    }
+                }
+                else
+                {
+                    ForSteps(r, step, step, [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
+                }
+            }
+            __syncthreads();
+            // The first part that reaches past the number's share, else the last with anything kept.
+            uint32_t part = 0;
+            double upToPart = 0.0;
+            for (uint32_t p = 0; p < a.parts; ++p)
+            {
+                const double ofPart = s.partWeight[p] + static_cast<double>(s.partMass[p]) * s.unit[step];
+                if (ofPart > 0.0)
+                {
+                    part = p;
+                    passed = upToPart;
+                    upToPart += ofPart;
+                    if (upToPart > reach)
+                    {
+                        break;
                     }
                 }
             }
-            else
-            {
-                ForSteps(r, step, step, [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
-            }
+            begin = part * a.partLength;
+            end = min(begin + a.partLength, a.vocab);
         }
-        __syncthreads();
-        // The first part that reaches past the number's share, else the last with anything kept.
-        uint32_t part = 0;
-        double upToPart = 0.0;
-        for (uint32_t p = 0; p < a.parts; ++p)
+        // Sums of groups of logits, and the first group that reaches past it, else the last with anything kept.
+        const uint32_t groups = (end - begin + kGroup - 1) / kGroup;
+        uint32_t group = 0;
+        double sum = passed;
+        bool past = false;
+        for (uint32_t first = 0; first < groups && !past; first += kGroups)
         {
-            const double of = s.partWeight[p] + static_cast<double>(s.partMass[p]) * s.unit[step];
-            if (of > 0.0)
+            const uint32_t here = min(groups - first, kGroups);
+            __syncthreads();
+            for (uint32_t i = wave; i < here; i += kPickWaves)
             {
-                part = p;
-                passed = upToPart;
-                upToPart += of;
-                if (upToPart > reach)
+                float v[kPickLoads];
+                const uint32_t at = begin + (first + i) * kGroup + lane;
+#pragma unroll
+                for (uint32_t j = 0; j < kPickLoads; ++j)
                 {
-                    break;
+                    v[j] = r.x[min(at + j * kWave, end - 1)];
+                }
+                double own = 0.0;
+#pragma unroll
+                for (uint32_t j = 0; j < kPickLoads; ++j)
+                {
+                    own += at + j * kWave < end ? weightAt(v[j], at + j * kWave) : 0.0;
+                }
+                own = WaveSum(own);
+                if (lane == 0)
+                {
+                    s.groupWeights[i] = own;
+                }
+            }
+            __syncthreads();
+            for (uint32_t i = 0; i < here && !past; ++i)
+            {
+                const double ofGroup = s.groupWeights[i];
+                if (ofGroup > 0.0)
+                {
+                    group = first + i;
+                    passed = sum;
+                    sum += ofGroup;
+                    past = sum > reach;
                 }
             }
         }
-        begin = part * a.partLength;
-        end = min(begin + a.partLength, a.vocab);
-    }
-    // Sums of groups of logits, and the first group that reaches past it, else the last with anything kept.
-    const uint32_t groups = (end - begin + kGroup - 1) / kGroup;
-    uint32_t group = 0;
-    double sum = passed;
-    bool past = false;
-    for (uint32_t first = 0; first < groups && !past; first += kPickBlock)
-    {
-        const uint32_t here = min(groups - first, static_cast<uint32_t>(kPickBlock));
-        __syncthreads();
-        for (uint32_t i = wave; i < here; i += kPickWaves)
+        if (wave != 0)
         {
-            float v[kPickLoads];
-            const uint32_t from = begin + (first + i) * kGroup + lane;
-#pragma unroll
-            for (uint32_t j = 0; j < kPickLoads; ++j)
-            {
-                v[j] = r.x[min(from + j * kWave, end - 1)];
-            }
-            double own = 0.0;
-#pragma unroll
-            for (uint32_t j = 0; j < kPickLoads; ++j)
-            {
-                own += from + j * kWave < end ? weightAt(v[j], from + j * kWave) : 0.0;
-            }
-            own = WaveSum(own);
-            if (lane == 0)
-            {
-                s.groupWeights[i] = own;
-            }
+            return;
         }
-        __syncthreads();
-        for (uint32_t i = 0; i < here && !past; ++i)
+        // The first of its logits that reaches past it, else its last that is kept.
+        const uint32_t first = begin + group * kGroup;
+#pragma unroll 1
+        for (uint32_t j = 0; j < kPickLoads; ++j)
         {
-            const double of = s.groupWeights[i];
-            if (of > 0.0)
+            const uint32_t at = first + j * kWave + lane;
+            const double own = at < end ? weightAt(r.x[at], at) : 0.0;
+            const double upToOwn = WaveInclusive(own);
+            const uint64_t kept = __ballot(own > 0.0);
+            const uint64_t over = __ballot(own > 0.0 && passed + upToOwn > reach);
+            if (kept != 0)
             {
-                group = first + i;
-                passed = sum;
-                sum += of;
-                past = sum > reach;
+                const int which = over != 0 ? __ffsll(static_cast<unsigned long long>(over)) - 1
+                                            : 63 - __clzll(static_cast<long long>(kept));
+                index = first + j * kWave + which;
+                ofToken = __shfl(own, which);
             }
+            if (over != 0)
+            {
+                break;
+            }
+            passed += __shfl(upToOwn, kWave - 1);
         }
+        writes = lane == 0;
     }
-    if (wave != 0)
+    if (writes)
     {
-        return;
-    }
-    // The first of its logits that reaches past it, else its last that is kept.
-    uint32_t token = ~0u;
-    double of = 0.0;
-    const uint32_t from = begin + group * kGroup;
-    for (uint32_t j = 0; j < kPickLoads; ++j)
-    {
-        const uint32_t index = from + j * kWave + lane;
-        const double own = index < end ? weightAt(r.x[index], index) : 0.0;
-        const double upToOwn = WaveInclusive(own);
-        const uint64_t kept = __ballot(own > 0.0);
-        const uint64_t over = __ballot(own > 0.0 && passed + upToOwn > reach);
-        if (kept != 0)
-        {
-            const int which = over != 0 ? __ffsll(static_cast<unsigned long long>(over)) - 1
-                                        : 63 - __clzll(static_cast<long long>(kept));
-            token = from + j * kWave + which;
-            of = __shfl(own, which);
-        }
-        if (over != 0)
-        {
-            break;
-        }
-        passed += __shfl(upToOwn, kWave - 1);
-    }
-    if (lane == 0)
-    {
-        a.tokens[row] = static_cast<int32_t>(token);
+        a.tokens[row] = static_cast<int32_t>(index);
         if (a.logprobs != nullptr)
         {
-            a.logprobs[row] = static_cast<float>(log(of / total));
+            a.logprobs[row] = static_cast<float>(log(ofToken / total));
         }
     }
 }
@@ -1228,7 +1315,7 @@ Parts PartsOf(uint32_t rows, uint32_t vocab)
 {
     const uint32_t batches = CeilDiv(vocab, kBatch);
     const uint32_t most = std::min(kMaxParts, CeilDiv(batches, kWaves));
-    const uint32_t wanted = std::max(1u, std::min(most, kBlocksAtOnce / std::max(rows, 1u)));
+    const uint32_t wanted = std::max(1u, std::min(most, kCountBlocks / std::max(rows, 1u)));
     const uint32_t length = CeilDiv(batches, wanted) * kBatch;
     return Parts{CeilDiv(vocab, length), length};
 }
