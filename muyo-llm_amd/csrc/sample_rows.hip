@@ -35,6 +35,8 @@ constexpr uint32_t kMaxRows = (1u << 22) - 1;  // a launch has fewer than 2^32 t
 constexpr uint32_t kMaxVocab = 1u << 24;       // masses of so many logits fit in 63 bits
 constexpr uint32_t kCountBlocks = 2048;        // workgroups to aim at that count
 constexpr double kLog2e = 1.44269504088896340736;
+constexpr uint32_t kListRows = 4096;           // rows whose lists get workgroups of their own
+constexpr uint32_t kListLength = 8192;         // logits that one of those looks through
 constexpr double kFar = 0x1p48;                // places past which steps are not whole numbers apart
 constexpr double kWhole = 0x1.8p52;            // added, the whole part's last 32 bits come last
 constexpr double kFixed = 0x1p50;              // units of the top step's weight, for sums of listed logits
@@ -45,6 +47,18 @@ struct PartHead
     double top;    // the grid's place of its first step, -inf: it has none
     float most;    // its largest logit
     uint32_t at;   // the first place of that, of a greedy row
+};
+
+/// What is known of a row's steps before its token is chosen, and the list of those near the cut.
+struct RowSteps
+{
+    double upTo[kSteps];
+    uint32_t counts[kSteps];
+    double top;
+    uint32_t first, last;  // steps that are listed: none if first > last
+    uint32_t listed;
+    uint32_t unused;
+    uint64_t keys[kListed];
 };
 
 struct SampleArgs
@@ -63,6 +77,7 @@ struct SampleArgs
     PartHead* heads;     // [rows][parts]
     uint64_t* masses;    // [rows][parts][kSteps]
     uint32_t* counts;    // [rows][parts][kSteps]
+    RowSteps* steps;     // [rows], of at most kListRows
 };
 
 /// What a row asks for.
@@ -482,19 +497,20 @@ __device__ __forceinline__ bool Reaches(const RowGrid& r, const Place& at)
     return (at.step - r.largest.step) + (at.rest - r.largest.rest) >= r.lowest;
 }
 
-/// Calls use(key, step, mass) for the row's logits in steps first..last, by all threads.
-///
-/// What bounds it: the row's arrival at one CU. Bounds in f32, a little wide, tell which of a thread's 32 logits may be
+/// Calls use(key, step, mass) for the logits begin..end - 1 of a row that are in steps first..last, by kThreads threads.
+/// Bounds in f32, a little wide, tell which of a thread's 32 logits may be
 /// meant; those are placed one by one (a copy of that for each of them filled the instruction cache).
-template <typename Use>
-__device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, Use use)
+template <int kThreads, typename Use>
+__device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t begin, uint32_t end, uint32_t first, uint32_t last,
+                                         Use use)
 {
+    const float* const part = r.x + begin;
     const double wide = 0.5 + 1e-6 + 1e-9 * fabs(r.top);
     const float low = __double2float_rd((r.top - last - wide) / r.perUnit);
     const float high = __double2float_ru((r.top - first + wide) / r.perUnit);
-    const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(r.x) / 4 % 4)) % 4u, r.vocab);
-    const uint32_t quads = (r.vocab - head) / 4;
-    const uint32_t edges = r.vocab - 4 * quads;  // before the first quad and behind the last
+    const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(part) / 4 % 4)) % 4u, end - begin);
+    const uint32_t quads = (end - begin - head) / 4;
+    const uint32_t edges = end - begin - 4 * quads;  // before the first quad and behind the last
     // +inf is not above `high`, which is rounded up, where it counts as f32's last number.
     const float most = high >= 0x1.fffffep127f ? INFINITY : high;
     constexpr uint32_t kAhead = 8;  // quads of a thread in a round; the next round's are on their way
@@ -503,8 +519,8 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint3
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i)
         {
-            const uint32_t quad = min(from + i * kPickBlock + threadIdx.x, quads - 1);
-            next[i] = *reinterpret_cast<const float4v*>(r.x + head + 4 * quad);
+            const uint32_t quad = min(from + i * kThreads + threadIdx.x, quads - 1);
+            next[i] = *reinterpret_cast<const float4v*>(part + head + 4 * quad);
         }
     };
     if (quads > 0)
@@ -515,7 +531,7 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint3
     uint32_t may = threadIdx.x < edges ? 1u : 0u;
     bool edge = true;
     const uint32_t edgeIndex = threadIdx.x < head ? threadIdx.x : threadIdx.x + 4 * quads;
-    v[0][0] = r.x[threadIdx.x < edges ? edgeIndex : 0];
+    v[0][0] = part[threadIdx.x < edges ? edgeIndex : 0];
     uint32_t from = 0;
     while (true)
     {
@@ -529,16 +545,16 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint3
             {
                 logit = bit == i ? v[i / 4][i % 4] : logit;
             }
-            const uint32_t index = edge ? edgeIndex : head + 4 * (from + bit / 4 * kPickBlock + threadIdx.x) + bit % 4;
+            const uint32_t at = edge ? edgeIndex : head + 4 * (from + bit / 4 * kThreads + threadIdx.x) + bit % 4;
             const float x = Counted(logit);
-            const Place at = PlaceOf(x, r.perUnit);
-            const double d = r.top - at.step;
+            const Place place = PlaceOf(x, r.perUnit);
+            const double d = r.top - place.step;
             if (x > -INFINITY && d >= first && d <= last)
             {
-                use(OrderKey(x, index), static_cast<uint32_t>(d), MassOf(at.rest));
+                use(OrderKey(x, begin + at), static_cast<uint32_t>(d), MassOf(place.rest));
             }
         }
-        from += edge ? 0 : kPickBlock * kAhead;
+        from += edge ? 0 : kThreads * kAhead;
         edge = false;
         if (from >= quads)
         {
@@ -549,11 +565,11 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint3
         {
             v[i] = next[i];
         }
-        load(from + kPickBlock * kAhead);
+        load(from + kThreads * kAhead);
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i)
         {
-            const bool there = from + i * kPickBlock + threadIdx.x < quads;
+            const bool there = from + i * kThreads + threadIdx.x < quads;
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e)
             {
@@ -572,7 +588,7 @@ __device__ __forceinline__ void ListSteps(const RowGrid& r, uint32_t first, uint
         s.listed = 0;
     }
     __syncthreads();
-    ForSteps(r, first, last, [&](uint64_t key, uint32_t, uint64_t) {
+    ForSteps<kPickBlock>(r, 0, r.vocab, first, last, [&](uint64_t key, uint32_t, uint64_t) {
         const uint32_t at = atomicAdd(&s.listed, 1u);
         if (at < kListed)
         {
@@ -771,7 +787,7 @@ __device__ Cut LastKeptOfRow(const RowGrid& r, uint32_t d, uint32_t most, uint64
             s.digitMasses[i] = 0;
         }
         __syncthreads();
-        ForSteps(r, d, d, [&](uint64_t key, uint32_t, uint64_t mass) {
+        ForSteps<kPickBlock>(r, 0, r.vocab, d, d, [&](uint64_t key, uint32_t, uint64_t mass) {
             if ((shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))) &&
                 Reaches(r, PlaceOf(KeyValue(key), r.perUnit)))
             {
@@ -812,9 +828,19 @@ __device__ Cut LastKeptOfRow(const RowGrid& r, uint32_t d, uint32_t most, uint64
     return Cut{prefix, aboveMass};
 }
 
+/// What the launches of a row's end do: everything; or the steps and what of them is to be listed, and then, with the
+/// list made by workgroups all over the GPU, the rest.
+enum PickPhase
+{
+    kPickAll,
+    kPickSteps,
+    kPickToken
+};
+
 /// Decides a row: where the cuts lie in the steps' counts and masses, and which token the number lands on. Where the
 /// logits of the steps down to the cut are few they are listed, in one pass over the row; else the step of the cut is,
 /// and the token is looked for in the part of the row that the parts' masses name.
+template <PickPhase kPhase>
 __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
 {
     __shared__ PickSpace s;
@@ -841,6 +867,18 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     for (int step = 1; step < kWave; step *= 2)
     {
         top = fmax(top, __shfl_xor(top, step));
+    }
+    RowSteps* const kept = kPhase == kPickAll ? nullptr : a.steps + row;
+    if (kPhase == kPickSteps && threadIdx.x == 0)
+    {
+        kept->top = top;
+        kept->first = 1;
+        kept->last = 0;
+        kept->listed = 0;
+    }
+    if (kPhase == kPickSteps && (most == -INFINITY || mode.perUnit < 0.0))
+    {
+        return;
     }
     if (most == -INFINITY || mode.perUnit < 0.0)
     {
@@ -883,40 +921,54 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     s.unit[d] = UnitOf(d);
     __syncthreads();
 
-    // The row's steps, a thread each, several parts' on their way at a time.
-    uint64_t mass = 0;
     uint32_t count = 0;
-    constexpr uint32_t kDeep = 20;
-    for (uint32_t p0 = 0; p0 < a.parts; p0 += kDeep)
+    double weight = 0.0;
+    if constexpr (kPhase == kPickToken)
     {
-        uint64_t m[kDeep];
-        uint32_t c[kDeep];
-#pragma unroll
-        for (uint32_t i = 0; i < kDeep; ++i)
-        {
-            const uint32_t p = min(p0 + i, a.parts - 1);
-            const uint32_t shift = s.partShift[p];
-            const uint64_t from = (slot + p) * kSteps + (d >= shift ? d - shift : 0);
-            const bool is = p0 + i < a.parts && d >= shift;
-            m[i] = is && mode.weighed ? a.masses[from] : 0;
-            c[i] = is && mode.counted ? a.counts[from] : 0;
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < kDeep; ++i)
-        {
-            mass += m[i];
-            count += c[i];
-        }
+        count = kept->counts[d];
+        weight = kept->upTo[d];
     }
-    double weight = static_cast<double>(mass) * s.unit[d];
-    if (!mode.counted)
+    else
     {
-        // A bound: a logit's mass is at least 2^(-1/16) of a unit's.
-        count = static_cast<uint32_t>(static_cast<double>(mass) * (0x1p-38 * 1.0443)) + (mass != 0 ? 1u : 0u);
+        // The row's steps, a thread each, several parts' on their way at a time.
+        uint64_t mass = 0;
+        constexpr uint32_t kDeep = 20;
+        for (uint32_t p0 = 0; p0 < a.parts; p0 += kDeep)
+        {
+            uint64_t m[kDeep];
+            uint32_t c[kDeep];
+    #pragma unroll
+            for (uint32_t i = 0; i < kDeep; ++i)
+            {
+                const uint32_t p = min(p0 + i, a.parts - 1);
+                const uint32_t shift = s.partShift[p];
+                const uint64_t from = (slot + p) * kSteps + (d >= shift ? d - shift : 0);
+                const bool is = p0 + i < a.parts && d >= shift;
+                m[i] = is && mode.weighed ? a.masses[from] : 0;
+                c[i] = is && mode.counted ? a.counts[from] : 0;
+            }
+    #pragma unroll
+            for (uint32_t i = 0; i < kDeep; ++i)
+            {
+                mass += m[i];
+                count += c[i];
+            }
+        }
+        weight = static_cast<double>(mass) * s.unit[d];
+        if (!mode.counted)
+        {
+            // A bound: a logit's mass is at least 2^(-1/16) of a unit's.
+            count = static_cast<uint32_t>(static_cast<double>(mass) * (0x1p-38 * 1.0443)) + (mass != 0 ? 1u : 0u);
+        }
+        StepSums(count, weight, s);
     }
-    StepSums(count, weight, s);
     s.counts[d] = count;
     s.upTo[d] = weight;
+    if (kPhase == kPickSteps)
+    {
+        kept->counts[d] = count;
+        kept->upTo[d] = weight;
+    }
     __syncthreads();
     // The step in which the first k end.
     uint32_t stepK = kSteps - 1;
@@ -936,12 +988,12 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     }
     auto countOf = [&](uint32_t step) { return s.counts[step] - (step > 0 ? s.counts[step - 1] : 0); };
     auto weightBefore = [&](uint32_t step) { return step > 0 ? s.upTo[step - 1] : 0.0; };
-    if (mode.weighed == false && s.counts[stepK] > kListed)
+    if (kPhase != kPickSteps && !mode.weighed && s.counts[stepK] > kListed)
     {
         // Counted alone, and too many for the list after all: the masses by a pass of their own.
         s.masses[d] = 0;
         __syncthreads();
-        ForSteps(r, 0, stepK, [&](uint64_t, uint32_t step, uint64_t one) {
+        ForSteps<kPickBlock>(r, 0, r.vocab, 0, stepK, [&](uint64_t, uint32_t step, uint64_t one) {
             atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[step]), one);
         });
     }
@@ -959,6 +1011,21 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     Task task = !mode.weighed ? kMassesOfK : narrow && !wholeK ? kCutOfK : kCutOfAll;
     uint32_t listFirst = 1;  // steps that are listed: none
     uint32_t listLast = 0;
+    if constexpr (kPhase == kPickToken)
+    {
+        listFirst = kept->first;
+        listLast = kept->last;
+        const uint32_t listed = listFirst <= listLast ? min(kept->listed, kListed) : 0;
+        for (uint32_t i = threadIdx.x; i < listed; i += kPickBlock)
+        {
+            s.keys[i] = kept->keys[i];
+        }
+        if (threadIdx.x == 0)
+        {
+            s.listed = listed;
+        }
+        __syncthreads();
+    }
     uint32_t step = 0;       // of the cut of all
     bool whole = false;      // nothing of that step is cut off
     bool all = false;        // all that is kept is listed
@@ -1015,6 +1082,15 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                 to = step;
             }
             total = s.upTo[step];
+        }
+        if constexpr (kPhase == kPickSteps)
+        {
+            if (threadIdx.x == 0)
+            {
+                kept->first = from;
+                kept->last = to;
+            }
+            return;
         }
         if (from <= to && !(listFirst <= from && to <= listLast))
         {
@@ -1199,7 +1275,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                 }
                 else
                 {
-                    ForSteps(r, step, step, [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
+                    ForSteps<kPickBlock>(r, 0, r.vocab, step, step, [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
                 }
             }
             __syncthreads();
@@ -1305,6 +1381,35 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     }
 }
 
+/// Lists the logits of the rows' chosen steps, a workgroup for each kListLength logits. The last rows first: the count
+/// has just read them.
+///
+/// What bounds it: the logits' arrival, at one CU if the workgroup that decides the row listed them (608 KB in 13 us).
+__global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
+{
+    const uint32_t row = a.rows - 1 - blockIdx.y;
+    RowSteps* const kept = a.steps + row;
+    const uint32_t first = kept->first;
+    const uint32_t last = kept->last;
+    if (first > last)
+    {
+        return;
+    }
+    RowGrid r;
+    r.x = a.logits + row * a.stride;
+    r.vocab = a.vocab;
+    r.perUnit = ModeOf(a, row).perUnit;
+    r.top = kept->top;
+    const uint32_t begin = blockIdx.x * kListLength;
+    ForSteps<kBlock>(r, begin, min(begin + kListLength, a.vocab), first, last, [&](uint64_t key, uint32_t, uint64_t) {
+        const uint32_t at = atomicAdd(&kept->listed, 1u);
+        if (at < kListed)
+        {
+            kept->keys[at] = key;  // in any order: what is made of them goes by their own
+        }
+    });
+}
+
 /// Workgroups of a row, and its logits that one counts.
 struct Parts
 {
@@ -1330,7 +1435,8 @@ extern "C" size_t muyo_sample_rows_workspace_bytes(uint32_t rows, uint32_t vocab
     {
         return 0;
     }
-    return (sizeof(PartHead) + 12ull * kSteps) * rows * PartsOf(rows, vocab).count;
+    return (sizeof(PartHead) + 12ull * kSteps) * rows * PartsOf(rows, vocab).count +
+           (rows <= kListRows ? sizeof(RowSteps) * rows : 0);
 }
 
 extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
@@ -1394,11 +1500,24 @@ extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, ui
     const uint64_t blocks = static_cast<uint64_t>(rows) * parts.count;
     char* space = static_cast<char*>(workspace);
     SampleArgs a{logits, row_stride, rows, vocab, temperatures, top_ks, top_ps, min_ps, randoms, tokens, logprobs,
-                 parts.count, parts.length, nullptr, nullptr, nullptr};
+                 parts.count, parts.length, nullptr, nullptr, nullptr, nullptr};
+    const bool lists = rows <= kListRows;
+    a.steps = reinterpret_cast<RowSteps*>(space);
+    space += lists ? sizeof(RowSteps) * rows : 0;
     a.masses = reinterpret_cast<uint64_t*>(space);
     a.heads = reinterpret_cast<PartHead*>(space + 8ull * kSteps * blocks);
     a.counts = reinterpret_cast<uint32_t*>(space + (8ull * kSteps + sizeof(PartHead)) * blocks);
-    hipLaunchKernelGGL(SampleCountKernel, dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, AsStream(stream), a);
-    hipLaunchKernelGGL(SamplePickKernel, dim3(rows), dim3(kPickBlock), 0, AsStream(stream), a);
+    const hipStream_t s = AsStream(stream);
+    hipLaunchKernelGGL(SampleCountKernel, dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, a);
+    if (lists)
+    {
+        hipLaunchKernelGGL(SamplePickKernel<kPickSteps>, dim3(rows), dim3(kPickBlock), 0, s, a);
+        hipLaunchKernelGGL(SampleListKernel, dim3(CeilDiv(vocab, kListLength), rows), dim3(kBlock), 0, s, a);
+        hipLaunchKernelGGL(SamplePickKernel<kPickToken>, dim3(rows), dim3(kPickBlock), 0, s, a);
+    }
+    else
+    {
+        hipLaunchKernelGGL(SamplePickKernel<kPickAll>, dim3(rows), dim3(kPickBlock), 0, s, a);
+    }
     return LaunchStatus(name);
 }
