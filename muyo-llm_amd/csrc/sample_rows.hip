@@ -33,10 +33,11 @@ constexpr uint32_t kFew = kWave;               // candidates that a wave looks a
 constexpr uint32_t kMaxParts = 64;             // workgroups of a row
 constexpr uint32_t kMaxRows = (1u << 22) - 1;  // a launch has fewer than 2^32 threads
 constexpr uint32_t kMaxVocab = 1u << 24;       // masses of so many logits fit in 63 bits
-constexpr uint32_t kCountBlocks = 2048;        // workgroups to aim at that count
+constexpr uint32_t kCountBlocks = 1024;        // workgroups to aim at that count
+constexpr uint32_t kFewestParts = 4;           // of a row, if it has the batches
 constexpr double kLog2e = 1.44269504088896340736;
 constexpr uint32_t kListRows = 4096;           // rows whose lists get workgroups of their own
-constexpr uint32_t kListLength = 8192;         // logits that one of those looks through
+constexpr uint32_t kListBatches = 2;           // batches that a wave of those looks through
 constexpr double kFar = 0x1p48;                // places past which steps are not whole numbers apart
 constexpr double kWhole = 0x1.8p52;            // added, the whole part's last 32 bits come last
 constexpr double kFixed = 0x1p50;              // units of the top step's weight, for sums of listed logits
@@ -77,6 +78,8 @@ struct SampleArgs
     PartHead* heads;     // [rows][parts]
     uint64_t* masses;    // [rows][parts][kSteps]
     uint32_t* counts;    // [rows][parts][kSteps]
+    float* batchMost;    // [rows][parts][batches]: the largest logit of each
+    uint32_t batches;    // of a part, at most
     RowSteps* steps;     // [rows], of at most kListRows
 };
 
@@ -196,10 +199,56 @@ __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double 
     }
 }
 
+/// A part of a row in batches of kBatch logits from the last 16-byte address at or before its first one on.
+struct PartRange
+{
+    uint32_t begin, end;
+    uint32_t before;   // logits of the first batch that are the part's before
+    uint32_t batches;
+};
+
+__device__ __forceinline__ PartRange RangeOf(const float* x, uint32_t begin, uint32_t end)
+{
+    PartRange r{begin, end, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x + begin) / 4 % 4), 0};
+    r.batches = (end - begin + r.before + kBatch - 1) / kBatch;
+    return r;
+}
+
+/// A lane's i-th logit of a batch: four in a row from each quad. Before the part's first logit it wraps or is too small.
+__device__ __forceinline__ uint32_t IndexOf(const PartRange& r, uint32_t batch, uint32_t i)
+{
+    return r.begin - r.before + batch * kBatch + (i / 4 * kWave + threadIdx.x % kWave) * 4 + i % 4;
+}
+
+/// A batch in 16-byte loads, logit by logit where it reaches over an end of the part (-inf outside).
+__device__ __forceinline__ void LoadBatch(const float* x, const PartRange& r, uint32_t batch, float4v (&v)[kQuads])
+{
+    const uint32_t first = batch * kBatch;
+    if (first >= r.before && first + kBatch <= r.end - r.begin + r.before)
+    {
+#pragma unroll
+        for (uint32_t q = 0; q < kQuads; ++q)
+        {
+            v[q] = *reinterpret_cast<const float4v*>(x + IndexOf(r, batch, 4 * q));
+        }
+    }
+    else if (batch < r.batches)
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * kQuads; ++i)
+        {
+            const uint32_t index = IndexOf(r, batch, i);
+            const bool inside = index >= r.begin && index < r.end;
+            const float one = x[inside ? index : r.begin];
+            v[i / 4][i % 4] = inside ? one : -INFINITY;
+        }
+    }
+}
+
 /// Counts the logits of a part of a row in steps of the grid, and their masses. A wave has counters of its own in
 /// LDS, from a step above the largest logit that it has met; a larger one moves them down, which is rare.
 ///
-__global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
+__global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
 {
     __shared__ uint64_t massOf[kWaves][kSteps];
     __shared__ uint32_t countOf[kWaves][kSteps];
@@ -227,44 +276,17 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
     bool near = false;
     float most = -INFINITY;   // of the wave; of a greedy row's lane
     uint32_t at = 0;
-    // 16-byte loads from the last such address at or before the part's first logit; batches that reach over an end
-    // of the part go logit by logit. A batch is on its way while the one before is counted.
-    const uint32_t before = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x + begin) / 4 % 4);
-    const uint32_t length = end - begin + before;
-    // A lane's logits: four in a row from each quad.
-    auto indexOf = [&](uint32_t first, uint32_t i) { return begin - before + first + (i / 4 * kWave + lane) * 4 + i % 4; };
-    auto load = [&](uint32_t first, float4v (&v)[kQuads]) {
-        if (first >= before && first + kBatch <= length)
-        {
-#pragma unroll
-            for (uint32_t q = 0; q < kQuads; ++q)
-            {
-                v[q] = *reinterpret_cast<const float4v*>(x + indexOf(first, 4 * q));
-            }
-        }
-        else if (first < length)
-        {
-#pragma unroll
-            for (uint32_t i = 0; i < 4 * kQuads; ++i)
-            {
-                // Before the part's first logit the index wraps or is too small: both are left out.
-                const uint32_t index = indexOf(first, i);
-                const bool inside = index >= begin && index < end;
-                const float one = x[inside ? index : begin];
-                v[i / 4][i % 4] = inside ? one : -INFINITY;
-            }
-        }
-    };
+    const PartRange range = RangeOf(x, begin, end);
     float4v v[kQuads], next[kQuads];
-    load(wave * kBatch, next);
-    for (uint32_t first = wave * kBatch; first < length; first += kWaves * kBatch)
+    LoadBatch(x, range, wave, next);
+    for (uint32_t batch = wave; batch < range.batches; batch += kWaves)
     {
 #pragma unroll
         for (int q = 0; q < kQuads; ++q)
         {
             v[q] = next[q];
         }
-        load(first + kWaves * kBatch, next);
+        LoadBatch(x, range, batch + kWaves, next);
         float batchMost = -INFINITY;
 #pragma unroll
         for (uint32_t i = 0; i < 4 * kQuads; ++i)
@@ -280,13 +302,17 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
 #pragma unroll
                 for (int i = 4 * kQuads - 1; i >= 0; --i)
                 {
-                    at = Counted(v[i / 4][i % 4]) == batchMost ? indexOf(first, i) : at;
+                    at = Counted(v[i / 4][i % 4]) == batchMost ? IndexOf(range, batch, i) : at;
                 }
             }
             continue;
         }
         batchMost = GroupMax<kWave>(batchMost);
         most = fmaxf(most, batchMost);
+        if (lane == 0)
+        {
+            a.batchMost[static_cast<uint64_t>(blockIdx.x) * a.batches + batch] = batchMost;
+        }
         if (batchMost == -INFINITY)
         {
             continue;
@@ -330,7 +356,7 @@ __global__ __launch_bounds__(kBlock) void SampleCountKernel(SampleArgs a)
 #pragma unroll 1
             for (uint32_t i = 0; i < 4 * kQuads; ++i)
             {
-                const uint32_t index = indexOf(first, i);
+                const uint32_t index = IndexOf(range, batch, i);
                 const bool inside = index >= begin && index < end;
                 AddOne(inside ? x[index] : -INFINITY, top, mode.perUnit, masses, counts);
             }
@@ -497,30 +523,35 @@ __device__ __forceinline__ bool Reaches(const RowGrid& r, const Place& at)
     return (at.step - r.largest.step) + (at.rest - r.largest.rest) >= r.lowest;
 }
 
-/// Calls use(key, step, mass) for the logits begin..end - 1 of a row that are in steps first..last, by kThreads threads.
+/// Bounds in f32, a little wide, of the logits in steps first..last.
+__device__ __forceinline__ void BoundsOf(const RowGrid& r, uint32_t first, uint32_t last, float& low, float& high)
+{
+    const double wide = 0.5 + 1e-6 + 1e-9 * fabs(r.top);
+    low = __double2float_rd((r.top - last - wide) / r.perUnit);
+    high = __double2float_ru((r.top - first + wide) / r.perUnit);
+    // +inf is not above the last number, as which it counts.
+    high = high >= 0x1.fffffep127f ? INFINITY : high;
+}
+
+/// Calls use(key, step, mass) for a row's logits in steps first..last, by all threads.
 /// Bounds in f32, a little wide, tell which of a thread's 32 logits may be
 /// meant; those are placed one by one (a copy of that for each of them filled the instruction cache).
-template <int kThreads, typename Use>
-__device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t begin, uint32_t end, uint32_t first, uint32_t last,
-                                         Use use)
+template <typename Use>
+__device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, Use use)
 {
-    const float* const part = r.x + begin;
-    const double wide = 0.5 + 1e-6 + 1e-9 * fabs(r.top);
-    const float low = __double2float_rd((r.top - last - wide) / r.perUnit);
-    const float high = __double2float_ru((r.top - first + wide) / r.perUnit);
-    const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(part) / 4 % 4)) % 4u, end - begin);
-    const uint32_t quads = (end - begin - head) / 4;
-    const uint32_t edges = end - begin - 4 * quads;  // before the first quad and behind the last
-    // +inf is not above `high`, which is rounded up, where it counts as f32's last number.
-    const float most = high >= 0x1.fffffep127f ? INFINITY : high;
+    float low, high;
+    BoundsOf(r, first, last, low, high);
+    const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(r.x) / 4 % 4)) % 4u, r.vocab);
+    const uint32_t quads = (r.vocab - head) / 4;
+    const uint32_t edges = r.vocab - 4 * quads;  // before the first quad and behind the last
     constexpr uint32_t kAhead = 8;  // quads of a thread in a round; the next round's are on their way
     float4v v[kAhead], next[kAhead];
     auto load = [&](uint32_t from) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i)
         {
-            const uint32_t quad = min(from + i * kThreads + threadIdx.x, quads - 1);
-            next[i] = *reinterpret_cast<const float4v*>(part + head + 4 * quad);
+            const uint32_t quad = min(from + i * kPickBlock + threadIdx.x, quads - 1);
+            next[i] = *reinterpret_cast<const float4v*>(r.x + head + 4 * quad);
         }
     };
     if (quads > 0)
@@ -531,7 +562,7 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t begin, uint3
     uint32_t may = threadIdx.x < edges ? 1u : 0u;
     bool edge = true;
     const uint32_t edgeIndex = threadIdx.x < head ? threadIdx.x : threadIdx.x + 4 * quads;
-    v[0][0] = part[threadIdx.x < edges ? edgeIndex : 0];
+    v[0][0] = r.x[threadIdx.x < edges ? edgeIndex : 0];
     uint32_t from = 0;
     while (true)
     {
@@ -545,16 +576,16 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t begin, uint3
             {
                 logit = bit == i ? v[i / 4][i % 4] : logit;
             }
-            const uint32_t at = edge ? edgeIndex : head + 4 * (from + bit / 4 * kThreads + threadIdx.x) + bit % 4;
+            const uint32_t at = edge ? edgeIndex : head + 4 * (from + bit / 4 * kPickBlock + threadIdx.x) + bit % 4;
             const float x = Counted(logit);
             const Place place = PlaceOf(x, r.perUnit);
             const double d = r.top - place.step;
             if (x > -INFINITY && d >= first && d <= last)
             {
-                use(OrderKey(x, begin + at), static_cast<uint32_t>(d), MassOf(place.rest));
+                use(OrderKey(x, at), static_cast<uint32_t>(d), MassOf(place.rest));
             }
         }
-        from += edge ? 0 : kThreads * kAhead;
+        from += edge ? 0 : kPickBlock * kAhead;
         edge = false;
         if (from >= quads)
         {
@@ -565,15 +596,15 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t begin, uint3
         {
             v[i] = next[i];
         }
-        load(from + kThreads * kAhead);
+        load(from + kPickBlock * kAhead);
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i)
         {
-            const bool there = from + i * kThreads + threadIdx.x < quads;
+            const bool there = from + i * kPickBlock + threadIdx.x < quads;
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e)
             {
-                may |= there && v[i][e] >= low && v[i][e] <= most ? 1u << (4 * i + e) : 0u;
+                may |= there && v[i][e] >= low && v[i][e] <= high ? 1u << (4 * i + e) : 0u;
             }
         }
     }
@@ -588,7 +619,7 @@ __device__ __forceinline__ void ListSteps(const RowGrid& r, uint32_t first, uint
         s.listed = 0;
     }
     __syncthreads();
-    ForSteps<kPickBlock>(r, 0, r.vocab, first, last, [&](uint64_t key, uint32_t, uint64_t) {
+    ForSteps(r, first, last, [&](uint64_t key, uint32_t, uint64_t) {
         const uint32_t at = atomicAdd(&s.listed, 1u);
         if (at < kListed)
         {
@@ -787,7 +818,7 @@ __device__ Cut LastKeptOfRow(const RowGrid& r, uint32_t d, uint32_t most, uint64
             s.digitMasses[i] = 0;
         }
         __syncthreads();
-        ForSteps<kPickBlock>(r, 0, r.vocab, d, d, [&](uint64_t key, uint32_t, uint64_t mass) {
+        ForSteps(r, d, d, [&](uint64_t key, uint32_t, uint64_t mass) {
             if ((shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))) &&
                 Reaches(r, PlaceOf(KeyValue(key), r.perUnit)))
             {
@@ -993,7 +1024,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         // Counted alone, and too many for the list after all: the masses by a pass of their own.
         s.masses[d] = 0;
         __syncthreads();
-        ForSteps<kPickBlock>(r, 0, r.vocab, 0, stepK, [&](uint64_t, uint32_t step, uint64_t one) {
+        ForSteps(r, 0, stepK, [&](uint64_t, uint32_t step, uint64_t one) {
             atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[step]), one);
         });
     }
@@ -1229,6 +1260,25 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                               (dist == static_cast<double>(step) && OrderKey(x, at) >= cut.key);
             return kept ? static_cast<double>(MassOf(place.rest)) * s.unit[static_cast<uint32_t>(dist)] : 0.0;
         };
+        // The same of logits of which none is far, with fewer operations (AddNearBatch): by the cut's own logit.
+        const double bound = (top - (kSteps + 2)) / r.perUnit;
+        const bool near = fabs(top) < kFar && bound > -0x1p127;
+        const float least = static_cast<float>(bound);
+        const uint32_t topStep = static_cast<uint32_t>(__double_as_longlong(top + kWhole));
+        const bool none = cut.key == ~0ull;  // of the step of the cut
+        const uint32_t lastStep = none ? step - 1 : step;
+        const float cutLogit = whole || none ? -INFINITY : KeyValue(cut.key);
+        const uint32_t cutIndex = ~static_cast<uint32_t>(cut.key);
+        auto nearWeightAt = [&](float v, uint32_t at) {
+            const float x = Counted(v);
+            const double y = static_cast<double>(fmaxf(x, least));
+            const double place = WholeOf(y, r.perUnit);
+            const uint32_t dist = topStep - static_cast<uint32_t>(__double_as_longlong(place));
+            const double weight = static_cast<double>(MassOf(fma(y, r.perUnit, -(place - kWhole)))) *
+                                  s.unit[min(dist, static_cast<uint32_t>(kSteps - 1))];
+            const bool kept = dist <= lastStep && (x > cutLogit || (x == cutLogit && at <= cutIndex));
+            return kept ? weight : 0.0;
+        };
         const double reach = number * total;
         uint32_t begin = 0;
         uint32_t end = a.vocab;
@@ -1238,19 +1288,36 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
             // What each part has of it: the steps before from its masses, this one's kept logits by a look at them.
             __syncthreads();
             const uint32_t until = whole ? step + 1 : step;
-            for (uint32_t p = wave; p < a.parts; p += kPickWaves)
+            for (uint32_t p0 = wave; p0 < a.parts; p0 += 2 * kPickWaves)
             {
-                const uint32_t shift = s.partShift[p];
-                double sum = 0.0;
-#pragma unroll 4
-                for (uint32_t i = shift + lane; i < until; i += kWave)
+                // Two parts' at a time.
+                uint64_t m[2][kSteps / kWave];
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
                 {
-                    sum += static_cast<double>(a.masses[(slot + p) * kSteps + i - shift]) * s.unit[i];
+                    const uint32_t p = min(p0 + h * kPickWaves, a.parts - 1);
+                    const uint32_t shift = s.partShift[p];
+#pragma unroll
+                    for (uint32_t j = 0; j < kSteps / kWave; ++j)
+                    {
+                        const uint32_t i = j * kWave + lane;
+                        m[h][j] = i >= shift && i < until ? a.masses[(slot + p) * kSteps + i - shift] : 0;
+                    }
                 }
-                sum = WaveSum(sum);
-                if (lane == 0)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
                 {
-                    s.partWeight[p] = sum;
+                    double sum = 0.0;
+#pragma unroll
+                    for (uint32_t j = 0; j < kSteps / kWave; ++j)
+                    {
+                        sum += static_cast<double>(m[h][j]) * s.unit[j * kWave + lane];
+                    }
+                    sum = WaveSum(sum);
+                    if (lane == 0 && p0 + h * kPickWaves < a.parts)
+                    {
+                        s.partWeight[p0 + h * kPickWaves] = sum;
+                    }
                 }
             }
             if (!whole)
@@ -1275,7 +1342,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                 }
                 else
                 {
-                    ForSteps<kPickBlock>(r, 0, r.vocab, step, step, [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
+                    ForSteps(r, step, step, [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
                 }
             }
             __syncthreads();
@@ -1318,10 +1385,21 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                     v[j] = r.x[min(at + j * kWave, end - 1)];
                 }
                 double own = 0.0;
-#pragma unroll
-                for (uint32_t j = 0; j < kPickLoads; ++j)
+                if (near)
                 {
-                    own += at + j * kWave < end ? weightAt(v[j], at + j * kWave) : 0.0;
+#pragma unroll
+                    for (uint32_t j = 0; j < kPickLoads; ++j)
+                    {
+                        own += at + j * kWave < end ? nearWeightAt(v[j], at + j * kWave) : 0.0;
+                    }
+                }
+                else
+                {
+#pragma unroll 1
+                    for (uint32_t j = 0; j < kPickLoads; ++j)
+                    {
+                        own += at + j * kWave < end ? weightAt(r.x[at + j * kWave], at + j * kWave) : 0.0;
+                    }
                 }
                 own = WaveSum(own);
                 if (lane == 0)
@@ -1381,17 +1459,25 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     }
 }
 
-/// Lists the logits of the rows' chosen steps, a workgroup for each kListLength logits. The last rows first: the count
-/// has just read them.
+/// Lists the logits of the rows' chosen steps, kListBatches batches a wave. Batches whose largest logit is below the
+/// steps are not read: tokens that stand out of a row are in few of them.
 ///
-/// What bounds it: the logits' arrival, at one CU if the workgroup that decides the row listed them (608 KB in 13 us).
+/// What bounds it: the arrival of the others, at one CU if the workgroup that decides the row listed them (608 KB in
+/// 13 us).
 __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
 {
-    const uint32_t row = a.rows - 1 - blockIdx.y;
+    const uint32_t row = blockIdx.y;
     RowSteps* const kept = a.steps + row;
     const uint32_t first = kept->first;
     const uint32_t last = kept->last;
     if (first > last)
+    {
+        return;
+    }
+    const uint32_t wave = blockIdx.x * kWaves + threadIdx.x / kWave;
+    const uint32_t perPart = (a.batches + kListBatches - 1) / kListBatches;  // waves
+    const uint32_t part = wave / perPart;
+    if (part >= a.parts)
     {
         return;
     }
@@ -1400,14 +1486,63 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
     r.vocab = a.vocab;
     r.perUnit = ModeOf(a, row).perUnit;
     r.top = kept->top;
-    const uint32_t begin = blockIdx.x * kListLength;
-    ForSteps<kBlock>(r, begin, min(begin + kListLength, a.vocab), first, last, [&](uint64_t key, uint32_t, uint64_t) {
-        const uint32_t at = atomicAdd(&kept->listed, 1u);
-        if (at < kListed)
+    float low, high;
+    BoundsOf(r, first, last, low, high);
+    const uint64_t slot = static_cast<uint64_t>(row) * a.parts + part;
+    const uint32_t begin = part * a.partLength;
+    const PartRange range = RangeOf(r.x, begin, min(begin + a.partLength, a.vocab));
+    const uint32_t batch0 = (wave - part * perPart) * kListBatches;
+    bool reads[kListBatches];
+    float4v v[kListBatches][kQuads];
+#pragma unroll
+    for (uint32_t b = 0; b < kListBatches; ++b)
+    {
+        reads[b] = batch0 + b < range.batches && a.batchMost[slot * a.batches + batch0 + b] >= low;
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < kListBatches; ++b)
+    {
+        if (reads[b])
         {
-            kept->keys[at] = key;  // in any order: what is made of them goes by their own
+            LoadBatch(r.x, range, batch0 + b, v[b]);
         }
-    });
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < kListBatches; ++b)
+    {
+        if (!reads[b])
+        {
+            continue;
+        }
+        uint32_t may = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4 * kQuads; ++i)
+        {
+            may |= v[b][i / 4][i % 4] >= low && v[b][i / 4][i % 4] <= high ? 1u << i : 0u;
+        }
+        while (may != 0)
+        {
+            const uint32_t bit = __ffs(static_cast<int>(may)) - 1;
+            may &= may - 1;
+            float logit = v[b][0][0];
+#pragma unroll
+            for (uint32_t i = 1; i < 4 * kQuads; ++i)
+            {
+                logit = bit == i ? v[b][i / 4][i % 4] : logit;
+            }
+            const float x = Counted(logit);
+            const double d = r.top - PlaceOf(x, r.perUnit).step;
+            if (x > -INFINITY && d >= first && d <= last)
+            {
+                const uint32_t at = atomicAdd(&kept->listed, 1u);
+                if (at < kListed)
+                {
+                    // In any order: what is made of them goes by their own.
+                    kept->keys[at] = OrderKey(x, IndexOf(range, batch0 + b, bit));
+                }
+            }
+        }
+    }
 }
 
 /// Workgroups of a row, and its logits that one counts.
@@ -1420,10 +1555,14 @@ Parts PartsOf(uint32_t rows, uint32_t vocab)
 {
     const uint32_t batches = CeilDiv(vocab, kBatch);
     const uint32_t most = std::min(kMaxParts, CeilDiv(batches, kWaves));
-    const uint32_t wanted = std::max(1u, std::min(most, kCountBlocks / std::max(rows, 1u)));
+    // Four batches a wave, where that leaves workgroups enough; the end of a row looks through a part of it.
+    const uint32_t wanted = std::min(most, std::max(kCountBlocks / rows, kFewestParts));
     const uint32_t length = CeilDiv(batches, wanted) * kBatch;
     return Parts{CeilDiv(vocab, length), length};
 }
+
+/// Batches of a part: one more than its logits fill, since they may begin anywhere.
+uint32_t BatchesOf(const Parts& parts) { return parts.length / kBatch + 1; }
 }  // namespace
 }  // namespace muyo
 
@@ -1435,7 +1574,8 @@ extern "C" size_t muyo_sample_rows_workspace_bytes(uint32_t rows, uint32_t vocab
     {
         return 0;
     }
-    return (sizeof(PartHead) + 12ull * kSteps) * rows * PartsOf(rows, vocab).count +
+    const Parts parts = PartsOf(rows, vocab);
+    return (sizeof(PartHead) + 12ull * kSteps + 4ull * BatchesOf(parts)) * rows * parts.count +
            (rows <= kListRows ? sizeof(RowSteps) * rows : 0);
 }
 
@@ -1500,19 +1640,21 @@ extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, ui
     const uint64_t blocks = static_cast<uint64_t>(rows) * parts.count;
     char* space = static_cast<char*>(workspace);
     SampleArgs a{logits, row_stride, rows, vocab, temperatures, top_ks, top_ps, min_ps, randoms, tokens, logprobs,
-                 parts.count, parts.length, nullptr, nullptr, nullptr, nullptr};
+                 parts.count, parts.length, nullptr, nullptr, nullptr, nullptr, BatchesOf(parts), nullptr};
     const bool lists = rows <= kListRows;
     a.steps = reinterpret_cast<RowSteps*>(space);
     space += lists ? sizeof(RowSteps) * rows : 0;
     a.masses = reinterpret_cast<uint64_t*>(space);
     a.heads = reinterpret_cast<PartHead*>(space + 8ull * kSteps * blocks);
     a.counts = reinterpret_cast<uint32_t*>(space + (8ull * kSteps + sizeof(PartHead)) * blocks);
+    a.batchMost = reinterpret_cast<float*>(space + (12ull * kSteps + sizeof(PartHead)) * blocks);
     const hipStream_t s = AsStream(stream);
     hipLaunchKernelGGL(SampleCountKernel, dim3(static_cast<uint32_t>(blocks)), dim3(kBlock), 0, s, a);
     if (lists)
     {
         hipLaunchKernelGGL(SamplePickKernel<kPickSteps>, dim3(rows), dim3(kPickBlock), 0, s, a);
-        hipLaunchKernelGGL(SampleListKernel, dim3(CeilDiv(vocab, kListLength), rows), dim3(kBlock), 0, s, a);
+        const uint32_t waves = CeilDiv(a.batches, kListBatches) * parts.count;
+        hipLaunchKernelGGL(SampleListKernel, dim3(CeilDiv(waves, kWaves), rows), dim3(kBlock), 0, s, a);
         hipLaunchKernelGGL(SamplePickKernel<kPickToken>, dim3(rows), dim3(kPickBlock), 0, s, a);
     }
     else
