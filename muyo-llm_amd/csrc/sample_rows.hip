@@ -175,25 +175,37 @@ __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double 
 {
     const uint32_t topStep = static_cast<uint32_t>(__double_as_longlong(top + kWhole));
 #pragma unroll
-    for (int i = 0; i < 4 * kQuads; ++i)
+    for (int q = 0; q < kQuads; ++q)
     {
-        // The smaller of a signalling NaN and a number is a quiet NaN, the larger of that and a number the number.
-        float x;
-        asm("v_min_f32 %0, %1, %2" : "=v"(x) : "v"(v[i / 4][i % 4]), "v"(0x1.fffffep127f));
-        asm("v_max_f32 %0, %1, %2" : "=v"(x) : "v"(x), "v"(least));
-        const double y = static_cast<double>(x);
-        const double whole = WholeOf(y, perUnit);
-        const uint32_t step = topStep - static_cast<uint32_t>(__double_as_longlong(whole));
-        if (step < kSteps)
+        // Four at a time, side by side up to the counters.
+        uint32_t step[4];
+        uint64_t mass[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
         {
-            if (kMass)
+            // The smaller of a signalling NaN and a number is a quiet NaN, the larger of that and a number the number.
+            float x;
+            asm("v_min_f32 %0, %1, %2" : "=v"(x) : "v"(v[q][e]), "v"(0x1.fffffep127f));
+            asm("v_max_f32 %0, %1, %2" : "=v"(x) : "v"(x), "v"(least));
+            const double y = static_cast<double>(x);
+            const double whole = WholeOf(y, perUnit);
+            step[e] = topStep - static_cast<uint32_t>(__double_as_longlong(whole));
+            mass[e] = kMass ? MassOf(fma(y, perUnit, -(whole - kWhole))) : 0;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+        {
+            if (step[e] < kSteps)
             {
-                atomicAdd(reinterpret_cast<unsigned long long*>(masses + step),
-                          MassOf(fma(y, perUnit, -(whole - kWhole))));
-            }
-            if (kCount)
-            {
-                atomicAdd(counts + step, 1u);
+                if (kMass)
+                {
+                    atomicAdd(reinterpret_cast<unsigned long long*>(masses + step[e]), mass[e]);
+                }
+                if (kCount)
+                {
+                    atomicAdd(counts + step[e], 1u);
+                }
             }
         }
     }
@@ -534,7 +546,7 @@ __device__ __forceinline__ void BoundsOf(const RowGrid& r, uint32_t first, uint3
 }
 
 /// Calls use(key, step, mass) for a row's logits in steps first..last, by all threads.
-/// Bounds in f32, a little wide, tell which of a thread's 32 logits may be
+/// Bounds in f32, a little wide, tell which of a thread's 16 logits may be
 /// meant; those are placed one by one (a copy of that for each of them filled the instruction cache).
 template <typename Use>
 __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, Use use)
@@ -544,7 +556,7 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint3
     const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(r.x) / 4 % 4)) % 4u, r.vocab);
     const uint32_t quads = (r.vocab - head) / 4;
     const uint32_t edges = r.vocab - 4 * quads;  // before the first quad and behind the last
-    constexpr uint32_t kAhead = 8;  // quads of a thread in a round; the next round's are on their way
+    constexpr uint32_t kAhead = 4;  // quads of a thread in a round; the next round's are on their way
     float4v v[kAhead], next[kAhead];
     auto load = [&](uint32_t from) {
 #pragma unroll
@@ -1367,6 +1379,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
             end = min(begin + a.partLength, a.vocab);
         }
         // Sums of groups of logits, and the first group that reaches past it, else the last with anything kept.
+        constexpr uint32_t kAtOnce = 4;  // groups of a wave
         const uint32_t groups = (end - begin + kGroup - 1) / kGroup;
         uint32_t group = 0;
         double sum = passed;
@@ -1375,49 +1388,78 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         {
             const uint32_t here = min(groups - first, kGroups);
             __syncthreads();
-            for (uint32_t i = wave; i < here; i += kPickWaves)
+            for (uint32_t i0 = wave; i0 < here; i0 += kAtOnce * kPickWaves)
             {
-                float v[kPickLoads];
-                const uint32_t at = begin + (first + i) * kGroup + lane;
+                float v[kAtOnce][kPickLoads];
 #pragma unroll
-                for (uint32_t j = 0; j < kPickLoads; ++j)
-                {
-                    v[j] = r.x[min(at + j * kWave, end - 1)];
-                }
-                double own = 0.0;
-                if (near)
+                for (uint32_t b = 0; b < kAtOnce; ++b)
                 {
 #pragma unroll
                     for (uint32_t j = 0; j < kPickLoads; ++j)
                     {
-                        own += at + j * kWave < end ? nearWeightAt(v[j], at + j * kWave) : 0.0;
+                        const uint32_t at = begin + (first + i0 + b * kPickWaves) * kGroup + lane + j * kWave;
+                        v[b][j] = r.x[min(at, end - 1)];
                     }
                 }
-                else
+                double own[kAtOnce];
+#pragma unroll
+                for (uint32_t b = 0; b < kAtOnce; ++b)
                 {
+                    const uint32_t i = i0 + b * kPickWaves;
+                    const uint32_t at = begin + (first + i) * kGroup + lane;
+                    own[b] = 0.0;
+                    if (near)
+                    {
+#pragma unroll
+                        for (uint32_t j = 0; j < kPickLoads; ++j)
+                        {
+                            own[b] += i < here && at + j * kWave < end ? nearWeightAt(v[b][j], at + j * kWave) : 0.0;
+                        }
+                    }
+                    else
+                    {
 #pragma unroll 1
-                    for (uint32_t j = 0; j < kPickLoads; ++j)
-                    {
-                        own += at + j * kWave < end ? weightAt(r.x[at + j * kWave], at + j * kWave) : 0.0;
+                        for (uint32_t j = 0; j < kPickLoads; ++j)
+                        {
+                            own[b] += i < here && at + j * kWave < end ? weightAt(r.x[at + j * kWave], at + j * kWave) : 0.0;
+                        }
                     }
                 }
-                own = WaveSum(own);
-                if (lane == 0)
+#pragma unroll
+                for (int step = 1; step < kWave; step *= 2)
                 {
-                    s.groupWeights[i] = own;
+#pragma unroll
+                    for (uint32_t b = 0; b < kAtOnce; ++b)
+                    {
+                        own[b] += __shfl_xor(own[b], step);
+                    }
+                }
+#pragma unroll
+                for (uint32_t b = 0; b < kAtOnce; ++b)
+                {
+                    if (lane == 0 && i0 + b * kPickWaves < here)
+                    {
+                        s.groupWeights[i0 + b * kPickWaves] = own[b];
+                    }
                 }
             }
             __syncthreads();
-            for (uint32_t i = 0; i < here && !past; ++i)
+            // Every wave finds the same, a group a lane.
+            for (uint32_t i0 = 0; i0 < here && !past; i0 += kWave)
             {
-                const double ofGroup = s.groupWeights[i];
-                if (ofGroup > 0.0)
+                const double ofGroup = i0 + lane < here ? s.groupWeights[i0 + lane] : 0.0;
+                const double upToGroup = WaveInclusive(ofGroup);
+                const uint64_t kept = __ballot(ofGroup > 0.0);
+                const uint64_t over = __ballot(ofGroup > 0.0 && sum + upToGroup > reach);
+                if (kept != 0)
                 {
-                    group = first + i;
-                    passed = sum;
-                    sum += ofGroup;
-                    past = sum > reach;
+                    const int which = over != 0 ? __ffsll(static_cast<unsigned long long>(over)) - 1
+                                                : 63 - __clzll(static_cast<long long>(kept));
+                    group = first + i0 + which;
+                    passed = sum + __shfl(upToGroup - ofGroup, which);
                 }
+                past = over != 0;
+                sum += __shfl(upToGroup, kWave - 1);
             }
         }
         if (wave != 0)
