@@ -12,10 +12,6 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kTile = 32;            // keys of a tile: what a wave takes at a time
 constexpr int kHalves = kTile / 16;       // matrix operands of 16 keys
-// Softmax weights are held in two planes of f16, which ends at 2^16: the weight of the maximum is 2^kWeightBias, and
-// 2^15 when a later one has run kLag binary orders ahead.
-constexpr float kLag = 4.0f;
-constexpr float kWeightBias = 15.0f - kLag;
 constexpr float kLowScale = 2048.0f;      // of the low plane: what 11 bits of the high one leave, in f16's range again
 
 template <bool kOnce>

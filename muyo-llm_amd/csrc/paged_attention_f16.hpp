@@ -5,6 +5,11 @@
 
 namespace muyo
 {
+// Softmax weights over own keys are held in two planes of f16, which ends at 2^16: the weight of the maximum is
+// 2^kWeightBias, and 2^15 when a later one has run kLag binary orders ahead.
+constexpr float kLag = 4.0f;
+constexpr float kWeightBias = 15.0f - kLag;
+
 struct PagedAttentionF16Args : PagedAttentionArgs
 {
     const uint16_t* kcache;

@@ -18,7 +18,7 @@ constexpr uint32_t kRowsOfBlock = kRowsOfWave * kWaves;
 constexpr uint32_t kPrefixBlocks = 512;   // workgroups to aim at: two on each of 256 CUs
 constexpr uint32_t kMaxChunks = 128;
 // Softmax weights as in the attention over a query's own keys: the maximum's is 2^kPrefixBias, 2^15 at most.
-constexpr float kPrefixLag = 4.0f;
+constexpr float kPrefixLag = 10.0f;
 constexpr float kPrefixBias = 15.0f - kPrefixLag;
 constexpr float kPrefixLowScale = 2048.0f;
 
@@ -493,7 +493,8 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
             const float4v result = *reinterpret_cast<const float4v*>(out);
             const float best = fmaxf(base, own.x);
             const float factor = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((base - best) * own.z);
-            const float w = own.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((own.x - best) * own.z);
+            float w = own.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((own.x - best) * own.z);
+            w *= __builtin_amdgcn_exp2f(kPrefixBias - kWeightBias);
             scaleLog2 = own.z;
             base = best;
             den = fmaf(w, own.y, den * factor);
