@@ -564,6 +564,8 @@ hipError_t LaunchOwnKeys(hipStream_t s, const PagedAttentionF16Args& a)
                                                   PagedAttentionKernel<kHd, true, true>);
 }
 
+bool OwnKeysSplit(const PagedAttentionF16Args& a) { return SplitKeys<kTile>(a); }
+
 template hipError_t LaunchOwnKeys<64>(hipStream_t, const PagedAttentionF16Args&);
 template hipError_t LaunchOwnKeys<128>(hipStream_t, const PagedAttentionF16Args&);
 

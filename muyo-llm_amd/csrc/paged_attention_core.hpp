@@ -25,7 +25,7 @@ struct PagedAttentionArgs
     uint32_t* costSums;  // [queries + 1]: CostOf of one kv head of the queries before
     uint4* cuts;         // what to join: query, kv head, first share, pieces (0: nothing)
     uint32_t cutsByUnit; // cuts has an entry per (query, kv head); else one per share
-    float4* stats;       // of kStats: base, sum, a score's log2 units, -, of each query's heads
+    float4* stats;       // of kStats, for what no share cut: base, sum, a score's log2 units, -, of each query's heads
     float* partials;     // [2 * shares][group][4 + headDim]: base, sum, a score's log2 units, -, weighted values
 };
 
@@ -306,7 +306,7 @@ __device__ __forceinline__ Share FirstShare(const PagedAttentionArgs& a, uint32_
 /// 256 threads have 32 pieces of 128 channels in flight, 512 have 128: one sequence of 32749 keys (28 / 4
 /// heads, 28 workgroups of 128 pieces) takes 4.9 us with 512 threads and 7.6 with 256; 64 sequences (1792
 /// workgroups, most with three pieces) take 8.4 us with 512, whose waves start no faster, and 4.7 with 256.
-template <int kHd, uint32_t kTile, int kThreads, bool kStats>
+template <int kHd, uint32_t kTile, int kThreads>
 __global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAttentionArgs a)
 {
     constexpr uint32_t kLanes = kHd / 4;
@@ -392,10 +392,6 @@ __global__ __launch_bounds__(kThreads) void PagedAttentionMergeKernel(PagedAtten
         const float4v result = den == 0.0f ? float4v{} : num / den;
         const uint64_t head = (static_cast<uint64_t>(cut.x) * a.kvHeads + cut.y) * a.group + h;
         *reinterpret_cast<float4v*>(a.out + head * kHd + 4 * lane) = result;
-        if (kStats && lane == 0)
-        {
-            a.stats[head] = make_float4(best, den, scaleLog2, 0.0f);
-        }
     }
 }
 
@@ -449,14 +445,23 @@ inline size_t DecodeWorkspaceBytes(uint32_t queries, uint32_t heads, uint32_t kv
     return CostSumBytes(queries) + kCutBytes + sizeof(float) * 2 * kSplitBlocks * (heads / kvHeads) * (headDim + 4);
 }
 
-/// Split launches take `split` and the join, tables or windows of at most kWholeKeys keys `whole`.
-template <int kHd, uint32_t kTile, bool kStats, typename Args>
-hipError_t LaunchPagedAttention(hipStream_t s, Args a, void (*whole)(Args), void (*split)(Args))
+/// Whether a call's keys are dealt out in shares: not those of tables or windows of at most kWholeKeys keys.
+template <uint32_t kTile>
+bool SplitKeys(const PagedAttentionArgs& a)
 {
     const uint64_t keys = std::min<uint64_t>(static_cast<uint64_t>(a.tablePages) << a.pageShift,
                                              a.window != 0 ? a.window : 0xFFFFFFFFull);
     const uint64_t units = static_cast<uint64_t>(a.queries) * a.kvHeads;
-    if (keys <= kWholeKeys || units * (keys / kTile + 2 + kSetupTiles<kTile>) > 0x7FFFFFFFull)
+    return keys > kWholeKeys && units * (keys / kTile + 2 + kSetupTiles<kTile>) <= 0x7FFFFFFFull;
+}
+
+/// Split launches take `split` and the join, others `whole`. With kStats the caller joins: `cuts` has an entry per
+/// (query, kv head).
+template <int kHd, uint32_t kTile, bool kStats, typename Args>
+hipError_t LaunchPagedAttention(hipStream_t s, Args a, void (*whole)(Args), void (*split)(Args))
+{
+    const uint64_t units = static_cast<uint64_t>(a.queries) * a.kvHeads;
+    if (!SplitKeys<kTile>(a))
     {
         hipLaunchKernelGGL(whole, dim3(a.kvHeads, a.queries), dim3(kBlock), 0, s, a);
         return hipGetLastError();
@@ -465,18 +470,20 @@ hipError_t LaunchPagedAttention(hipStream_t s, Args a, void (*whole)(Args), void
     {
         hipLaunchKernelGGL(PagedCostSumsKernel<kTile>, dim3(1), dim3(1024), 0, s, a);
     }
-    a.cutsByUnit = units < kSplitBlocks ? 1 : 0;
+    a.cutsByUnit = kStats || units < kSplitBlocks ? 1 : 0;
     const uint32_t joins = a.cutsByUnit != 0 ? static_cast<uint32_t>(units) : kSplitBlocks - 1;
     hipLaunchKernelGGL(split, dim3(kSplitBlocks), dim3(kBlock), 0, s, a);
+    if (kStats)
+    {
+        return hipGetLastError();
+    }
     if (joins * a.group <= 256)
     {
-        hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, kTile, 512, kStats>), dim3(joins, a.group), dim3(512), 0, s,
-                           a);
+        hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, kTile, 512>), dim3(joins, a.group), dim3(512), 0, s, a);
     }
     else
     {
-        hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, kTile, 256, kStats>), dim3(joins, a.group), dim3(256), 0, s,
-                           a);
+        hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, kTile, 256>), dim3(joins, a.group), dim3(256), 0, s, a);
     }
     return hipGetLastError();
 }

@@ -16,9 +16,12 @@ struct PagedAttentionF16Args : PagedAttentionArgs
     const uint16_t* vcache;
 };
 
-/// muyo_paged_attention_decode_f16kv's launches, with `stats` written.
+/// muyo_paged_attention_decode_f16kv's launches but for the join of what shares cut: OwnKeysSplit says if there is any.
+/// What no share cut is in `out` and `stats`.
 template <int kHd>
 hipError_t LaunchOwnKeys(hipStream_t s, const PagedAttentionF16Args& a);
+
+bool OwnKeysSplit(const PagedAttentionF16Args& a);
 
 extern template hipError_t LaunchOwnKeys<64>(hipStream_t, const PagedAttentionF16Args&);
 extern template hipError_t LaunchOwnKeys<128>(hipStream_t, const PagedAttentionF16Args&);

@@ -37,6 +37,8 @@ struct PagedPrefixArgs
     float scale;
     uint32_t chunks;        // of the prefix, at most
     const float4* stats;    // of the own keys: base, sum, a score's log2 units, -
+    const uint4* cuts;      // of the own keys of each (query, kv head), and what to join; null if none is cut
+    const float* pieces;
     float* partials;        // [kv_heads][queries * group][chunks][4 + headDim]: the same, weighted values
 };
 
@@ -280,6 +282,7 @@ __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a
         {
             const uint8_t* kTile = kRows + first * kRowBytes;
             const uint8_t* vTile = vRows + first * kRowBytes;
+            __builtin_amdgcn_s_setprio(1);  // matrix work before the other wave's weights: 182 -> 180 us
             floatx16 score = floatx16{};
             floatx16 low = floatx16{};
 #pragma unroll
@@ -289,6 +292,7 @@ __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a
                 low = Mfma(k, qlo[s], low);
                 score = Mfma(k, qhi[s], score);
             }
+            __builtin_amdgcn_s_setprio(0);
             score += low;
             if (!inside)
             {
@@ -422,8 +426,9 @@ __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a
     }
 }
 
-/// Joins a row's chunks and its own keys' output (in `out`, with its base and sum in `stats`): kThreads threads a row,
-/// kHd / 4 of them over the channels, so many pieces side by side, kDeep of each on their way. In a fixed order.
+/// Joins a row's chunks with its own keys' pieces, or their output where these were not cut (in `out`, with its base
+/// and sum in `stats`): kThreads threads a row, kHd / 4 of them over the channels, so many pieces side by side, kDeep of
+/// each on their way. In a fixed order.
 template <int kHd, int kThreads>
 __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
 {
@@ -441,8 +446,17 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
     const uint32_t at = threadIdx.x / kLanes;
     const uint32_t query = static_cast<uint32_t>(min(item, items - 1) / heads);
     const uint32_t head = static_cast<uint32_t>(min(item, items - 1) % heads);
-    const bool is = item < items && prefix.chunks > 0 &&
-                    static_cast<uint32_t>(a.querySequence[query]) < a.sequences;
+    uint32_t first = 0;  // share of the own keys
+    uint32_t pieces = 0;
+    if (a.cuts != nullptr && static_cast<uint32_t>(a.querySequence[query]) < a.sequences)
+    {
+        const uint4 cut = a.cuts[query * a.kvHeads + head / a.group];
+        first = cut.z;
+        pieces = cut.w;
+    }
+    const uint32_t parts = prefix.chunks + pieces;
+    const bool is = item < items && parts > 0 && static_cast<uint32_t>(a.querySequence[query]) < a.sequences;
+    const float ownUnits = __builtin_amdgcn_exp2f(kPrefixBias - kWeightBias);  // of its weights, in the prefix's
     float base = -INFINITY;
     float den = 0.0f;
     float scaleLog2 = 1.0f;
@@ -454,21 +468,26 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
         const float* const from = a.partials +
                                   ((head / a.group) * rows + static_cast<uint64_t>(query) * a.group + head % a.group) *
                                       a.chunks * (kHd + 4);
-        for (uint32_t p0 = slice; p0 < prefix.chunks; p0 += kDeep * kSlices)
+        for (uint32_t p0 = slice; p0 < parts; p0 += kDeep * kSlices)
         {
             float4v of[kDeep], x[kDeep];
             float best = base;
 #pragma unroll
             for (uint32_t i = 0; i < kDeep; ++i)
             {
-                const uint32_t p = min(p0 + i * kSlices, prefix.chunks - 1);
-                of[i] = *reinterpret_cast<const float4v*>(from + static_cast<uint64_t>(p) * (kHd + 4));
-                x[i] = *reinterpret_cast<const float4v*>(from + static_cast<uint64_t>(p) * (kHd + 4) + 4 + 4 * lane);
+                const uint32_t p = min(p0 + i * kSlices, parts - 1);
+                const uint32_t own = p - prefix.chunks;  // piece 0 begins the own keys, the others are their shares' first
+                const float* at = p < prefix.chunks
+                                      ? from + static_cast<uint64_t>(p) * (kHd + 4)
+                                      : a.pieces + (static_cast<uint64_t>(2 * (first + own) + (own == 0 ? 1 : 0)) *
+                                                        a.group + head % a.group) * (kHd + 4);
+                of[i] = *reinterpret_cast<const float4v*>(at);
+                x[i] = *reinterpret_cast<const float4v*>(at + 4 + 4 * lane);
             }
 #pragma unroll
             for (uint32_t i = 0; i < kDeep; ++i)
             {
-                best = p0 + i * kSlices < prefix.chunks ? fmaxf(best, of[i][0]) : best;
+                best = p0 + i * kSlices < parts ? fmaxf(best, of[i][0]) : best;
             }
             scaleLog2 = of[0][2];
             const float factor = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((base - best) * scaleLog2);
@@ -478,24 +497,24 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
 #pragma unroll
             for (uint32_t i = 0; i < kDeep; ++i)
             {
-                if (p0 + i * kSlices < prefix.chunks)
+                if (p0 + i * kSlices < parts)
                 {
                     // A piece without keys is all 0; one of NaN scores has this base too, and stays NaN.
-                    const float w = of[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((of[i][0] - best) * scaleLog2);
+                    float w = of[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((of[i][0] - best) * scaleLog2);
+                    w *= p0 + i * kSlices < prefix.chunks ? 1.0f : ownUnits;
                     den = fmaf(w, of[i][1], den);
                     num += w * x[i];
                 }
             }
         }
-        if (slice == kSlices - 1)
+        if (slice == kSlices - 1 && pieces == 0)
         {
             const float4 own = a.stats[static_cast<uint64_t>(query) * heads + head];
             const float4v result = *reinterpret_cast<const float4v*>(out);
             const float best = fmaxf(base, own.x);
             const float factor = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((base - best) * own.z);
             float w = own.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((own.x - best) * own.z);
-            w *= __builtin_amdgcn_exp2f(kPrefixBias - kWeightBias);
-            scaleLog2 = own.z;
+            w *= ownUnits;
             base = best;
             den = fmaf(w, own.y, den * factor);
             num = num * factor + result * (w * own.y);
@@ -509,39 +528,38 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
     __syncthreads();
     if (is && slice == kSlices - 1)
     {
-        const uint32_t first = at - (kSlices - 1);
+        const uint32_t slice0 = at - (kSlices - 1);
+        scaleLog2 = sliceHead[slice0][2];  // slice 0 has a part
         float best = -INFINITY;
 #pragma unroll
         for (uint32_t s = 0; s < kSlices; ++s)
         {
-            best = fmaxf(best, sliceHead[first + s][0]);
+            best = fmaxf(best, sliceHead[slice0 + s][0]);
         }
         num = float4v{};
         den = 0.0f;
 #pragma unroll
         for (uint32_t s = 0; s < kSlices; ++s)
         {
-            const float b = sliceHead[first + s][0];
+            const float b = sliceHead[slice0 + s][0];
             const float w = b == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((b - best) * scaleLog2);
-            den = fmaf(w, sliceHead[first + s][1], den);
-            num += w * sliceNum[first + s][lane];
+            den = fmaf(w, sliceHead[slice0 + s][1], den);
+            num += w * sliceNum[slice0 + s][lane];
         }
         *reinterpret_cast<float4v*>(out) = den == 0.0f ? float4v{} : num / den;
     }
 }
 
-/// Chunks of the prefix: as many as there are workgroups to aim at, a number of (kv head, chunk) that is a multiple
-/// of eight where that costs little.
+/// Chunks of the prefix: as many as there are workgroups to aim at. (A number of workgroups of the same rows that is a
+/// multiple of eight, which keeps those of the same keys on one XCD, was slower where it left CUs with one fewer: 250
+/// queries of 28 / 4 heads, 16381 keys in 8 chunks 187 us, in 9 182.)
 uint32_t PrefixChunks(uint32_t queries, uint32_t heads, uint32_t kvHeads)
 {
     const uint32_t blocks = CeilDiv(static_cast<uint64_t>(queries) * (heads / kvHeads), kRowsOfBlock);
-    uint32_t chunks = std::max(1u, std::min(kMaxChunks, kPrefixBlocks / std::max(1u, kvHeads * blocks)));
-    while (chunks > 8 && kvHeads * chunks % 8 != 0)
-    {
-        --chunks;
-    }
-    return chunks;
+    return std::max(1u, std::min(kMaxChunks, kPrefixBlocks / std::max(1u, kvHeads * blocks)));
 }
+
+size_t CutBytes(uint32_t queries, uint32_t kvHeads) { return sizeof(uint4) * static_cast<size_t>(queries) * kvHeads; }
 
 size_t StatBytes(uint32_t queries, uint32_t heads) { return sizeof(float4) * static_cast<size_t>(queries) * heads; }
 
@@ -556,7 +574,9 @@ hipError_t LaunchPrefix(hipStream_t s, const PagedPrefixArgs& a, const PagedAtte
         return launched;
     }
     const uint64_t items = static_cast<uint64_t>(a.queries) * a.kvHeads * a.group;
-    if (items <= 512)
+    // 256 threads have 32 parts of 128 channels on their way, 64 have 8: 64 queries of 28 heads with 32 chunks (1792
+    // rows) take 53.6 us in all with 256 and 56.2 with 64, 250 queries with 9 chunks about the same with either.
+    if (a.chunks > 16)
     {
         hipLaunchKernelGGL((PagedPrefixJoinKernel<kHd, 256>), dim3(static_cast<uint32_t>(items)), dim3(256), 0, s, a);
     }
@@ -579,6 +599,7 @@ extern "C" size_t muyo_paged_attention_prefix_f16kv_workspace_bytes(uint32_t que
         return 0;
     }
     return DecodeWorkspaceBytes(queries, heads, kv_heads, head_dim) + StatBytes(queries, heads) +
+           CutBytes(queries, kv_heads) +
            sizeof(float) * static_cast<size_t>(queries) * heads * PrefixChunks(queries, heads, kv_heads) *
                (head_dim + 4);
 }
@@ -608,10 +629,12 @@ extern "C" int muyo_paged_attention_prefix_f16kv(const float* q, const void* kca
     own.vcache = static_cast<const uint16_t*>(vcache);
     char* const behind = static_cast<char*>(workspace) + DecodeWorkspaceBytes(queries, heads, kv_heads, head_dim);
     own.stats = reinterpret_cast<float4*>(behind);
+    own.cuts = reinterpret_cast<uint4*>(behind + StatBytes(queries, heads));
     const PagedPrefixArgs a{q, own.kcache, own.vcache, out, tables, sequences, table_pages, query_sequence, queries,
                             heads / kv_heads, kv_heads, prefix, pages, own.pageShift, scale,
                             PrefixChunks(queries, heads, kv_heads), own.stats,
-                            reinterpret_cast<float*>(behind + StatBytes(queries, heads))};
+                            OwnKeysSplit(own) ? own.cuts : nullptr, own.partials,
+                            reinterpret_cast<float*>(behind + StatBytes(queries, heads) + CutBytes(queries, kv_heads))};
     const hipError_t launched =
         head_dim == 64 ? LaunchPrefix<64>(AsStream(stream), a, own) : LaunchPrefix<128>(AsStream(stream), a, own);
     return launched == hipSuccess ? MUYO_OK : HipStatus(launched, name);
