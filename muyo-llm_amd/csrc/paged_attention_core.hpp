@@ -25,7 +25,7 @@ struct PagedAttentionArgs
     uint32_t* costSums;  // [queries + 1]: CostOf of one kv head of the queries before
     uint4* cuts;         // what to join: query, kv head, first share, pieces (0: nothing)
     uint32_t cutsByUnit; // cuts has an entry per (query, kv head); else one per share
-    float4* stats;       // of kStats, for what no share cut: base, sum, a score's log2 units, -, of each query's heads
+    float* wholes;       // of kPieces: [queries][heads], as partials, of what no share cut
     float* partials;     // [2 * shares][group][4 + headDim]: base, sum, a score's log2 units, -, weighted values
 };
 
@@ -223,9 +223,9 @@ struct ShareSpace
     uint32_t firstAt[2];  // the share's first query, and the costs before it
 };
 
-/// The share of this workgroup; one that is empty has at >= stop.
+/// Share `block`; one that is empty has at >= stop.
 template <uint32_t kTile>
-__device__ __forceinline__ Share FirstShare(const PagedAttentionArgs& a, uint32_t lane, ShareSpace& space)
+__device__ __forceinline__ Share FirstShare(const PagedAttentionArgs& a, uint32_t block, uint32_t lane, ShareSpace& space)
 {
     Share first;
     uint32_t total;
@@ -238,7 +238,7 @@ __device__ __forceinline__ Share FirstShare(const PagedAttentionArgs& a, uint32_
         const uint32_t sum = WaveSums(cost);
         total = __builtin_amdgcn_readlane(sum, kWave - 1);
         first.share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
-        first.at = blockIdx.x * first.share;
+        first.at = block * first.share;
         const uint64_t has = __ballot((sum - cost) * a.kvHeads <= first.at && first.at < sum * a.kvHeads);
         first.query = has != 0 ? static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(has)) - 1) : 0;
         first.queryAt = __builtin_amdgcn_readlane(sum - cost, first.query) * a.kvHeads;
@@ -265,7 +265,7 @@ __device__ __forceinline__ Share FirstShare(const PagedAttentionArgs& a, uint32_
         const uint32_t all = sum;
         sum = BlockSums<kBlock>(sum, space.waveSum, total) - all;
         first.share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
-        first.at = blockIdx.x * first.share;
+        first.at = block * first.share;
 #pragma unroll
         for (uint32_t e = 0; e < kPer; ++e)
         {
@@ -287,7 +287,7 @@ __device__ __forceinline__ Share FirstShare(const PagedAttentionArgs& a, uint32_
     {
         total = a.costSums[a.queries];
         first.share = max((total * a.kvHeads + kSplitBlocks - 1) / kSplitBlocks, kMinShare);
-        first.at = blockIdx.x * first.share;
+        first.at = block * first.share;
         first.query = OwnerOf(a.costSums, a.queries, min(first.at / a.kvHeads, total - 1));
         first.queryAt = a.costSums[first.query] * a.kvHeads;
         first.range = RangeOf<kTile>(a, first.query);
@@ -435,7 +435,7 @@ inline void FillAttentionArgs(PagedAttentionArgs& a, const AttentionCall& c, uin
     a.costSums = reinterpret_cast<uint32_t*>(space);
     a.cuts = reinterpret_cast<uint4*>(space + CostSumBytes(c.queries));
     a.cutsByUnit = 0;
-    a.stats = nullptr;
+    a.wholes = nullptr;
     a.partials = reinterpret_cast<float*>(space + CostSumBytes(c.queries) + kCutBytes);
 }
 
@@ -455,9 +455,8 @@ bool SplitKeys(const PagedAttentionArgs& a)
     return keys > kWholeKeys && units * (keys / kTile + 2 + kSetupTiles<kTile>) <= 0x7FFFFFFFull;
 }
 
-/// Split launches take `split` and the join, others `whole`. With kStats the caller joins: `cuts` has an entry per
-/// (query, kv head).
-template <int kHd, uint32_t kTile, bool kStats, typename Args>
+/// Split launches take `split` and the join, others `whole`.
+template <int kHd, uint32_t kTile, typename Args>
 hipError_t LaunchPagedAttention(hipStream_t s, Args a, void (*whole)(Args), void (*split)(Args))
 {
     const uint64_t units = static_cast<uint64_t>(a.queries) * a.kvHeads;
@@ -470,13 +469,9 @@ hipError_t LaunchPagedAttention(hipStream_t s, Args a, void (*whole)(Args), void
     {
         hipLaunchKernelGGL(PagedCostSumsKernel<kTile>, dim3(1), dim3(1024), 0, s, a);
     }
-    a.cutsByUnit = kStats || units < kSplitBlocks ? 1 : 0;
+    a.cutsByUnit = units < kSplitBlocks ? 1 : 0;
     const uint32_t joins = a.cutsByUnit != 0 ? static_cast<uint32_t>(units) : kSplitBlocks - 1;
     hipLaunchKernelGGL(split, dim3(kSplitBlocks), dim3(kBlock), 0, s, a);
-    if (kStats)
-    {
-        return hipGetLastError();
-    }
     if (joins * a.group <= 256)
     {
         hipLaunchKernelGGL((PagedAttentionMergeKernel<kHd, kTile, 512>), dim3(joins, a.group), dim3(512), 0, s, a);

@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 3 : 2) void PagedAttentionQ8Ker
     uint4 cut = make_uint4(0, 0, 0, 0);
     if constexpr (kSplit)
     {
-        const Share first = FirstShare<kTile>(a, lane, space);
+        const Share first = FirstShare<kTile>(a, blockIdx.x, lane, space);
         share = first.share;
         at = first.at;
         stop = first.stop;
@@ -688,7 +688,7 @@ __global__ __launch_bounds__(kBlock, kHd == 64 ? 3 : 2) void PagedAttentionQ8Ker
 template <int kHd, int kFormat>
 hipError_t LaunchQ8(hipStream_t s, const PagedAttentionQ8Args& a)
 {
-    return LaunchPagedAttention<kHd, kTile, false>(s, a, PagedAttentionQ8Kernel<kHd, kFormat, false>,
+    return LaunchPagedAttention<kHd, kTile>(s, a, PagedAttentionQ8Kernel<kHd, kFormat, false>,
                                                    PagedAttentionQ8Kernel<kHd, kFormat, true>);
 }
 }  // namespace

@@ -9,14 +9,13 @@ namespace muyo
 {
 namespace
 {
-typedef short short4v __attribute__((ext_vector_type(4)));
-
 constexpr uint32_t kStep = 64;            // keys of one step: an LDS buffer of K and V rows
 constexpr uint32_t kStepPages = kStep / 16;
 constexpr uint32_t kRowsOfWave = 32;      // rows are (query, head of a kv head's group)
 constexpr uint32_t kRowsOfBlock = kRowsOfWave * kWaves;
 constexpr uint32_t kPrefixBlocks = 512;   // workgroups to aim at: two on each of 256 CUs
 constexpr uint32_t kMaxChunks = 128;
+constexpr uint32_t kTurn = 256;           // workgroups of a kind in turn: one on each CU
 // Softmax weights as in the attention over a query's own keys: the maximum's is 2^kPrefixBias, 2^15 at most.
 constexpr float kPrefixLag = 10.0f;
 constexpr float kPrefixBias = 15.0f - kPrefixLag;
@@ -36,10 +35,11 @@ struct PagedPrefixArgs
     uint32_t pages, pageShift;
     float scale;
     uint32_t chunks;        // of the prefix, at most
-    const float4* stats;    // of the own keys: base, sum, a score's log2 units, -
-    const uint4* cuts;      // of the own keys of each (query, kv head), and what to join; null if none is cut
+    // The own keys': what no share cut, and where shares are dealt out those of each (query, kv head) and their pieces.
+    const float* wholes;
+    const uint4* cuts;
     const float* pieces;
-    float* partials;        // [kv_heads][queries * group][chunks][4 + headDim]: the same, weighted values
+    float* partials;        // [kv_heads][queries * group][chunks][4 + headDim]: base, sum, a score's log2 units, -, values
 };
 
 /// The prefix's keys, and the steps of a chunk of them.
@@ -61,6 +61,13 @@ __device__ __forceinline__ PrefixKeys KeysOf(const PagedPrefixArgs& a)
     return p;
 }
 
+template <int kHd>
+inline constexpr int kPrefixStages = kHd == 128 ? 2 : 3;
+
+/// LDS of PrefixKeysOfRows: K and V of its steps, and later the rows' results.
+template <int kHd>
+inline constexpr uint32_t kPrefixBytes = kPrefixStages<kHd> * 2 * kStep * 2 * kHd;
+
 /// A wave has 32 rows, the columns of its matrix operations; a workgroup's four waves share each step of 64 keys of K
 /// and V through LDS, where they go straight from memory a step ahead. Per 32 keys a wave
 ///   - forms S^T (keys x rows) = K . q^T, K from LDS, q in registers as two planes of f16 (of q / 2^e, e by the row's
@@ -74,12 +81,11 @@ __device__ __forceinline__ PrefixKeys KeysOf(const PagedPrefixArgs& a)
 /// Steps that reach past the prefix, or into a page that is not there, are masked: scores to -inf, and V's rows to 0 in
 /// LDS, since 0 * NaN would be NaN.
 ///
-/// Grid: (kv head, chunk of keys) fastest, then blocks of 128 rows: those of the same keys come a multiple of eight
-/// workgroups apart, on one XCD.
+/// `block` goes over (kv head, chunk) fastest, then blocks of 128 rows.
 template <int kHd>
-__global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a)
+__device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint32_t block, uint8_t* lds)
 {
-    constexpr int kStages = kHd == 128 ? 2 : 3;
+    constexpr int kStages = kPrefixStages<kHd>;
     constexpr bool kKeepLow = kHd == 64;
     constexpr uint32_t kRowBytes = 2 * kHd;
     constexpr uint32_t kChunks = kHd / 8;                // 16-byte chunks of a row
@@ -88,21 +94,18 @@ __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a
     constexpr int kMatrixLoads = kMatrixBytes / 1024 / kWaves;  // of a wave
     constexpr int kLoads = 2 * kMatrixLoads;
     constexpr int kChannels = kHd / 32;                  // 32-channel blocks of the output
-    static_assert(kStages * 2 * kMatrixBytes >= kRowsOfBlock * kHd * 4, "O fits where K and V were");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * 2 * kMatrixBytes];
-
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t h = lane / 32;
-    const uint32_t g = blockIdx.x % a.kvHeads;
-    const uint32_t chunk = blockIdx.x / a.kvHeads;
+    const uint32_t g = block % a.kvHeads;
+    const uint32_t chunk = block / a.kvHeads % a.chunks;
     const PrefixKeys prefix = KeysOf(a);
     if (chunk >= prefix.chunks)
     {
         return;
     }
     const uint32_t rows = a.queries * a.group;
-    const uint32_t row0 = blockIdx.y * kRowsOfBlock + wave * kRowsOfWave;
+    const uint32_t row0 = block / (a.kvHeads * a.chunks) * kRowsOfBlock + wave * kRowsOfWave;
     const bool active = row0 < rows;  // a wave past the rows only loads
     const uint32_t row = min(row0 + lane % 32, rows - 1);
     const uint32_t firstStep = chunk * prefix.perChunk;
@@ -426,9 +429,45 @@ __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a
     }
 }
 
-/// Joins a row's chunks with its own keys' pieces, or their output where these were not cut (in `out`, with its base
-/// and sum in `stats`): kThreads threads a row, kHd / 4 of them over the channels, so many pieces side by side, kDeep of
-/// each on their way. In a fixed order.
+/// Both kinds of keys in one launch: workgroups for the prefix, whose matrix operations bound them, and for own keys,
+/// which wait for memory, in turns of a CU each. The q of a workgroup may be read when others have ended, so none
+/// writes `out`.
+///
+/// What it took as two launches, the prefix's before the own keys': %%.
+template <int kHd, bool kSplit>
+__global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a, PagedAttentionF16Args own,
+                                                               uint32_t prefixBlocks, uint32_t ownBlocks)
+{
+    static_assert(kPrefixBytes<kHd> >= kOwnKeysBytes<kHd> && kPrefixBytes<kHd> >= kRowsOfBlock * kHd * 4,
+                  "own keys' V and all results fit");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kPrefixBytes<kHd>];
+    __shared__ OwnKeysSpace space;
+    const uint32_t turns = min(prefixBlocks, ownBlocks) / kTurn * kTurn;  // of each kind
+    uint32_t at = blockIdx.x;
+    bool isOwn;
+    if (at < 2 * turns)
+    {
+        isOwn = at / kTurn % 2 != 0;
+        at = at / (2 * kTurn) * kTurn + at % kTurn;
+    }
+    else
+    {
+        at -= turns;
+        isOwn = at >= prefixBlocks;
+        at -= isOwn ? prefixBlocks - turns : 0;
+    }
+    if (!isOwn)
+    {
+        PrefixKeysOfRows<kHd>(a, at, lds);
+    }
+    else
+    {
+        OwnKeys<kHd, kSplit, true>(own, kSplit ? at : at % a.kvHeads, at / a.kvHeads, lds, space);
+    }
+}
+
+/// Joins a row's chunks with its own keys' pieces: kThreads threads a row, kHd / 4 of them over the channels, so many
+/// pieces side by side, kDeep of each on their way. In a fixed order.
 template <int kHd, int kThreads>
 __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
 {
@@ -446,16 +485,16 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
     const uint32_t at = threadIdx.x / kLanes;
     const uint32_t query = static_cast<uint32_t>(min(item, items - 1) / heads);
     const uint32_t head = static_cast<uint32_t>(min(item, items - 1) % heads);
+    const bool is = item < items && static_cast<uint32_t>(a.querySequence[query]) < a.sequences;
     uint32_t first = 0;  // share of the own keys
     uint32_t pieces = 0;
-    if (a.cuts != nullptr && static_cast<uint32_t>(a.querySequence[query]) < a.sequences)
+    if (a.cuts != nullptr && is)
     {
         const uint4 cut = a.cuts[query * a.kvHeads + head / a.group];
         first = cut.z;
         pieces = cut.w;
     }
-    const uint32_t parts = prefix.chunks + pieces;
-    const bool is = item < items && parts > 0 && static_cast<uint32_t>(a.querySequence[query]) < a.sequences;
+    const uint32_t parts = prefix.chunks + max(pieces, 1u);
     const float ownUnits = __builtin_amdgcn_exp2f(kPrefixBias - kWeightBias);  // of its weights, in the prefix's
     float base = -INFINITY;
     float den = 0.0f;
@@ -477,10 +516,11 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
             {
                 const uint32_t p = min(p0 + i * kSlices, parts - 1);
                 const uint32_t own = p - prefix.chunks;  // piece 0 begins the own keys, the others are their shares' first
-                const float* at = p < prefix.chunks
-                                      ? from + static_cast<uint64_t>(p) * (kHd + 4)
-                                      : a.pieces + (static_cast<uint64_t>(2 * (first + own) + (own == 0 ? 1 : 0)) *
-                                                        a.group + head % a.group) * (kHd + 4);
+                const float* at = p < prefix.chunks ? from + static_cast<uint64_t>(p) * (kHd + 4)
+                                  : pieces == 0     ? a.wholes + (static_cast<uint64_t>(query) * heads + head) * (kHd + 4)
+                                                    : a.pieces + (static_cast<uint64_t>(2 * (first + own) +
+                                                                                        (own == 0 ? 1 : 0)) * a.group +
+                                                                  head % a.group) * (kHd + 4);
                 of[i] = *reinterpret_cast<const float4v*>(at);
                 x[i] = *reinterpret_cast<const float4v*>(at + 4 + 4 * lane);
             }
@@ -506,18 +546,6 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
                     num += w * x[i];
                 }
             }
-        }
-        if (slice == kSlices - 1 && pieces == 0)
-        {
-            const float4 own = a.stats[static_cast<uint64_t>(query) * heads + head];
-            const float4v result = *reinterpret_cast<const float4v*>(out);
-            const float best = fmaxf(base, own.x);
-            const float factor = base == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((base - best) * own.z);
-            float w = own.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((own.x - best) * own.z);
-            w *= ownUnits;
-            base = best;
-            den = fmaf(w, own.y, den * factor);
-            num = num * factor + result * (w * own.y);
         }
     }
     sliceNum[at][lane] = num;
@@ -561,17 +589,29 @@ uint32_t PrefixChunks(uint32_t queries, uint32_t heads, uint32_t kvHeads)
 
 size_t CutBytes(uint32_t queries, uint32_t kvHeads) { return sizeof(uint4) * static_cast<size_t>(queries) * kvHeads; }
 
-size_t StatBytes(uint32_t queries, uint32_t heads) { return sizeof(float4) * static_cast<size_t>(queries) * heads; }
+size_t WholeBytes(uint32_t queries, uint32_t heads, uint32_t headDim)
+{
+    return sizeof(float) * static_cast<size_t>(queries) * heads * (headDim + 4);
+}
 
 template <int kHd>
 hipError_t LaunchPrefix(hipStream_t s, const PagedPrefixArgs& a, const PagedAttentionF16Args& own)
 {
-    const uint32_t blocks = CeilDiv(static_cast<uint64_t>(a.queries) * a.group, kRowsOfBlock);
-    hipLaunchKernelGGL(PagedPrefixKernel<kHd>, dim3(a.kvHeads * a.chunks, blocks), dim3(kBlock), 0, s, a);
-    const hipError_t launched = LaunchOwnKeys<kHd>(s, own);
-    if (launched != hipSuccess)
+    const uint32_t prefixBlocks = a.kvHeads * a.chunks * CeilDiv(static_cast<uint64_t>(a.queries) * a.group, kRowsOfBlock);
+    if (a.cuts != nullptr)
     {
-        return launched;
+        if (a.queries > kScanQueries)
+        {
+            hipLaunchKernelGGL(PagedCostSumsKernel<kTile>, dim3(1), dim3(1024), 0, s, own);
+        }
+        hipLaunchKernelGGL((PagedPrefixKernel<kHd, true>), dim3(prefixBlocks + kSplitBlocks), dim3(kBlock), 0, s, a, own,
+                           prefixBlocks, kSplitBlocks);
+    }
+    else
+    {
+        const uint32_t ownBlocks = a.queries * a.kvHeads;
+        hipLaunchKernelGGL((PagedPrefixKernel<kHd, false>), dim3(prefixBlocks + ownBlocks), dim3(kBlock), 0, s, a, own,
+                           prefixBlocks, ownBlocks);
     }
     const uint64_t items = static_cast<uint64_t>(a.queries) * a.kvHeads * a.group;
     // 256 threads have 32 parts of 128 channels on their way, 64 have 8: 64 queries of 28 heads with 32 chunks (1792
@@ -598,7 +638,7 @@ extern "C" size_t muyo_paged_attention_prefix_f16kv_workspace_bytes(uint32_t que
     {
         return 0;
     }
-    return DecodeWorkspaceBytes(queries, heads, kv_heads, head_dim) + StatBytes(queries, heads) +
+    return DecodeWorkspaceBytes(queries, heads, kv_heads, head_dim) + WholeBytes(queries, heads, head_dim) +
            CutBytes(queries, kv_heads) +
            sizeof(float) * static_cast<size_t>(queries) * heads * PrefixChunks(queries, heads, kv_heads) *
                (head_dim + 4);
@@ -628,13 +668,14 @@ extern "C" int muyo_paged_attention_prefix_f16kv(const float* q, const void* kca
     own.kcache = static_cast<const uint16_t*>(kcache);
     own.vcache = static_cast<const uint16_t*>(vcache);
     char* const behind = static_cast<char*>(workspace) + DecodeWorkspaceBytes(queries, heads, kv_heads, head_dim);
-    own.stats = reinterpret_cast<float4*>(behind);
-    own.cuts = reinterpret_cast<uint4*>(behind + StatBytes(queries, heads));
+    own.wholes = reinterpret_cast<float*>(behind);
+    own.cutsByUnit = 1;
+    own.cuts = reinterpret_cast<uint4*>(behind + WholeBytes(queries, heads, head_dim));
     const PagedPrefixArgs a{q, own.kcache, own.vcache, out, tables, sequences, table_pages, query_sequence, queries,
                             heads / kv_heads, kv_heads, prefix, pages, own.pageShift, scale,
-                            PrefixChunks(queries, heads, kv_heads), own.stats,
-                            OwnKeysSplit(own) ? own.cuts : nullptr, own.partials,
-                            reinterpret_cast<float*>(behind + StatBytes(queries, heads) + CutBytes(queries, kv_heads))};
+                            PrefixChunks(queries, heads, kv_heads), own.wholes,
+                            SplitKeys<kTile>(own) ? own.cuts : nullptr, own.partials,
+                            reinterpret_cast<float*>(behind + WholeBytes(queries, heads, head_dim) + CutBytes(queries, kv_heads))};
     const hipError_t launched =
         head_dim == 64 ? LaunchPrefix<64>(AsStream(stream), a, own) : LaunchPrefix<128>(AsStream(stream), a, own);
     return launched == hipSuccess ? MUYO_OK : HipStatus(launched, name);
