@@ -13,8 +13,8 @@ constexpr uint32_t kStep = 64;            // keys of one step: an LDS buffer of 
 constexpr uint32_t kStepPages = kStep / 16;
 constexpr uint32_t kRowsOfWave = 32;      // rows are (query, head of a kv head's group)
 constexpr uint32_t kRowsOfBlock = kRowsOfWave * kWaves;
-constexpr uint32_t kPrefixBlocks = 512;   // workgroups to aim at: two on each of 256 CUs
 constexpr uint32_t kMaxChunks = 128;
+constexpr uint32_t kFewChunks = 8;
 constexpr uint32_t kTurn = 256;           // workgroups of a kind in turn: one on each CU
 // Softmax weights as in the attention over a query's own keys: the maximum's is 2^kPrefixBias, 2^15 at most.
 constexpr float kPrefixLag = 10.0f;
@@ -433,7 +433,9 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 /// which wait for memory, in turns of a CU each. The q of a workgroup may be read when others have ended, so none
 /// writes `out`.
 ///
-/// What it took as two launches, the prefix's before the own keys': %%.
+/// Two launches, the prefix's before the own keys', took 14.3 us for 3 queries (1009 keys and up to 100 own, 14 / 2 heads
+/// of 64), together 10.3; 64 queries (8190 and up to 2000, 28 / 4 of 128) 53 and 45; 250 (16381 and up to 500) 183 and
+/// 172. In turns of 8, 128 and 512 workgroups, or with the own keys first, 1 to 70 us more.
 template <int kHd, bool kSplit>
 __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a, PagedAttentionF16Args own,
                                                                uint32_t prefixBlocks, uint32_t ownBlocks)
@@ -578,13 +580,16 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
     }
 }
 
-/// Chunks of the prefix: as many as there are workgroups to aim at. (A number of workgroups of the same rows that is a
-/// multiple of eight, which keeps those of the same keys on one XCD, was slower where it left CUs with one fewer: 250
-/// queries of 28 / 4 heads, 16381 keys in 8 chunks 187 us, in 9 182.)
+/// Chunks of the prefix: workgroups for one on each of 256 CUs, beside one of own keys; two where that would be few
+/// chunks, so that rounding their number down leaves many CUs without. 28 / 4 heads of 128: 64 queries, 8190 keys in 16
+/// chunks 44.7 us, in 32 47.8; 16 queries, 16000 keys in 64 chunks 31.3 us, in 128 38.0; 250 queries, 16381 keys in 9
+/// chunks 170 us, in 4 207. (A number of workgroups of the same rows that is a multiple of eight, which keeps those of
+/// the same keys on one XCD, gained nothing: the last in 8 chunks 5 us slower.)
 uint32_t PrefixChunks(uint32_t queries, uint32_t heads, uint32_t kvHeads)
 {
-    const uint32_t blocks = CeilDiv(static_cast<uint64_t>(queries) * (heads / kvHeads), kRowsOfBlock);
-    return std::max(1u, std::min(kMaxChunks, kPrefixBlocks / std::max(1u, kvHeads * blocks)));
+    const uint32_t blocks = kvHeads * CeilDiv(static_cast<uint64_t>(queries) * (heads / kvHeads), kRowsOfBlock);
+    const uint32_t chunks = kTurn / blocks;
+    return std::max(1u, std::min(kMaxChunks, chunks < kFewChunks ? 2 * kTurn / blocks : chunks));
 }
 
 size_t CutBytes(uint32_t queries, uint32_t kvHeads) { return sizeof(uint4) * static_cast<size_t>(queries) * kvHeads; }
