@@ -619,9 +619,9 @@ hipError_t LaunchPrefix(hipStream_t s, const PagedPrefixArgs& a, const PagedAtte
                            prefixBlocks, ownBlocks);
     }
     const uint64_t items = static_cast<uint64_t>(a.queries) * a.kvHeads * a.group;
-    // 256 threads have 32 parts of 128 channels on their way, 64 have 8: 64 queries of 28 heads with 32 chunks (1792
-    // rows) take 53.6 us in all with 256 and 56.2 with 64, 250 queries with 9 chunks about the same with either.
-    if (a.chunks > 16)
+    // 256 threads have 32 parts of 128 channels on their way, 64 have 8: 16 queries of 28 heads with 64 chunks take
+    // 31.0 us in all with 256 and 38.8 with 64, 64 queries with 16 chunks 43.3 and 44.3, 250 with 9 178 and 171.
+    if (a.chunks >= 16)
     {
         hipLaunchKernelGGL((PagedPrefixJoinKernel<kHd, 256>), dim3(static_cast<uint32_t>(items)), dim3(256), 0, s, a);
     }

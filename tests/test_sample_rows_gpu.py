@@ -125,6 +125,35 @@ def test_rows(mh, gpu, rows, vocab):
     Batch(mh, gpu, logits_of(rng, rows, vocab), settings, rng.random(rows), stride=vocab + 5).check()
 
 
+@pytest.mark.parametrize("vocab", [1, 70, 1501, 4999])
+def test_thousands_of_rows(mh, gpu, vocab):
+    """More rows than get workgroups of their own for their lists, the first of them also in a call that has these."""
+    rng = np.random.default_rng(vocab)
+    rows = 4100
+    settings = [SETTINGS[i] for i in rng.integers(0, len(SETTINGS), rows)]
+    x = logits_of(rng, 41, vocab)[rng.integers(0, 41, rows)]
+    x[rng.random(rows) < 0.05] = -np.inf
+    randoms = rng.random(rows)
+    batch = Batch(mh, gpu, x, settings, randoms, stride=vocab + 3)
+    batch.check()
+    less = Batch(mh, gpu, x[:4096], settings[:4096], randoms[:4096], stride=vocab + 1)
+    less.call()
+    gpu.cuda.synchronize()
+    assert np.array_equal(host(less.tokens)[:4096], host(batch.tokens)[:4096])
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_logits_that_begin_anywhere(mh, gpu, shift):
+    """Rows at any multiple of four bytes."""
+    torch, rng = gpu, np.random.default_rng(shift)
+    for rows, vocab, stride in ((22, 5001, 5001), (22, 151936, 151937), (3, 3, 7)):
+        batch = Batch(mh, torch, logits_of(rng, rows, vocab), SETTINGS[:rows], rng.random(rows), stride=stride)
+        wide = torch.full((rows * stride + 8,), 1e9, device="cuda")
+        wide[shift:shift + rows * stride] = batch.d[0].flatten()
+        batch.d[0] = wide[shift:]
+        batch.check()
+
+
 def test_settings_that_are_off(mh, gpu):
     rng = np.random.default_rng(2)
     settings = [(0.6, 9, 0.8, 0.1)] * 8
