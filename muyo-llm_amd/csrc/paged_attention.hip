@@ -8,7 +8,8 @@ namespace muyo
 namespace
 {
 template <int kHd, bool kSplit>
-__global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void PagedAttentionKernel(PagedAttentionF16Args a)
+__global__ __launch_bounds__(kBlock, kHd == 64 ? (kSplit ? 3 : 4) : 2) void PagedAttentionKernel(
+    PagedAttentionF16Args a)
 {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kOwnKeysBytes<kHd>];
     __shared__ OwnKeysSpace space;
@@ -113,7 +114,7 @@ extern "C" int muyo_paged_attention_decode_f16kv(const float* q, const void* kca
     const char* name = "paged_attention_decode_f16kv";
     const uint64_t cacheBytes = 2ull * pages * page_size * kv_heads * head_dim;
     const Range caches[] = {{kcache, cacheBytes, "kcache"}, {vcache, cacheBytes, "vcache"}};
-    const AttentionCall call{q,       out,      tables,   sequences, table_pages, query_sequence, positions, queries, heads,
+    const AttentionCall call{q, out, tables, sequences, table_pages, query_sequence, positions, queries, heads,
                              kv_heads, head_dim, pages, page_size, scale, workspace, workspace_bytes,
                              muyo_paged_attention_decode_f16kv_workspace_bytes(queries, heads, kv_heads, head_dim)};
     const int checked = CheckAttention(name, call, caches, 2, 2);

@@ -104,8 +104,8 @@ __device__ __forceinline__ KeyRange RangeOf(const PagedAttentionArgs& a, uint32_
 
 /// What a (query, kv head) of `tiles` tiles counts in the shares. A change to it (its q, its first tile's
 /// round trips, joining the waves) takes 3 to 4 us, a tile of each wave about one: dealt out by tiles alone,
-/// shares of short sequences had up to four of them. 28 / 4 heads of 128, with a cost of 0, 4, 8 and 12 tiles of 32 keys:
-/// 64 sequences of 1 to 500 keys 27, 15.7, 14.4 and 15.2 us; 250 of 1 to 2000, most short, -, 41, 38 and 43.
+/// shares of short sequences had up to four of them. 28 / 4 heads of 128, with a cost of 0, 4, 8 and 12 tiles of
+/// 32 keys: 64 sequences of 1 to 500 keys 27, 15.7, 14.4 and 15.2 us; 250 of 1 to 2000, most short, -, 41, 38 and 43.
 template <uint32_t kTile>
 inline constexpr uint32_t kSetupTiles = 256 / kTile;
 
@@ -225,7 +225,8 @@ struct ShareSpace
 
 /// Share `block`; one that is empty has at >= stop.
 template <uint32_t kTile>
-__device__ __forceinline__ Share FirstShare(const PagedAttentionArgs& a, uint32_t block, uint32_t lane, ShareSpace& space)
+__device__ __forceinline__ Share FirstShare(const PagedAttentionArgs& a, uint32_t block, uint32_t lane,
+                                            ShareSpace& space)
 {
     Share first;
     uint32_t total;

@@ -95,7 +95,8 @@ struct OwnKeysSpace
 /// (position, page, rows), 5.2 us: 8 or 16 waves a workgroup, tiles of 64 keys, and two or three tiles in
 /// flight at head_dim 64 all measured no better or worse.
 ///
-/// kPieces: nothing is joined here, what is not cut goes to `wholes`. `block` is the share, or the kv head of `wholeQuery`.
+/// kPieces: nothing is joined here, what is not cut goes to `wholes`. `block` is the share, or the kv head of
+/// `wholeQuery`.
 template <int kHd, bool kSplit, bool kPieces>
 __device__ __forceinline__ void OwnKeys(const PagedAttentionF16Args& a, uint32_t block, uint32_t wholeQuery,
                                         uint8_t* lds, OwnKeysSpace& shared)
@@ -531,10 +532,9 @@ __device__ __forceinline__ void OwnKeys(const PagedAttentionF16Args& a, uint32_t
             }
             else
             {
-                float* slot = kPieces && isWhole
-                                  ? a.wholes + head * (kHd + 4)
-                                  : a.partials + (static_cast<uint64_t>(2 * block + (tile0 == 0 ? 1 : 0)) * a.group + h) *
-                                                     (kHd + 4);
+                const uint64_t piece = 2 * block + (tile0 == 0 ? 1 : 0);
+                float* slot = kPieces && isWhole ? a.wholes + head * (kHd + 4)
+                                                 : a.partials + (piece * a.group + h) * (kHd + 4);
                 *reinterpret_cast<float4v*>(slot + 4 + channel) = num;
                 if (channel == 0)
                 {

@@ -14,7 +14,7 @@ typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 constexpr uint32_t kTile = 32;       // keys of a tile
 constexpr int kParts = kTile / 16;   // matrix operands of 16 keys
 constexpr int kPlanes = 3;           // of weights, 8 bits each: what f32 holds
-constexpr float kLag = 4.0f;         // binary orders that a weight may be above 1
+constexpr float kLag = 8.0f;         // binary orders that a weight may be above 1: with 4 a long batch takes 2 % more
 
 struct PagedAttentionQ8Args : PagedAttentionArgs
 {
@@ -134,15 +134,22 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
     return row * (2 * kHd) + (chunk ^ by) * 16;
 }
 
-/// The fp16 cache's attention (paged_attention.hip) with codes for K and V: the same shares, tiles, masks and joins,
-/// and v_mfma_f32_16x16x32_bf16 with its operands in the same places. What differs:
-///   - codes are widened to bf16, which holds them exactly, K's in registers on the way to the matrix cores, V's on
-///     the way to LDS; a key's scale multiplies its score, and its weight before that meets V;
-///   - q and the weights (times V's scales) are three planes of bf16, whose exponent is f32's: all 24 bits of each,
-///     whatever the scales and however small a weight beside the largest. (Two planes of f16 would want the
-///     products of weights and scales kept in f16's range, a second running maximum.) A matrix operation more for
-///     each of the fp16 cache's two; the cache's arrival hides them.
-///   - scores are raw, q (taken to 1 .. 2 by a power of two) times code times scale, and weights 2^kLag at most.
+/// The fp16 cache's attention (paged_attention_f16.hpp) with codes for K and V: the same shares, masks and joins, and
+/// operands in the same places. What differs:
+///   - K's codes are widened to f16, which holds them exactly, in registers on the way to the matrix cores, where they
+///     meet the same two planes of q; a key's scale multiplies its score;
+///   - V's are widened to bf16, as exact, on the way to LDS; a key's weight is multiplied by its scale before it meets
+///     them, in three planes of bf16, whose exponent is f32's: all 24 bits, whatever the scale and however small the
+///     weight beside the largest. (Two planes of f16 would want those products kept in f16's range, a second running
+///     maximum.) Three matrix operations for the fp16 cache's two;
+///   - a tile is half the bytes, so two are on their way.
+///
+/// What bounds it: two waves of a SIMD taking turns at the codes' widening (176 vector operations of 390 for a tile of
+/// 128 channels), the matrix cores and the wait for either. 64 sequences of 1 to 16384 keys (28 / 4 heads of 128, pages
+/// of 16, 554 MB): 97 us and 5 for the join, 5.7 TB/s where the best streaming read here has 6.9; the vector units are
+/// busy for 42 us of it, the matrix cores for 17. Three waves, of one tile each, spill their registers (168) and take
+/// 147 us in all, two waves of one tile 125. One sequence of 32749 keys 13 us and 5
+/// for the join; 16 of up to 500 keys 6.1.
 template <int kHd, int kFormat, bool kSplit>
 __global__ __launch_bounds__(kBlock, kHd == 64 ? 3 : 2) void PagedAttentionQ8Kernel(PagedAttentionQ8Args a)
 {
@@ -725,7 +732,7 @@ extern "C" int muyo_paged_attention_decode_q8kv(const float* q, const void* kcac
                             {vcache, cacheBytes, "vcache"},
                             {kscales, scaleBytes, "kscales"},
                             {vscales, scaleBytes, "vscales"}};
-    const AttentionCall call{q,       out,      tables,   sequences, table_pages, query_sequence, positions, queries, heads,
+    const AttentionCall call{q, out, tables, sequences, table_pages, query_sequence, positions, queries, heads,
                              kv_heads, head_dim, pages, page_size, scale, workspace, workspace_bytes,
                              muyo_paged_attention_decode_q8kv_workspace_bytes(queries, heads, kv_heads, head_dim)};
     const int checked = CheckAttention(name, call, caches, 4, 4);

@@ -39,7 +39,7 @@ struct PagedPrefixArgs
     const float* wholes;
     const uint4* cuts;
     const float* pieces;
-    float* partials;        // [kv_heads][queries * group][chunks][4 + headDim]: base, sum, a score's log2 units, -, values
+    float* partials;        // [kv_heads][queries * group][chunks][4 + headDim], as the own keys' partials
 };
 
 /// The prefix's keys, and the steps of a chunk of them.
@@ -142,8 +142,9 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
             const bool isV = i >= kMatrixLoads;
             const uint32_t first = (wave + i % kMatrixLoads * kWaves) * kRowsPerLoad;  // row of the step
             // The part is known up to the wave's half of 32 rows.
-            const uint32_t id = kHd == 128 ? ids.of[i % kMatrixLoads]
-                                           : (wave < 2 ? ids.of[2 * (i % kMatrixLoads)] : ids.of[2 * (i % kMatrixLoads) + 1]);
+            const int part = i % kMatrixLoads;
+            const uint32_t id =
+                kHd == 128 ? ids.of[part] : wave < 2 ? ids.of[2 * part] : ids.of[2 * part + 1];
             const uint32_t page = id < a.pages ? id : 0;  // read, and masked
             const uint32_t at = ((firstStep + step) * kStep + first) & (pageSize - 1);
             const uint16_t* base = (isV ? a.vcache : a.kcache) +
@@ -283,15 +284,16 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 #pragma unroll 1
         for (uint32_t first = 0; first < kStep; first += 32)
         {
-            const uint8_t* kTile = kRows + first * kRowBytes;
-            const uint8_t* vTile = vRows + first * kRowBytes;
+            const uint8_t* keys = kRows + first * kRowBytes;
+            const uint8_t* values = vRows + first * kRowBytes;
             __builtin_amdgcn_s_setprio(1);  // matrix work before the other wave's weights: 182 -> 180 us
             floatx16 score = floatx16{};
             floatx16 low = floatx16{};
 #pragma unroll
             for (int s = 0; s < kHd / 16; ++s)
             {
-                const half8 k = *reinterpret_cast<const half8*>(kTile + kRow * kRowBytes + ((2 * s + h) ^ (kRow & 7u)) * 16);
+                const half8 k = *reinterpret_cast<const half8*>(keys + kRow * kRowBytes +
+                                                                ((2 * s + h) ^ (kRow & 7u)) * 16);
                 low = Mfma(k, qlo[s], low);
                 score = Mfma(k, qhi[s], score);
             }
@@ -356,7 +358,7 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
                 {
-                    const uint8_t* at = vTile + vAt + 16 * s * kRowBytes + (vChunk ^ (4u * c)) * 16;
+                    const uint8_t* at = values + vAt + 16 * s * kRowBytes + (vChunk ^ (4u * c)) * 16;
                     const half4 one = __builtin_bit_cast(
                         half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                    (__attribute__((address_space(3))) short4v*)(const_cast<uint8_t*>(at))));
@@ -433,9 +435,9 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 /// which wait for memory, in turns of a CU each. The q of a workgroup may be read when others have ended, so none
 /// writes `out`.
 ///
-/// Two launches, the prefix's before the own keys', took 14.3 us for 3 queries (1009 keys and up to 100 own, 14 / 2 heads
-/// of 64), together 10.3; 64 queries (8190 and up to 2000, 28 / 4 of 128) 53 and 45; 250 (16381 and up to 500) 183 and
-/// 172. In turns of 8, 128 and 512 workgroups, or with the own keys first, 1 to 70 us more.
+/// Two launches, the prefix's before the own keys', took 14.3 us for 3 queries (1009 keys and up to 100 own, 14 / 2
+/// heads of 64), together 10.3; 64 queries (8190 and up to 2000, 28 / 4 of 128) 53 and 45; 250 (16381 and up to 500)
+/// 183 and 172. In turns of 8, 128 and 512 workgroups, or with the own keys first, 1 to 70 us more.
 template <int kHd, bool kSplit>
 __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a, PagedAttentionF16Args own,
                                                                uint32_t prefixBlocks, uint32_t ownBlocks)
@@ -445,7 +447,11 @@ __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kPrefixBytes<kHd>];
     __shared__ OwnKeysSpace space;
     const uint32_t turns = min(prefixBlocks, ownBlocks) / kTurn * kTurn;  // of each kind
-    uint32_t at = blockIdx.x;
+    uint32_t at = blockIdx.y * gridDim.x + blockIdx.x;
+    if (at >= prefixBlocks + ownBlocks)
+    {
+        return;
+    }
     bool isOwn;
     if (at < 2 * turns)
     {
@@ -509,6 +515,7 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
         const float* const from = a.partials +
                                   ((head / a.group) * rows + static_cast<uint64_t>(query) * a.group + head % a.group) *
                                       a.chunks * (kHd + 4);
+        const float* const whole = a.wholes + (static_cast<uint64_t>(query) * heads + head) * (kHd + 4);
         for (uint32_t p0 = slice; p0 < parts; p0 += kDeep * kSlices)
         {
             float4v of[kDeep], x[kDeep];
@@ -517,12 +524,12 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
             for (uint32_t i = 0; i < kDeep; ++i)
             {
                 const uint32_t p = min(p0 + i * kSlices, parts - 1);
-                const uint32_t own = p - prefix.chunks;  // piece 0 begins the own keys, the others are their shares' first
+                // Piece 0 begins the own keys, the others are their shares' first.
+                const uint32_t own = p - prefix.chunks;
+                const uint64_t piece = 2 * (first + own) + (own == 0 ? 1 : 0);
                 const float* at = p < prefix.chunks ? from + static_cast<uint64_t>(p) * (kHd + 4)
-                                  : pieces == 0     ? a.wholes + (static_cast<uint64_t>(query) * heads + head) * (kHd + 4)
-                                                    : a.pieces + (static_cast<uint64_t>(2 * (first + own) +
-                                                                                        (own == 0 ? 1 : 0)) * a.group +
-                                                                  head % a.group) * (kHd + 4);
+                                  : pieces == 0     ? whole
+                                                    : a.pieces + (piece * a.group + head % a.group) * (kHd + 4);
                 of[i] = *reinterpret_cast<const float4v*>(at);
                 x[i] = *reinterpret_cast<const float4v*>(at + 4 + 4 * lane);
             }
@@ -602,20 +609,25 @@ size_t WholeBytes(uint32_t queries, uint32_t heads, uint32_t headDim)
 template <int kHd>
 hipError_t LaunchPrefix(hipStream_t s, const PagedPrefixArgs& a, const PagedAttentionF16Args& own)
 {
-    const uint32_t prefixBlocks = a.kvHeads * a.chunks * CeilDiv(static_cast<uint64_t>(a.queries) * a.group, kRowsOfBlock);
+    const uint32_t rowBlocks = CeilDiv(static_cast<uint64_t>(a.queries) * a.group, kRowsOfBlock);
+    const uint32_t prefixBlocks = a.kvHeads * a.chunks * rowBlocks;
+    auto grid = [](uint32_t blocks) {  // a dimension's threads are below 2^32
+        constexpr uint32_t kMost = 1u << 23;
+        return dim3(std::min(blocks, kMost), CeilDiv(blocks, kMost));
+    };
     if (a.cuts != nullptr)
     {
         if (a.queries > kScanQueries)
         {
             hipLaunchKernelGGL(PagedCostSumsKernel<kTile>, dim3(1), dim3(1024), 0, s, own);
         }
-        hipLaunchKernelGGL((PagedPrefixKernel<kHd, true>), dim3(prefixBlocks + kSplitBlocks), dim3(kBlock), 0, s, a, own,
-                           prefixBlocks, kSplitBlocks);
+        hipLaunchKernelGGL((PagedPrefixKernel<kHd, true>), grid(prefixBlocks + kSplitBlocks), dim3(kBlock), 0, s, a,
+                           own, prefixBlocks, kSplitBlocks);
     }
     else
     {
         const uint32_t ownBlocks = a.queries * a.kvHeads;
-        hipLaunchKernelGGL((PagedPrefixKernel<kHd, false>), dim3(prefixBlocks + ownBlocks), dim3(kBlock), 0, s, a, own,
+        hipLaunchKernelGGL((PagedPrefixKernel<kHd, false>), grid(prefixBlocks + ownBlocks), dim3(kBlock), 0, s, a, own,
                            prefixBlocks, ownBlocks);
     }
     const uint64_t items = static_cast<uint64_t>(a.queries) * a.kvHeads * a.group;
@@ -660,7 +672,7 @@ extern "C" int muyo_paged_attention_prefix_f16kv(const float* q, const void* kca
     const char* name = "paged_attention_prefix_f16kv";
     const uint64_t cacheBytes = 2ull * pages * page_size * kv_heads * head_dim;
     const Range more[] = {{kcache, cacheBytes, "kcache"}, {vcache, cacheBytes, "vcache"}, {prefix, 8, "prefix"}};
-    const AttentionCall call{q,       out,      tables,   sequences, table_pages, query_sequence, positions, queries, heads,
+    const AttentionCall call{q, out, tables, sequences, table_pages, query_sequence, positions, queries, heads,
                              kv_heads, head_dim, pages, page_size, scale, workspace, workspace_bytes,
                              muyo_paged_attention_prefix_f16kv_workspace_bytes(queries, heads, kv_heads, head_dim)};
     const int checked = CheckAttention(name, call, more, 3, 2);
@@ -680,7 +692,8 @@ extern "C" int muyo_paged_attention_prefix_f16kv(const float* q, const void* kca
                             heads / kv_heads, kv_heads, prefix, pages, own.pageShift, scale,
                             PrefixChunks(queries, heads, kv_heads), own.wholes,
                             SplitKeys<kTile>(own) ? own.cuts : nullptr, own.partials,
-                            reinterpret_cast<float*>(behind + WholeBytes(queries, heads, head_dim) + CutBytes(queries, kv_heads))};
+                            reinterpret_cast<float*>(behind + WholeBytes(queries, heads, head_dim) +
+                                                     CutBytes(queries, kv_heads))};
     const hipError_t launched =
         head_dim == 64 ? LaunchPrefix<64>(AsStream(stream), a, own) : LaunchPrefix<128>(AsStream(stream), a, own);
     return launched == hipSuccess ? MUYO_OK : HipStatus(launched, name);

@@ -305,8 +305,8 @@ extern "C" int muyo_paged_rope_append_q8kv(const float* q, const float* k, const
                             {kscales, scaleBytes, "kscales"},
                             {vscales, scaleBytes, "vscales"}};
     const uint64_t items = static_cast<uint64_t>(tokens) * (heads + 2ull * kv_heads) * (head_dim / 8);
-    const AppendCall call{q,     k,        v,        q_stride, k_stride,  v_stride,    q_out,      positions, slots, tokens,
-                          heads, kv_heads, head_dim, pages,    page_size, rope_layout, rotary_dim, turns, magnitude, items};
+    const AppendCall call{q, k, v, q_stride, k_stride, v_stride, q_out, positions, slots, tokens, heads, kv_heads,
+                          head_dim, pages, page_size, rope_layout, rotary_dim, turns, magnitude, items};
     const int checked = CheckAppend(name, call, caches, 4);
     if (checked != MUYO_OK)
     {

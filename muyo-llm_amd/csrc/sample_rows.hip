@@ -167,8 +167,8 @@ __device__ __forceinline__ void AddOne(float v, double top, double perUnit, uint
     }
 }
 
-/// The same of a batch, for places below kFar, with fewer operations: a step is the last 32 bits of a place's sum with kWhole. Logits
-/// below `least`, past the last step, count as that, so that no place is far.
+/// The same of a batch, for places below kFar, with fewer operations: a step is the last 32 bits of a place's sum with
+/// kWhole. Logits below `least`, past the last step, count as that, so that no place is far.
 template <bool kCount, bool kMass>
 __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double top, float least, double perUnit,
                                              uint64_t* masses, uint32_t* counts)
@@ -1421,7 +1421,8 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
 #pragma unroll 1
                         for (uint32_t j = 0; j < kPickLoads; ++j)
                         {
-                            own[b] += i < here && at + j * kWave < end ? weightAt(r.x[at + j * kWave], at + j * kWave) : 0.0;
+                            const uint32_t here1 = at + j * kWave;
+                            own[b] += i < here && here1 < end ? weightAt(r.x[here1], here1) : 0.0;
                         }
                     }
                 }

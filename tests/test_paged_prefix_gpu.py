@@ -257,6 +257,43 @@ def test_past_four_gigabytes_of_cache(mh, gpu):
     batch.compare(host(out))
 
 
+def test_more_queries_than_are_scanned(mh, gpu):
+    """Shares whose sums a kernel of its own makes, and a last sequence that shares cut."""
+    rng = np.random.default_rng(21)
+    positions = rng.integers(-1, 60, 1300)
+    positions[[3, 700, 1299]] = [1400, 1100, 2047]
+    for heads, kv, hd in ((14, 2, 64), (28, 4, 128)):
+        batch = Shared(mh, gpu, rng, heads, kv, hd, 16, positions, 90)
+        batch.poison_unseen()
+        out = batch.call()
+        gpu.cuda.synchronize()
+        batch.compare(host(out), some=np.r_[:8, 700, rng.integers(0, 1300, 12), 1298, 1299])
+
+
+def test_the_largest_batch(mh, gpu):
+    """65535 queries of 264 heads: more workgroups than a dimension of a launch takes."""
+    torch, rng = gpu, np.random.default_rng(22)
+    heads, hd, n = 264, 64, 65535
+    small = np.array([5, 0, -1, 17, 30])
+    batch = Shared(mh, torch, rng, heads, heads, hd, 16, small, 20)
+    batch.poison_unseen()
+    batch.call()
+    batch.d[0] = torch.randn((n, heads, hd), device="cuda")
+    which = np.arange(n) % len(small)
+    some = np.r_[:6, 4095:4100, rng.integers(0, n, 6), n - 6:n]
+    batch.sequence, batch.positions = batch.sequence[which], batch.positions[which]
+    batch.d[4], batch.d[5] = (dev(torch, x.astype(np.int32)) for x in (batch.sequence, batch.positions))
+    batch.q = np.zeros((n, 1))
+    batch.nbytes = mh.load().muyo_paged_attention_prefix_f16kv_workspace_bytes(n, heads, heads, hd)
+    batch.space = torch.empty(batch.nbytes, dtype=torch.uint8, device="cuda")
+    out = batch.call(where=True)
+    torch.cuda.synchronize()
+    pick = torch.from_numpy(some).cuda()
+    batch.q, got = host(batch.d[0][pick]), host(out[pick])
+    batch.sequence, batch.positions = batch.sequence[some], batch.positions[some]
+    batch.compare(got)
+
+
 def test_a_steps_operators_in_one_graph(mh, gpu):
     """Plan, append, attention and sampling of chats that share a prompt, captured together and replayed: the prompt is
     a sequence of the plan with its own pages, the chats' rope positions go on behind it."""
