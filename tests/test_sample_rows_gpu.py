@@ -228,6 +228,26 @@ def test_a_large_vocabulary(mh, gpu):
     few.check()
 
 
+def test_the_largest_vocabulary(mh, gpu):
+    """2^24 logits, of a few values so that steps hold millions, and of as many as there are."""
+    rng = np.random.default_rng(8)
+    x = rng.normal(0, 1, (2, 2 ** 24)).astype(np.float32)
+    x[0] = np.round(x[0])
+    Batch(mh, gpu, x, [(1.0, 0, 0.97, 0.0), (1.0, 5000, 0.8, 0.0)], [0.6, 0.7]).check()
+
+
+@pytest.mark.parametrize("rows, vocab, stride", [(5, 5003, 2 ** 29 + 3), (4101, 700, 270001)])
+def test_rows_past_four_gigabytes(mh, gpu, rows, vocab, stride):
+    torch, rng = gpu, np.random.default_rng(rows)
+    settings = [SETTINGS[i] for i in rng.integers(0, len(SETTINGS), rows)]
+    x = logits_of(rng, 41, vocab)[rng.integers(0, 41, rows)]
+    batch = Batch(mh, torch, x, settings, rng.random(rows))
+    wide = torch.empty((rows - 1) * stride + vocab, device="cuda")
+    torch.as_strided(wide, (rows, vocab), (stride, 1)).copy_(batch.d[0])
+    batch.d[0], batch.stride = wide, stride
+    batch.check()
+
+
 def test_the_same_twice_and_on_other_streams(mh, gpu):
     torch, rng = gpu, np.random.default_rng(7)
     batches = []
