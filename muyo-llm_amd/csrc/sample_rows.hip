@@ -492,7 +492,7 @@ struct PickSpace
     unsigned long long partMass[kMaxParts];
     double partWeight[kMaxParts];
     unsigned long long low, high, sum;
-    uint32_t listed, active, few;
+    uint32_t listed, few;
     uint32_t stepK, stepP;
 };
 
@@ -651,17 +651,18 @@ struct Cut
 /// Of `n` items in falling order of their keys (which differ), those that have fewer than `most` before them and
 /// less than `limit` of mass: the last one's key, and their mass. item(i, key, mass) says whether there is one.
 ///
-/// Keys are taken apart into 256 equal ranges between the smallest and the largest, the range with the last one is
-/// found from counts and masses of all, and so on until a wave can look at the rest one by one.
+/// All keys are in low..high. That is taken apart into 256 equal ranges, the one with the last item is found from
+/// counts and masses of all, and so on between the smallest and the largest there, until a wave can look at the rest
+/// one by one.
 template <typename Item>
-__device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, uint64_t limit, PickSpace& s)
+__device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, uint64_t limit, uint64_t low,
+                                        uint64_t high, PickSpace& s)
 {
     const uint32_t lane = threadIdx.x % kWave;
-    uint64_t low = 0;
-    uint64_t high = ~0ull;
     uint32_t above = 0;
     uint64_t aboveMass = 0;
     bool few = n <= kFew;
+    bool narrow = true;  // the range is not worth a look for its ends
     while (true)
     {
         __syncthreads();
@@ -669,7 +670,6 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, ui
         {
             s.low = ~0ull;
             s.high = 0;
-            s.active = 0;
             s.few = 0;
         }
         for (uint32_t i = threadIdx.x; i < kDigits; i += kPickBlock)
@@ -678,11 +678,10 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, ui
             s.digitMasses[i] = 0;
         }
         __syncthreads();
-        if (!few)
+        if (!few && !narrow)
         {
             uint64_t least = ~0ull;
             uint64_t largest = 0;
-            uint32_t count = 0;
             for (uint32_t i = threadIdx.x; i < n; i += kPickBlock)
             {
                 uint64_t key, mass;
@@ -690,7 +689,6 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, ui
                 {
                     least = least < key ? least : key;
                     largest = largest > key ? largest : key;
-                    ++count;
                 }
             }
 #pragma unroll
@@ -700,23 +698,17 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, ui
                 const uint64_t h = __shfl_xor(static_cast<unsigned long long>(largest), step);
                 least = least < l ? least : l;
                 largest = largest > h ? largest : h;
-                count += __shfl_xor(count, step);
             }
-            if (lane == 0 && count > 0)
+            if (lane == 0 && least <= largest)
             {
                 atomicMin(&s.low, static_cast<unsigned long long>(least));
                 atomicMax(&s.high, static_cast<unsigned long long>(largest));
-                atomicAdd(&s.active, count);
             }
             __syncthreads();
             low = s.low;
             high = s.high;
-            if (s.active == 0)
-            {
-                return Cut{~0ull, aboveMass};
-            }
-            few = s.active <= kFew;
         }
+        narrow = false;
         if (few)
         {
             for (uint32_t i = threadIdx.x; i < n; i += kPickBlock)
@@ -785,6 +777,7 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, ui
         uint64_t massBefore =
             aboveMass + WaveInclusive(static_cast<unsigned long long>(massOfLane)) - massOfLane;
         uint32_t which = ~0u;
+        uint32_t ofIt = 0;
         uint32_t beforeIt = 0;
         uint64_t massBeforeIt = 0;
 #pragma unroll
@@ -793,6 +786,7 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, ui
             if (c[e] > 0 && before < most && massBefore < limit)
             {
                 which = lane * kPer + e;
+                ofIt = c[e];
                 beforeIt = before;
                 massBeforeIt = massBefore;
             }
@@ -806,6 +800,7 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, ui
         }
         const int owner = 63 - __clzll(static_cast<long long>(has));
         which = __shfl(which, owner);
+        few = __shfl(ofIt, owner) <= kFew;
         above = __shfl(beforeIt, owner);
         aboveMass = __shfl(static_cast<unsigned long long>(massBeforeIt), owner);
         high -= static_cast<uint64_t>(which) << shift;
@@ -1221,8 +1216,19 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         if (needed)
         {
             const uint64_t below = limit < 0x1p63 ? static_cast<uint64_t>(ceil(limit)) : ~0ull;
-            found = task == kToken || (listFirst <= of && of <= listLast) ? LastKept(s.listed, item, atMost, below, s)
-                                                                          : LastKeptOfRow(r, of, atMost, below, s);
+            // Of the token's search keys are indices, else those of the step's logits.
+            uint64_t low = static_cast<uint32_t>(~(a.vocab - 1));
+            uint64_t high = 0xFFFFFFFFull;
+            if (task != kToken)
+            {
+                float least, largest;
+                BoundsOf(r, of, of, least, largest);
+                low = static_cast<uint64_t>(OrderBits(least)) << 32;
+                high |= static_cast<uint64_t>(OrderBits(largest)) << 32;
+            }
+            found = task == kToken || (listFirst <= of && of <= listLast)
+                        ? LastKept(s.listed, item, atMost, below, low, high, s)
+                        : LastKeptOfRow(r, of, atMost, below, s);
         }
         if (task == kCutOfK)
         {
