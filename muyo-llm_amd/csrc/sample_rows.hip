@@ -37,6 +37,7 @@ constexpr uint32_t kCountBlocks = 1024;        // workgroups to aim at that coun
 constexpr uint32_t kFewestParts = 4;           // of a row, if it has the batches
 constexpr double kLog2e = 1.44269504088896340736;
 constexpr uint32_t kListRows = 4096;           // rows whose lists get workgroups of their own
+constexpr uint32_t kPickAtOnce = 256;          // rows that are decided at once: one on each CU
 constexpr uint32_t kListBatches = 2;           // batches that a wave of those looks through
 constexpr double kFar = 0x1p48;                // places past which steps are not whole numbers apart
 constexpr double kWhole = 0x1.8p52;            // added, the whole part's last 32 bits come last
@@ -58,7 +59,7 @@ struct RowSteps
     double top;
     uint32_t first, last;  // steps that are listed: none if first > last
     uint32_t listed;
-    uint32_t unused;
+    uint32_t walk;         // the list will not do: the token is looked for in the row
     uint64_t keys[kListed];
 };
 
@@ -649,19 +650,20 @@ struct Cut
 };
 
 /// Of `n` items in falling order of their keys (which differ), those that have fewer than `most` before them and
-/// less than `limit` of mass: the last one's key, and their mass. item(i, key, mass) says whether there is one.
+/// less than `limit` of mass: the last one's key, and their mass. item(i, key, mass) says whether there is one; there
+/// are `some` at most.
 ///
 /// All keys are in low..high. That is taken apart into 256 equal ranges, the one with the last item is found from
 /// counts and masses of all, and so on between the smallest and the largest there, until a wave can look at the rest
 /// one by one.
 template <typename Item>
-__device__ __forceinline__ Cut LastKept(uint32_t n, Item item, uint32_t most, uint64_t limit, uint64_t low,
-                                        uint64_t high, PickSpace& s)
+__device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, uint32_t most, uint64_t limit,
+                                        uint64_t low, uint64_t high, PickSpace& s)
 {
     const uint32_t lane = threadIdx.x % kWave;
     uint32_t above = 0;
     uint64_t aboveMass = 0;
-    bool few = n <= kFew;
+    bool few = min(n, some) <= kFew;
     bool narrow = true;  // the range is not worth a look for its ends
     while (true)
     {
@@ -882,10 +884,15 @@ template <PickPhase kPhase>
 __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
 {
     __shared__ PickSpace s;
-    const uint32_t row = blockIdx.x;
+    const uint32_t row = blockIdx.x % a.rows;
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = threadIdx.x / kWave;
     const uint64_t slot = static_cast<uint64_t>(row) * a.parts;
+    // In two turns, what takes longest is begun first.
+    if (kPhase == kPickToken && gridDim.x > a.rows && (a.steps[row].walk != 0) != (blockIdx.x < a.rows))
+    {
+        return;
+    }
 
     // Every wave looks at the parts, a lane each.
     static_assert(kMaxParts == kWave, "a lane for each part");
@@ -913,6 +920,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         kept->first = 1;
         kept->last = 0;
         kept->listed = 0;
+        kept->walk = 0;
     }
     if (kPhase == kPickSteps && (most == -INFINITY || mode.perUnit < 0.0))
     {
@@ -995,8 +1003,8 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         weight = static_cast<double>(mass) * s.unit[d];
         if (!mode.counted)
         {
-            // A bound: a logit's mass is at least 2^(-1/16) of a unit's.
-            count = static_cast<uint32_t>(static_cast<double>(mass) * (0x1p-38 * 1.0443)) + (mass != 0 ? 1u : 0u);
+            // A bound: a logit's mass is at least 2^(-3/32) of a unit's.
+            count = static_cast<uint32_t>(static_cast<double>(mass) * (0x1p-38 * 1.0672)) + (mass != 0 ? 1u : 0u);
         }
         StepSums(count, weight, s);
     }
@@ -1127,6 +1135,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
             {
                 kept->first = from;
                 kept->last = to;
+                kept->walk = (task == kCutOfAll ? all : from <= to) ? 0 : 1;
             }
             return;
         }
@@ -1217,9 +1226,17 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         {
             const uint64_t below = limit < 0x1p63 ? static_cast<uint64_t>(ceil(limit)) : ~0ull;
             // Of the token's search keys are indices, else those of the step's logits.
+            const uint32_t some = task != kToken ? countOf(of)
+                                  : mode.counted ? min(s.counts[of], static_cast<uint32_t>(mode.topK))
+                                                 : s.counts[of];
             uint64_t low = static_cast<uint32_t>(~(a.vocab - 1));
             uint64_t high = 0xFFFFFFFFull;
-            if (task != kToken)
+            if (task != kToken && min(s.listed, some) <= kFew)
+            {
+                low = 0;
+                high = ~0ull;
+            }
+            else if (task != kToken)
             {
                 float least, largest;
                 BoundsOf(r, of, of, least, largest);
@@ -1227,7 +1244,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                 high |= static_cast<uint64_t>(OrderBits(largest)) << 32;
             }
             found = task == kToken || (listFirst <= of && of <= listLast)
-                        ? LastKept(s.listed, item, atMost, below, low, high, s)
+                        ? LastKept(s.listed, some, item, atMost, below, low, high, s)
                         : LastKeptOfRow(r, of, atMost, below, s);
         }
         if (task == kCutOfK)
@@ -1704,7 +1721,8 @@ extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, ui
         hipLaunchKernelGGL(SamplePickKernel<kPickSteps>, dim3(rows), dim3(kPickBlock), 0, s, a);
         const uint32_t waves = CeilDiv(a.batches, kListBatches) * parts.count;
         hipLaunchKernelGGL(SampleListKernel, dim3(CeilDiv(waves, kWaves), rows), dim3(kBlock), 0, s, a);
-        hipLaunchKernelGGL(SamplePickKernel<kPickToken>, dim3(rows), dim3(kPickBlock), 0, s, a);
+        hipLaunchKernelGGL(SamplePickKernel<kPickToken>, dim3(rows > kPickAtOnce ? 2 * rows : rows), dim3(kPickBlock), 0,
+                           s, a);
     }
     else
     {

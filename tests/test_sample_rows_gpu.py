@@ -179,6 +179,15 @@ def test_equal_logits(mh, gpu, vocab, step):
     Batch(mh, gpu, x, settings, rng.random(len(settings))).check()
 
 
+@pytest.mark.parametrize("vocab", [61, 4000, 4096, 4150, 4300])
+def test_equal_logits_at_tiny_temperatures(mh, gpu, vocab):
+    """Places so far out that what a step leaves of them is any number: as many as a list holds, and more."""
+    rng = np.random.default_rng(vocab)
+    x = np.repeat(rng.normal(0, 3, (24, 1)), vocab, 1)
+    settings = [(1e-20, 0, 1.0, 0.0), (1e-18, 0, 0.9, 0.0), (1e-25, 4140, 1.0, 0.0), (1e-20, 0, 1.0, 0.5)] * 6
+    Batch(mh, gpu, x, settings, rng.random(24)).check()
+
+
 def test_masked_infinite_and_missing_logits(mh, gpu):
     rng = np.random.default_rng(4)
     vocab = 5000
