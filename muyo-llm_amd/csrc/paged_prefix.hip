@@ -69,14 +69,20 @@ template <int kHd>
 inline constexpr uint32_t kPrefixBytes = kPrefixStages<kHd> * 2 * kStep * 2 * kHd;
 
 /// A wave has 32 rows, the columns of its matrix operations; a workgroup's four waves share each step of 64 keys of K
-/// and V through LDS, where they go straight from memory a step ahead. Per 32 keys a wave
+/// and V through LDS, where they go straight from memory a step ahead. Per step a wave
 ///   - forms S^T (keys x rows) = K . q^T, K from LDS, q in registers as two planes of f16 (of q / 2^e, e by the row's
 ///     largest value, as in the attention over own keys: the two are joined by their raw scores);
-///   - makes the softmax weights of a row's 16 keys in a lane, one exchange with the lane 32 away, in two planes;
+///   - makes the softmax weights of a row's 32 keys in a lane, one exchange with the lane 32 away, in two planes;
 ///   - O^T (channels x rows) += V^T . P^T, V^T by transposing LDS reads, keys in the order that the scores have.
 /// The weights' low plane, times 2048, has sums of its own, so that small weights count beside a key that has most of
 /// the weight: at head_dim 64 accumulators beside the others, at 128, where these would not fit the registers, sums of
-/// the 32 keys that are added to the others by a multiply-add.
+/// the step that are added to the others by a multiply-add.
+///
+/// What bounds it: vector and matrix work, which a SIMD's two waves overlap little. 250 queries of 28 / 4 heads of 128
+/// with 16381 keys: 140 us, the vector units busy for 69 of them and the matrix cores for 48. 32 keys at a time took 2 %
+/// more; one wave a SIMD, with the next step's matrix operations between this one's weights, 200 us; other orders of
+/// the chunks in LDS, with fewer bank conflicts (0.4 of its time), and a wave's priority in either kind of work, no
+/// less.
 ///
 /// Steps that reach past the prefix, or into a page that is not there, are masked: scores to -inf, and V's rows to 0 in
 /// LDS, since 0 * NaN would be NaN.
@@ -94,6 +100,7 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
     constexpr int kMatrixLoads = kMatrixBytes / 1024 / kWaves;  // of a wave
     constexpr int kLoads = 2 * kMatrixLoads;
     constexpr int kChannels = kHd / 32;                  // 32-channel blocks of the output
+    constexpr int kHalves = kStep / 32;                  // matrix operands of 32 keys
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t h = lane / 32;
@@ -281,108 +288,100 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
         {
             continue;
         }
-#pragma unroll 1
-        for (uint32_t first = 0; first < kStep; first += 32)
+        floatx16 score[kHalves];
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half)
         {
-            const uint8_t* keys = kRows + first * kRowBytes;
-            const uint8_t* values = vRows + first * kRowBytes;
-            __builtin_amdgcn_s_setprio(1);  // matrix work before the other wave's weights: 182 -> 180 us
-            floatx16 score = floatx16{};
-            floatx16 low = floatx16{};
+            const uint8_t* keys = kRows + half * 32 * kRowBytes;
+            score[half] = floatx16{};
 #pragma unroll
             for (int s = 0; s < kHd / 16; ++s)
             {
                 const half8 k = *reinterpret_cast<const half8*>(keys + kRow * kRowBytes +
                                                                 ((2 * s + h) ^ (kRow & 7u)) * 16);
-                low = Mfma(k, qlo[s], low);
-                score = Mfma(k, qhi[s], score);
+                score[half] = Mfma(k, qlo[s], score[half]);
+                score[half] = Mfma(k, qhi[s], score[half]);
             }
-            __builtin_amdgcn_s_setprio(0);
-            score += low;
             if (!inside)
             {
-                const bool there0 = (first == 0 ? now.of[0] : now.of[2]) < a.pages;
-                const bool there1 = (first == 0 ? now.of[1] : now.of[3]) < a.pages;
+                const bool there0 = now.of[2 * half] < a.pages;
+                const bool there1 = now.of[2 * half + 1] < a.pages;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                 {
-                    const uint32_t key = key0 + first + 8 * (r / 4) + 4 * h + r % 4;
+                    const uint32_t key = key0 + 32 * half + 8 * (r / 4) + 4 * h + r % 4;
                     if (key >= prefix.keys || !(r < 8 ? there0 : there1))
                     {
-                        score[r] = -INFINITY;
+                        score[half][r] = -INFINITY;
                     }
                 }
             }
-            float tileMax = -INFINITY;
+        }
+        float stepMax = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-            {
-                tileMax = fmaxf(tileMax, score[r]);
-            }
-            tileMax = fmaxf(tileMax, PartnerLane<32>(tileMax));
-            const bool rises =
-                tileMax != -INFINITY && (base == -INFINITY || (tileMax - base) * scaleLog2 > kPrefixLag);
-            if (__any(rises))
-            {
-                const float factor =
-                    rises ? (base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((base - tileMax) * scaleLog2)) : 1.0f;
-                base = rises ? tileMax : base;
-                runSum *= factor;
-#pragma unroll
-                for (int c = 0; c < kChannels; ++c)
-                {
-                    o[c] *= factor;
-                    if (kKeepLow)
-                    {
-                        oLow[c] *= factor;
-                    }
-                }
-            }
-            const float from = base == -INFINITY ? 0.0f : base;  // without keys so far every score is -inf
-            half8 phi[2], plo[2];
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-            {
-                const float p = __builtin_amdgcn_exp2f(fmaf(score[r] - from, scaleLog2, kPrefixBias));
-                sum[r % 4] += p;
-                const _Float16 hi = static_cast<_Float16>(p);
-                phi[r / 8][r % 8] = hi;
-                plo[r / 8][r % 8] = static_cast<_Float16>(kPrefixLowScale * (p - static_cast<float>(hi)));
-            }
-            runSum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        for (int r = 0; r < 16; ++r)
+        {
+            stepMax = fmaxf(stepMax, fmaxf(score[0][r], score[1][r]));
+        }
+        stepMax = fmaxf(stepMax, PartnerLane<32>(stepMax));
+        const bool rises = stepMax != -INFINITY && (base == -INFINITY || (stepMax - base) * scaleLog2 > kPrefixLag);
+        if (__any(rises))
+        {
+            const float factor =
+                rises ? (base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((base - stepMax) * scaleLog2)) : 1.0f;
+            base = rises ? stepMax : base;
+            runSum *= factor;
 #pragma unroll
             for (int c = 0; c < kChannels; ++c)
             {
-                half8 vt[2];
-#pragma unroll
-                for (int s = 0; s < 2; ++s)
-                {
-                    const uint8_t* at = values + vAt + 16 * s * kRowBytes + (vChunk ^ (4u * c)) * 16;
-                    const half4 one = __builtin_bit_cast(
-                        half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                   (__attribute__((address_space(3))) short4v*)(const_cast<uint8_t*>(at))));
-                    const half4 two = __builtin_bit_cast(
-                        half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
-                                   const_cast<uint8_t*>(at + 8 * kRowBytes))));
-                    vt[s] = __builtin_shufflevector(one, two, 0, 1, 2, 3, 4, 5, 6, 7);
-                }
-                floatx16 add = kKeepLow ? oLow[c] : floatx16{};
-                add = Mfma(vt[0], plo[0], add);
-                add = Mfma(vt[1], plo[1], add);
-                o[c] = Mfma(vt[0], phi[0], o[c]);
-                o[c] = Mfma(vt[1], phi[1], o[c]);
+                o[c] *= factor;
                 if (kKeepLow)
                 {
-                    oLow[c] = add;
+                    oLow[c] *= factor;
                 }
-                else
-                {
+            }
+        }
+        const float from = base == -INFINITY ? 0.0f : base;  // without keys so far every score is -inf
+        half8 phi[2 * kHalves], plo[2 * kHalves];
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                    {
-                        o[c][r] = fmaf(add[r], 1.0f / kPrefixLowScale, o[c][r]);
-                    }
+        for (int i = 0; i < 16 * kHalves; ++i)
+        {
+            const float p = __builtin_amdgcn_exp2f(fmaf(score[i / 16][i % 16] - from, scaleLog2, kPrefixBias));
+            sum[i % 4] += p;
+            const _Float16 hi = static_cast<_Float16>(p);
+            phi[i / 8][i % 8] = hi;
+            plo[i / 8][i % 8] = static_cast<_Float16>(kPrefixLowScale * (p - static_cast<float>(hi)));
+        }
+        runSum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int c = 0; c < kChannels; ++c)
+        {
+            floatx16 add = kKeepLow ? oLow[c] : floatx16{};
+#pragma unroll
+            for (int s = 0; s < 2 * kHalves; ++s)
+            {
+                const uint8_t* at = vRows + vAt + 16 * s * kRowBytes + (vChunk ^ (4u * c)) * 16;
+                const half4 one = __builtin_bit_cast(
+                    half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                               (__attribute__((address_space(3))) short4v*)(const_cast<uint8_t*>(at))));
+                const half4 two = __builtin_bit_cast(
+                    half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
+                               const_cast<uint8_t*>(at + 8 * kRowBytes))));
+                const half8 vt = __builtin_shufflevector(one, two, 0, 1, 2, 3, 4, 5, 6, 7);
+                add = Mfma(vt, plo[s], add);
+                o[c] = Mfma(vt, phi[s], o[c]);
+            }
+            if (kKeepLow)
+            {
+                oLow[c] = add;
+            }
+            else
+            {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                {
+                    o[c][r] = fmaf(add[r], 1.0f / kPrefixLowScale, o[c][r]);
                 }
             }
         }
