@@ -9,6 +9,8 @@ namespace muyo
 {
 namespace
 {
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
 constexpr uint32_t kStep = 64;            // keys of one step: an LDS buffer of K and V rows
 constexpr uint32_t kStepPages = kStep / 16;
 constexpr uint32_t kRowsOfWave = 32;      // rows are (query, head of a kv head's group)
@@ -345,13 +347,24 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
         half8 phi[2 * kHalves], plo[2 * kHalves];
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 16 * kHalves; ++i)
+        for (int i = 0; i < 16 * kHalves; i += 2)
         {
-            const float p = __builtin_amdgcn_exp2f(fmaf(score[i / 16][i % 16] - from, scaleLog2, kPrefixBias));
-            sum[i % 4] += p;
-            const _Float16 hi = static_cast<_Float16>(p);
-            phi[i / 8][i % 8] = hi;
-            plo[i / 8][i % 8] = static_cast<_Float16>(kPrefixLowScale * (p - static_cast<float>(hi)));
+            float p[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                p[e] = __builtin_amdgcn_exp2f(fmaf(score[i / 16][i % 16 + e] - from, scaleLog2, kPrefixBias));
+                sum[(i + e) % 4] += p[e];
+            }
+            // The high plane is cut off, the low one has what that leaves: one operation a pair and one a weight.
+            const half2v hi = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(p[0], p[1]));
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+            {
+                phi[i / 8][i % 8 + e] = hi[e];
+                plo[i / 8][i % 8 + e] = static_cast<_Float16>(
+                    fmaf(static_cast<float>(hi[e]), -kPrefixLowScale, kPrefixLowScale * p[e]));
+            }
         }
         runSum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
