@@ -81,10 +81,10 @@ inline constexpr uint32_t kPrefixBytes = kPrefixStages<kHd> * 2 * kStep * 2 * kH
 /// the step that are added to the others by a multiply-add.
 ///
 /// What bounds it: vector and matrix work, which a SIMD's two waves overlap little. 250 queries of 28 / 4 heads of 128
-/// with 16381 keys: 140 us, the vector units busy for 69 of them and the matrix cores for 48. 32 keys at a time took 2 %
-/// more; one wave a SIMD, with the next step's matrix operations between this one's weights, 200 us; other orders of
-/// the chunks in LDS, with fewer bank conflicts (0.4 of its time), and a wave's priority in either kind of work, no
-/// less.
+/// with 16381 keys: 121 us, of which at 2.4 GHz the vector units are busy for 45 and the matrix cores for 44 (the
+/// clock is below that here). 32 keys at a time took 2 % more, without V's reads ahead of the weights 2 to 4; one wave
+/// a SIMD, with the next step's matrix operations between this one's weights, 200 us; other orders of the chunks in
+/// LDS, with fewer bank conflicts (0.4 of its time), and a wave's priority in either kind of work, no less.
 ///
 /// Steps that reach past the prefix, or into a page that is not there, are masked: scores to -inf, and V's rows to 0 in
 /// LDS, since 0 * NaN would be NaN.
@@ -319,6 +319,24 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
                 }
             }
         }
+        // V of 32 channels, transposed; the first are on their way while the weights are made.
+        auto valuesOf = [&](int c, half8 (&vt)[2 * kHalves]) {
+#pragma unroll
+            for (int s = 0; s < 2 * kHalves; ++s)
+            {
+                const uint8_t* at = vRows + vAt + 16 * s * kRowBytes + (vChunk ^ (4u * c)) * 16;
+                const half4 one = __builtin_bit_cast(
+                    half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                               (__attribute__((address_space(3))) short4v*)(const_cast<uint8_t*>(at))));
+                const half4 two = __builtin_bit_cast(
+                    half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
+                               const_cast<uint8_t*>(at + 8 * kRowBytes))));
+                vt[s] = __builtin_shufflevector(one, two, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        };
+        half8 vt[2 * kHalves];
+        valuesOf(0, vt);
+        __builtin_amdgcn_sched_barrier(0);
         float stepMax = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -370,20 +388,22 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 #pragma unroll
         for (int c = 0; c < kChannels; ++c)
         {
+            half8 later[2 * kHalves];
+            if (c + 1 < kChannels)
+            {
+                valuesOf(c + 1, later);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             floatx16 add = kKeepLow ? oLow[c] : floatx16{};
 #pragma unroll
             for (int s = 0; s < 2 * kHalves; ++s)
             {
-                const uint8_t* at = vRows + vAt + 16 * s * kRowBytes + (vChunk ^ (4u * c)) * 16;
-                const half4 one = __builtin_bit_cast(
-                    half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                               (__attribute__((address_space(3))) short4v*)(const_cast<uint8_t*>(at))));
-                const half4 two = __builtin_bit_cast(
-                    half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(
-                               const_cast<uint8_t*>(at + 8 * kRowBytes))));
-                const half8 vt = __builtin_shufflevector(one, two, 0, 1, 2, 3, 4, 5, 6, 7);
-                add = Mfma(vt, plo[s], add);
-                o[c] = Mfma(vt, phi[s], o[c]);
+                add = Mfma(vt[s], plo[s], add);
+                o[c] = Mfma(vt[s], phi[s], o[c]);
+                if (c + 1 < kChannels)
+                {
+                    vt[s] = later[s];
+                }
             }
             if (kKeepLow)
             {
