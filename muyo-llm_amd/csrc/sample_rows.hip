@@ -132,23 +132,56 @@ __device__ __forceinline__ Place PlaceOf(float x, double perUnit)
 }
 
 /// 2^(rest / 8) in units of 2^-38, by a polynomial (the fit of least error over half a step each way: 2^-41.6), to
-/// a whole number by 2^52, whose bits then go.
+/// a whole number by 2^52, whose bits then go. kCount side by side.
+template <int kCount>
+__device__ __forceinline__ void MassesOf(const double (&rest)[kCount], uint64_t (&mass)[kCount])
+{
+    constexpr double kOne = 0x1p38;
+    constexpr double c0 = 4.069392558613428e-08 * kOne;
+    constexpr double c1 = 2.3483963990465326e-06 * kOne;
+    constexpr double c2 = 0.00010840646184941278 * kOne;
+    constexpr double c3 = 0.0037535391505790455 * kOne;
+    constexpr double c4 = 0.08664339757000515 * kOne;
+    constexpr double c5 = 1.0000000000002864 * kOne + 0x1p52;
+    // As it stands, with the summands in scalar registers: the compiler would take the form that overwrites its summand,
+    // and copy each first.
+    double m[kCount];
+    if constexpr (kCount == 4)
+    {
+        asm("v_fma_f64 %0, %8, %4, %9\n\tv_fma_f64 %1, %8, %5, %9\n\t"
+            "v_fma_f64 %2, %8, %6, %9\n\tv_fma_f64 %3, %8, %7, %9\n\t"
+            "v_fma_f64 %0, %0, %4, %10\n\tv_fma_f64 %1, %1, %5, %10\n\t"
+            "v_fma_f64 %2, %2, %6, %10\n\tv_fma_f64 %3, %3, %7, %10\n\t"
+            "v_fma_f64 %0, %0, %4, %11\n\tv_fma_f64 %1, %1, %5, %11\n\t"
+            "v_fma_f64 %2, %2, %6, %11\n\tv_fma_f64 %3, %3, %7, %11\n\t"
+            "v_fma_f64 %0, %0, %4, %12\n\tv_fma_f64 %1, %1, %5, %12\n\t"
+            "v_fma_f64 %2, %2, %6, %12\n\tv_fma_f64 %3, %3, %7, %12\n\t"
+            "v_fma_f64 %0, %0, %4, %13\n\tv_fma_f64 %1, %1, %5, %13\n\t"
+            "v_fma_f64 %2, %2, %6, %13\n\tv_fma_f64 %3, %3, %7, %13"
+            : "=&v"(m[0]), "=&v"(m[1]), "=&v"(m[2]), "=&v"(m[3])
+            : "v"(rest[0]), "v"(rest[1]), "v"(rest[2]), "v"(rest[3]), "v"(c0), "s"(c1), "s"(c2), "s"(c3), "s"(c4),
+              "s"(c5));
+    }
+    else
+    {
+        static_assert(kCount == 1, "one, or four");
+        asm("v_fma_f64 %0, %2, %1, %3\n\tv_fma_f64 %0, %0, %1, %4\n\tv_fma_f64 %0, %0, %1, %5\n\t"
+            "v_fma_f64 %0, %0, %1, %6\n\tv_fma_f64 %0, %0, %1, %7"
+            : "=&v"(m[0])
+            : "v"(rest[0]), "v"(c0), "s"(c1), "s"(c2), "s"(c3), "s"(c4), "s"(c5));
+    }
+#pragma unroll
+    for (int e = 0; e < kCount; ++e)
+    {
+        mass[e] = static_cast<uint64_t>(__double_as_longlong(m[e])) & 0xFFFFFFFFFFFFFull;
+    }
+}
+
 __device__ __forceinline__ uint64_t MassOf(double rest)
 {
-    // As it stands: the compiler would take the form that overwrites its summand, and copy each constant first.
-    auto add = [](double x, double y, double z) {
-        double d;
-        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(x), "v"(y), "v"(z));
-        return d;
-    };
-    constexpr double kOne = 0x1p38;
-    double s = 4.069392558613428e-08 * kOne;
-    s = add(s, rest, 2.3483963990465326e-06 * kOne);
-    s = add(s, rest, 0.00010840646184941278 * kOne);
-    s = add(s, rest, 0.0037535391505790455 * kOne);
-    s = add(s, rest, 0.08664339757000515 * kOne);
-    s = add(s, rest, 1.0000000000002864 * kOne + 0x1p52);
-    return static_cast<uint64_t>(__double_as_longlong(s)) & 0xFFFFFFFFFFFFFull;
+    uint64_t mass[1];
+    MassesOf<1>({rest}, mass);
+    return mass[0];
 }
 
 /// Weight of a unit of mass in step d, relative to the top's.
@@ -181,17 +214,23 @@ __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double 
         // Four at a time, side by side up to the counters.
         uint32_t step[4];
         uint64_t mass[4];
+        double rest[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
             // The smaller of a signalling NaN and a number is a quiet NaN, the larger of that and a number the number.
             float x;
-            asm("v_min_f32 %0, %1, %2" : "=v"(x) : "v"(v[q][e]), "v"(0x1.fffffep127f));
-            asm("v_max_f32 %0, %1, %2" : "=v"(x) : "v"(x), "v"(least));
+            asm("v_min_f32 %0, %2, %1\n\tv_max_f32 %0, %0, %3"
+                : "=&v"(x)
+                : "v"(v[q][e]), "s"(0x1.fffffep127f), "v"(least));
             const double y = static_cast<double>(x);
             const double whole = WholeOf(y, perUnit);
             step[e] = topStep - static_cast<uint32_t>(__double_as_longlong(whole));
-            mass[e] = kMass ? MassOf(fma(y, perUnit, -(whole - kWhole))) : 0;
+            rest[e] = fma(y, perUnit, -(whole - kWhole));
+        }
+        if (kMass)
+        {
+            MassesOf<4>(rest, mass);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
