@@ -154,6 +154,25 @@ def test_logits_that_begin_anywhere(mh, gpu, shift):
         batch.check()
 
 
+def test_results_between_rows_of_logits(mh, gpu):
+    torch, rng = gpu, np.random.default_rng(11)
+    rows, vocab = 22, 4999
+    batch = Batch(mh, torch, logits_of(rng, rows, vocab), SETTINGS, rng.random(rows), stride=vocab + 60)
+    wide = batch.d[0].flatten()
+    before = host(wide).copy()
+    first, second = vocab + 2, 3 * (vocab + 60) + vocab + 1
+    batch.tokens, batch.logprobs = wide[first:first + rows].view(torch.int32), wide[second:second + rows]
+    batch.call()
+    torch.cuda.synchronize()
+    after = host(wide)
+    changed = np.flatnonzero(after.view(np.uint32) != before.view(np.uint32))
+    assert np.isin(changed, np.r_[first:first + rows, second:second + rows]).all()
+    for r in range(rows):
+        token, lp = sample64(batch.logits[r], SETTINGS[r], batch.randoms[r])
+        assert after[first + r].view(np.int32) == token
+        assert abs(after[second + r] - lp) <= 2 * U * max(1.0, abs(lp))
+
+
 def test_settings_that_are_off(mh, gpu):
     rng = np.random.default_rng(2)
     settings = [(0.6, 9, 0.8, 0.1)] * 8
