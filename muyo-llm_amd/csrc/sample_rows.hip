@@ -105,6 +105,75 @@ __device__ __forceinline__ RowMode ModeOf(const SampleArgs& a, uint32_t row)
     return mode;
 }
 
+/// move(word) of each 32-bit word of v.
+template <typename T, typename Move>
+__device__ __forceinline__ T ByWords(T v, Move move)
+{
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "words");
+    if constexpr (sizeof(T) == 4)
+    {
+        return __builtin_bit_cast(T, move(__builtin_bit_cast(int, v)));
+    }
+    else
+    {
+        const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+        const uint32_t low = static_cast<uint32_t>(move(static_cast<int>(static_cast<uint32_t>(bits))));
+        const uint32_t high = static_cast<uint32_t>(move(static_cast<int>(static_cast<uint32_t>(bits >> 32))));
+        return __builtin_bit_cast(T, static_cast<uint64_t>(high) << 32 | low);
+    }
+}
+
+/// The same of all of a wave's lanes: join(a, b) of all, in pairs, pairs of pairs and so on.
+template <typename T, typename Join>
+__device__ __forceinline__ T WaveJoin(T v, Join join)
+{
+    v = join(v, ByWords(v, [](int w) { return PartnerLane<1>(w); }));
+    v = join(v, ByWords(v, [](int w) { return PartnerLane<2>(w); }));
+    v = join(v, ByWords(v, [](int w) { return PartnerLane<4>(w); }));
+    v = join(v, ByWords(v, [](int w) { return PartnerLane<8>(w); }));
+    v = join(v, ByWords(v, [](int w) { return PartnerLane<16>(w); }));
+    return join(v, ByWords(v, [](int w) { return PartnerLane<32>(w); }));
+}
+
+template <typename T>
+__device__ __forceinline__ T WaveSum(T v)
+{
+    return WaveJoin(v, [](T a, T b) { return a + b; });
+}
+
+/// The smallest of a wave's values.
+template <typename T>
+__device__ __forceinline__ T WaveLeast(T v)
+{
+    return WaveJoin(v, [](T a, T b) { return a < b ? a : b; });
+}
+
+/// v plus that of the lane a DPP control names, in the given rows of 16 lanes; 0 from no lane.
+template <int kControl, int kRows, typename T>
+__device__ __forceinline__ T PlusLane(T v)
+{
+    return v + ByWords(v, [](int w) { return __builtin_amdgcn_update_dpp(0, w, kControl, kRows, 0xF, false); });
+}
+
+/// Inclusive sum over the wave's lanes: shifts inside rows of 16 lanes, then the last lanes of rows to those behind.
+template <typename T>
+__device__ __forceinline__ T WaveInclusive(T v)
+{
+    v = PlusLane<0x111, 0xF>(v);  // row_shr:1
+    v = PlusLane<0x112, 0xF>(v);
+    v = PlusLane<0x114, 0xF>(v);
+    v = PlusLane<0x118, 0xF>(v);
+    v = PlusLane<0x142, 0xA>(v);     // row_bcast:15
+    return PlusLane<0x143, 0xC>(v);  // row_bcast:31
+}
+
+/// A lane's value, the lane the same in the whole wave.
+template <typename T>
+__device__ __forceinline__ T OfLane(T v, int lane)
+{
+    return ByWords(v, [&](int w) { return __builtin_amdgcn_readlane(w, lane); });
+}
+
 /// A logit as it counts: -inf for NaN (the larger of a NaN and a number is the number), the largest finite one for
 /// +inf.
 __device__ __forceinline__ float Counted(float x) { return fminf(fmaxf(x, -INFINITY), 0x1.fffffep127f); }
@@ -431,11 +500,7 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
         // The wave's largest and its first place.
         const float waveMost = GroupMax<kWave>(most);
         at = most == waveMost && most > -INFINITY ? at : ~0u;
-#pragma unroll
-        for (int step = 1; step < kWave; step *= 2)
-        {
-            at = min(at, static_cast<uint32_t>(__shfl_xor(at, step)));
-        }
+        at = WaveLeast(at);
         most = waveMost;
     }
     if (lane == 0)
@@ -488,30 +553,6 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
             a.counts[slot * kSteps + i] = count;
         }
     }
-}
-
-template <typename T>
-__device__ __forceinline__ T WaveInclusive(T v)
-{
-    const uint32_t lane = threadIdx.x % kWave;
-#pragma unroll
-    for (int step = 1; step < kWave; step *= 2)
-    {
-        const T other = __shfl_up(v, step);
-        v += lane >= static_cast<uint32_t>(step) ? other : T{};
-    }
-    return v;
-}
-
-template <typename T>
-__device__ __forceinline__ T WaveSum(T v)
-{
-#pragma unroll
-    for (int step = 1; step < kWave; step *= 2)
-    {
-        v += __shfl_xor(v, step);
-    }
-    return v;
 }
 
 struct PickSpace
@@ -732,14 +773,8 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, ui
                     largest = largest > key ? largest : key;
                 }
             }
-#pragma unroll
-            for (int step = 1; step < kWave; step *= 2)
-            {
-                const uint64_t l = __shfl_xor(static_cast<unsigned long long>(least), step);
-                const uint64_t h = __shfl_xor(static_cast<unsigned long long>(largest), step);
-                least = least < l ? least : l;
-                largest = largest > h ? largest : h;
-            }
+            least = WaveLeast(least);
+            largest = ~WaveLeast(~largest);
             if (lane == 0 && least <= largest)
             {
                 atomicMin(&s.low, static_cast<unsigned long long>(least));
@@ -776,16 +811,14 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, ui
                 massBefore += is ? s.fewMasses[j] : 0;
             }
             const bool kept = lane < count && before < most && massBefore < limit;
-            Cut last{kept ? key : ~0ull, kept ? massBefore + mass : aboveMass};
-#pragma unroll
-            for (int step = 1; step < kWave; step *= 2)
+            // The last one kept is the smallest of them.
+            const uint64_t last = WaveLeast(kept ? key : ~0ull);
+            const uint64_t is = __ballot(kept && key == last);
+            if (is == 0)
             {
-                const uint64_t k = __shfl_xor(static_cast<unsigned long long>(last.key), step);
-                const uint64_t m = __shfl_xor(static_cast<unsigned long long>(last.mass), step);
-                last.mass = k < last.key ? m : last.mass;
-                last.key = k < last.key ? k : last.key;
+                return Cut{~0ull, aboveMass};
             }
-            return last;
+            return Cut{last, OfLane(massBefore + mass, __ffsll(static_cast<unsigned long long>(is)) - 1)};
         }
         const int bits = 64 - __clzll(static_cast<long long>(high - low));
         const int shift = max(bits - 8, 0);
@@ -816,7 +849,7 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, ui
         }
         uint32_t before = above + WaveInclusive(ofLane) - ofLane;
         uint64_t massBefore =
-            aboveMass + WaveInclusive(static_cast<unsigned long long>(massOfLane)) - massOfLane;
+            aboveMass + WaveInclusive(massOfLane) - massOfLane;
         uint32_t which = ~0u;
         uint32_t ofIt = 0;
         uint32_t beforeIt = 0;
@@ -840,10 +873,10 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, ui
             return Cut{~0ull, aboveMass};
         }
         const int owner = 63 - __clzll(static_cast<long long>(has));
-        which = __shfl(which, owner);
-        few = __shfl(ofIt, owner) <= kFew;
-        above = __shfl(beforeIt, owner);
-        aboveMass = __shfl(static_cast<unsigned long long>(massBeforeIt), owner);
+        which = OfLane(which, owner);
+        few = OfLane(ofIt, owner) <= kFew;
+        above = OfLane(beforeIt, owner);
+        aboveMass = OfLane(massBeforeIt, owner);
         high -= static_cast<uint64_t>(which) << shift;
         const uint64_t span = (1ull << shift) - 1;
         low = high - low > span ? high - span : low;
@@ -947,11 +980,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     }
     const float most = GroupMax<kWave>(head.most);
     double top = head.top;
-#pragma unroll
-    for (int step = 1; step < kWave; step *= 2)
-    {
-        top = fmax(top, __shfl_xor(top, step));
-    }
+    top = WaveJoin(top, [](double x, double y) { return fmax(x, y); });
     RowSteps* const kept = kPhase == kPickAll ? nullptr : a.steps + row;
     if (kPhase == kPickSteps && threadIdx.x == 0)
     {
@@ -968,11 +997,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     if (most == -INFINITY || mode.perUnit < 0.0)
     {
         uint32_t at = head.most == most ? head.at : ~0u;
-#pragma unroll
-        for (int step = 1; step < kWave; step *= 2)
-        {
-            at = min(at, static_cast<uint32_t>(__shfl_xor(at, step)));
-        }
+        at = WaveLeast(at);
         if (threadIdx.x == 0)
         {
             a.tokens[row] = most == -INFINITY ? -1 : static_cast<int32_t>(at);
@@ -1251,7 +1276,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                 uint64_t key, fixed;
                 sum += item(i, key, fixed) ? fixed : 0;
             }
-            sum = WaveSum(static_cast<unsigned long long>(sum));
+            sum = WaveSum(sum);
             if (lane == 0 && sum != 0)
             {
                 atomicAdd(&s.sum, static_cast<unsigned long long>(sum));
@@ -1489,20 +1514,12 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                     }
                 }
 #pragma unroll
-                for (int step = 1; step < kWave; step *= 2)
-                {
-#pragma unroll
-                    for (uint32_t b = 0; b < kAtOnce; ++b)
-                    {
-                        own[b] += __shfl_xor(own[b], step);
-                    }
-                }
-#pragma unroll
                 for (uint32_t b = 0; b < kAtOnce; ++b)
                 {
+                    const double ofGroup = WaveSum(own[b]);
                     if (lane == 0 && i0 + b * kPickWaves < here)
                     {
-                        s.groupWeights[i0 + b * kPickWaves] = own[b];
+                        s.groupWeights[i0 + b * kPickWaves] = ofGroup;
                     }
                 }
             }
@@ -1519,10 +1536,10 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                     const int which = over != 0 ? __ffsll(static_cast<unsigned long long>(over)) - 1
                                                 : 63 - __clzll(static_cast<long long>(kept));
                     group = first + i0 + which;
-                    passed = sum + __shfl(upToGroup - ofGroup, which);
+                    passed = sum + OfLane(upToGroup - ofGroup, which);
                 }
                 past = over != 0;
-                sum += __shfl(upToGroup, kWave - 1);
+                sum += OfLane(upToGroup, kWave - 1);
             }
         }
         if (wave != 0)
@@ -1544,13 +1561,13 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                 const int which = over != 0 ? __ffsll(static_cast<unsigned long long>(over)) - 1
                                             : 63 - __clzll(static_cast<long long>(kept));
                 index = first + j * kWave + which;
-                ofToken = __shfl(own, which);
+                ofToken = OfLane(own, which);
             }
             if (over != 0)
             {
                 break;
             }
-            passed += __shfl(upToOwn, kWave - 1);
+            passed += OfLane(upToOwn, kWave - 1);
         }
         writes = lane == 0;
     }
