@@ -200,10 +200,10 @@ __device__ __forceinline__ Place PlaceOf(float x, double perUnit)
     return at;
 }
 
-/// 2^(rest / 8) in units of 2^-38, by a polynomial (the fit of least error over half a step each way: 2^-41.6), to
-/// a whole number by 2^52, whose bits then go. kCount side by side.
+/// 2^52 and 2^(rest / 8) in units of 2^-38, by a polynomial (the fit of least error over half a step each way:
+/// 2^-41.6), to a whole number. kCount side by side.
 template <int kCount>
-__device__ __forceinline__ void MassesOf(const double (&rest)[kCount], uint64_t (&mass)[kCount])
+__device__ __forceinline__ void MassSums(const double (&rest)[kCount], double (&m)[kCount])
 {
     constexpr double kOne = 0x1p38;
     constexpr double c0 = 4.069392558613428e-08 * kOne;
@@ -214,7 +214,6 @@ __device__ __forceinline__ void MassesOf(const double (&rest)[kCount], uint64_t 
     constexpr double c5 = 1.0000000000002864 * kOne + 0x1p52;
     // As it stands, with the summands in scalar registers: the compiler would take the form that overwrites its summand,
     // and copy each first.
-    double m[kCount];
     if constexpr (kCount == 4)
     {
         asm("v_fma_f64 %0, %8, %4, %9\n\tv_fma_f64 %1, %8, %5, %9\n\t"
@@ -239,18 +238,19 @@ __device__ __forceinline__ void MassesOf(const double (&rest)[kCount], uint64_t 
             : "=&v"(m[0])
             : "v"(rest[0]), "v"(c0), "s"(c1), "s"(c2), "s"(c3), "s"(c4), "s"(c5));
     }
-#pragma unroll
-    for (int e = 0; e < kCount; ++e)
-    {
-        mass[e] = static_cast<uint64_t>(__double_as_longlong(m[e])) & 0xFFFFFFFFFFFFFull;
-    }
+}
+
+/// The mass of a sum with 2^52.
+__device__ __forceinline__ uint64_t MassIn(double sum)
+{
+    return static_cast<uint64_t>(__double_as_longlong(sum)) & 0xFFFFFFFFFFFFFull;
 }
 
 __device__ __forceinline__ uint64_t MassOf(double rest)
 {
-    uint64_t mass[1];
-    MassesOf<1>({rest}, mass);
-    return mass[0];
+    double sum[1];
+    MassSums<1>({rest}, sum);
+    return MassIn(sum[0]);
 }
 
 /// Weight of a unit of mass in step d, relative to the top's.
@@ -282,8 +282,7 @@ __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double 
     {
         // Four at a time, side by side up to the counters.
         uint32_t step[4];
-        uint64_t mass[4];
-        double rest[4];
+        double rest[4], mass[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
@@ -299,7 +298,7 @@ __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double 
         }
         if (kMass)
         {
-            MassesOf<4>(rest, mass);
+            MassSums<4>(rest, mass);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -309,7 +308,7 @@ __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double 
             {
                 if (kMass)
                 {
-                    atomicAdd(reinterpret_cast<unsigned long long*>(masses + step[e]), mass[e]);
+                    atomicAdd(reinterpret_cast<unsigned long long*>(masses + step[e]), MassIn(mass[e]));
                 }
                 if (kCount)
                 {
@@ -1368,19 +1367,34 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         const uint32_t lastStep = none ? step - 1 : step;
         const float cutLogit = whole || none ? -INFINITY : KeyValue(cut.key);
         const uint32_t cutIndex = ~static_cast<uint32_t>(cut.key);
-        auto nearWeightAt = [&](float v, uint32_t at) {
-            const float x = Counted(v);
-            const double y = static_cast<double>(fmaxf(x, least));
-            const double place = WholeOf(y, r.perUnit);
-            const uint32_t dist = topStep - static_cast<uint32_t>(__double_as_longlong(place));
-            const double weight = static_cast<double>(MassOf(fma(y, r.perUnit, -(place - kWhole)))) *
-                                  s.unit[min(dist, static_cast<uint32_t>(kSteps - 1))];
-            const bool kept = dist <= lastStep && (x > cutLogit || (x == cutLogit && at <= cutIndex));
-            return kept ? weight : 0.0;
-        };
-        const double reach = number * total;
         uint32_t begin = 0;
         uint32_t end = a.vocab;
+        // Adds those of four logits, kWave apart.
+        auto nearWeights = [&](const float (&v)[4], uint32_t at, double& sum) {
+            float x[4];
+            uint32_t dist[4];
+            double rest[4], mass[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+            {
+                x[e] = Counted(v[e]);
+                const double y = static_cast<double>(fmaxf(x[e], least));
+                const double place = WholeOf(y, r.perUnit);
+                dist[e] = topStep - static_cast<uint32_t>(__double_as_longlong(place));
+                rest[e] = fma(y, r.perUnit, -(place - kWhole));
+            }
+            MassSums<4>(rest, mass);
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+            {
+                const uint32_t index = at + e * kWave;
+                const bool kept = index < end && dist[e] <= lastStep &&
+                                  (x[e] > cutLogit || (x[e] == cutLogit && index <= cutIndex));
+                const double weight = (mass[e] - 0x1p52) * s.unit[min(dist[e], static_cast<uint32_t>(kSteps - 1))];
+                sum += kept ? weight : 0.0;
+            }
+        };
+        const double reach = number * total;
         double passed = 0.0;
         if (mode.weighed)
         {
@@ -1497,10 +1511,13 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                     own[b] = 0.0;
                     if (near)
                     {
-#pragma unroll
-                        for (uint32_t j = 0; j < kPickLoads; ++j)
+                        if (i < here)
                         {
-                            own[b] += i < here && at + j * kWave < end ? nearWeightAt(v[b][j], at + j * kWave) : 0.0;
+#pragma unroll
+                            for (uint32_t j = 0; j < kPickLoads; j += 4)
+                            {
+                                nearWeights({v[b][j], v[b][j + 1], v[b][j + 2], v[b][j + 3]}, at + j * kWave, own[b]);
+                            }
                         }
                     }
                     else
