@@ -25,7 +25,7 @@ constexpr int kPickBlock = 512;                // threads that decide a row
 constexpr int kPickWaves = kPickBlock / kWave;
 constexpr int kPickLoads = 8;
 constexpr uint32_t kGroup = kWave * kPickLoads;  // logits of a sum on the way to the token
-constexpr uint32_t kGroups = 1024;             // such sums at a time
+constexpr uint32_t kGroups = 32;               // such sums at a time, four of each wave: half a part on average
 constexpr uint32_t kListed = 4096;             // logits that are listed
 constexpr int32_t kListedK = 2048;             // a top-k up to which listing the tokens is likely to do
 constexpr uint32_t kDigits = 256;
@@ -38,7 +38,7 @@ constexpr uint32_t kFewestParts = 4;           // of a row, if it has the batche
 constexpr double kLog2e = 1.44269504088896340736;
 constexpr uint32_t kListRows = 4096;           // rows whose lists get workgroups of their own
 constexpr uint32_t kPickAtOnce = 256;          // rows that are decided at once: one on each CU
-constexpr uint32_t kListBatches = 2;           // batches that a wave of those looks through
+constexpr uint32_t kListAtOnce = 16384;        // waves of those that fit the GPU at about once
 constexpr double kFar = 0x1p48;                // places past which steps are not whole numbers apart
 constexpr double kWhole = 0x1.8p52;            // added, the whole part's last 32 bits come last
 constexpr double kFixed = 0x1p50;              // units of the top step's weight, for sums of listed logits
@@ -212,8 +212,8 @@ __device__ __forceinline__ void MassSums(const double (&rest)[kCount], double (&
     constexpr double c3 = 0.0037535391505790455 * kOne;
     constexpr double c4 = 0.08664339757000515 * kOne;
     constexpr double c5 = 1.0000000000002864 * kOne + 0x1p52;
-    // As it stands, with the summands in scalar registers: the compiler would take the form that overwrites its summand,
-    // and copy each first.
+    // As it stands, with the summands in scalar registers: the compiler would take the form that overwrites its
+    // summand, and copy each first.
     if constexpr (kCount == 4)
     {
         asm("v_fma_f64 %0, %8, %4, %9\n\tv_fma_f64 %1, %8, %5, %9\n\t"
@@ -334,7 +334,8 @@ __device__ __forceinline__ PartRange RangeOf(const float* x, uint32_t begin, uin
     return r;
 }
 
-/// A lane's i-th logit of a batch: four in a row from each quad. Before the part's first logit it wraps or is too small.
+/// A lane's i-th logit of a batch: four in a row from each quad. Before the part's first logit it wraps or is too
+/// small.
 __device__ __forceinline__ uint32_t IndexOf(const PartRange& r, uint32_t batch, uint32_t i)
 {
     return r.begin - r.before + batch * kBatch + (i / 4 * kWave + threadIdx.x % kWave) * 4 + i % 4;
@@ -368,6 +369,9 @@ __device__ __forceinline__ void LoadBatch(const float* x, const PartRange& r, ui
 /// Counts the logits of a part of a row in steps of the grid, and their masses. A wave has counters of its own in
 /// LDS, from a step above the largest logit that it has met; a larger one moves them down, which is rare.
 ///
+/// What bounds it: some 20 vector operations a logit, ten of them in 64 bits, beside the logits' arrival: 500 rows of
+/// 151936 in 76 us, 4.0 TB/s, the vector units busy for 0.6 of that at 2.4 GHz. Two batches on their way, or three or
+/// five waves a SIMD, were slower.
 __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
 {
     __shared__ uint64_t massOf[kWaves][kSteps];
@@ -625,9 +629,9 @@ __device__ __forceinline__ void BoundsOf(const RowGrid& r, uint32_t first, uint3
     high = high >= 0x1.fffffep127f ? INFINITY : high;
 }
 
-/// Calls use(key, step, mass) for a row's logits in steps first..last, by all threads.
-/// Bounds in f32, a little wide, tell which of a thread's 16 logits may be
-/// meant; those are placed one by one (a copy of that for each of them filled the instruction cache).
+/// Calls use(key, step, mass) for a row's logits in steps first..last, by all threads. Bounds in f32, a little wide,
+/// tell which of a thread's 16 logits may be meant; those are placed one by one (a copy of that for each of them filled
+/// the instruction cache).
 template <typename Use>
 __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, Use use)
 {
@@ -951,6 +955,10 @@ enum PickPhase
 /// Decides a row: where the cuts lie in the steps' counts and masses, and which token the number lands on. Where the
 /// logits of the steps down to the cut are few they are listed, in one pass over the row; else the step of the cut is,
 /// and the token is looked for in the part of the row that the parts' masses name.
+///
+/// What bounds it: a workgroup's chain of searches, each some passes over the list between barriers (1.3 us where a
+/// wave can look at all, 4 for thousands), and where the list does not do, 64-bit work for half a part of the row (10 us
+/// of 30, where 500 rows have 4 parts). One workgroup fits a CU at 171 registers; at 128 they spill and it was slower.
 template <PickPhase kPhase>
 __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
 {
@@ -1598,11 +1606,13 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
     }
 }
 
-/// Lists the logits of the rows' chosen steps, kListBatches batches a wave. Batches whose largest logit is below the
+/// Lists the logits of the rows' chosen steps, kBatches batches a wave. Batches whose largest logit is below the
 /// steps are not read: tokens that stand out of a row are in few of them.
 ///
 /// What bounds it: the arrival of the others, at one CU if the workgroup that decides the row listed them (608 KB in
-/// 13 us).
+/// 13 us). A batch a wave where all fit the GPU at about once, else two: one row 28.3 us in all with one and 29.3 with
+/// two, 61 rows 54.8 and 55.4, 500 154.0 and 149.5 (with four 153).
+template <uint32_t kBatches>
 __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
 {
     const uint32_t row = blockIdx.y;
@@ -1614,7 +1624,7 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
         return;
     }
     const uint32_t wave = blockIdx.x * kWaves + threadIdx.x / kWave;
-    const uint32_t perPart = (a.batches + kListBatches - 1) / kListBatches;  // waves
+    const uint32_t perPart = (a.batches + kBatches - 1) / kBatches;  // waves
     const uint32_t part = wave / perPart;
     if (part >= a.parts)
     {
@@ -1630,16 +1640,16 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
     const uint64_t slot = static_cast<uint64_t>(row) * a.parts + part;
     const uint32_t begin = part * a.partLength;
     const PartRange range = RangeOf(r.x, begin, min(begin + a.partLength, a.vocab));
-    const uint32_t batch0 = (wave - part * perPart) * kListBatches;
-    bool reads[kListBatches];
-    float4v v[kListBatches][kQuads];
+    const uint32_t batch0 = (wave - part * perPart) * kBatches;
+    bool reads[kBatches];
+    float4v v[kBatches][kQuads];
 #pragma unroll
-    for (uint32_t b = 0; b < kListBatches; ++b)
+    for (uint32_t b = 0; b < kBatches; ++b)
     {
         reads[b] = batch0 + b < range.batches && a.batchMost[slot * a.batches + batch0 + b] >= low;
     }
 #pragma unroll
-    for (uint32_t b = 0; b < kListBatches; ++b)
+    for (uint32_t b = 0; b < kBatches; ++b)
     {
         if (reads[b])
         {
@@ -1647,7 +1657,7 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
         }
     }
 #pragma unroll
-    for (uint32_t b = 0; b < kListBatches; ++b)
+    for (uint32_t b = 0; b < kBatches; ++b)
     {
         if (!reads[b])
         {
@@ -1731,8 +1741,8 @@ extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, ui
     const size_t need = muyo_sample_rows_workspace_bytes(rows, vocab);
     if (need == 0)
     {
-        return Fail(MUYO_E_RANGE, "%s: needs 1..%u rows of 1..%u logits (got %u of %u)", name, kMaxRows, kMaxVocab, rows,
-                    vocab);
+        return Fail(MUYO_E_RANGE, "%s: needs 1..%u rows of 1..%u logits (got %u of %u)", name, kMaxRows, kMaxVocab,
+                    rows, vocab);
     }
     if (row_stride < vocab || (reinterpret_cast<uintptr_t>(logits) & 3u) != 0 ||
         (reinterpret_cast<uintptr_t>(randoms) & 7u) != 0)
@@ -1792,10 +1802,18 @@ extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, ui
     if (lists)
     {
         hipLaunchKernelGGL(SamplePickKernel<kPickSteps>, dim3(rows), dim3(kPickBlock), 0, s, a);
-        const uint32_t waves = CeilDiv(a.batches, kListBatches) * parts.count;
-        hipLaunchKernelGGL(SampleListKernel, dim3(CeilDiv(waves, kWaves), rows), dim3(kBlock), 0, s, a);
-        hipLaunchKernelGGL(SamplePickKernel<kPickToken>, dim3(rows > kPickAtOnce ? 2 * rows : rows), dim3(kPickBlock), 0,
-                           s, a);
+        const auto waves = [&](uint32_t each) { return CeilDiv(a.batches, each) * parts.count; };
+        if (static_cast<uint64_t>(waves(1)) * rows <= kListAtOnce)
+        {
+            hipLaunchKernelGGL(SampleListKernel<1>, dim3(CeilDiv(waves(1), kWaves), rows), dim3(kBlock), 0, s, a);
+        }
+        else
+        {
+            hipLaunchKernelGGL(SampleListKernel<2>, dim3(CeilDiv(waves(2), kWaves), rows), dim3(kBlock), 0, s, a);
+        }
+        // More rows than are decided at once: in two turns, 157 us instead of 159.5 for 500 of 151936.
+        const uint32_t turns = rows > kPickAtOnce ? 2 : 1;
+        hipLaunchKernelGGL(SamplePickKernel<kPickToken>, dim3(turns * rows), dim3(kPickBlock), 0, s, a);
     }
     else
     {
