@@ -957,8 +957,9 @@ enum PickPhase
 /// and the token is looked for in the part of the row that the parts' masses name.
 ///
 /// What bounds it: a workgroup's chain of searches, each some passes over the list between barriers (1.3 us where a
-/// wave can look at all, 4 for thousands), and where the list does not do, 64-bit work for half a part of the row (10 us
-/// of 30, where 500 rows have 4 parts). One workgroup fits a CU at 171 registers; at 128 they spill and it was slower.
+/// wave can look at all, 4 for thousands), and where the list does not do, 64-bit work for half a part of the row
+/// (10 us of 30, where 500 rows have 4 parts). One workgroup fits a CU at 171 registers; at 128 they spill and it was
+/// slower.
 template <PickPhase kPhase>
 __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
 {
