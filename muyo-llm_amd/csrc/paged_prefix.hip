@@ -82,9 +82,10 @@ inline constexpr uint32_t kPrefixBytes = kPrefixStages<kHd> * 2 * kStep * 2 * kH
 ///
 /// What bounds it: vector and matrix work, which a SIMD's two waves overlap little. 250 queries of 28 / 4 heads of 128
 /// with 16381 keys: 121 us alone, 141 with up to 500 own keys, of which at 2.4 GHz the vector units are busy for 55 and
-/// the matrix cores for 49 (the clock is below that here). 32 keys at a time took 2 % more, without V's reads ahead of the weights 2 to 4; one wave
-/// a SIMD, with the next step's matrix operations between this one's weights, 200 us; other orders of the chunks in
-/// LDS, with fewer bank conflicts (0.4 of its time), and a wave's priority in either kind of work, no less.
+/// the matrix cores for 49 (the clock is below that here). 32 keys at a time took 2 % more, without V's reads ahead of
+/// the weights 2 to 4; one wave a SIMD, with the next step's matrix operations between this one's weights, 200 us; other
+/// orders of the chunks in LDS, with fewer bank conflicts (0.4 of its time), and a wave's priority in either kind of
+/// work, no less.
 ///
 /// Steps that reach past the prefix, or into a page that is not there, are masked: scores to -inf, and V's rows to 0 in
 /// LDS, since 0 * NaN would be NaN.
@@ -469,7 +470,8 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 ///
 /// Two launches, the prefix's before the own keys', took 14.3 us for 3 queries (1009 keys and up to 100 own, 14 / 2
 /// heads of 64), together 10.3; 64 queries (8190 and up to 2000, 28 / 4 of 128) 53 and 45; 250 (16381 and up to 500)
-/// 183 and 172 (with faster weights since then 41 and 150). In turns of 8, 128 and 512 workgroups, or with the own keys first, 1 to 70 us more.
+/// 183 and 172 (with faster weights since then 41 and 150). In turns of 8, 128 and 512 workgroups, or with the own keys
+/// first, 1 to 70 us more.
 template <int kHd, bool kSplit>
 __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a, PagedAttentionF16Args own,
                                                                uint32_t prefixBlocks, uint32_t ownBlocks)

@@ -219,12 +219,19 @@ __global__ __launch_bounds__(256) void PagedAppendQ8Kernel(AppendQ8Args a)
     // A row that is not finite is told by its scale.
     const float scale = finite ? static_cast<float>(size / kMost) : NAN;
     const bool codes = finite && scale > 0.0f;
+    // Quotients by the reciprocal and a step from what is left, which rounds them as a division does (Markstein).
+    const double wide = codes ? static_cast<double>(scale) : 1.0;
+    const double per = 1.0 / wide;
+    auto scaled = [&](double y) {
+        const double x = y * per;
+        // A scale next to f32's end is rounded by more than half a code.
+        return codes ? fmin(fmax(fma(fma(-x, wide, y), per, x), -kMost), kMost) : 0.0;
+    };
 #pragma unroll
     for (int e = 0; e < 4; ++e)
     {
-        // A scale next to f32's end is rounded by more than half a code.
-        y0[e] = codes ? fmin(fmax(y0[e] / scale, -kMost), kMost) : 0.0;
-        y1[e] = codes ? fmin(fmax(y1[e] / scale, -kMost), kMost) : 0.0;
+        y0[e] = scaled(y0[e]);
+        y1[e] = scaled(y1[e]);
     }
     const uint32_t page = static_cast<uint32_t>(slot) >> a.pageShift;
     const uint32_t row = static_cast<uint32_t>(slot) & ((1u << a.pageShift) - 1);
