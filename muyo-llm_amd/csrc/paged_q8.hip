@@ -100,9 +100,9 @@ __device__ __forceinline__ double TurnFraction(double turns, int32_t position)
 ///
 /// A row's scale is its largest size over the type's, rounded to f32, and its codes are the values over that
 /// scale, rounded once (half steps to even): k is rotated in 64 bits and scaled in 64 bits, so that a value next
-/// to the border between two codes gets the one that is nearer (from f32, one value in 2^16 got the other).
-/// q stays f32, as in the fp16 cache's append. (Two heads of q a lane, which share their angles, take 62 us instead of 63.5
-/// for 8191 tokens of 28 / 4 heads of 128, and 7.2 instead of 5.8 for 253.)
+/// to the border between two codes gets the one that is nearer (from f32, about one value in 2^16 would get the
+/// other). q stays f32, as in the fp16 cache's append. (Two heads of q a lane, which share their angles, take 62 us
+/// instead of 63.5 for 8191 tokens of 28 / 4 heads of 128, and 7.2 instead of 5.8 for 253.)
 ///
 /// What bounds it: round trips for few tokens; for many, reads and writes together (277 MB, 4.4 TB/s, where a copy has
 /// 5.1) beside vector work: angles, and codes in 64 bits.
