@@ -341,11 +341,30 @@ __device__ __forceinline__ uint32_t IndexOf(const PartRange& r, uint32_t batch, 
     return r.begin - r.before + batch * kBatch + (i / 4 * kWave + threadIdx.x % kWave) * 4 + i % 4;
 }
 
-/// A batch in 16-byte loads, logit by logit where it reaches over an end of the part (-inf outside).
-__device__ __forceinline__ void LoadBatch(const float* x, const PartRange& r, uint32_t batch, float4v (&v)[kQuads])
+/// Whether a batch lies in the part as a whole.
+__device__ __forceinline__ bool IsWhole(const PartRange& r, uint32_t batch)
 {
     const uint32_t first = batch * kBatch;
-    if (first >= r.before && first + kBatch <= r.end - r.begin + r.before)
+    return first >= r.before && first + kBatch <= r.end - r.begin + r.before;
+}
+
+/// A batch logit by logit, -inf outside of the part.
+__device__ __forceinline__ void LoadOneByOne(const float* x, const PartRange& r, uint32_t batch, float4v (&v)[kQuads])
+{
+#pragma unroll
+    for (uint32_t i = 0; i < 4 * kQuads; ++i)
+    {
+        const uint32_t index = IndexOf(r, batch, i);
+        const bool inside = index >= r.begin && index < r.end;
+        const float one = x[inside ? index : r.begin];
+        v[i / 4][i % 4] = inside ? one : -INFINITY;
+    }
+}
+
+/// A batch in 16-byte loads, logit by logit where it reaches over an end of the part.
+__device__ __forceinline__ void LoadBatch(const float* x, const PartRange& r, uint32_t batch, float4v (&v)[kQuads])
+{
+    if (IsWhole(r, batch))
     {
 #pragma unroll
         for (uint32_t q = 0; q < kQuads; ++q)
@@ -355,14 +374,7 @@ __device__ __forceinline__ void LoadBatch(const float* x, const PartRange& r, ui
     }
     else if (batch < r.batches)
     {
-#pragma unroll
-        for (uint32_t i = 0; i < 4 * kQuads; ++i)
-        {
-            const uint32_t index = IndexOf(r, batch, i);
-            const bool inside = index >= r.begin && index < r.end;
-            const float one = x[inside ? index : r.begin];
-            v[i / 4][i % 4] = inside ? one : -INFINITY;
-        }
+        LoadOneByOne(x, r, batch, v);
     }
 }
 
@@ -401,8 +413,24 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
     float most = -INFINITY;   // of the wave; of a greedy row's lane
     uint32_t at = 0;
     const PartRange range = RangeOf(x, begin, end);
+    // The next batch is on its way, always in as many loads: under a condition they would all be waited for at once. What
+    // lies outside the part's whole quads is read as the nearest of these, and again one by one; without any, as what
+    // the workspace holds.
+    const uint32_t firstQuad = range.before != 0 ? 1 : 0;
+    const uint32_t quads = (end - begin + range.before) / 4;
+    const float4v* const wide = quads > firstQuad ? reinterpret_cast<const float4v*>(x + begin - range.before)
+                                                  : reinterpret_cast<const float4v*>(a.masses);
+    const uint32_t low = quads > firstQuad ? firstQuad : 0;
+    const uint32_t high = quads > firstQuad ? quads - 1 : 0;
+    auto request = [&](uint32_t batch, float4v (&to)[kQuads]) {
+#pragma unroll
+        for (uint32_t q = 0; q < kQuads; ++q)
+        {
+            to[q] = wide[min(max(batch * (kBatch / 4) + q * kWave + lane, low), high)];
+        }
+    };
     float4v v[kQuads], next[kQuads];
-    LoadBatch(x, range, wave, next);
+    request(wave, next);
     for (uint32_t batch = wave; batch < range.batches; batch += kWaves)
     {
 #pragma unroll
@@ -410,7 +438,11 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
         {
             v[q] = next[q];
         }
-        LoadBatch(x, range, batch + kWaves, next);
+        request(batch + kWaves, next);
+        if (!IsWhole(range, batch))
+        {
+            LoadOneByOne(x, range, batch, v);
+        }
         float batchMost = -INFINITY;
 #pragma unroll
         for (uint32_t i = 0; i < 4 * kQuads; ++i)
