@@ -56,8 +56,9 @@ struct RowSteps
 {
     double upTo[kSteps];
     uint32_t counts[kSteps];
-    double top;
+    double top, perUnit;
     uint32_t first, last;  // steps that are listed: none if first > last
+    float low, high;       // bounds of their logits
     uint32_t listed;
     uint32_t walk;         // the list will not do: the token is looked for in the row
     uint64_t keys[kListed];
@@ -1237,6 +1238,8 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         {
             if (threadIdx.x == 0)
             {
+                kept->perUnit = r.perUnit;
+                BoundsOf(r, from, to, kept->low, kept->high);
                 kept->first = from;
                 kept->last = to;
                 kept->walk = (task == kCutOfAll ? all : from <= to) ? 0 : 1;
@@ -1663,16 +1666,14 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
     {
         return;
     }
-    RowGrid r;
-    r.x = a.logits + row * a.stride;
-    r.vocab = a.vocab;
-    r.perUnit = ModeOf(a, row).perUnit;
-    r.top = kept->top;
-    float low, high;
-    BoundsOf(r, first, last, low, high);
+    const float* const x = a.logits + row * a.stride;
+    const double perUnit = kept->perUnit;
+    const double top = kept->top;
+    const float low = kept->low;
+    const float high = kept->high;
     const uint64_t slot = static_cast<uint64_t>(row) * a.parts + part;
     const uint32_t begin = part * a.partLength;
-    const PartRange range = RangeOf(r.x, begin, min(begin + a.partLength, a.vocab));
+    const PartRange range = RangeOf(x, begin, min(begin + a.partLength, a.vocab));
     const uint32_t batch0 = (wave - part * perPart) * kBatches;
     bool reads[kBatches];
     float4v v[kBatches][kQuads];
@@ -1686,7 +1687,7 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
     {
         if (reads[b])
         {
-            LoadBatch(r.x, range, batch0 + b, v[b]);
+            LoadBatch(x, range, batch0 + b, v[b]);
         }
     }
 #pragma unroll
@@ -1712,15 +1713,15 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
             {
                 logit = bit == i ? v[b][i / 4][i % 4] : logit;
             }
-            const float x = Counted(logit);
-            const double d = r.top - PlaceOf(x, r.perUnit).step;
-            if (x > -INFINITY && d >= first && d <= last)
+            const float counted = Counted(logit);
+            const double d = top - PlaceOf(counted, perUnit).step;
+            if (counted > -INFINITY && d >= first && d <= last)
             {
                 const uint32_t at = atomicAdd(&kept->listed, 1u);
                 if (at < kListed)
                 {
                     // In any order: what is made of them goes by their own.
-                    kept->keys[at] = OrderKey(x, IndexOf(range, batch0 + b, bit));
+                    kept->keys[at] = OrderKey(counted, IndexOf(range, batch0 + b, bit));
                 }
             }
         }
