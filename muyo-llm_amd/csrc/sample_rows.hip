@@ -647,6 +647,14 @@ struct RowGrid
     double lowest;  // of y - largest, by min-p; -inf: none
 };
 
+/// Keys from low to high.
+struct KeyRange
+{
+    uint64_t low, high;
+};
+
+constexpr KeyRange kAllKeys{0, ~0ull};
+
 __device__ __forceinline__ bool Reaches(const RowGrid& r, const Place& at)
 {
     return (at.step - r.largest.step) + (at.rest - r.largest.rest) >= r.lowest;
@@ -662,19 +670,20 @@ __device__ __forceinline__ void BoundsOf(const RowGrid& r, uint32_t first, uint3
     high = high >= 0x1.fffffep127f ? INFINITY : high;
 }
 
-/// Calls use(key, step, mass) for a row's logits in steps first..last, by all threads. Bounds in f32, a little wide,
-/// tell which of a thread's 16 logits may be meant; those are placed one by one (a copy of that for each of them filled
-/// the instruction cache).
-template <typename Use>
-__device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, Use use)
+/// Calls use(key, step, mass) for a row's logits in steps first..last with keys in keys.low..high, by all threads. Bounds
+/// in f32, a little wide, tell which of a thread's logits of a round may be meant; those are placed one by one (a copy
+/// of that for each of them filled the instruction cache). kAhead: 16-byte loads of a thread in a round.
+template <uint32_t kAhead, typename Use>
+__device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, KeyRange keys, Use use)
 {
     float low, high;
     BoundsOf(r, first, last, low, high);
+    low = fmaxf(low, KeyValue(keys.low));
+    high = KeyValue(keys.high) < 0x1.fffffep127f ? fminf(high, KeyValue(keys.high)) : high;
     const uint32_t head = min((4u - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(r.x) / 4 % 4)) % 4u, r.vocab);
     const uint32_t quads = (r.vocab - head) / 4;
     const uint32_t edges = r.vocab - 4 * quads;  // before the first quad and behind the last
-    constexpr uint32_t kAhead = 4;  // quads of a thread in a round; the next round's are on their way
-    float4v v[kAhead], next[kAhead];
+    float4v v[kAhead], next[kAhead];  // quads of a round; the next round's are on their way
     auto load = [&](uint32_t from) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i)
@@ -709,9 +718,10 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint3
             const float x = Counted(logit);
             const Place place = PlaceOf(x, r.perUnit);
             const double d = r.top - place.step;
-            if (x > -INFINITY && d >= first && d <= last)
+            const uint64_t key = OrderKey(x, at);
+            if (x > -INFINITY && d >= first && d <= last && key >= keys.low && key <= keys.high)
             {
-                use(OrderKey(x, at), static_cast<uint32_t>(d), MassOf(place.rest));
+                use(key, static_cast<uint32_t>(d), MassOf(place.rest));
             }
         }
         from += edge ? 0 : kPickBlock * kAhead;
@@ -739,8 +749,9 @@ __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint3
     }
 }
 
-/// Lists the keys of the logits in steps first..last (at most kListed, as the caller has seen).
-__device__ __forceinline__ void ListSteps(const RowGrid& r, uint32_t first, uint32_t last, PickSpace& s)
+/// Lists the keys of those (at most kListed, as the caller has seen).
+template <uint32_t kAhead>
+__device__ __forceinline__ void ListSteps(const RowGrid& r, uint32_t first, uint32_t last, KeyRange keys, PickSpace& s)
 {
     __syncthreads();
     if (threadIdx.x == 0)
@@ -748,7 +759,7 @@ __device__ __forceinline__ void ListSteps(const RowGrid& r, uint32_t first, uint
         s.listed = 0;
     }
     __syncthreads();
-    ForSteps(r, first, last, [&](uint64_t key, uint32_t, uint64_t) {
+    ForSteps<kAhead>(r, first, last, keys, [&](uint64_t key, uint32_t, uint64_t) {
         const uint32_t at = atomicAdd(&s.listed, 1u);
         if (at < kListed)
         {
@@ -765,16 +776,74 @@ struct Cut
     uint64_t mass;
 };
 
+/// Of 256 equal ranges from the high end of keys down, `shift` says how many bits of a distance they leave.
+__device__ __forceinline__ int DigitShift(KeyRange keys)
+{
+    return max(56 - __clzll(static_cast<long long>(keys.high - keys.low)), 0);
+}
+
+__device__ __forceinline__ KeyRange DigitOf(KeyRange keys, uint32_t which, int shift)
+{
+    keys.high -= static_cast<uint64_t>(which) << shift;
+    const uint64_t span = (1ull << shift) - 1;
+    keys.low = keys.high - keys.low > span ? keys.high - span : keys.low;
+    return keys;
+}
+
+/// The last such range that begins before both limits, by the counts and masses of all (the first after `above` items
+/// of `aboveMass`), and what it begins after; ~0: none. Every wave finds the same, four ranges a lane.
+struct Digit
+{
+    uint32_t which, count, above;
+    uint64_t aboveMass;
+};
+
+__device__ __forceinline__ Digit LastDigit(uint32_t most, uint64_t limit, uint32_t above, uint64_t aboveMass,
+                                           const PickSpace& s)
+{
+    const uint32_t lane = threadIdx.x % kWave;
+    constexpr uint32_t kPer = kDigits / kWave;
+    uint32_t c[kPer];
+    uint64_t m[kPer];
+    uint32_t ofLane = 0;
+    uint64_t massOfLane = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; ++e)
+    {
+        c[e] = s.digitCounts[lane * kPer + e];
+        m[e] = s.digitMasses[lane * kPer + e];
+        ofLane += c[e];
+        massOfLane += m[e];
+    }
+    uint32_t before = above + WaveInclusive(ofLane) - ofLane;
+    uint64_t massBefore = aboveMass + WaveInclusive(massOfLane) - massOfLane;
+    Digit last{~0u, 0, above, aboveMass};
+#pragma unroll
+    for (uint32_t e = 0; e < kPer; ++e)
+    {
+        if (c[e] > 0 && before < most && massBefore < limit)
+        {
+            last = Digit{lane * kPer + e, c[e], before, massBefore};
+        }
+        before += c[e];
+        massBefore += m[e];
+    }
+    const uint64_t has = __ballot(last.which != ~0u);
+    const int owner = has != 0 ? 63 - __clzll(static_cast<long long>(has)) : 0;
+    return Digit{OfLane(last.which, owner), OfLane(last.count, owner), OfLane(last.above, owner),
+                 OfLane(last.aboveMass, owner)};
+}
+
 /// Of `n` items in falling order of their keys (which differ), those that have fewer than `most` before them and
 /// less than `limit` of mass: the last one's key, and their mass. item(i, key, mass) says whether there is one; there
 /// are `some` at most.
 ///
-/// All keys are in low..high. That is taken apart into 256 equal ranges, the one with the last item is found from
+/// All keys are in `keys`. That is taken apart into 256 equal ranges, the one with the last item is found from
 /// counts and masses of all, and so on between the smallest and the largest there, until a wave can look at the rest
 /// one by one.
 template <typename Item>
 __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, uint32_t most, uint64_t limit,
-                                        uint64_t low, uint64_t high, PickSpace& s)
+                                        KeyRange keys, PickSpace& s)
 {
     const uint32_t lane = threadIdx.x % kWave;
     uint32_t above = 0;
@@ -803,7 +872,7 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, ui
             for (uint32_t i = threadIdx.x; i < n; i += kPickBlock)
             {
                 uint64_t key, mass;
-                if (item(i, key, mass) && key >= low && key <= high)
+                if (item(i, key, mass) && key >= keys.low && key <= keys.high)
                 {
                     least = least < key ? least : key;
                     largest = largest > key ? largest : key;
@@ -817,8 +886,7 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, ui
                 atomicMax(&s.high, static_cast<unsigned long long>(largest));
             }
             __syncthreads();
-            low = s.low;
-            high = s.high;
+            keys = KeyRange{s.low, s.high};
         }
         narrow = false;
         if (few)
@@ -826,7 +894,7 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, ui
             for (uint32_t i = threadIdx.x; i < n; i += kPickBlock)
             {
                 uint64_t key, mass;
-                if (item(i, key, mass) && key >= low && key <= high)
+                if (item(i, key, mass) && key >= keys.low && key <= keys.high)
                 {
                     const uint32_t at = atomicAdd(&s.few, 1u);
                     s.fewKeys[at] = key;
@@ -856,124 +924,83 @@ __device__ __forceinline__ Cut LastKept(uint32_t n, uint32_t some, Item item, ui
             }
             return Cut{last, OfLane(massBefore + mass, __ffsll(static_cast<unsigned long long>(is)) - 1)};
         }
-        const int bits = 64 - __clzll(static_cast<long long>(high - low));
-        const int shift = max(bits - 8, 0);
+        const int shift = DigitShift(keys);
         for (uint32_t i = threadIdx.x; i < n; i += kPickBlock)
         {
             uint64_t key, mass;
-            if (item(i, key, mass) && key >= low && key <= high)
+            if (item(i, key, mass) && key >= keys.low && key <= keys.high)
             {
-                const uint32_t digit = static_cast<uint32_t>((high - key) >> shift);
+                const uint32_t digit = static_cast<uint32_t>((keys.high - key) >> shift);
                 atomicAdd(&s.digitCounts[digit], 1u);
                 atomicAdd(reinterpret_cast<unsigned long long*>(&s.digitMasses[digit]), mass);
             }
         }
         __syncthreads();
-        // Every wave finds the last range that begins before both limits, four of them a lane.
-        constexpr uint32_t kPer = kDigits / kWave;
-        uint32_t c[kPer];
-        uint64_t m[kPer];
-        uint32_t ofLane = 0;
-        uint64_t massOfLane = 0;
-#pragma unroll
-        for (uint32_t e = 0; e < kPer; ++e)
-        {
-            c[e] = s.digitCounts[lane * kPer + e];
-            m[e] = s.digitMasses[lane * kPer + e];
-            ofLane += c[e];
-            massOfLane += m[e];
-        }
-        uint32_t before = above + WaveInclusive(ofLane) - ofLane;
-        uint64_t massBefore =
-            aboveMass + WaveInclusive(massOfLane) - massOfLane;
-        uint32_t which = ~0u;
-        uint32_t ofIt = 0;
-        uint32_t beforeIt = 0;
-        uint64_t massBeforeIt = 0;
-#pragma unroll
-        for (uint32_t e = 0; e < kPer; ++e)
-        {
-            if (c[e] > 0 && before < most && massBefore < limit)
-            {
-                which = lane * kPer + e;
-                ofIt = c[e];
-                beforeIt = before;
-                massBeforeIt = massBefore;
-            }
-            before += c[e];
-            massBefore += m[e];
-        }
-        const uint64_t has = __ballot(which != ~0u);
-        if (has == 0)
+        const Digit digit = LastDigit(most, limit, above, aboveMass, s);
+        if (digit.which == ~0u)
         {
             return Cut{~0ull, aboveMass};
         }
-        const int owner = 63 - __clzll(static_cast<long long>(has));
-        which = OfLane(which, owner);
-        few = OfLane(ofIt, owner) <= kFew;
-        above = OfLane(beforeIt, owner);
-        aboveMass = OfLane(massBeforeIt, owner);
-        high -= static_cast<uint64_t>(which) << shift;
-        const uint64_t span = (1ull << shift) - 1;
-        low = high - low > span ? high - span : low;
+        few = digit.count <= kFew;
+        above = digit.above;
+        aboveMass = digit.aboveMass;
+        keys = DigitOf(keys, digit.which, shift);
     }
 }
 
-/// The cut in a step of more logits than are listed: digit by digit of the keys, from the highest, with a pass over
-/// the row for each.
-__device__ Cut LastKeptOfRow(const RowGrid& r, uint32_t d, uint32_t most, uint64_t limit, PickSpace& s)
+/// In a step of more logits than are listed: takes `keys` to a range that has the last of what is kept, of few enough
+/// to list, and returns what that begins after (which ~0: nothing is kept). Range by range of 256 and between the
+/// smallest and the largest key there, with a pass over the row for each.
+template <uint32_t kAhead>
+__device__ __forceinline__ Digit NarrowStep(const RowGrid& r, uint32_t d, uint32_t most, uint64_t limit, KeyRange& keys,
+                                            PickSpace& s)
 {
-    uint64_t prefix = 0;
-    uint32_t above = 0;
-    uint64_t aboveMass = 0;
-    for (int shift = 56; shift >= 0; shift -= 8)
+    Digit last{0, ~0u, 0, 0};
+    while (last.count > kListed)
     {
         __syncthreads();
+        if (threadIdx.x == 0)
+        {
+            s.low = ~0ull;
+            s.high = 0;
+        }
         for (uint32_t i = threadIdx.x; i < kDigits; i += kPickBlock)
         {
             s.digitCounts[i] = 0;
             s.digitMasses[i] = 0;
         }
         __syncthreads();
-        ForSteps(r, d, d, [&](uint64_t key, uint32_t, uint64_t mass) {
-            if ((shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))) &&
-                Reaches(r, PlaceOf(KeyValue(key), r.perUnit)))
+        const int shift = DigitShift(keys);
+        uint64_t least = ~0ull;
+        uint64_t largest = 0;
+        ForSteps<kAhead>(r, d, d, keys, [&](uint64_t key, uint32_t, uint64_t mass) {
+            if (Reaches(r, PlaceOf(KeyValue(key), r.perUnit)))
             {
-                const uint32_t digit = 255u - (static_cast<uint32_t>(key >> shift) & 255u);
+                const uint32_t digit = static_cast<uint32_t>((keys.high - key) >> shift);
                 atomicAdd(&s.digitCounts[digit], 1u);
                 atomicAdd(reinterpret_cast<unsigned long long*>(&s.digitMasses[digit]), mass);
+                least = least < key ? least : key;
+                largest = largest > key ? largest : key;
             }
         });
+        least = WaveLeast(least);
+        largest = ~WaveLeast(~largest);
+        if (threadIdx.x % kWave == 0 && least <= largest)
+        {
+            atomicMin(&s.low, static_cast<unsigned long long>(least));
+            atomicMax(&s.high, static_cast<unsigned long long>(largest));
+        }
         __syncthreads();
-        uint32_t before = above;
-        uint64_t massBefore = aboveMass;
-        uint32_t which = ~0u;
-        uint64_t massOfIt = 0;
-        for (uint32_t digit = 0; digit < kDigits; ++digit)
+        last = LastDigit(most, limit, last.above, last.aboveMass, s);
+        if (last.which == ~0u)
         {
-            const uint32_t c = s.digitCounts[digit];
-            const uint64_t m = s.digitMasses[digit];
-            if (c > 0 && before < most && massBefore < limit)
-            {
-                which = digit;
-                above = before;
-                aboveMass = massBefore;
-                massOfIt = m;
-            }
-            before += c;
-            massBefore += m;
+            return last;
         }
-        if (which == ~0u)  // nothing in the step reaches min-p
-        {
-            return Cut{~0ull, aboveMass};
-        }
-        prefix |= static_cast<uint64_t>(255u - which) << shift;
-        if (shift == 0)
-        {
-            aboveMass += massOfIt;  // keys differ: one
-        }
+        keys = DigitOf(keys, last.which, shift);
+        keys.low = keys.low > s.low ? keys.low : s.low;
+        keys.high = keys.high < s.high ? keys.high : s.high;
     }
-    return Cut{prefix, aboveMass};
+    return last;
 }
 
 /// What the launches of a row's end do: everything; or the steps and what of them is to be listed, and then, with the
@@ -994,9 +1021,11 @@ enum PickPhase
 /// (10 us of 30, where 500 rows have 4 parts). One workgroup fits a CU at 171 registers; at 128 they spill and it was
 /// slower.
 template <PickPhase kPhase>
-__global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
+__global__ __launch_bounds__(kPickBlock, kPhase == kPickAll ? 1 : 4) void SamplePickKernel(SampleArgs a)
 {
     __shared__ PickSpace s;
+    // Without lists made before, passes over the row are the rule; else the registers of more loads cost a workgroup.
+    constexpr uint32_t kAhead = kPhase == kPickAll ? 4 : 1;
     const uint32_t row = blockIdx.x % a.rows;
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = threadIdx.x / kWave;
@@ -1144,7 +1173,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         // Counted alone, and too many for the list after all: the masses by a pass of their own.
         s.masses[d] = 0;
         __syncthreads();
-        ForSteps(r, 0, stepK, [&](uint64_t, uint32_t step, uint64_t one) {
+        ForSteps<kAhead>(r, 0, stepK, kAllKeys, [&](uint64_t, uint32_t step, uint64_t one) {
             atomicAdd(reinterpret_cast<unsigned long long*>(&s.masses[step]), one);
         });
     }
@@ -1248,7 +1277,7 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         }
         if (from <= to && !(listFirst <= from && to <= listLast))
         {
-            ListSteps(r, from, to, s);
+            ListSteps<kAhead>(r, from, to, kAllKeys, s);
             listFirst = from;
             listLast = to;
         }
@@ -1333,26 +1362,40 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
         {
             const uint64_t below = limit < 0x1p63 ? static_cast<uint64_t>(ceil(limit)) : ~0ull;
             // Of the token's search keys are indices, else those of the step's logits.
-            const uint32_t some = task != kToken ? countOf(of)
-                                  : mode.counted ? min(s.counts[of], static_cast<uint32_t>(mode.topK))
-                                                 : s.counts[of];
-            uint64_t low = static_cast<uint32_t>(~(a.vocab - 1));
-            uint64_t high = 0xFFFFFFFFull;
-            if (task != kToken && min(s.listed, some) <= kFew)
+            uint32_t some = task != kToken ? countOf(of)
+                            : mode.counted ? min(s.counts[of], static_cast<uint32_t>(mode.topK))
+                                           : s.counts[of];
+            KeyRange keys{static_cast<uint32_t>(~(a.vocab - 1)), 0xFFFFFFFFull};
+            const bool inList = task == kToken || (listFirst <= of && of <= listLast);
+            if (task != kToken && inList && min(s.listed, some) <= kFew)
             {
-                low = 0;
-                high = ~0ull;
+                keys = kAllKeys;
             }
             else if (task != kToken)
             {
                 float least, largest;
                 BoundsOf(r, of, of, least, largest);
-                low = static_cast<uint64_t>(OrderBits(least)) << 32;
-                high |= static_cast<uint64_t>(OrderBits(largest)) << 32;
+                keys.low = static_cast<uint64_t>(OrderBits(least)) << 32;
+                keys.high |= static_cast<uint64_t>(OrderBits(largest)) << 32;
             }
-            found = task == kToken || (listFirst <= of && of <= listLast)
-                        ? LastKept(s.listed, some, item, atMost, below, low, high, s)
-                        : LastKeptOfRow(r, of, atMost, below, s);
+            Digit before{0, 0, 0, 0};
+            if (!inList)
+            {
+                before = NarrowStep<kAhead>(r, of, atMost, below, keys, s);
+                some = before.count;
+                listFirst = 1;
+                listLast = 0;
+                if (before.which != ~0u)
+                {
+                    ListSteps<kAhead>(r, of, of, keys, s);
+                }
+            }
+            found = Cut{~0ull, 0};
+            if (before.which != ~0u)
+            {
+                found = LastKept(s.listed, some, item, atMost - before.above, below - before.aboveMass, keys, s);
+            }
+            found.mass += before.aboveMass;
         }
         if (task == kCutOfK)
         {
@@ -1499,7 +1542,8 @@ __global__ __launch_bounds__(kPickBlock) void SamplePickKernel(SampleArgs a)
                 }
                 else
                 {
-                    ForSteps(r, step, step, [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
+                    ForSteps<kAhead>(r, step, step, KeyRange{cut.key, ~0ull},
+                                     [&](uint64_t key, uint32_t, uint64_t one) { use(key, one); });
                 }
             }
             __syncthreads();

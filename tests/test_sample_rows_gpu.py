@@ -198,6 +198,21 @@ def test_equal_logits(mh, gpu, vocab, step):
     Batch(mh, gpu, x, settings, rng.random(len(settings))).check()
 
 
+@pytest.mark.parametrize("std", [1.0, 0.3, 0.01, 1e-4])
+def test_flat_rows(mh, gpu, std):
+    """Tens of thousands of logits in the steps of the cuts, few of them equal."""
+    rng = np.random.default_rng(int(1 / std))
+    more = [(1.0, 30000, 1.0, 0.0), (1.0, 30000, 0.5, 0.0), (1.0, 0, 0.5, 0.0), (1.0, 0, 0.999, 0.0), (1.0, 0, 1.0, 0.7),
+            (0.9, 40000, 0.9, 0.5), (2.0, 69999, 0.9999, 0.0), (1.0, 0, 1e-6, 0.0), (1.0, 5000, 0.99, 0.001)]
+    settings = SETTINGS + more
+    rows = len(settings)
+    x = rng.normal(0, std, (rows, 70000)).astype(np.float32)
+    Batch(mh, gpu, x, settings, rng.random(rows)).check()
+    x[:, ::3] = -np.inf
+    batch = Batch(mh, gpu, np.tile(x, (9, 1)), settings * 9, rng.random(9 * rows))
+    batch.check()
+
+
 @pytest.mark.parametrize("vocab", [61, 4000, 4096, 4150, 4300])
 def test_equal_logits_at_tiny_temperatures(mh, gpu, vocab):
     """Places so far out that what a step leaves of them is any number: as many as a list holds, and more."""
