@@ -37,7 +37,6 @@ constexpr uint32_t kCountBlocks = 1024;        // workgroups to aim at that coun
 constexpr uint32_t kFewestParts = 4;           // of a row, if it has the batches
 constexpr double kLog2e = 1.44269504088896340736;
 constexpr uint32_t kListRows = 4096;           // rows whose lists get workgroups of their own
-constexpr uint32_t kPickAtOnce = 256;          // rows that are decided at once: one on each CU
 constexpr uint32_t kListAtOnce = 16384;        // waves of those that fit the GPU at about once
 constexpr double kFar = 0x1p48;                // places past which steps are not whole numbers apart
 constexpr double kWhole = 0x1.8p52;            // added, the whole part's last 32 bits come last
@@ -60,7 +59,7 @@ struct RowSteps
     uint32_t first, last;  // steps that are listed: none if first > last
     float low, high;       // bounds of their logits
     uint32_t listed;
-    uint32_t walk;         // the list will not do: the token is looked for in the row
+    uint32_t unused;
     uint64_t keys[kListed];
 };
 
@@ -414,9 +413,9 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
     float most = -INFINITY;   // of the wave; of a greedy row's lane
     uint32_t at = 0;
     const PartRange range = RangeOf(x, begin, end);
-    // The next batch is on its way, always in as many loads: under a condition they would all be waited for at once. What
-    // lies outside the part's whole quads is read as the nearest of these, and again one by one; without any, as what
-    // the workspace holds.
+    // The next batch is on its way, always in as many loads: under a condition they would all be waited for at once.
+    // What lies outside the part's whole quads is read as the nearest of these, and again one by one; without any, as
+    // what the workspace holds.
     const uint32_t firstQuad = range.before != 0 ? 1 : 0;
     const uint32_t quads = (end - begin + range.before) / 4;
     const float4v* const wide = quads > firstQuad ? reinterpret_cast<const float4v*>(x + begin - range.before)
@@ -670,9 +669,9 @@ __device__ __forceinline__ void BoundsOf(const RowGrid& r, uint32_t first, uint3
     high = high >= 0x1.fffffep127f ? INFINITY : high;
 }
 
-/// Calls use(key, step, mass) for a row's logits in steps first..last with keys in keys.low..high, by all threads. Bounds
-/// in f32, a little wide, tell which of a thread's logits of a round may be meant; those are placed one by one (a copy
-/// of that for each of them filled the instruction cache). kAhead: 16-byte loads of a thread in a round.
+/// Calls use(key, step, mass) for a row's logits in steps first..last with keys in keys.low..high, by all threads.
+/// Bounds in f32, a little wide, tell which of a thread's logits of a round may be meant; those are placed one by one
+/// (a copy of that for each of them filled the instruction cache). kAhead: 16-byte loads of a thread in a round.
 template <uint32_t kAhead, typename Use>
 __device__ __forceinline__ void ForSteps(const RowGrid& r, uint32_t first, uint32_t last, KeyRange keys, Use use)
 {
@@ -1017,24 +1016,22 @@ enum PickPhase
 /// and the token is looked for in the part of the row that the parts' masses name.
 ///
 /// What bounds it: a workgroup's chain of searches, each some passes over the list between barriers (1.3 us where a
-/// wave can look at all, 4 for thousands), and where the list does not do, 64-bit work for half a part of the row
-/// (10 us of 30, where 500 rows have 4 parts). One workgroup fits a CU at 171 registers; at 128 they spill and it was
-/// slower.
+/// wave can look at all, 4 for thousands); where the list does not do, 64-bit work for half a part of the row (10 us of
+/// 30, where 500 rows have 4 parts); and where a cut's step is not to be listed, a pass over the row for each range of
+/// it (500 rows of 151936 of standard deviation 0.75 take 337 us in all, of 2.5 with some that stand out 129; by digits
+/// of the keys, eight passes, the former took 980). Two workgroups fit a CU at 123 registers: with more loads on their
+/// way in such passes, 171 and one, 500 rows with lists took 142 us.
 template <PickPhase kPhase>
 __global__ __launch_bounds__(kPickBlock, kPhase == kPickAll ? 1 : 4) void SamplePickKernel(SampleArgs a)
 {
     __shared__ PickSpace s;
-    // Without lists made before, passes over the row are the rule; else the registers of more loads cost a workgroup.
+    // Without lists made before, passes over the row are the rule; else the registers of more loads on their way would
+    // take the second workgroup's place on a CU.
     constexpr uint32_t kAhead = kPhase == kPickAll ? 4 : 1;
-    const uint32_t row = blockIdx.x % a.rows;
+    const uint32_t row = blockIdx.x;
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = threadIdx.x / kWave;
     const uint64_t slot = static_cast<uint64_t>(row) * a.parts;
-    // In two turns, what takes longest is begun first.
-    if (kPhase == kPickToken && gridDim.x > a.rows && (a.steps[row].walk != 0) != (blockIdx.x < a.rows))
-    {
-        return;
-    }
 
     // Every wave looks at the parts, a lane each.
     static_assert(kMaxParts == kWave, "a lane for each part");
@@ -1058,7 +1055,6 @@ __global__ __launch_bounds__(kPickBlock, kPhase == kPickAll ? 1 : 4) void Sample
         kept->first = 1;
         kept->last = 0;
         kept->listed = 0;
-        kept->walk = 0;
     }
     if (kPhase == kPickSteps && (most == -INFINITY || mode.perUnit < 0.0))
     {
@@ -1271,7 +1267,6 @@ __global__ __launch_bounds__(kPickBlock, kPhase == kPickAll ? 1 : 4) void Sample
                 BoundsOf(r, from, to, kept->low, kept->high);
                 kept->first = from;
                 kept->last = to;
-                kept->walk = (task == kCutOfAll ? all : from <= to) ? 0 : 1;
             }
             return;
         }
@@ -1889,9 +1884,7 @@ extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, ui
         {
             hipLaunchKernelGGL(SampleListKernel<2>, dim3(CeilDiv(waves(2), kWaves), rows), dim3(kBlock), 0, s, a);
         }
-        // More rows than are decided at once: in two turns, 157 us instead of 159.5 for 500 of 151936.
-        const uint32_t turns = rows > kPickAtOnce ? 2 : 1;
-        hipLaunchKernelGGL(SamplePickKernel<kPickToken>, dim3(turns * rows), dim3(kPickBlock), 0, s, a);
+        hipLaunchKernelGGL(SamplePickKernel<kPickToken>, dim3(rows), dim3(kPickBlock), 0, s, a);
     }
     else
     {
