@@ -81,7 +81,7 @@ struct SampleArgs
     uint32_t* counts;    // [rows][parts][kSteps]
     float* batchMost;    // [rows][parts][batches]: the largest logit of each
     uint32_t batches;    // of a part, at most
-    RowSteps* steps;     // [rows], of at most kListRows
+    RowSteps* steps;     // [rows], of at most kListRows; where the workspace begins
 };
 
 /// What a row asks for.
@@ -415,11 +415,11 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
     const PartRange range = RangeOf(x, begin, end);
     // The next batch is on its way, always in as many loads: under a condition they would all be waited for at once.
     // What lies outside the part's whole quads is read as the nearest of these, and again one by one; without any, as
-    // what the workspace holds.
+    // what the workspace begins with.
     const uint32_t firstQuad = range.before != 0 ? 1 : 0;
     const uint32_t quads = (end - begin + range.before) / 4;
     const float4v* const wide = quads > firstQuad ? reinterpret_cast<const float4v*>(x + begin - range.before)
-                                                  : reinterpret_cast<const float4v*>(a.masses);
+                                                  : reinterpret_cast<const float4v*>(a.steps);
     const uint32_t low = quads > firstQuad ? firstQuad : 0;
     const uint32_t high = quads > firstQuad ? quads - 1 : 0;
     auto request = [&](uint32_t batch, float4v (&to)[kQuads]) {

@@ -117,7 +117,8 @@ def test_settings_and_vocabularies(mh, gpu, vocab):
     Batch(mh, gpu, logits_of(rng, rows, vocab), SETTINGS, rng.random(rows)).check()
 
 
-@pytest.mark.parametrize("rows, vocab", [(1, 152064), (2, 151937), (64, 20000), (300, 5003), (1700, 999), (3000, 40)])
+@pytest.mark.parametrize("rows, vocab", [(1, 152064), (2, 151937), (64, 20000), (300, 5003), (1700, 999), (3000, 40),
+                                         (1, 1), (5, 2), (7, 3), (4095, 7)])
 def test_rows(mh, gpu, rows, vocab):
     """From many workgroups a row to one."""
     rng = np.random.default_rng(rows)
