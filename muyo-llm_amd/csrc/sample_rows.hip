@@ -256,6 +256,18 @@ __device__ __forceinline__ uint64_t MassOf(double rest)
 /// Weight of a unit of mass in step d, relative to the top's.
 __device__ __forceinline__ double UnitOf(uint32_t d) { return exp2(-38.0 - static_cast<double>(d) * 0.125); }
 
+/// Whether places of logits that are at least `least` are near the top step's, so that steps are whole numbers of 32
+/// bits apart; `least` lies past the last step.
+__device__ __forceinline__ bool NearPlaces(double top, double perUnit, float& least)
+{
+    const double bound = (top - (kSteps + 2)) / perUnit;
+    // Down: at small temperatures all steps are less than a unit in the last place of the largest logit, and the f32
+    // nearest to the bound is that logit itself.
+    least = __double2float_rd(bound);
+    // (At huge temperatures the bound is below all numbers, and does not tell -inf from them.)
+    return fabs(top) < kFar && bound > -0x1p127;
+}
+
 /// Adds a lane's logit to the counters of steps below `top`.
 __device__ __forceinline__ void AddOne(float v, double top, double perUnit, uint64_t* masses, uint32_t* counts)
 {
@@ -408,7 +420,7 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
         counts[i] = 0;
     }
     double top = -INFINITY;
-    float least = -INFINITY;  // past the last step, where places are near
+    float least = -INFINITY;  // NearPlaces
     bool near = false;
     float most = -INFINITY;   // of the wave; of a greedy row's lane
     uint32_t at = 0;
@@ -502,10 +514,7 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
                 __builtin_amdgcn_wave_barrier();
             }
             top = moved;
-            const double bound = (top - (kSteps + 2)) / mode.perUnit;
-            least = static_cast<float>(bound);
-            // (At huge temperatures the bound is below all numbers, and does not tell -inf from them.)
-            near = fabs(top) < kFar && bound > -0x1p127;
+            near = NearPlaces(top, mode.perUnit, least);
         }
         if (!near)
         {
@@ -1441,9 +1450,8 @@ __global__ __launch_bounds__(kPickBlock, kPhase == kPickAll ? 1 : 4) void Sample
             return kept ? static_cast<double>(MassOf(place.rest)) * s.unit[static_cast<uint32_t>(dist)] : 0.0;
         };
         // The same of logits of which none is far, with fewer operations (AddNearBatch): by the cut's own logit.
-        const double bound = (top - (kSteps + 2)) / r.perUnit;
-        const bool near = fabs(top) < kFar && bound > -0x1p127;
-        const float least = static_cast<float>(bound);
+        float least;
+        const bool near = NearPlaces(top, r.perUnit, least);
         const uint32_t topStep = static_cast<uint32_t>(__double_as_longlong(top + kWhole));
         const bool none = cut.key == ~0ull;  // of the step of the cut
         const uint32_t lastStep = none ? step - 1 : step;

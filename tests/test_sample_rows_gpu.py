@@ -354,3 +354,33 @@ def test_agrees_with_the_log_probabilities(mh, gpu):
     torch.cuda.synchronize()
     # Logits of a few units: some eight roundings of that size.
     assert np.abs(host(out) - host(batch.logprobs)[:rows]).max() <= 64 * U * np.abs(host(out)).max()
+
+
+def peaked_rows(rng, rows, vocab, ties):
+    """Rows whose largest logit is alone or 37 times there, 23 others the next f32 numbers below it; some have masked
+    and missing logits."""
+    x = rng.normal(0, 2.5, (rows, vocab)).astype(np.float32)
+    for r, row in enumerate(x):
+        peak = np.float32([3.3, 20.3, 1000.7, -20.3][(r // 5 + r) % 4])
+        row[:] = np.minimum(row, 2.0) if peak > 0 else np.minimum(row, 2.0) - np.float32(30.0)
+        if r % 3:
+            row[rng.random(vocab) < 0.2] = -np.inf
+            row[rng.random(vocab) < 0.1] = np.nan
+        at = rng.choice(vocab, 60, replace=False)
+        row[at[:37 if ties[r] else 1]] = peak
+        row[at[37:]] = peak - np.spacing(peak) * np.arange(1, 24, dtype=np.float32)
+    return x
+
+
+@pytest.mark.parametrize("rows, vocab", [(1, 151936), (61, 151936), (500, 151936), (55, 3001), (4100, 500)])
+def test_small_temperatures(mh, gpu, rows, vocab):
+    """Where a unit in the last place of the largest logit is less than a step of weights, as many, and more than all
+    of them."""
+    rng = np.random.default_rng(rows)
+    temperatures = [1e-4, 1e-5, 1e-6, 1e-7, 2e-8, 1e-8, 1e-9, 1e-10, 1e-11, 1e-12, 1e-13, 1e-14]
+    cuts = [(0, 1.0, 0.0), (0, 1.0, 0.5), (0, 0.6, 0.0), (3000, 1.0, 0.0), (40, 0.9, 0.0)]
+    settings = [(t, *c) for t in temperatures for c in cuts]
+    for first in range(0, len(settings) if rows == 1 else 1):
+        these = [settings[(first + r) % len(settings)] for r in range(rows)]
+        x = peaked_rows(rng, rows, vocab, [s[2] == 0.6 or r % 2 for r, s in enumerate(these)])
+        Batch(mh, gpu, x, these, rng.random(rows)).check()
