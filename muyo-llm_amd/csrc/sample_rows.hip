@@ -283,7 +283,8 @@ __device__ __forceinline__ void AddOne(float v, double top, double perUnit, uint
 }
 
 /// The same of a batch, for places below kFar, with fewer operations: a step is the last 32 bits of a place's sum with
-/// kWhole. Logits below `least`, past the last step, count as that, so that no place is far.
+/// kWhole. Logits below `least`, past the last step, count as that, as does a NaN, so that no place is far; none is past
+/// the top or infinite.
 template <bool kCount, bool kMass>
 __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double top, float least, double perUnit,
                                              uint64_t* masses, uint32_t* counts)
@@ -298,11 +299,9 @@ __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double 
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            // The smaller of a signalling NaN and a number is a quiet NaN, the larger of that and a number the number.
+            // The larger of a signalling NaN and a number is a quiet NaN, of that and a number the number.
             float x;
-            asm("v_min_f32 %0, %2, %1\n\tv_max_f32 %0, %0, %3"
-                : "=&v"(x)
-                : "v"(v[q][e]), "s"(0x1.fffffep127f), "v"(least));
+            asm("v_max_f32 %0, %1, %2\n\tv_max_f32 %0, %0, %2" : "=&v"(x) : "v"(v[q][e]), "v"(least));
             const double y = static_cast<double>(x);
             const double whole = WholeOf(y, perUnit);
             step[e] = topStep - static_cast<uint32_t>(__double_as_longlong(whole));
@@ -516,7 +515,8 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
             top = moved;
             near = NearPlaces(top, mode.perUnit, least);
         }
-        if (!near)
+        // What counts as the largest number may be an infinity.
+        if (!near || batchMost == 0x1.fffffep127f)
         {
 #pragma unroll 1
             for (uint32_t i = 0; i < 4 * kQuads; ++i)

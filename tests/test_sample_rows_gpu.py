@@ -384,3 +384,48 @@ def test_small_temperatures(mh, gpu, rows, vocab):
         these = [settings[(first + r) % len(settings)] for r in range(rows)]
         x = peaked_rows(rng, rows, vocab, [s[2] == 0.6 or r % 2 for r, s in enumerate(these)])
         Batch(mh, gpu, x, these, rng.random(rows)).check()
+
+
+# Temperatures at which the largest f32's place on a grid of eighths of an octave, cut to 32 bits, is that of ordinary
+# logits.
+WRAPPED = [0.037677984684705734, 0.04902310296893120, 0.07893555611371994, 0.12279371172189713, 0.17001739144325256]
+
+
+@pytest.mark.parametrize("rows", [1, 61, 600])
+@pytest.mark.parametrize("temperature", WRAPPED)
+def test_missing_logits_are_not_large_ones(mh, gpu, temperature, rows):
+    """NaN at temperatures and peaks where the largest number's place would be one that counts."""
+    rng = np.random.default_rng(rows)
+    per_unit = 8.0 * 1.44269504088896340736 / temperature
+    assert np.float32(temperature) == temperature
+    wrapped = (np.float64(np.finfo(np.float32).max) * per_unit + 1.5 * 2.0 ** 52).view(np.int64).astype(np.int32)
+    cuts = [(0, 1.0, 0.0), (0, 0.9, 0.0), (3000, 1.0, 0.0), (40, 0.95, 0.0), (0, 1.0, 0.1)]
+    nans = np.array([0x7FC00000, 0xFFC00000, 0x7FFFFFFF], np.uint32).view(np.float32)
+    vocab = 20011
+    x = rng.normal(0, 2.5, (rows, vocab)).astype(np.float32)
+    for r, row in enumerate(x):
+        below = (8, 9, 40, 300, 500)[r % 5]  # steps that the wrapped place is below the first one
+        peak = np.float32((wrapped + below - 8) / per_unit)
+        row[:] = peak - np.abs(row) * np.float32(4.0 * temperature)
+        row[rng.integers(vocab)] = peak
+        missing = np.flatnonzero(rng.random(vocab) < (0.0002, 0.01, 0.3)[r // 5 % 3])
+        missing = missing[row[missing] != peak]
+        row[missing] = np.resize(nans, len(missing))
+    settings = [(temperature, *cuts[(r // 15 + r) % 5]) for r in range(rows)]
+    Batch(mh, gpu, x, settings, rng.random(rows)).check()
+
+
+@pytest.mark.parametrize("temperature", [1e24, 1e28, 1e33, 1e36, 1e38])
+def test_infinite_and_missing_logits_at_huge_temperatures(mh, gpu, temperature):
+    """The largest number, as which an infinity counts, near enough to the others for a step of its own or theirs."""
+    rng = np.random.default_rng(3)
+    vocab = 9001
+    most = np.finfo(np.float32).max
+    x = rng.normal(0, 1, (20, vocab)).astype(np.float32)
+    for r, row in enumerate(x):
+        row *= np.float32([1.0, 1e30, 1e36, 3e37][r % 4])
+        row[rng.integers(0, vocab, 30)] = (np.inf, most)[r // 4 % 2]
+        row[rng.integers(0, vocab, 2000)] = np.nan
+        row[rng.integers(0, vocab, 20)] = -np.inf
+    cuts = [(0, 1.0, 0.0), (0, 0.9, 0.0), (3000, 1.0, 0.0), (40, 0.95, 0.0), (0, 1.0, 0.1)]
+    Batch(mh, gpu, x, [(temperature, *cuts[r // 4]) for r in range(20)], rng.random(20)).check()
