@@ -174,9 +174,12 @@ __device__ __forceinline__ T OfLane(T v, int lane)
     return ByWords(v, [&](int w) { return __builtin_amdgcn_readlane(w, lane); });
 }
 
-/// A logit as it counts: -inf for NaN (the larger of a NaN and a number is the number), the largest finite one for
-/// +inf.
-__device__ __forceinline__ float Counted(float x) { return fminf(fmaxf(x, -INFINITY), 0x1.fffffep127f); }
+/// `x`, of a signalling NaN the quiet one: the larger of that and a number is the number, of a signalling one and a
+/// number a quiet NaN, so that the number would be lost.
+__device__ __forceinline__ float Quiet(float x) { return __builtin_canonicalizef(x); }
+
+/// A logit as it counts: -inf for NaN, the largest finite one for +inf.
+__device__ __forceinline__ float Counted(float x) { return fminf(fmaxf(Quiet(x), -INFINITY), 0x1.fffffep127f); }
 
 /// A logit's place on the grid.
 struct Place
@@ -284,7 +287,7 @@ __device__ __forceinline__ void AddOne(float v, double top, double perUnit, uint
 
 /// The same of a batch, for places below kFar, with fewer operations: a step is the last 32 bits of a place's sum with
 /// kWhole. Logits below `least`, past the last step, count as that, as does a NaN, so that no place is far; none is past
-/// the top or infinite.
+/// the top, infinite or a signalling NaN.
 template <bool kCount, bool kMass>
 __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double top, float least, double perUnit,
                                              uint64_t* masses, uint32_t* counts)
@@ -299,9 +302,9 @@ __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double 
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            // The larger of a signalling NaN and a number is a quiet NaN, of that and a number the number.
+            // As it stands: the compiler would make both quiet again.
             float x;
-            asm("v_max_f32 %0, %1, %2\n\tv_max_f32 %0, %0, %2" : "=&v"(x) : "v"(v[q][e]), "v"(least));
+            asm("v_max_f32 %0, %1, %2" : "=v"(x) : "v"(v[q][e]), "v"(least));
             const double y = static_cast<double>(x);
             const double whole = WholeOf(y, perUnit);
             step[e] = topStep - static_cast<uint32_t>(__double_as_longlong(whole));
@@ -458,6 +461,7 @@ __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
 #pragma unroll
         for (uint32_t i = 0; i < 4 * kQuads; ++i)
         {
+            v[i / 4][i % 4] = Quiet(v[i / 4][i % 4]);
             batchMost = fmaxf(batchMost, v[i / 4][i % 4]);
         }
         batchMost = fminf(batchMost, 0x1.fffffep127f);

@@ -429,3 +429,19 @@ def test_infinite_and_missing_logits_at_huge_temperatures(mh, gpu, temperature):
         row[rng.integers(0, vocab, 20)] = -np.inf
     cuts = [(0, 1.0, 0.0), (0, 0.9, 0.0), (3000, 1.0, 0.0), (40, 0.95, 0.0), (0, 1.0, 0.1)]
     Batch(mh, gpu, x, [(temperature, *cuts[r // 4]) for r in range(20)], rng.random(20)).check()
+
+
+@pytest.mark.parametrize("rows, vocab", [(1, 151936), (61, 20011), (700, 5003), (4100, 300)])
+def test_signalling_missing_logits(mh, gpu, rows, vocab):
+    """NaN of every kind before, behind and between the largest logits, in all settings."""
+    rng = np.random.default_rng(rows)
+    nans = np.array([0x7F800001, 0xFFBFFFFF, 0x7FC00000, 0xFFC00000, 0x7FA00000], np.uint32).view(np.float32)
+    for first in range(0, len(SETTINGS) if rows == 1 else 1):
+        x = logits_of(rng, rows, vocab)
+        for r, row in enumerate(x):
+            missing = np.flatnonzero(rng.random(vocab) < (0.001, 0.05, 0.6)[r % 3])
+            row[missing] = np.resize(nans, len(missing))
+            order = np.argsort(np.where(np.isnan(row), -np.inf, -row))[:40]  # and next to the largest
+            row[np.minimum(order[::2] + 1, vocab - 1)] = nans[0]
+        settings = [SETTINGS[(first + r) % len(SETTINGS)] for r in range(rows)]
+        Batch(mh, gpu, x, settings, rng.random(rows)).check()
