@@ -18,10 +18,6 @@ constexpr uint32_t kRowsOfBlock = kRowsOfWave * kWaves;
 constexpr uint32_t kMaxChunks = 128;
 constexpr uint32_t kFewChunks = 8;
 constexpr uint32_t kTurn = 256;           // workgroups of a kind in turn: one on each CU
-// Softmax weights as in the attention over a query's own keys: the maximum's is 2^kPrefixBias, 2^15 at most.
-constexpr float kPrefixLag = 10.0f;
-constexpr float kPrefixBias = 15.0f - kPrefixLag;
-constexpr float kPrefixLowScale = 2048.0f;
 
 struct PagedPrefixArgs
 {
@@ -74,7 +70,9 @@ inline constexpr uint32_t kPrefixBytes = kPrefixStages<kHd> * 2 * kStep * 2 * kH
 /// and V through LDS, where they go straight from memory a step ahead. Per step a wave
 ///   - forms S^T (keys x rows) = K . q^T, K from LDS, q in registers as two planes of f16 (of q / 2^e, e by the row's
 ///     largest value, as in the attention over own keys: the two are joined by their raw scores);
-///   - makes the softmax weights of a row's 32 keys in a lane, one exchange with the lane 32 away, in two planes;
+///   - makes the softmax weights of a row's 32 keys in a lane, one exchange with the lane 32 away, in two planes that
+///     keep the bits of own keys' weights (accumulators that follow a maximum only 2^10 ahead would save 1.5 % of the
+///     time and cost 1e-4 of a result 20 nats below a key with a value of 0);
 ///   - O^T (channels x rows) += V^T . P^T, V^T by transposing LDS reads, keys in the order that the scores have.
 /// The weights' low plane, times 2048, has sums of its own, so that small weights count beside a key that has most of
 /// the weight: at head_dim 64 accumulators beside the others, at 128, where these would not fit the registers, sums of
@@ -345,7 +343,7 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
             stepMax = fmaxf(stepMax, fmaxf(score[0][r], score[1][r]));
         }
         stepMax = fmaxf(stepMax, PartnerLane<32>(stepMax));
-        const bool rises = stepMax != -INFINITY && (base == -INFINITY || (stepMax - base) * scaleLog2 > kPrefixLag);
+        const bool rises = stepMax != -INFINITY && (base == -INFINITY || (stepMax - base) * scaleLog2 > kLag);
         if (__any(rises))
         {
             const float factor =
@@ -372,7 +370,7 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 #pragma unroll
             for (int e = 0; e < 2; ++e)
             {
-                p[e] = __builtin_amdgcn_exp2f(fmaf(score[i / 16][i % 16 + e] - from, scaleLog2, kPrefixBias));
+                p[e] = __builtin_amdgcn_exp2f(fmaf(score[i / 16][i % 16 + e] - from, scaleLog2, kWeightBias));
                 sum[(i + e) % 4] += p[e];
             }
             // The high plane is cut off, the low one has what that leaves: one operation a pair and one a weight.
@@ -382,7 +380,7 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
             {
                 phi[i / 8][i % 8 + e] = hi[e];
                 plo[i / 8][i % 8 + e] = static_cast<_Float16>(
-                    fmaf(static_cast<float>(hi[e]), -kPrefixLowScale, kPrefixLowScale * p[e]));
+                    fmaf(static_cast<float>(hi[e]), -kLowScale, kLowScale * p[e]));
             }
         }
         runSum += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -415,7 +413,7 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
                 {
-                    o[c][r] = fmaf(add[r], 1.0f / kPrefixLowScale, o[c][r]);
+                    o[c][r] = fmaf(add[r], 1.0f / kLowScale, o[c][r]);
                 }
             }
         }
@@ -435,7 +433,7 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
     {
         if (kKeepLow)
         {
-            o[c] += oLow[c] * (1.0f / kPrefixLowScale);
+            o[c] += oLow[c] * (1.0f / kLowScale);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -537,7 +535,6 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
         pieces = cut.w;
     }
     const uint32_t parts = prefix.chunks + max(pieces, 1u);
-    const float ownUnits = __builtin_amdgcn_exp2f(kPrefixBias - kWeightBias);  // of its weights, in the prefix's
     float base = -INFINITY;
     float den = 0.0f;
     float scaleLog2 = 1.0f;
@@ -583,8 +580,8 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
                 if (p0 + i * kSlices < parts)
                 {
                     // A piece without keys is all 0; one of NaN scores has this base too, and stays NaN.
-                    float w = of[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((of[i][0] - best) * scaleLog2);
-                    w *= p0 + i * kSlices < prefix.chunks ? 1.0f : ownUnits;
+                    const float w =
+                        of[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((of[i][0] - best) * scaleLog2);
                     den = fmaf(w, of[i][1], den);
                     num += w * x[i];
                 }

@@ -197,6 +197,32 @@ def test_a_key_that_has_most_of_the_weight(mh, gpu, heads, kv, hd, value):
         batch.check(rtol=ATTENTION_RTOL * 2.0)
 
 
+@pytest.mark.parametrize("heads, kv, hd", [(14, 2, 64), (28, 4, 128), (16, 1, 128)])
+@pytest.mark.parametrize("value, spread", [(0.0, 0.1), (0.01, 0.1), (0.0, 1.0)])
+def test_small_weights_as_in_the_attention_over_own_keys(mh, gpu, heads, kv, hd, value, spread):
+    """Its test of a key with most of the weight, at its tolerance, with that key a query's own or the prefix's."""
+    rng = np.random.default_rng(hd + heads)
+    nats = np.array([20.0, 8.0, 17.0, 14.0, 12.0, 0.0])
+    batch = Shared(mh, gpu, rng, heads, kv, hd, 16, np.array([100, 300, 1000, 20, 2000, 64]), 3000)
+    batch.caches[0] *= np.float16(spread)
+    with_sinks(batch, rng, nats, value)
+    out = batch.call()
+    gpu.cuda.synchronize()
+    for i in range(len(nats)):
+        batch.compare(host(out), rtol=ATTENTION_RTOL * max(1.0, nats[i] / 10), some=[i])
+    for which in range(3):
+        batch = Shared(mh, gpu, rng, heads, kv, hd, 16, np.array([100, 300, -1]), 3000)
+        batch.caches[0] *= np.float16(spread)
+        key = [0, 1700, 2999][which]
+        at = batch.tables[batch.prefix[0], key // 16], slice(None), key % 16
+        for g, q in enumerate(batch.q[which].astype(np.float64).reshape(kv, heads // kv, hd)):
+            batch.caches[0][at][g] = np.linalg.pinv(q) @ np.full(heads // kv, nats[which] / batch.scale)
+        batch.caches[1][at] = rng.normal(0, value, (kv, hd))
+        out = batch.call()
+        gpu.cuda.synchronize()
+        batch.compare(host(out), rtol=ATTENTION_RTOL * max(1.0, nats[which] / 10), some=[which])
+
+
 @pytest.mark.parametrize("q_std, scale", [(2.0, 1e9), (2.0, -1e12), (2.0, 3e38), (1e20, 1e25), (1e-20, 1e38)])
 def test_scores_far_past_any_exponent(mh, gpu, q_std, scale):
     """The largest score's value is the output, but for the weights' planes and the joins' products, and keys that are
