@@ -669,9 +669,10 @@ enum
 
 /* muyo_paged_rope_append_f16kv into such a cache. A row y of a kv head (k rotated, or v) is stored with
  *   scale = max|y| / 127 (int8) or / 448 (e4m3), rounded to f32, codes = y / scale, rounded to the nearest (even)
- * from 64 bits, k's rotation included. A row of zeros has scale 0, as has one too small for f32 to hold its scale;
- * one with an infinity or a NaN has scale NaN and codes 0. head_dim 64 or 128; else as above. Caches and scales are
- * 16-byte aligned and overlap nothing else. */
+ * from 64 bits, k's rotation included, and at most 127 or 448 in size (scales next to f32's smallest are rounded by
+ * more than half a code). A row of zeros has scale 0, as has one too small for f32 to hold its scale; one that a
+ * magnitude makes too large for that has an infinite scale, one with an infinity or a NaN scale NaN, and all of them
+ * codes 0. head_dim 64 or 128; else as above. Caches and scales are 16-byte aligned and overlap nothing else. */
 int muyo_paged_rope_append_q8kv(const float* q, const float* k, const float* v, uint64_t q_stride, uint64_t k_stride,
                                 uint64_t v_stride, float* q_out, void* kcache, void* vcache, float* kscales,
                                 float* vscales, const int32_t* positions, const int32_t* slots, uint32_t tokens,

@@ -220,9 +220,9 @@ __global__ __launch_bounds__(256) void PagedAppendQ8Kernel(AppendQ8Args a)
     constexpr double kMost = kFormat == MUYO_KV_INT8 ? 127.0 : 448.0;
     const double size = __longlong_as_double(static_cast<long long>(largest));
     const bool finite = size < INFINITY;
-    // A row that is not finite is told by its scale.
+    // A row that is not finite, or that a magnitude has taken past f32, is told by its scale.
     const float scale = finite ? static_cast<float>(size / kMost) : NAN;
-    const bool codes = finite && scale > 0.0f;
+    const bool codes = scale > 0.0f && scale < INFINITY;
     // Quotients by the reciprocal and a step from what is left, which rounds them as a division does (Markstein).
     const double wide = codes ? static_cast<double>(scale) : 1.0;
     const double per = 1.0 / wide;

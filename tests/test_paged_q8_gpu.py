@@ -181,6 +181,27 @@ def test_append_of_borders_and_extreme_rows(mh, gpu, hd, form):
     batch.check(0, hd, turns, 1.0)
 
 
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("layout, rotary", [(0, 64), (1, 64), (0, 20)])
+def test_append_of_rows_past_f32(mh, gpu, layout, rotary, form):
+    """A magnitude that takes some rows of k to where f32 ends, and past it: their scale is infinite, their codes 0."""
+    rng = np.random.default_rng(5)
+    n, hd, size = 40, 64, 16
+    turns, _ = mh.rope_frequencies(1e4, rotary)
+    k = rng.uniform(0.5, 1, (n, 1, hd)) * 2.0 ** (np.arange(n) + 88.0)[:, None, None]
+    batch = Append(mh, gpu, rng, 1, 1, hd, size, form, [np.zeros((n, 1, hd)), k, np.ones((n, 1, hd))],
+                   rng.integers(0, 3000, n), rng.permutation(48)[:n], 3)
+    batch.call(layout, rotary, turns, 2.0 ** 30)
+    gpu.cuda.synchronize()
+    rotated, _ = rotate64(batch.parts[1].reshape(n, 1, hd), batch.positions, turns, 2.0 ** 30, layout, rotary)
+    codes, scales = quantise(rotated[:, 0], form)
+    codes[np.isinf(scales)] = 0  # of either sign
+    assert np.isinf(scales).any() and (scales < np.inf).any()
+    at = batch.slots // size, 0, batch.slots % size
+    assert np.array_equal(host(batch.d[2])[at], scales)
+    assert np.array_equal(host(batch.d[0])[at], codes)
+
+
 def test_append_in_place_is_the_fp16_caches_rotation(mh, gpu):
     """q_out may be q, and q is rotated as by the fp16 cache's append, bit for bit."""
     torch, rng = gpu, np.random.default_rng(3)
