@@ -682,8 +682,10 @@ int muyo_paged_rope_append_q8kv(const float* q, const float* k, const float* v, 
 
 /* muyo_paged_attention_decode_f16kv over such a cache, of the values as they are stored:
  *   out[i][h] = sum_j softmax_j(scale * kscale_j * (q[i][h].kcode[j])) * vscale_j * vcode[j]
- * Rows and scales that a query sees are finite; the others may hold anything. The rest, the workspace too, as
- * above. */
+ * Rows and scales that a query sees are finite, K's scales at most 2^96 in size and V's at most 2^110 over the number
+ * of keys that it sees (sums of weights of up to 2^8 times a scale and a code are f32); where V's are below 2^-79, out
+ * is good to 2^-84 and not to its own last bits. What a query does not see may hold anything. The rest, the workspace
+ * too, as above. */
 size_t muyo_paged_attention_decode_q8kv_workspace_bytes(uint32_t queries, uint32_t heads, uint32_t kv_heads,
                                                         uint32_t head_dim); /* 0: unsupported shape */
 int muyo_paged_attention_decode_q8kv(const float* q, const void* kcache, const void* vcache, const float* kscales,

@@ -139,9 +139,11 @@ __device__ __forceinline__ uint32_t ValueAt(uint32_t row, uint32_t chunk)
 ///   - K's codes are widened to f16, which holds them exactly, in registers on the way to the matrix cores, where they
 ///     meet the same two planes of q; a key's scale multiplies its score;
 ///   - V's are widened to bf16, as exact, on the way to LDS; a key's weight is multiplied by its scale before it meets
-///     them, in three planes of bf16, whose exponent is f32's: all 24 bits, whatever the scale and however small the
-///     weight beside the largest. (Two planes of f16 would want those products kept in f16's range, a second running
-///     maximum.) Three matrix operations for the fp16 cache's two;
+///     them, in three planes of bf16, whose exponent is f32's: all 24 bits of weights down to 2^-31 with scales down to
+///     2^-79. (Two planes of f16 would want those products kept in f16's range, a second running maximum.) Three matrix
+///     operations for the fp16 cache's two;
+///   - f32 ends: raw scores are below 2^30 (q / 2^e below 2^14, codes of up to 448, 128 channels) before a K scale of up
+///     to 2^96, and a sum over n keys is of weights of up to 2^kLag, codes and V scales of up to 2^110 / n;
 ///   - a tile is half the bytes, so two are on their way.
 ///
 /// What bounds it: two waves of a SIMD taking turns at the codes' widening (176 vector operations of 390 for a tile of

@@ -435,6 +435,58 @@ def test_attention_of_scores_far_past_any_exponent(mh, gpu, q_std, scale):
         batch.check()
 
 
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("heads, kv, hd, position", [(14, 2, 64, 700), (28, 4, 128, 3000)])
+def test_attention_of_the_largest_and_smallest_scales(mh, gpu, heads, kv, hd, position, form):
+    """Scales at the ends that the call is stated for."""
+    rng = np.random.default_rng(7)
+    for k_most, v_most in ((96, 110 - np.log2(position + 1)), (96, -72), (-140, -72), (-140, 96)):
+        batch = Attend8(mh, gpu, rng, heads, kv, hd, 16, np.array([position, 40]), form=form)
+        k_size, v_size = (2.0 ** np.floor(most - np.log2(float(batch.scales[i].max())))
+                          for i, most in enumerate((k_most, v_most)))
+        # K's rows are then of that size, and scores as elsewhere.
+        batch.scales[0] *= np.float32(k_size)
+        batch.scales[1] *= np.float32(v_size)
+        assert batch.scales[0].max() <= 2.0 ** 96 and batch.scales[1].max() <= 2.0 ** 110 / (position + 1)
+        batch.scale /= max(k_size, 2.0 ** -120)
+        batch.q *= np.float32(max(k_size, 2.0 ** -120) / k_size)
+        batch.caches = batch.values()
+        batch.check()
+
+
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("keys", [1000, 3000])
+def test_attention_of_equal_values_at_the_largest_scale(mh, gpu, keys, form):
+    """Weights that a later maximum leaves above 1, each of the largest code and scale: the sum is the largest that a
+    call is stated for, and the output that value."""
+    heads, kv, hd = 28, 4, 128
+    batch = Attend8(mh, gpu, np.random.default_rng(2), heads, kv, hd, 16, np.array([keys - 1]), form=form)
+    batch.q[:] = 1.0
+    batch.scale = 0.125 / hd
+    batch.codes[1] = 127 if form == INT8 else 126  # the largest
+    batch.scales[1] = 2.0 ** 110 / keys
+    batch.codes[0] = 56 if form == E4M3 else 1     # 1
+    batch.scales[0] = 1.0
+    later = batch.tables[0][np.arange(128, keys) // 16], slice(None), np.arange(128, keys) % 16
+    batch.scales[0][later] = 8.0 * 5.4             # nats above the first 128 keys' 1 / 8: 2^7.6 of their weight
+    batch.caches = batch.values()
+    want = LARGEST[form] * float(np.float32(2.0 ** 110 / keys))
+    out = host(batch.call())
+    assert np.abs(out / want - 1).max() <= ATTENTION_RTOL
+
+
+@pytest.mark.parametrize("form", FORMATS)
+def test_attention_of_vanishing_scales(mh, gpu, form):
+    for most in (-80, -100, -120, -126, -140):
+        batch = Attend8(mh, gpu, np.random.default_rng(3), 14, 2, 64, 16, np.array([2000, 15]), form=form)
+        batch.scales[1] = batch.scales[1] / batch.scales[1].max() * 2.0 ** most
+        batch.caches = batch.values()
+        out = host(batch.call())
+        for i, p in enumerate(batch.positions):
+            want = attend64(batch.q[i], *batch.caches, batch.tables[i], int(p), 0, batch.scale)
+            assert np.abs(out[i] - want).max() <= 2.0 ** -84 + ATTENTION_RTOL * np.abs(want).max(), most
+
+
 def test_attention_past_four_gigabytes_of_cache(mh, gpu):
     """Pages whose codes lie past 2^32 bytes of the cache."""
     torch, rng = gpu, np.random.default_rng(14)
