@@ -50,7 +50,7 @@ struct PartHead
     uint32_t at;   // the first place of that, of a greedy row
 };
 
-/// What is known of a row's steps before its token is chosen, and the list of those near the cut.
+/// What is known of a row's steps before its token is chosen, and which are listed.
 struct RowSteps
 {
     double upTo[kSteps];
@@ -60,7 +60,6 @@ struct RowSteps
     float low, high;       // bounds of their logits
     uint32_t listed;
     uint32_t unused;
-    uint64_t keys[kListed];
 };
 
 struct SampleArgs
@@ -82,6 +81,8 @@ struct SampleArgs
     float* batchMost;    // [rows][parts][batches]: the largest logit of each
     uint32_t batches;    // of a part, at most
     RowSteps* steps;     // [rows], of at most kListRows; where the workspace begins
+    uint64_t* listKeys;  // [rows][listRoom] of these
+    uint32_t listRoom;
 };
 
 /// What a row asks for.
@@ -286,8 +287,8 @@ __device__ __forceinline__ void AddOne(float v, double top, double perUnit, uint
 }
 
 /// The same of a batch, for places below kFar, with fewer operations: a step is the last 32 bits of a place's sum with
-/// kWhole. Logits below `least`, past the last step, count as that, as does a NaN, so that no place is far; none is past
-/// the top, infinite or a signalling NaN.
+/// kWhole. Logits below `least`, past the last step, count as that, as does a NaN, so that no place is far; none is
+/// past the top, infinite or a signalling NaN.
 template <bool kCount, bool kMass>
 __device__ __forceinline__ void AddNearBatch(const float4v (&v)[kQuads], double top, float least, double perUnit,
                                              uint64_t* masses, uint32_t* counts)
@@ -1204,10 +1205,11 @@ __global__ __launch_bounds__(kPickBlock, kPhase == kPickAll ? 1 : 4) void Sample
     {
         listFirst = kept->first;
         listLast = kept->last;
-        const uint32_t listed = listFirst <= listLast ? min(kept->listed, kListed) : 0;
+        const uint32_t listed = listFirst <= listLast ? min(kept->listed, a.listRoom) : 0;
+        const uint64_t* const keys = a.listKeys + static_cast<uint64_t>(row) * a.listRoom;
         for (uint32_t i = threadIdx.x; i < listed; i += kPickBlock)
         {
-            s.keys[i] = kept->keys[i];
+            s.keys[i] = keys[i];
         }
         if (threadIdx.x == 0)
         {
@@ -1718,6 +1720,7 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
         return;
     }
     const float* const x = a.logits + row * a.stride;
+    uint64_t* const keys = a.listKeys + static_cast<uint64_t>(row) * a.listRoom;
     const double perUnit = kept->perUnit;
     const double top = kept->top;
     const float low = kept->low;
@@ -1769,10 +1772,10 @@ __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
             if (counted > -INFINITY && d >= first && d <= last)
             {
                 const uint32_t at = atomicAdd(&kept->listed, 1u);
-                if (at < kListed)
+                if (at < a.listRoom)
                 {
                     // In any order: what is made of them goes by their own.
-                    kept->keys[at] = OrderKey(counted, IndexOf(range, batch0 + b, bit));
+                    keys[at] = OrderKey(counted, IndexOf(range, batch0 + b, bit));
                 }
             }
         }
@@ -1797,6 +1800,9 @@ Parts PartsOf(uint32_t rows, uint32_t vocab)
 
 /// Batches of a part: one more than its logits fill, since they may begin anywhere.
 uint32_t BatchesOf(const Parts& parts) { return parts.length / kBatch + 1; }
+
+/// Keys of a row's list.
+uint32_t ListRoom(uint32_t vocab) { return std::min(vocab, kListed); }
 }  // namespace
 }  // namespace muyo
 
@@ -1810,7 +1816,7 @@ extern "C" size_t muyo_sample_rows_workspace_bytes(uint32_t rows, uint32_t vocab
     }
     const Parts parts = PartsOf(rows, vocab);
     return (sizeof(PartHead) + 12ull * kSteps + 4ull * BatchesOf(parts)) * rows * parts.count +
-           (rows <= kListRows ? sizeof(RowSteps) * rows : 0);
+           (rows <= kListRows ? (sizeof(RowSteps) + sizeof(uint64_t) * ListRoom(vocab)) * rows : 0);
 }
 
 extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab,
@@ -1874,10 +1880,13 @@ extern "C" int muyo_sample_rows_f32(const float* logits, uint64_t row_stride, ui
     const uint64_t blocks = static_cast<uint64_t>(rows) * parts.count;
     char* space = static_cast<char*>(workspace);
     SampleArgs a{logits, row_stride, rows, vocab, temperatures, top_ks, top_ps, min_ps, randoms, tokens, logprobs,
-                 parts.count, parts.length, nullptr, nullptr, nullptr, nullptr, BatchesOf(parts), nullptr};
+                 parts.count, parts.length, nullptr, nullptr, nullptr, nullptr, BatchesOf(parts), nullptr, nullptr,
+                 ListRoom(vocab)};
     const bool lists = rows <= kListRows;
     a.steps = reinterpret_cast<RowSteps*>(space);
     space += lists ? sizeof(RowSteps) * rows : 0;
+    a.listKeys = reinterpret_cast<uint64_t*>(space);
+    space += lists ? sizeof(uint64_t) * a.listRoom * rows : 0;
     a.masses = reinterpret_cast<uint64_t*>(space);
     a.heads = reinterpret_cast<PartHead*>(space + 8ull * kSteps * blocks);
     a.counts = reinterpret_cast<uint32_t*>(space + (8ull * kSteps + sizeof(PartHead)) * blocks);

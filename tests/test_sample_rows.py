@@ -42,3 +42,10 @@ def test_workspace_sizes_of_unsupported_shapes_are_zero(mh):
     assert size(1, 1) > 0 and size((1 << 22) - 1, 1000) > 0 and size(1, 1 << 24) > 0
     for shape in ((0, 100), (1, 0), (1 << 22, 100), (1, (1 << 24) + 1)):
         assert size(*shape) == 0, shape
+
+
+def test_lists_take_no_more_than_their_rows_have(mh):
+    """What rows that are listed need beside others: a row's steps, and a key for each logit up to 4096."""
+    size = mh.load().muyo_sample_rows_workspace_bytes
+    for vocab in (1, 7, 1000, 4096, 30000):
+        assert size(4096, vocab) - size(4097, vocab) <= 4096 * (6200 + 8 * min(vocab, 4096)), vocab
