@@ -78,12 +78,13 @@ inline constexpr uint32_t kPrefixBytes = kPrefixStages<kHd> * 2 * kStep * 2 * kH
 /// the weight: at head_dim 64 accumulators beside the others, at 128, where these would not fit the registers, sums of
 /// the step that are added to the others by a multiply-add.
 ///
-/// What bounds it: vector and matrix work, which a SIMD's two waves overlap little. 250 queries of 28 / 4 heads of 128
-/// with 16381 keys: 121 us alone, 141 with up to 500 own keys, of which at 2.4 GHz the vector units are busy for 55 and
-/// the matrix cores for 49 (the clock is below that here). 32 keys at a time took 2 % more, without V's reads ahead of
-/// the weights 2 to 4; one wave a SIMD, with the next step's matrix operations between this one's weights, 200 us; other
-/// orders of the chunks in LDS, with fewer bank conflicts (0.4 of its time), and a wave's priority in either kind of
-/// work, no less.
+/// What bounds it: vector work, matrix work and LDS reads, which a SIMD's two waves overlap little: each wave reads all
+/// of a step's K and V for its 32 rows. 250 queries of 28 / 4 heads of 128 with 16381 keys: 137 us with one own key
+/// each, 146 with up to 500, of which at 2.4 GHz the vector units are busy for 57, the matrix cores for 49 and LDS for
+/// 26 (24 of them K's and V's reads at 128 bytes a clock), and 12 more in bank conflicts (the clock is below that
+/// here). 32 keys at a time took 2 % more, without V's reads ahead of the weights 2 to 4; one wave a SIMD, with the
+/// next step's matrix operations between this one's weights, 200 us; other orders of the chunks in LDS, with fewer bank
+/// conflicts, and a wave's priority in either kind of work, no less.
 ///
 /// Steps that reach past the prefix, or into a page that is not there, are masked: scores to -inf, and V's rows to 0 in
 /// LDS, since 0 * NaN would be NaN.
@@ -466,10 +467,10 @@ __device__ __forceinline__ void PrefixKeysOfRows(const PagedPrefixArgs& a, uint3
 /// which wait for memory, in turns of a CU each. The q of a workgroup may be read when others have ended, so none
 /// writes `out`.
 ///
-/// Two launches, the prefix's before the own keys', took 14.3 us for 3 queries (1009 keys and up to 100 own, 14 / 2
-/// heads of 64), together 10.3; 64 queries (8190 and up to 2000, 28 / 4 of 128) 53 and 45; 250 (16381 and up to 500)
-/// 183 and 172 (with faster weights since then 41 and 150). In turns of 8, 128 and 512 workgroups, or with the own keys
-/// first, 1 to 70 us more.
+/// When both were built, two launches, the prefix's before the own keys', took 14.3 us for 3 queries (1009 keys and up
+/// to 100 own, 14 / 2 heads of 64) and one 10.3; for 64 queries (8190 and up to 2000, 28 / 4 of 128) 53 and 45; for 250
+/// (16381 and up to 500) 183 and 172. One takes 10.3, 39.4 and 157 now (each with 4 to 10 for the join); in turns of 8,
+/// 128 and 512 workgroups the latter two take 49, 44 and 39, and 216, 178 and 167, with the own keys first 41 and 155.
 template <int kHd, bool kSplit>
 __global__ __launch_bounds__(kBlock, 2) void PagedPrefixKernel(PagedPrefixArgs a, PagedAttentionF16Args own,
                                                                uint32_t prefixBlocks, uint32_t ownBlocks)
@@ -620,9 +621,9 @@ __global__ __launch_bounds__(256) void PagedPrefixJoinKernel(PagedPrefixArgs a)
 
 /// Chunks of the prefix: workgroups for one on each of 256 CUs, beside one of own keys; two where that would be few
 /// chunks, so that rounding their number down leaves many CUs without. 28 / 4 heads of 128: 64 queries, 8190 keys in 16
-/// chunks 44.7 us, in 32 47.8; 16 queries, 16000 keys in 64 chunks 31.3 us, in 128 38.0; 250 queries, 16381 keys in 9
-/// chunks 170 us, in 4 207. (A number of workgroups of the same rows that is a multiple of eight, which keeps those of
-/// the same keys on one XCD, gained nothing: the last in 8 chunks 5 us slower.)
+/// chunks 40.1 us, in 32 44.5; 16 queries, 16000 keys in 64 chunks 29.7 us, in 128 36.6; 250 queries, 16381 keys in 9
+/// chunks 157 us, in 4 182. (A number of workgroups of the same rows that is a multiple of eight, which keeps those of
+/// the same keys on one XCD, gained nothing: the last in 8 chunks 5 us slower, when it took 187.)
 uint32_t PrefixChunks(uint32_t queries, uint32_t heads, uint32_t kvHeads)
 {
     const uint32_t blocks = kvHeads * CeilDiv(static_cast<uint64_t>(queries) * (heads / kvHeads), kRowsOfBlock);
@@ -663,7 +664,7 @@ hipError_t LaunchPrefix(hipStream_t s, const PagedPrefixArgs& a, const PagedAtte
     }
     const uint64_t items = static_cast<uint64_t>(a.queries) * a.kvHeads * a.group;
     // 256 threads have 32 parts of 128 channels on their way, 64 have 8: 16 queries of 28 heads with 64 chunks take
-    // 31.0 us in all with 256 and 38.8 with 64, 64 queries with 16 chunks 43.3 and 44.3, 250 with 9 178 and 171.
+    // 29.7 us in all with 256 and 37.5 with 64, 64 queries with 16 chunks 40.0 and 41.2, 250 with 9 164 and 157.
     if (a.chunks >= 16)
     {
         hipLaunchKernelGGL((PagedPrefixJoinKernel<kHd, 256>), dim3(static_cast<uint32_t>(items)), dim3(256), 0, s, a);

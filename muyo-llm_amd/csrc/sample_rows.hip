@@ -397,8 +397,8 @@ __device__ __forceinline__ void LoadBatch(const float* x, const PartRange& r, ui
 /// LDS, from a step above the largest logit that it has met; a larger one moves them down, which is rare.
 ///
 /// What bounds it: some 20 vector operations a logit, ten of them in 64 bits, beside the logits' arrival: 500 rows of
-/// 151936 in 76 us, 4.0 TB/s, the vector units busy for 0.6 of that at 2.4 GHz. Two batches on their way, or three or
-/// five waves a SIMD, were slower.
+/// 151936 in 70 us, 4.4 TB/s, the vector units busy for 0.65 of that at 2.4 GHz, and 0.6 of the LDS operations' time in
+/// bank conflicts. Two batches on their way, or three or five waves a SIMD, were slower.
 __global__ __launch_bounds__(kBlock, 4) void SampleCountKernel(SampleArgs a)
 {
     __shared__ uint64_t massOf[kWaves][kSteps];
@@ -1032,9 +1032,9 @@ enum PickPhase
 /// What bounds it: a workgroup's chain of searches, each some passes over the list between barriers (1.3 us where a
 /// wave can look at all, 4 for thousands); where the list does not do, 64-bit work for half a part of the row (10 us of
 /// 30, where 500 rows have 4 parts); and where a cut's step is not to be listed, a pass over the row for each range of
-/// it (500 rows of 151936 of standard deviation 0.75 take 337 us in all, of 2.5 with some that stand out 129; by digits
+/// it (500 rows of 151936 of standard deviation 0.75 take 311 us in all, of 2.5 with some that stand out 131; by digits
 /// of the keys, eight passes, the former took 980). Two workgroups fit a CU at 123 registers: with more loads on their
-/// way in such passes, 171 and one, 500 rows with lists took 142 us.
+/// way in such passes, 169 and one, 500 rows with lists take 143 us.
 template <PickPhase kPhase>
 __global__ __launch_bounds__(kPickBlock, kPhase == kPickAll ? 1 : 4) void SamplePickKernel(SampleArgs a)
 {
@@ -1699,8 +1699,8 @@ __global__ __launch_bounds__(kPickBlock, kPhase == kPickAll ? 1 : 4) void Sample
 /// steps are not read: tokens that stand out of a row are in few of them.
 ///
 /// What bounds it: the arrival of the others, at one CU if the workgroup that decides the row listed them (608 KB in
-/// 13 us). A batch a wave where all fit the GPU at about once, else two: one row 28.3 us in all with one and 29.3 with
-/// two, 61 rows 54.8 and 55.4, 500 154.0 and 149.5 (with four 153).
+/// 13 us). A batch a wave where all fit the GPU at about once, else two: one row 27.5 us in all with one and 28.6 with
+/// two, 61 rows 53.3 and 54.5, 500 134.3 and 131.2 (with four 135.2).
 template <uint32_t kBatches>
 __global__ __launch_bounds__(kBlock) void SampleListKernel(SampleArgs a)
 {
